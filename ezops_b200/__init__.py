@@ -1,13 +1,19 @@
 """ezops_b200: the Qwen3 dense-decode path of ez-ops as hand-written sm_100a
-kernels behind ez-ops' own operator / registry API."""
+kernels behind ez-ops' own operator / registry API, and the operators that take
+prompts through the same model over the same paged caches."""
 
 from . import kernels as _kernels  # noqa: F401  (registers the backends; needs libezb200.so)
 from .ops import (
     AttnDecodeOp,
+    AttnPromptOp,
     FusedOProjFfnOp,
     FusedQkNormRopeOp,
     GemvOp,
+    LinearOp,
     Op,
+    PagedPlan,
+    PagedPlanOp,
+    PagedQkNormRopeOp,
     PdlGemmOp,
     Qwen3DecodeStackOp,
     Qwen3DenseDecodeOp,
@@ -21,10 +27,15 @@ from .registry import get_kernel, list_backends, list_ops, register_kernel
 
 __all__ = [
     "AttnDecodeOp",
+    "AttnPromptOp",
     "FusedOProjFfnOp",
     "FusedQkNormRopeOp",
     "GemvOp",
+    "LinearOp",
     "Op",
+    "PagedPlan",
+    "PagedPlanOp",
+    "PagedQkNormRopeOp",
     "PdlGemmOp",
     "Qwen3DecodeStackOp",
     "Qwen3DenseDecodeOp",

@@ -1,0 +1,721 @@
+// Causal attention of ragged rows over paged KV caches, on the 5th-generation tensor cores:
+//   row b has n_b queries (tokens cu[b] .. cu[b+1]) behind c_b = len_b - n_b cached keys; query i of it sees the keys
+//   0 .. c_b + i:   out = softmax(q K^T / sqrt(D)) V,   H query heads share NKV key/value heads (G = H / NKV).
+//
+// Tile: the G heads of a group are packed next to each other, so 128 rows of an MMA are floor(128/G) tokens x G heads and
+// every key and value is read once per group.  A unit of work is 256 such rows (two tiles, two softmax warpgroups) of one
+// (row, kv head); it walks the keys 128 at a time.  Scores S (fp32) live in tensor memory, one thread owns a whole row of
+// them: running maximum and sum without a shuffle.  P is written back over S in bf16 and is the MMA's A operand from tensor
+// memory; O (fp32) stays there too.  2 x (128 + D) columns of the 512.  While one warpgroup exponentiates, the other tile's
+// products run.  The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the
+// result does not depend on which maximum is subtracted; sums and P stay far inside their ranges).
+// A unit with at most 128 rows (single tokens, the end of a prompt) uses the second tile for every other block of keys.
+//
+// Work is dealt out on the device, since the lengths are there: all units form one line, weighted by their keys, and CTA c
+// takes the c-th equal share; a unit that is cut leaves (max, sum, O) parts in the workspace, and the CTA that finishes its
+// last part joins them in the order of the keys (equal calls give equal bits).
+//
+// What bounds it: for prompts the exponentials and the products together - 128 x 128 scores take 512 cycles each for QK^T
+// and PV (D = 128) and 1024 cycles of the MUFU, twice per step; for single tokens the bytes of the caches.
+// Keys behind a row's last one, entries outside the pools and everything masked are never added: K there is masked after
+// the product, V is zero (out-of-range TMA boxes, or cleared in shared memory where a box straddles the end).
+#include "prompt.h"
+#include "tc.cuh"
+
+namespace ezb {
+
+static constexpr int kApThreads = 384;  // warps 0-3 and 4-7: softmax of tile 0 / 1; 8: TMA; 9: MMA; 10 and 11 fill up their warpgroup
+static constexpr int kApStages = 5;     // ring of K and V tiles
+static constexpr int kApKeys = 128;     // keys per tile
+static constexpr int kApUnitCost = 256;  // a unit's fixed cost in keys; at least 127, so that its last tile lies inside its cost
+static constexpr int kApMinShare = 256;  // keys below which a further CTA is not worth its merge
+
+struct ApParams {
+    bf16* Out;
+    long long ldo;
+    const int *table, *lens, *cu;
+    float* parts;        // [2 * grid slots][2 tiles][D + 2][128] fp32
+    unsigned int* count;  // [grid], zero between calls
+    int B, T, H, NKV, G, tpt, max_pages, page_shift, num_pages;
+    float scale_log2;  // log2(e) / sqrt(D)
+    unsigned int* status;
+};
+
+// ---- wrappers -----------------------------------------------------------------
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+        "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+          "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Descriptor of the B operand of P V: V is stored [key][64 elements] with the 128-byte swizzle, so the MMA's N runs along
+// the contiguous dimension; 64-element column blocks lie 16 KB apart, groups of eight keys 1 KB.
+template <int D>
+__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr) {
+    return umma_desc_sw128(smem_addr) | (D > 64 ? (uint64_t)(16384u >> 4) << 16 : 0ull);
+}
+
+// ---- the line of work ----------------------------------------------------------
+// A unit: 2 * tpt consecutive tokens of a row for one kv head.
+struct ApRow {
+    int q0, n, len, units;  // first token, tokens, valid keys
+    long long per_unit;     // cost of unit j: per_unit + (j + 1) * 2 * tpt
+    long long head_cost;    // cost of all units of one head
+};
+__device__ __forceinline__ ApRow ap_row(const ApParams& p, int b) {
+    ApRow r;
+    r.q0 = min(max(__ldg(p.cu + b), 0), p.T);
+    r.n = min(max(__ldg(p.cu + b + 1), r.q0), p.T) - r.q0;
+    r.len = min(max(__ldg(p.lens + b), 0), p.max_pages << p.page_shift);
+    const int u = 2 * p.tpt;
+    r.units = (r.n + u - 1) / u;
+    r.per_unit = max(r.len - r.n, 0) + kApUnitCost;
+    r.head_cost = r.units * r.per_unit + (long long)u * r.units * (r.units + 1) / 2;
+    return r;
+}
+__device__ __forceinline__ long long ap_unit_start(const ApParams& p, const ApRow& r, int j) {  // inside its head
+    return j * r.per_unit + (long long)p.tpt * j * (j + 1);
+}
+
+struct ApLine {
+    long long total;
+    int ctas;  // CTAs that take a share
+};
+__device__ __forceinline__ long long ap_share(const ApLine& l, int c) { return l.total * c / l.ctas; }
+
+struct ApCursor {
+    int b, h, j;
+    long long x0;  // where the unit starts on the line
+    ApRow row;
+};
+struct ApSegment {
+    int tokens, first;    // tokens of the unit, its first token within the row
+    int extent, tiles;    // keys that any of its queries sees, in tiles of 128
+    int ks, ke;           // tiles of this CTA
+    bool dual, whole;     // at most 128 rows; nothing cut
+};
+__device__ __forceinline__ int ap_tile_at(long long x, long long x0, int tiles) {
+    const long long k = (x - x0) >> 7;
+    return x <= x0 ? 0 : (k < tiles ? (int)k : tiles);
+}
+// The unit under the cursor as CTA share [lo, hi) sees it; false when none of its tiles belongs to the share.
+__device__ __forceinline__ bool ap_segment(const ApParams& p, const ApCursor& c, long long lo, long long hi, ApSegment& s) {
+    const int u = 2 * p.tpt;
+    s.first = c.j * u;
+    s.tokens = min(u, c.row.n - s.first);
+    s.extent = max(0, c.row.len - (c.row.n - s.first - s.tokens));
+    s.tiles = (s.extent + kApKeys - 1) / kApKeys;
+    s.ks = ap_tile_at(lo, c.x0, s.tiles), s.ke = ap_tile_at(hi, c.x0, s.tiles);
+    s.dual = s.tokens <= p.tpt;
+    s.whole = s.ke - s.ks == s.tiles;
+    return s.tiles ? s.ks < s.ke : lo <= c.x0;  // a unit without keys belongs to the share in which it starts
+}
+// Next unit; false at the end of the batch.
+__device__ __forceinline__ bool ap_advance(const ApParams& p, ApCursor& c) {
+    c.x0 += c.row.per_unit + (long long)(c.j + 1) * 2 * p.tpt;
+    if (++c.j < c.row.units) return true;
+    c.j = 0;
+    if (++c.h < p.NKV) return true;
+    c.h = 0;
+    do {
+        if (++c.b >= p.B) return false;
+        c.row = ap_row(p, c.b);
+    } while (c.row.units == 0);
+    return true;
+}
+
+template <int D>
+struct ApSmem {
+    static constexpr int kTile = kApKeys * D * 2;  // a K, V or Q tile
+    static constexpr int kQ = 0;
+    static constexpr int kRing = 2 * kTile;
+    static constexpr int kTail = kRing + kApStages * kTile;
+    static constexpr int kBytes = kTail + 2048 + 1024;  // tail, alignment
+};
+
+struct ApTail {
+    uint64_t full[kApStages], empty[kApStages];
+    uint64_t q_full, q_empty, fix;
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+    uint32_t tmem;
+    int abort_flag;
+    int last;  // this CTA joins the parts of the unit
+    ApLine line;
+    ApCursor start;
+    long long warp_sum[kApThreads / 32];
+    int list[2 * 160];  // parts of a unit in the order of its keys: 2 * slot + tile, or -1
+};
+static_assert(sizeof(ApTail) <= 2048, "tail of the shared memory");
+
+template <int D>
+__global__ void __launch_bounds__(kApThreads, 1)
+attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                   const __grid_constant__ CUtensorMap mapV, const __grid_constant__ ApParams p) {
+    using L = ApSmem<D>;
+    constexpr int BLOCKS = D / 64;  // column blocks of 64 elements (128 bytes)
+    constexpr uint32_t IDESC_QK = umma_idesc_bf16(128, kApKeys);
+    constexpr uint32_t IDESC_PV = umma_idesc_bf16(128, D) | (1u << 16);  // B transposed: N is the contiguous dimension
+    extern __shared__ unsigned char ap_raw[];
+    const uint32_t raw = smem_u32(ap_raw);
+    unsigned char* smem = ap_raw + (((raw + 1023u) & ~1023u) - raw);
+    ApTail& t = *reinterpret_cast<ApTail*>(smem + L::kTail);
+    volatile int* abort_flag = &t.abort_flag;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+
+    if (tid == 0) {
+        for (int s = 0; s < kApStages; ++s) mbar_init(smem_u32(&t.full[s]), 1), mbar_init(smem_u32(&t.empty[s]), 1);
+        mbar_init(smem_u32(&t.q_full), 1), mbar_init(smem_u32(&t.q_empty), 1), mbar_init(smem_u32(&t.fix), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&t.s_full[i]), 1), mbar_init(smem_u32(&t.o_full[i]), 1);
+            mbar_init(smem_u32(&t.p_full[i]), 4), mbar_init(smem_u32(&t.o_empty[i]), 4);  // one arrival per warp
+        }
+        t.abort_flag = 0;
+        mbar_fence_init();
+    }
+    pdl_open(1);
+
+    // ---- where this CTA's share starts: running sums of the rows' costs, rows spread over the threads
+    const int cta = blockIdx.x;
+    auto row_cost = [&](int b) { return b < p.B ? ap_row(p, b).head_cost * p.NKV : 0; };
+    auto chunk_scan = [&](long long v, long long& total) {  // exclusive prefix over the block
+        long long s = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += up;
+        }
+        __syncthreads();
+        if (lane == 31) t.warp_sum[warp] = s;
+        __syncthreads();
+        long long before = 0, all = 0;
+        for (int w = 0; w < kApThreads / 32; ++w) {
+            if (w == warp) before = all;
+            all += t.warp_sum[w];
+        }
+        total = all;
+        return before + s - v;
+    };
+    long long total = 0, first_cost = 0, first_prefix = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kApThreads) {
+        const long long v = row_cost(b0 + tid);
+        long long sum;
+        const long long pre = chunk_scan(v, sum);
+        if (b0 == 0) first_cost = v, first_prefix = pre;
+        total += sum;
+    }
+    ApLine line;
+    line.total = total;
+    {
+        const long long want = total / kApMinShare;
+        line.ctas = want < 1 ? 1 : (want < gridDim.x ? (int)want : (int)gridDim.x);
+    }
+    const bool idle = total == 0 || cta >= line.ctas;
+    const long long lo = idle ? 0 : ap_share(line, cta), hi = idle ? 0 : ap_share(line, cta + 1);
+    if (!idle) {
+        long long base = 0;
+        for (int b0 = 0; b0 < p.B; b0 += kApThreads) {
+            long long v = first_cost, pre = first_prefix, sum = 0;
+            if (p.B > kApThreads) {
+                v = row_cost(b0 + tid);
+                pre = chunk_scan(v, sum);
+            }
+            const long long x = base + pre;
+            if (v > 0 && x <= lo && lo < x + v) {
+                ApCursor c;
+                c.b = b0 + tid;
+                c.row = ap_row(p, c.b);
+                c.h = (int)((lo - x) / c.row.head_cost);
+                const long long rem = (lo - x) - c.h * c.row.head_cost;
+                int a = 0, z = c.row.units;  // last unit that starts at or before rem
+                while (z - a > 1) {
+                    const int mid = (a + z) >> 1;
+                    if (ap_unit_start(p, c.row, mid) <= rem) a = mid;
+                    else z = mid;
+                }
+                c.j = a;
+                c.x0 = x + c.h * c.row.head_cost + ap_unit_start(p, c.row, a);
+                t.start = c;
+            }
+            base += sum;
+        }
+    }
+    if (warp == 9) {
+        tmem_alloc(smem_u32(&t.tmem), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = t.tmem;
+    const uint32_t sm_q = smem_u32(smem), sm_ring = sm_q + L::kRing;
+    // A thread holds a row of scores: 384 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72.
+    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+
+    if (!idle) {
+        ApCursor cur = t.start;
+        ApSegment seg;
+        bool more = true;
+        if (warp == 8) {
+            // ------------------------------------------------------------ TMA producer
+            int it = 0, n_q = 0, n_fix = 0;  // ring tiles, query loads, repaired tiles so far
+            for (; more && cur.x0 < hi && !*abort_flag; more = ap_advance(p, cur)) {
+                if (!ap_segment(p, cur, lo, hi, seg) || seg.tiles == 0) continue;
+                const int cnt = seg.ke - seg.ks;
+                const int* table = p.table + (long long)cur.b * p.max_pages;
+                const bool clear_tail = ((seg.extent + 63) & ~63) > cur.row.len && (seg.extent & 63);
+                if (!mbar_wait_bounded(smem_u32(&t.q_empty), (uint32_t)((n_q & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&t.q_full), bytes = (uint32_t)(p.tpt * p.G * 128 * BLOCKS);
+                    const int tiles_q = seg.dual ? 1 : 2;
+                    mbar_arrive_expect_tx(bar, bytes * tiles_q);
+                    for (int m = 0; m < tiles_q; ++m)
+                        for (int k = 0; k < BLOCKS; ++k)
+                            tma_load_3d(sm_q + m * L::kTile + k * 16384, &mapQ, k * 64, cur.h * p.G, cur.row.q0 + seg.first + m * p.tpt, bar);
+                }
+                __syncwarp();
+                ++n_q;
+                int ids = 0, ids_from = -16;  // lane i: pool page of key block (ids_from * 2 + i), 64 keys each
+                // the tile of K (v = 0) or V (v = 1) number k of the unit
+                auto load = [&](int k, int v) {
+                    if (k < ids_from || k >= ids_from + 16) {
+                        ids_from = k;
+                        const long long key = ((long long)k * 2 + lane) * 64;
+                        ids = p.num_pages;  // out of range: zeros
+                        if (key < seg.extent) {
+                            const int id = __ldg(table + (key >> p.page_shift));
+                            if (id >= 0 && id < p.num_pages) ids = id;
+                            else report_fault(p.status, FAULT_PAGE_RANGE);
+                        }
+                    }
+                    const int stage = it % kApStages;
+                    if (!mbar_wait_bounded(smem_u32(&t.empty[stage]), (uint32_t)(((it / kApStages) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT))
+                        return;
+                    const int id0 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2), id1 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2 + 1);
+                    const bool repair = v && clear_tail && k == seg.tiles - 1;
+                    const uint32_t dst = sm_ring + stage * L::kTile, bar = smem_u32(repair ? &t.fix : &t.full[stage]);
+                    if (elect_one()) {
+                        const CUtensorMap* map = v ? &mapV : &mapK;
+                        const int mask = (1 << p.page_shift) - 1, y0 = (k * kApKeys) & mask, y1 = (k * kApKeys + 64) & mask;
+                        mbar_arrive_expect_tx(bar, L::kTile);
+#pragma unroll
+                        for (int c = 0; c < BLOCKS; ++c) {
+                            tma_load_3d(dst + c * 16384, map, c * 64, y0, id0 * p.NKV + cur.h, bar);
+                            tma_load_3d(dst + c * 16384 + 8192, map, c * 64, y1, id1 * p.NKV + cur.h, bar);
+                        }
+                    }
+                    __syncwarp();
+                    ++it;
+                    if (repair) {
+                        // rows behind the last key of the block that straddles it: P is zero there, and V has to be
+                        mbar_wait_bounded(bar, (uint32_t)(n_fix & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
+                        ++n_fix;
+                        const int r0 = seg.extent - k * kApKeys, r1 = (r0 + 63) & ~63;  // extent is no multiple of 64 here
+                        for (int i = lane; i < (r1 - r0) * 8 * BLOCKS; i += 32) {
+                            const int c = i / ((r1 - r0) * 8), o = i - c * (r1 - r0) * 8;
+                            *reinterpret_cast<uint4*>(smem + L::kRing + stage * L::kTile + c * 16384 + r0 * 128 + o * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&t.full[stage]));
+                    }
+                };
+                const int ahead = seg.dual ? 2 : 1;  // K tiles in front of the V tile they belong to
+                for (int i = 0; i < ahead && i < cnt; ++i) load(seg.ks + i, 0);
+                for (int i = 0; i < cnt && !*abort_flag; ++i) {
+                    load(seg.ks + i, 1);
+                    if (i + ahead < cnt) load(seg.ks + i + ahead, 0);
+                }
+            }
+            if (*abort_flag) {  // nothing may still be landing in this CTA's shared memory when it exits
+                const long long t0 = clock64();
+                while (clock64() - t0 < kWaitLimitCycles / 100) {}
+            }
+        } else if (warp == 9) {
+            // ------------------------------------------------------------ MMA issuer
+            if (elect_one()) {
+                int it = 0, n_q = 0, n_tile[2] = {0, 0}, n_unit[2] = {0, 0};
+                auto wait = [&](uint64_t* bar, int parity) {
+                    const bool ok = mbar_wait_bounded(smem_u32(bar), (uint32_t)parity, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    tc_fence_after();
+                    return ok;
+                };
+                auto wait_stage = [&](int i) { return wait(&t.full[i % kApStages], (i / kApStages) & 1); };
+                auto scores = [&](int m, int q_tile, int i) {  // S[m] = Q K^T
+                    const uint64_t a = umma_desc_sw128(sm_q + q_tile * L::kTile), b = umma_desc_sw128(sm_ring + (i % kApStages) * L::kTile);
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const int off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+                        tc_mma_bf16(tmem + m * 128, a + off, b + off, IDESC_QK, k > 0);
+                    }
+                    tc_commit(smem_u32(&t.s_full[m]));
+                };
+                auto values = [&](int m, int i, bool fresh) {  // O[m] (+)= P V
+                    const uint64_t b = umma_desc_sw128_mn<D>(sm_ring + (i % kApStages) * L::kTile);
+#pragma unroll
+                    for (int k = 0; k < kApKeys / 16; ++k)
+                        tc_mma_bf16_ts(tmem + 256 + m * D, tmem + m * 128 + k * 8, b + k * (2048 >> 4), IDESC_PV, !(fresh && k == 0));
+                };
+                for (; more && cur.x0 < hi && !*abort_flag; more = ap_advance(p, cur)) {
+                    if (!ap_segment(p, cur, lo, hi, seg) || seg.tiles == 0) continue;
+                    const int cnt = seg.ke - seg.ks;
+                    if (!wait(&t.q_full, n_q & 1)) break;
+                    ++n_q;
+                    if (!seg.dual) {
+                        // K(0) V(0) K(1) V(1) ... in the ring, each for both tiles
+                        if (!wait_stage(it)) break;
+                        scores(0, 0, it), scores(1, 1, it);
+                        tc_commit(smem_u32(&t.empty[it % kApStages]));
+                        ++it;
+                        if (cnt == 1) tc_commit(smem_u32(&t.q_empty));
+                        for (int i = 0; i < cnt && !*abort_flag; ++i) {
+                            const int v = it, k = it + 1;
+                            const bool next = i + 1 < cnt;
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                if (!wait(&t.p_full[m], n_tile[m] & 1)) break;
+                                ++n_tile[m];
+                                if (i == 0) {
+                                    if (!wait(&t.o_empty[m], (n_unit[m] & 1) ^ 1)) break;
+                                    ++n_unit[m];
+                                }
+                                if (m == 0 && !wait_stage(v)) break;
+                                values(m, v, i == 0);
+                                if (m == 1) tc_commit(smem_u32(&t.empty[v % kApStages]));
+                                if (next) {
+                                    if (m == 0 && !wait_stage(k)) break;
+                                    scores(m, m, k);
+                                    if (m == 1) {
+                                        tc_commit(smem_u32(&t.empty[k % kApStages]));
+                                        if (i + 2 == cnt) tc_commit(smem_u32(&t.q_empty));
+                                    }
+                                } else {
+                                    tc_commit(smem_u32(&t.o_full[m]));
+                                }
+                            }
+                            it += next ? 2 : 1;
+                        }
+                    } else {
+                        // K(0) K(1) V(0) K(2) V(1) K(3) ...: tile i of the keys belongs to warpgroup i & 1
+                        for (int i = 0; i < 2 && i < cnt; ++i) {
+                            if (!wait_stage(it)) break;
+                            scores(i, 0, it);
+                            tc_commit(smem_u32(&t.empty[it % kApStages]));
+                            ++it;
+                        }
+                        if (cnt <= 2) tc_commit(smem_u32(&t.q_empty));
+                        for (int i = 0; i < cnt && !*abort_flag; ++i) {
+                            const int m = i & 1;
+                            int& tiles = n_tile[m];
+                            if (!wait(&t.p_full[m], tiles & 1)) break;
+                            ++tiles;
+                            if (i < 2) {
+                                if (!wait(&t.o_empty[m], (n_unit[m] & 1) ^ 1)) break;
+                                ++n_unit[m];
+                            }
+                            if (!wait_stage(it)) break;
+                            values(m, it, i < 2);
+                            tc_commit(smem_u32(&t.empty[it % kApStages]));
+                            ++it;
+                            if (i + 2 < cnt) {
+                                if (!wait_stage(it)) break;
+                                scores(m, 0, it);
+                                tc_commit(smem_u32(&t.empty[it % kApStages]));
+                                ++it;
+                                if (i + 3 == cnt) tc_commit(smem_u32(&t.q_empty));
+                            } else {
+                                tc_commit(smem_u32(&t.o_full[m]));
+                            }
+                        }
+                    }
+                }
+            }
+        } else if (warp < 8) {
+            // ------------------------------------------------------------ softmax, one row per thread
+            const int m = warp >> 2;                                    // tile
+            const int r = (warp & 3) * 32 + lane;                       // row of the tile
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t t_s = tmem + lanes + m * 128, t_o = tmem + lanes + 256 + m * D;
+            const int r_tok = r / p.G, r_head = r - r_tok * p.G;
+            int n_tile = 0, n_unit = 0;
+            for (; more && cur.x0 < hi; more = ap_advance(p, cur)) {
+                if (!ap_segment(p, cur, lo, hi, seg)) continue;
+                const int cnt = seg.ke - seg.ks;
+                const int tok0 = seg.first + (seg.dual ? 0 : m * p.tpt);  // first token of this tile within the row
+                const int tok = tok0 + r_tok;
+                const bool live = r_tok < p.tpt && tok < seg.first + seg.tokens;
+                // keys that this query sees; for the tile: what all of its queries see
+                const int limit = live ? max(0, cur.row.len - (cur.row.n - 1 - tok)) : 0;
+                const int all_see = cur.row.len - (cur.row.n - 1 - tok0);
+                const int my0 = seg.dual ? m : 0, step = seg.dual ? 2 : 1;
+                const int mine = seg.dual ? (cnt + 1 - m) / 2 : cnt;
+                float mx = -INFINITY, sum = 0.f;
+                for (int i = my0; i < cnt; i += step) {
+                    const int key0 = (seg.ks + i) * kApKeys;
+                    mbar_wait_bounded(smem_u32(&t.s_full[m]), (uint32_t)(n_tile & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    ++n_tile;
+                    tc_fence_after();
+                    float s[kApKeys];
+#pragma unroll
+                    for (int c = 0; c < kApKeys; c += 32) tmem_ld32(t_s + c, s + c);
+                    tmem_ld_wait();
+                    if (key0 + kApKeys > all_see) {
+#pragma unroll
+                        for (int c = 0; c < kApKeys; ++c)
+                            if (key0 + c >= limit) s[c] = -INFINITY;
+                    }
+                    float top = s[0];
+#pragma unroll
+                    for (int c = 1; c < kApKeys; ++c) top = fmaxf(top, s[c]);
+                    if (i == my0) {
+                        mx = top;
+                    } else {
+                        // all keys so far masked: nothing has been summed, and the factor is exp2(-inf) = 0
+                        const float higher = fmaxf(mx, top);
+                        const bool grow = (higher - mx) * p.scale_log2 > 8.f;
+                        if (__any_sync(0xffffffffu, grow)) {
+                            const float f = grow ? exp2_approx((mx - higher) * p.scale_log2) : 1.f;
+                            if (grow) mx = higher;
+                            sum *= f;
+#pragma unroll
+                            for (int c = 0; c < D; c += 32) {
+                                float o[32];
+                                tmem_ld32(t_o + c, o);
+                                tmem_ld_wait();
+                                uint32_t w[32];
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+                                tmem_st16(t_o + c, w);
+                                tmem_st16(t_o + c + 16, w + 16);
+                            }
+                            tmem_st_wait();
+                        }
+                    }
+                    const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+                    float add[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < kApKeys; c += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float a = exp2_approx(fmaf(s[c + 2 * e], p.scale_log2, -shift));
+                            const float b = exp2_approx(fmaf(s[c + 2 * e + 1], p.scale_log2, -shift));
+                            add[(2 * e) & 3] += a, add[(2 * e + 1) & 3] += b;
+                            w[e] = pack_bf16(a, b);
+                        }
+                        tmem_st16(t_s + c / 2, w);
+                    }
+                    sum += (add[0] + add[1]) + (add[2] + add[3]);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&t.p_full[m]));
+                }
+                // ---- end of the segment
+                const bool direct = seg.tiles == 0 || (seg.whole && (!seg.dual || cnt == 1));
+                if (mine > 0) {
+                    mbar_wait_bounded(smem_u32(&t.o_full[m]), (uint32_t)(n_unit & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    ++n_unit;
+                    tc_fence_after();
+                }
+                if (direct) {
+                    if (seg.dual && m == 1) continue;  // tile 0 holds all rows
+                    const float inv = 1.0f / sum;
+                    bf16* out = p.Out + (long long)(cur.row.q0 + tok) * p.ldo + (long long)(cur.h * p.G + r_head) * D;
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        if (mine > 0) {
+                            tmem_ld32(t_o + c, o);
+                            tmem_ld_wait();
+                        }
+                        if (live && !*abort_flag) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int q = 0; q < 4; ++q)  // a query that sees no key gives zero
+                                    w[q] = limit == 0 ? 0u : pack_bf16(o[e + 2 * q] * inv, o[e + 2 * q + 1] * inv);
+                                *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                    }
+                    if (mine > 0) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&t.o_empty[m]));
+                    }
+                    continue;
+                }
+                // A part: slot 2 * cta holds the unit that the CTA in front began, 2 * cta + 1 one that starts here
+                const int slot = 2 * cta + (cur.x0 >= lo ? 1 : 0);
+                constexpr long long kPart = (long long)(D + 2) * 128;
+                if (mine > 0) {
+                    float* part = p.parts + (slot * 2 + m) * kPart;
+                    if (live) __stcg(part + (long long)D * 128 + r, mx), __stcg(part + (long long)(D + 1) * 128 + r, sum);
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        tmem_ld32(t_o + c, o);
+                        tmem_ld_wait();
+                        if (live) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                __stcg(reinterpret_cast<float4*>(part) + (c + e) / 4 * 128 + r, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&t.o_empty[m]));
+                }
+                __threadfence();
+                named_bar_sync(1, 256);
+                // the share in which the unit starts, and the last one with keys of it
+                int c0 = (int)(cur.x0 * line.ctas / line.total), c1;
+                while (c0 > 0 && ap_share(line, c0) > cur.x0) --c0;
+                while (ap_share(line, c0 + 1) <= cur.x0) ++c0;
+                if (tid == 0) {
+                    // One counter per share: of the units that start in it only the last can be cut.  (The others have to leave
+                    // it alone: the next CTA may already have added its part of that last one.)
+                    t.last = 1;
+                    if (!seg.whole) {
+                        t.last = atomicAdd(p.count + c0, (unsigned)cnt) + (unsigned)cnt == (unsigned)seg.tiles;
+                        if (t.last) p.count[c0] = 0u;
+                    }
+                }
+                c1 = c0;
+                while (c1 + 1 < line.ctas && ap_tile_at(ap_share(line, c1 + 1), cur.x0, seg.tiles) < seg.tiles) ++c1;
+                for (int c = c0 + tid; c <= c1; c += 256) {
+                    const int a = ap_tile_at(ap_share(line, c), cur.x0, seg.tiles), z = ap_tile_at(ap_share(line, c + 1), cur.x0, seg.tiles);
+                    const int sl = 2 * (2 * c + (c == c0 ? 1 : 0));
+                    t.list[2 * (c - c0)] = a < z ? sl : -1;
+                    t.list[2 * (c - c0) + 1] = seg.dual && z - a > 1 ? sl + 1 : -1;
+                }
+                named_bar_sync(1, 256);
+                if (t.last && !*abort_flag) {
+                    __threadfence();
+                    const int n_list = 2 * (c1 - c0 + 1), rows = seg.tokens * p.G;
+                    // dual: all rows in every part; else tile q of row / (tpt * G), which is the second of a pair of parts
+                    const int per_tile = p.tpt * p.G;
+                    for (int i = tid; i < rows * (D / 4); i += 256) {
+                        const int row = i % rows, c = i / rows;
+                        const int q = row / per_tile, rr = row - q * per_tile;
+                        float top = -INFINITY;
+                        for (int k = 0; k < n_list; ++k) {
+                            const int id = t.list[k];
+                            if (id >= 0) top = fmaxf(top, __ldcg(p.parts + (id + q) * kPart + (long long)D * 128 + rr));
+                        }
+                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                        float all = 0.f;
+                        for (int k = 0; k < n_list; ++k) {
+                            const int id = t.list[k];
+                            if (id < 0) continue;
+                            const float* part = p.parts + (id + q) * kPart;
+                            const float pm = __ldcg(part + (long long)D * 128 + rr);
+                            const float w = pm == -INFINITY ? 0.f : exp2_approx((pm - top) * p.scale_log2);
+                            const float4 o = __ldcg(reinterpret_cast<const float4*>(part) + c * 128 + rr);
+                            all += w * __ldcg(part + (long long)(D + 1) * 128 + rr);
+                            acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
+                        }
+                        const int token = seg.first + row / p.G, head = row % p.G;
+                        const float inv = 1.0f / all;
+                        uint2 w = make_uint2(0u, 0u);  // a query that sees no key
+                        if (cur.row.len - (cur.row.n - 1 - token) > 0)
+                            w = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+                        *reinterpret_cast<uint2*>(p.Out + (long long)(cur.row.q0 + token) * p.ldo + (long long)(cur.h * p.G + head) * D + c * 4) = w;
+                    }
+                }
+                named_bar_sync(1, 256);  // the list and the flag are free again
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------
+static constexpr int kApMaxGrid = 160;
+
+static int attn_prompt_grid() { return sm_count() < kApMaxGrid ? sm_count() : kApMaxGrid; }
+
+size_t attn_prompt_workspace_bytes(int D) {
+    return (size_t)kApMaxGrid * 4 + (size_t)attn_prompt_grid() * 4 * (D + 2) * 128 * sizeof(float);
+}
+
+// bf16 [d2][d1][d0] with element strides; box [b2][b1][64], 128-byte swizzle, zeros out of range
+static bool encode_3d(CUtensorMap* map, const bf16* base, long long d0, long long d1, long long d2, long long s1, long long s2, int b1, int b2) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+    cuuint64_t strides[2] = {(cuuint64_t)s1 * 2, (cuuint64_t)s2 * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2}, one[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<bf16*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+static cudaError_t launch_attn_prompt_d(const AttnPromptArgs& a, const ApParams& p, cudaStream_t stream) {
+    alignas(64) CUtensorMap mq, mk, mv;
+    const long long P = 1ll << a.page_shift, z = (long long)a.num_pages * a.NKV;
+    if (!encode_3d(&mq, a.Q, D, a.H, a.T, D, a.ldq, p.G, p.tpt) || !encode_3d(&mk, a.K, D, P, z, D, P * D, 64, 1) ||
+        !encode_3d(&mv, a.V, D, P, z, D, P * D, 64, 1))
+        return cudaErrorInvalidValue;
+    cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ApSmem<D>::kBytes);
+    if (e != cudaSuccess) return e;
+    chain_begin();
+    return launch_pdl(attn_prompt_kernel<D>, dim3((unsigned)attn_prompt_grid()), dim3(kApThreads), ApSmem<D>::kBytes, stream, mq, mk, mv, p);
+}
+
+cudaError_t launch_attn_prompt(const AttnPromptArgs& a, cudaStream_t stream) {
+    ApParams p;
+    p.Out = a.Out, p.ldo = a.ldo;
+    p.table = a.page_table, p.lens = a.seq_lens, p.cu = a.cu_tokens;
+    p.count = static_cast<unsigned int*>(a.workspace);
+    p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + kApMaxGrid * 4);
+    p.B = a.B, p.T = a.T, p.H = a.H, p.NKV = a.NKV, p.G = a.H / a.NKV, p.tpt = 128 / p.G;
+    p.max_pages = a.max_pages, p.page_shift = a.page_shift, p.num_pages = a.num_pages;
+    p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)a.D));
+    p.status = status_ptr();
+    if (!p.status) return cudaErrorUnknown;
+    return a.D == 64 ? launch_attn_prompt_d<64>(a, p, stream) : launch_attn_prompt_d<128>(a, p, stream);
+}
+
+}  // namespace ezb

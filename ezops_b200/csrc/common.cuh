@@ -28,7 +28,10 @@ enum DeviceFault : unsigned int {
     FAULT_GEMV_DRAIN = 0x103,       // copies still in flight at exit
     FAULT_TC_ACC_WAIT = 0x104,      // tensor-memory accumulator hand-over never happened
     FAULT_AR_FLAG_WAIT = 0x201,     // a peer's partial result never arrived in the inbox
+    FAULT_ROPE_POSITION = 0x301,    // a position lies behind the last row of the rotary tables
     FAULT_PAGE_RANGE = 0x302,       // a page-table entry points outside the page pools
+    FAULT_SLOT_RANGE = 0x303,       // a cache slot lies outside the page pools
+    FAULT_PROMPT_WAIT = 0x105,      // prompt attention: a tile, score or output hand-over never happened
     FAULT_MEGA_GRID_BARRIER = 0x400,  // + barrier index: a grid-wide barrier of the single-kernel layer never filled
 };
 

@@ -28,6 +28,8 @@
 
 #include "launchers.h"
 #include "map_table.h"
+#include "prompt.h"
+#include "tc.cuh"
 
 namespace ezb {
 
@@ -68,138 +70,10 @@ struct TcParams {
     Trace trace;
     int trace_id;
     TpLink link;  // fused tensor-parallel exchange (world 0: none); only the push side lives in this kernel
+    // EXT instance: out = act(product + bias) + residual, one rounding
+    const bf16* bias;  // [N], SwiGLU [2N] gate first, or null
+    int act, out_f32;
 };
-
-// ---- tcgen05 / TMA wrappers -------------------------------------------------
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_mma_bf16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// 32 lanes x 16 consecutive 32-bit columns: thread i of the warp gets lane (base lane + i)
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// Shared-memory matrix descriptor for a K-major bf16 tile whose rows are 128
-// bytes (64 elements) with the 128-byte swizzle that the tiled TMA wrote:
-// start address / 16, stride between 8-row groups 1024 bytes, descriptor
-// version 1 (sm_100), layout type 2 (128-byte swizzle).
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-    d |= (uint64_t)(1024u >> 4) << 32;
-    d |= 1ull << 46;
-    d |= 2ull << 61;
-    return d;
-}
-
-// Instruction descriptor, kind::f16: fp32 accumulator, bf16 A and B, both
-// K-major, N in units of 8 at bit 17, M in units of 16 at bit 24.
-__host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-// ---- cluster wrappers -------------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-// Relaxed: what the peers must see first is ordered otherwise (fence.mbarrier_init at the start; at the end every copy
-// and arrival towards a peer has been waited for by that peer).  The release form waited for every store in flight.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-// Address of `local` (a shared::cta address) in the shared memory of cluster CTA `rank`.
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t local, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// Bulk copy from this CTA's shared memory into another CTA's of the cluster; the bytes are counted on that CTA's barrier.
-__device__ __forceinline__ void bulk_s2cluster(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(src),
-                 "r"(bytes), "r"(bar)
-                 : "memory");
-}
-__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-// As mbar_wait_bounded, for arrivals from other CTAs of the cluster.
-__device__ __forceinline__ bool mbar_wait_bounded_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                                          unsigned int* status, unsigned int fault_code) {
-    const long long t0 = clock64();
-    while (!mbar_try_wait_cluster(bar, parity)) {
-        if (*abort_flag) return false;
-        if (clock64() - t0 > kWaitLimitCycles) {
-            *abort_flag = 1;
-            report_fault(status, fault_code);
-            return false;
-        }
-    }
-    return true;
-}
-
-// One thread of a converged warp.  Unlike `lane == 0`, the compiler knows that exactly one thread enters the branch and
-// keeps descriptors and addresses in uniform registers: four MMAs and their commit issue in 171 cycles instead of 264.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
-    return one != 0;
-}
-
-// 32 lanes x 8 columns, see tmem_ld16
-__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
-    uint32_t r[8];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-}
 
 // What bounds it: the weight stream.  A tile's parts meet in shared memory because the round trips of a reduction
 // through L2 (park, ticket, read 4..19 parts in one CTA) cost 5..13 us at the end of every projection.
@@ -209,7 +83,8 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
 // 2B layers above 488 -> 438 us, 28 layers of 0.6B at batch 4 1008 -> 858 us).
 // LINK: the instance for chains with the fused exchange: its epilogue can push fp32 results into the peers' inboxes (see
 // TpLink), and its waits start behind the gather of the kernel in front.
-template <int NB, bool LINK>
+// EXT: the instance for linear layers (LinearOp): bias, activation and residual in fp32, result in bf16 or fp32.
+template <int NB, bool LINK, bool EXT>
 __global__ void __launch_bounds__(kTcThreads, 2)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant__ CUtensorMap mapW1,
                const __grid_constant__ CUtensorMap mapX, const TcParams p) {
@@ -415,7 +290,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                     src += groups * p.ldres;
                 }
             };
-            if (p.epilogue == EPI_RESIDUAL && live_row) fetch_residual(cg);
+            if ((EXT ? p.residual != nullptr : p.epilogue == EPI_RESIDUAL) && live_row) fetch_residual(cg);
             const float next_w = (p.xw_out && live_row) ? __bfloat162float(p.next_norm_w[n]) : 0.f;
             mbar_wait_bounded(smem_u32(&acc_full[acc]), (uint32_t)((i >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             if (i == 0) trace_mark(trec, 4);
@@ -478,7 +353,30 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                         if (col + u * groups < n_cols) v[u] *= norm_r[col + u * groups];
                 }
             };
-            if (p.ssq_out) {
+            if constexpr (EXT) {
+                if (!*abort_flag && live_row) {
+                    const float b0 = p.bias ? __bfloat162float(p.bias[n]) : 0.f;
+                    const float b1 = p.bias && p.pair ? __bfloat162float(p.bias[p.N + n]) : 0.f;
+                    for (int col = cg; col < n_cols; col += CU * groups) {
+                        float v[CU], up[CU];
+                        gather(col, frow, v);
+                        if (p.pair) gather(col, frow + p.half_rows, up);
+                        if (p.residual && col != cg) fetch_residual(col);
+#pragma unroll
+                        for (int u = 0; u < CU; ++u) {
+                            const int c = col + u * groups;
+                            if (c < n_cols) {
+                                float x = v[u] + b0;
+                                x = p.pair ? silu_f32(x) * (up[u] + b1) : linear_act(x, p.act);
+                                if (p.residual) x += res[u];
+                                const long long o = (long long)(b_first + c) * p.ldout + n;
+                                if (p.out_f32) static_cast<float*>(p.out)[o] = x;
+                                else static_cast<bf16*>(p.out)[o] = __float2bfloat16_rn(x);
+                            }
+                        }
+                    }
+                }
+            } else if (p.ssq_out) {
                 // Residual epilogue in front of a norm: the result, the result with the norm weight, and the sum of
                 // squares of the warp's 32 rows of each column.
                 const int q32 = (et & 127) >> 5, q32s = (p.units + 31) >> 5;
@@ -569,22 +467,6 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(ptr);
-    }
-    return fn;
-}
-
 // 2-D bf16 row-major [rows, cols] with leading dimension ld; box = [64 cols, box_rows], 128-byte swizzle,
 // out-of-range elements read as zero.
 static bool encode_map(CUtensorMap* map, const bf16* base, long long rows, long long cols, long long ld, int box_rows) {
@@ -640,7 +522,7 @@ static constexpr size_t kTcHalfSm = 113 * 1024;  // two CTAs of this size share 
 
 // Clusters of 1 << log2c CTAs, one CTA per SM, that can be resident together (asked once per device): the clusters of
 // eight leave SMs of a GPC over, 15 of them fit at a whole SM per CTA and 16 at half an SM; 33 of four, 74 of two.
-template <int NB, bool LINK>
+template <int NB, bool LINK, bool EXT>
 static int tc_resident_clusters(int dev, int log2c, bool half) {
     static std::atomic<int> cache[64][4][2];
     const bool keep = dev >= 0 && dev < 64;
@@ -657,7 +539,7 @@ static int tc_resident_clusters(int dev, int log2c, bool half) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int n = 0;
-        return cudaOccupancyMaxActiveClusters(&n, gemm_tc_kernel<NB, LINK>, &cfg) == cudaSuccess ? n : 0;
+        return cudaOccupancyMaxActiveClusters(&n, gemm_tc_kernel<NB, LINK, EXT>, &cfg) == cudaSuccess ? n : 0;
     };
     int n = ask((size_t)max_smem_optin());
     if (half) {
@@ -678,14 +560,14 @@ static int tc_resident_clusters(int dev, int log2c, bool half) {
 // 32, layer us with clusters of 1 | 2 | 4 | 8: gate/up 174.5 | 168.9 | 171.1 | 185.1, down 191.4 | 175.0 | 171.0 | 172.3;
 // 0.6B o_proj 64.9 | 60.5 | 58.6 | 58.4).  A k-block costs 40 ns plus its bytes at a 148th of the HBM rate (never less
 // than 150 ns: waiting for a stage and issuing its MMAs, which read 128 rows of A whatever the tile holds).
-template <int NB, bool LINK>
+template <int NB, bool LINK, bool EXT>
 static bool tc_plan(TcParams& p, int dev, int& clusters, size_t& smem) {
     double best = 0.;
     for (int log2c = 0; (1 << log2c) <= kTcMaxCluster && (1 << log2c) <= p.kblocks; ++log2c) {
         const int C = 1 << log2c, max_units = p.pair ? kTcRows / 2 : kTcRows;
         const int cpc = (p.B + C - 1) / C, nk = (p.kblocks + C - 1) / C;
         for (int half = 0; half < 2; ++half) {
-            const int nc = tc_resident_clusters<NB, LINK>(dev, log2c, half != 0);
+            const int nc = tc_resident_clusters<NB, LINK, EXT>(dev, log2c, half != 0);
             if (nc < 1) continue;
             long long rounds = (p.N + (long long)nc * max_units - 1) / ((long long)nc * max_units);
             int units = (int)((p.N + nc * rounds - 1) / (nc * rounds));
@@ -723,9 +605,9 @@ static bool tc_plan(TcParams& p, int dev, int& clusters, size_t& smem) {
     return best > 0.;
 }
 
-template <int NB, bool LINK>
+template <int NB, bool LINK, bool EXT = false>
 static cudaError_t launch_tc_instance(const GemvArgs& a, const bf16* x, long long ldx, TcParams& p, cudaStream_t stream) {
-    auto kernel = gemm_tc_kernel<NB, LINK>;
+    auto kernel = gemm_tc_kernel<NB, LINK, EXT>;
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
@@ -736,12 +618,18 @@ static cudaError_t launch_tc_instance(const GemvArgs& a, const bf16* x, long lon
     }
     int clusters = 0;
     size_t smem = 0;
-    if (!tc_plan<NB, LINK>(p, dev, clusters, smem)) return cudaErrorInvalidConfiguration;
+    if (!tc_plan<NB, LINK, EXT>(p, dev, clusters, smem)) return cudaErrorInvalidConfiguration;
     if (a.tiling && a.prologue != PRO_SCALED) a.tiling->units = p.units, a.tiling->tiles = p.tiles;
     p.first = chain_waits_first();
     p.cols_pad = 1;
     while (p.cols_pad < p.cpc) p.cols_pad *= 2;
     alignas(64) CUtensorMap m0, m1, mx;
+    if (EXT) {  // called with ever new activation buffers: descriptors are encoded (1 us) instead of filling up the table
+        if (!encode_map(&m0, a.W0, a.N, a.K, a.ldw, p.units) || !encode_map(&m1, p.pair ? a.W1 : a.W0, a.N, a.K, a.ldw, p.units) ||
+            !encode_map(&mx, x, a.B, a.K, ldx, NB))
+            return cudaErrorInvalidValue;
+        return launch_pdl_cluster(kernel, dim3((unsigned)clusters << p.log2c), dim3(kTcThreads), 1 << p.log2c, smem, stream, m0, m1, mx, p);
+    }
     if (!make_map(&m0, a.W0, a.N, a.K, a.ldw, p.units)) return cudaErrorInvalidValue;
     if (!make_map(&m1, p.pair ? a.W1 : a.W0, a.N, a.K, a.ldw, p.units)) return cudaErrorInvalidValue;
     if (!make_map(&mx, x, a.B, a.K, ldx, NB)) return cudaErrorInvalidValue;
@@ -767,6 +655,7 @@ cudaError_t launch_gemm_tc(const GemvArgs& a, const bf16* x, long long ldx, cuda
     if (a.prologue == PRO_SCALED) p.ssq_in = a.ssq, p.ssq_parts = a.tiling->parts();
     else if (a.ssq && a.epilogue == EPI_RESIDUAL) p.ssq_out = a.ssq, p.xw_out = a.next_norm_w ? a.xw_out : nullptr;
     p.link = a.link;
+    p.bias = nullptr, p.act = 0, p.out_f32 = 0;
     if (a.link.world > 0 && (a.link.gather_inbox >= 0 || pair)) return cudaErrorNotSupported;  // only the push side lives here
     const int NB = tc_batch_tile(a.B);
     if (a.link.world > 0 || a.behind_gather) {
@@ -780,6 +669,29 @@ cudaError_t launch_gemm_tc(const GemvArgs& a, const bf16* x, long long ldx, cuda
         case 16: return launch_tc_instance<16, false>(a, x, ldx, p, stream);
         case 32: return launch_tc_instance<32, false>(a, x, ldx, p, stream);
         default: return launch_tc_instance<64, false>(a, x, ldx, p, stream);
+    }
+}
+
+cudaError_t launch_linear_few(const LinearArgs& l, cudaStream_t stream) {
+    GemvArgs a;
+    const bool pair = l.act == ACT_SWIGLU;
+    a.W0 = l.W, a.W1 = pair ? l.W + (long long)l.N * l.K : nullptr, a.ldw = l.K, a.N = l.N, a.K = l.K, a.B = l.M;
+    TcParams p = {};
+    p.N = l.N, p.K = l.K, p.B = l.M;
+    p.kblocks = (l.K + kTcBlockK - 1) / kTcBlockK;
+    p.pair = pair ? 1 : 0;
+    p.residual = l.residual, p.ldres = l.ldres;
+    p.out = l.out, p.ldout = l.ldout;
+    p.bias = l.bias, p.act = l.act, p.out_f32 = l.out_f32;
+    p.status = status_ptr();
+    if (!p.status) return cudaErrorUnknown;
+    p.trace = trace_handle();
+    p.link.push_inbox = p.link.gather_inbox = p.link.bump_inbox = -1;
+    chain_begin();
+    switch (tc_batch_tile(l.M)) {
+        case 16: return launch_tc_instance<16, false, true>(a, l.x, l.ldx, p, stream);
+        case 32: return launch_tc_instance<32, false, true>(a, l.x, l.ldx, p, stream);
+        default: return launch_tc_instance<64, false, true>(a, l.x, l.ldx, p, stream);
     }
 }
 

@@ -1,0 +1,319 @@
+// Linear layers of prompts on the 5th-generation tensor cores:
+//   out[m, n] = act( sum_k x[m, k] W[n, k] + bias[n] ) + residual[m, n],            fp32 until the one rounding,
+//   SwiGLU: silu(gate + bias_g) * (up + bias_u) with W = [gate rows | up rows].
+//
+// More than kLinearFewRows rows: two CTAs of a cluster share a tile of 256 rows of x by BN rows of W
+// (tcgen05.mma.cta_group::2: each CTA holds half of x's rows and half of W's, and 128 x BN of the result in its tensor
+// memory), so each operand byte that enters an SM is used by two.  One elected thread per CTA fills a ring of 64-element
+// K blocks by TMA (both CTAs' bytes are counted on the first CTA's barrier), one thread of the first CTA issues the MMAs,
+// four warps of each CTA drain one of two accumulators while the next tile is multiplied: bias, activation, residual and
+// rounding happen there, in registers.  Grid: one CTA per SM, tiles in groups of kLinearGroup row tiles so that the x and W
+// tiles in flight stay in L2.  BN = 256 reads least per product; narrower tiles (128, 64) are taken when the wide ones would
+// leave clusters without work (linear_plan).
+// What bounds it: the tensor cores (and from a few hundred rows down the weights' bytes).
+// Few rows: the kernel of the batched decode projections (gemm_tc.cu) with this epilogue.
+#include "prompt.h"
+#include "tc.cuh"
+
+namespace ezb {
+
+static constexpr int kLtThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+static constexpr int kLtBlockK = 64;
+static constexpr int kLtMaxStages = 12;
+static constexpr int kLtGroup = 8;  // row tiles per group of the tile order
+
+struct LtParams {
+    const bf16 *bias, *residual;
+    void* out;
+    long long ldres, ldout;
+    int M, N, kblocks;
+    int tiles_m, tiles_n, stages, act, out_f32;
+    int vec_out, vec_res, vec_bias;  // rows allow 16-byte accesses
+    unsigned int* status;
+};
+
+// ---- cta_group::2 wrappers ------------------------------------------------------
+// The same barrier (or address) in the first CTA of the pair.
+__device__ __forceinline__ uint32_t pair_leader(uint32_t shared_addr) { return shared_addr & 0xFEFFFFFFu; }
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(pair_leader(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void tc_mma_bf16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrives on this barrier in both CTAs once the MMAs issued so far have finished.
+__device__ __forceinline__ void tc_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void cluster_sync_full() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <int BN>
+struct LtSmem {
+    static constexpr int kA = 128 * kLtBlockK * 2;        // this CTA's rows of x
+    static constexpr int kB = BN / 2 * kLtBlockK * 2;     // this CTA's rows of W
+    static constexpr int kStage = kA + kB;
+    static constexpr int kTail = 1024;
+    static constexpr int kStages = (232448 - 1024 - kTail) / kStage < kLtMaxStages ? (232448 - 1024 - kTail) / kStage : kLtMaxStages;
+    static constexpr int kBytes = 1024 + kStages * kStage + kTail;
+};
+
+// Result rows leave in pieces of 16 columns per thread (32 or 64 contiguous bytes).
+template <int W>
+__device__ __forceinline__ void load_bf16(const bf16* src, int left, int vec, float (&v)[W]) {
+    if (vec && left >= W) {
+#pragma unroll
+        for (int e = 0; e < W; e += 8) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(src + e));
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[e + 2 * i] = bf16_lo(w[i]), v[e + 2 * i + 1] = bf16_hi(w[i]);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] = e < left ? __bfloat162float(src[e]) : 0.f;
+    }
+}
+
+template <int BN, bool PAIR>
+__global__ void __launch_bounds__(kLtThreads, 1)
+linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW0,
+                 const __grid_constant__ CUtensorMap mapW1, const __grid_constant__ LtParams p) {
+    using L = LtSmem<BN>;
+    constexpr uint32_t IDESC = umma_idesc_bf16(256, BN);
+    constexpr int UNITS = PAIR ? BN / 2 : BN;  // output columns of a tile
+    extern __shared__ unsigned char lt_raw[];
+    const uint32_t raw = smem_u32(lt_raw);
+    unsigned char* smem = lt_raw + (((raw + 1023u) & ~1023u) - raw);
+    unsigned char* tail = smem + L::kStages * L::kStage;
+    uint64_t* full = reinterpret_cast<uint64_t*>(tail);
+    uint64_t* empty = full + kLtMaxStages;
+    uint64_t* acc_full = empty + kLtMaxStages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int rank = (int)cluster_rank();
+
+    if (tid == 0) {
+        for (int s = 0; s < L::kStages; ++s) mbar_init(smem_u32(&full[s]), 1), mbar_init(smem_u32(&empty[s]), 1);
+        for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&acc_full[a]), 1), mbar_init(smem_u32(&acc_empty[a]), 8);  // warps of both CTAs
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(tmem_slot), 2 * BN);
+        tmem_relinquish_pair();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_full();  // the barriers of both CTAs exist
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_open(1);
+
+    const int n_tiles = p.tiles_m * p.tiles_n, n_clusters = gridDim.x >> 1;
+    auto tile_at = [&](int i, int& m, int& n) {  // groups of kLtGroup row tiles, column tile by column tile
+        const int per = kLtGroup * p.tiles_n, g = i / per, rows = min(kLtGroup, p.tiles_m - g * kLtGroup), r = i - g * per;
+        m = g * kLtGroup + r % rows, n = r / rows;
+    };
+    if (warp == 0) {
+        if (elect_one()) {
+            int it = 0;
+            for (int i = blockIdx.x >> 1; i < n_tiles && !*abort_flag; i += n_clusters) {
+                int tm, tn;
+                tile_at(i, tm, tn);
+                const int y_x = tm * 256 + rank * 128;
+                const CUtensorMap* mapB = PAIR && rank ? &mapW1 : &mapW0;  // SwiGLU: the second CTA brings the up rows
+                const int y_w = PAIR ? tn * UNITS : tn * BN + rank * (BN / 2);
+                for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+                    const int s = it % L::kStages;
+                    if (!mbar_wait_bounded(smem_u32(&empty[s]), (uint32_t)(((it / L::kStages) & 1) ^ 1), abort_flag, p.status, FAULT_GEMV_EMPTY_WAIT)) break;
+                    const uint32_t bar = smem_u32(&full[s]), a = smem_u32(smem) + s * L::kStage;
+                    if (rank == 0) mbar_arrive_expect_tx(bar, 2 * L::kStage);
+                    tma_load_2d_pair(a, &mapX, kb * kLtBlockK, y_x, bar);
+                    tma_load_2d_pair(a + L::kA, mapB, kb * kLtBlockK, y_w, bar);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            int it = 0, n = 0;
+            for (int i = blockIdx.x >> 1; i < n_tiles && !*abort_flag; i += n_clusters, ++n) {
+                const int acc = n & 1;
+                if (!mbar_wait_bounded_cluster(smem_u32(&acc_empty[acc]), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, p.status, FAULT_TC_ACC_WAIT)) break;
+                tc_fence_after();
+                for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+                    const int s = it % L::kStages;
+                    if (!mbar_wait_bounded_cluster(smem_u32(&full[s]), (uint32_t)((it / L::kStages) & 1), abort_flag, p.status, FAULT_GEMV_FULL_WAIT)) break;
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem) + s * L::kStage;
+                    const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + L::kA);
+#pragma unroll
+                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * BN, ad + 2 * k, bd + 2 * k, IDESC, kb > 0 || k > 0);
+                    tc_commit_pair(smem_u32(&empty[s]));
+                }
+                tc_commit_pair(smem_u32(&acc_full[acc]));
+            }
+        }
+    } else {
+        const int q = warp & 3, row = q * 32 + lane;
+        int n = 0;
+        for (int i = blockIdx.x >> 1; i < n_tiles; i += n_clusters, ++n) {
+            int tm, tn;
+            tile_at(i, tm, tn);
+            const int acc = n & 1;
+            const int m = tm * 256 + rank * 128 + row;
+            const bool live_row = m < p.M;
+            const int n0 = tn * UNITS;
+            const int cols = min(UNITS, p.N - n0);
+            mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
+            tc_fence_after();
+            const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * BN;
+            constexpr int W = 16;  // columns at a time
+#pragma unroll 1
+            for (int c = 0; c < cols; c += W) {
+                float v[W], up[W];
+                tmem_ld16(t + c, v);
+                if (PAIR) tmem_ld16(t + UNITS + c, up);
+                const int left = cols - c, col = n0 + c;
+                float res[W];
+                if (p.residual && live_row) load_bf16<W>(p.residual + (long long)m * p.ldres + col, left, p.vec_res, res);
+                tmem_ld_wait();
+                if (live_row && !*abort_flag) {
+                    if (p.bias) {
+                        float b[W];
+                        load_bf16<W>(p.bias + col, left, p.vec_bias, b);
+    #pragma unroll
+                        for (int e = 0; e < W; ++e) v[e] += b[e];
+                        if (PAIR) {
+                            load_bf16<W>(p.bias + p.N + col, left, p.vec_bias, b);
+    #pragma unroll
+                            for (int e = 0; e < W; ++e) up[e] += b[e];
+                        }
+                    }
+                    if (PAIR) {
+    #pragma unroll
+                        for (int e = 0; e < W; ++e) v[e] = silu_f32(v[e]) * up[e];
+                    } else if (p.act != ACT_NONE) {
+    #pragma unroll
+                        for (int e = 0; e < W; ++e) v[e] = linear_act(v[e], p.act);
+                    }
+                    if (p.residual) {
+    #pragma unroll
+                        for (int e = 0; e < W; ++e) v[e] += res[e];
+                    }
+                    const long long o = (long long)m * p.ldout + col;
+                    if (p.out_f32) {
+                        float* dst = static_cast<float*>(p.out) + o;
+                        if (p.vec_out && left >= W) {
+    #pragma unroll
+                            for (int e = 0; e < W; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        } else {
+    #pragma unroll
+                            for (int e = 0; e < W; ++e)
+                                if (e < left) dst[e] = v[e];
+                        }
+                    } else {
+                        bf16* dst = static_cast<bf16*>(p.out) + o;
+                        if (p.vec_out && left >= W) {
+    #pragma unroll
+                            for (int e = 0; e < W; e += 8)
+                                *reinterpret_cast<uint4*>(dst + e) =
+                                    make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]), pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
+                        } else {
+    #pragma unroll
+                            for (int e = 0; e < W; ++e)
+                                if (e < left) dst[e] = __float2bfloat16_rn(v[e]);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            __syncwarp();
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[acc]), 0));
+        }
+    }
+    __syncwarp();
+    if (*abort_flag) __nanosleep(200000);  // copies and products that may still be in flight
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_full();  // nothing is written to or signalled in a CTA that has left
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc_pair(tmem, 2 * BN);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------
+static bool encode_rows(CUtensorMap* map, const bf16* base, long long rows, long long cols, long long ld, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {(cuuint32_t)kLtBlockK, (cuuint32_t)box_rows}, one[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<bf16*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN, bool PAIR>
+static cudaError_t launch_linear_tile(const LinearArgs& a, LtParams& p, cudaStream_t stream) {
+    constexpr int UNITS = PAIR ? BN / 2 : BN;
+    alignas(64) CUtensorMap mx, w0, w1;
+    if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, 128) || !encode_rows(&w0, a.W, a.N, a.K, a.K, BN / 2) ||
+        !encode_rows(&w1, PAIR ? a.W + (long long)a.N * a.K : a.W, a.N, a.K, a.K, BN / 2))
+        return cudaErrorInvalidValue;
+    cudaError_t e = cudaFuncSetAttribute(linear_tc_kernel<BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, LtSmem<BN>::kBytes);
+    if (e != cudaSuccess) return e;
+    p.tiles_m = (a.M + 255) / 256, p.tiles_n = (a.N + UNITS - 1) / UNITS;
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    const int clusters = (int)(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
+    chain_begin();
+    return launch_pdl_cluster(linear_tc_kernel<BN, PAIR>, dim3(2u * clusters), dim3(kLtThreads), 2, LtSmem<BN>::kBytes, stream, mx, w0, w1, p);
+}
+
+cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
+    if (a.M <= kLinearFewRows) return launch_linear_few(a, stream);
+    LtParams p;
+    p.bias = a.bias, p.residual = a.residual, p.out = a.out, p.ldres = a.ldres, p.ldout = a.ldout;
+    p.M = a.M, p.N = a.N, p.kblocks = (a.K + kLtBlockK - 1) / kLtBlockK;
+    p.act = a.act, p.out_f32 = a.out_f32;
+    const int per16 = a.out_f32 ? 4 : 8;
+    p.vec_out = aligned16(a.out) && a.ldout % per16 == 0;
+    p.vec_res = a.residual && aligned16(a.residual) && a.ldres % 8 == 0;
+    p.vec_bias = a.bias && aligned16(a.bias) && (a.act != ACT_SWIGLU || a.N % 8 == 0);
+    p.status = status_ptr();
+    if (!p.status) return cudaErrorUnknown;
+    // The width of a tile: rounds of tiles over the clusters times what a tile of that width costs.
+    const bool pair = a.act == ACT_SWIGLU;
+    const long long rows = pair ? 2ll * a.N : a.N, tm = (a.M + 255) / 256, clusters = sm_count() / 2;
+    auto cost = [&](int bn, double per_block) {
+        const long long tiles = tm * ((rows + bn - 1) / bn);
+        return (double)((tiles + clusters - 1) / clusters) * per_block;
+    };
+    const double c256 = cost(256, 256.), c128 = cost(128, 160.), c64 = cost(64, 110.);
+    if (c256 <= c128 && c256 <= c64) return pair ? launch_linear_tile<256, true>(a, p, stream) : launch_linear_tile<256, false>(a, p, stream);
+    if (c128 <= c64) return pair ? launch_linear_tile<128, true>(a, p, stream) : launch_linear_tile<128, false>(a, p, stream);
+    return pair ? launch_linear_tile<64, true>(a, p, stream) : launch_linear_tile<64, false>(a, p, stream);
+}
+
+}  // namespace ezb

@@ -1,0 +1,291 @@
+// The small kernels of a step over paged KV caches that carries prompts as well as single tokens: the plan of the
+// step (page tables, slots and positions from request lengths) and the head norm + rotary embedding + cache write of
+// its tokens.
+#include "launchers.h"
+#include "prompt.h"
+
+namespace ezb {
+
+// ------------------------------------------------------------------- plan ---
+// With h(x) = ceil(x / page_size), c_b cached and n_b new tokens of row b (offsets cu = running sum of n, cut at
+// max_tokens):
+//   table[b, j] = free[count - 1 - (sum of rows before b of (h(c+n) - h(c))) - (j - h(c_b))],   h(c_b) <= j < h(c_b + n_b)
+//   token t of row b: position c_b + t - cu[b], slot = table[b, position / page_size] * page_size + position % page_size.
+// What bounds it: latency - three dependent reads (lengths, then table or free list) and two block-wide running sums.
+// Every CTA therefore forms the sums over all rows by itself (8 KB of lengths for 1024 rows, from L2) instead of
+// waiting for another CTA, keeps them in shared memory and finds the row of a token there by bisection.  A token in a page
+// that this call maps reads the free list itself, so no CTA reads a table entry that another one writes.
+// Measured (calls in a row, 148 SMs): 32 rows, 32 tokens and 512 rows, 16384 tokens: see the case table of the design notes.
+static constexpr int kPlanThreads = 256;
+static constexpr int kPlanTokens = 1024;  // tokens per CTA
+
+struct PlanParams {
+    const int *ctx, *fresh, *free_pages, *free_count;
+    int *table, *lens, *cu, *positions, *slots, *free_left;
+    int B, T, max_pages, page_shift, num_pages, free_size;
+};
+
+// Exclusive running sum over the block's threads; the total in `total`.  Sums are cut at `cap` (no overflow: every
+// value is at most cap <= 2^30).
+__device__ __forceinline__ int block_prefix(int v, int cap, int* warp_sums, int& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s = min(s + up, cap);
+    }
+    __syncthreads();  // warp_sums may still be read from the sum before
+    if (lane == 31) warp_sums[warp] = s;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+        if (w == warp) before = all;
+        all = min(all + warp_sums[w], cap);
+    }
+    total = all;
+    int up = __shfl_up_sync(0xffffffffu, s, 1);
+    if (lane == 0) up = 0;
+    return min(before + up, cap);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanParams p) {
+    pdl_open(1);
+    extern __shared__ int plan_smem[];
+    int* cu = plan_smem;             // [B + 1] first token of a row
+    int* base = plan_smem + p.B + 1;  // [B] new pages of the rows in front
+    __shared__ int warp_sums[kPlanThreads / 32];
+    const int tid = threadIdx.x;
+    const int page = 1 << p.page_shift, cap = p.max_pages << p.page_shift;
+    const int rows = (p.B + kPlanThreads - 1) / kPlanThreads;
+    const int b0 = min(tid * rows, p.B), b1 = min(b0 + rows, p.B);
+    const int count = min(__ldg(p.free_count), p.free_size);
+    auto cached = [&](int b) { return min(max(__ldg(p.ctx + b), 0), cap); };
+    auto held = [&](int c) { return (int)(((long long)c + page - 1) >> p.page_shift); };
+
+    int sum = 0, total = 0;
+    for (int b = b0; b < b1; ++b) sum = min(sum + min(max(__ldg(p.fresh + b), 0), p.T), p.T);
+    int at = block_prefix(sum, p.T, warp_sums, total);
+    if (tid == 0) cu[p.B] = total;
+    sum = 0;
+    for (int b = b0; b < b1; ++b) {
+        cu[b] = at;
+        const int next = min(at + min(max(__ldg(p.fresh + b), 0), p.T), p.T), c = cached(b);
+        base[b] = sum;  // completed below
+        sum += held(min(c + next - at, cap)) - held(c);
+        at = next;
+    }
+    int pages = 0;
+    const int first = block_prefix(sum, 1 << 30, warp_sums, pages);
+    for (int b = b0; b < b1; ++b) base[b] += first;
+    __syncthreads();
+
+    auto valid = [&](int id) { return id >= 0 && id < p.num_pages ? id : -1; };
+    auto new_page = [&](int k) {  // k-th page that this step takes
+        const int i = count - 1 - k;
+        return i >= 0 ? valid(__ldg(p.free_pages + i)) : -1;
+    };
+    if (blockIdx.x == 0) {
+        for (int b = tid; b <= p.B; b += kPlanThreads) {
+            p.cu[b] = cu[b];
+            if (b < p.B) p.lens[b] = min(cached(b) + cu[b + 1] - cu[b], cap);
+        }
+        if (tid == 0) *p.free_left = count - pages;
+    }
+    // table entries: a warp per row
+    for (int b = blockIdx.x * (kPlanThreads / 32) + (tid >> 5); b < p.B; b += gridDim.x * (kPlanThreads / 32)) {
+        const int n = cu[b + 1] - cu[b];
+        if (n == 0) continue;
+        const int c = cached(b), h = held(c), need = held(min(c + n, cap));
+        for (int j = h + (tid & 31); j < need; j += 32) p.table[(long long)b * p.max_pages + j] = new_page(base[b] + j - h);
+    }
+    for (int t = blockIdx.x * kPlanTokens + tid; t < min((blockIdx.x + 1) * kPlanTokens, p.T); t += kPlanThreads) {
+        int pos = -1, slot = -1;
+        if (t < total) {
+            int lo = 0, hi = p.B;  // the last row whose first token is at most t
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (cu[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            const int c = cached(lo), h = held(c);
+            pos = c + t - cu[lo];
+            if (pos < cap) {
+                const int j = pos >> p.page_shift;
+                const int id = j < h ? valid(p.table[(long long)lo * p.max_pages + j]) : new_page(base[lo] + j - h);
+                if (id >= 0) slot = (id << p.page_shift) + (pos & (page - 1));
+            }
+        }
+        p.positions[t] = pos;
+        p.slots[t] = slot;
+    }
+}
+
+cudaError_t launch_paged_plan(const PlanArgs& a, cudaStream_t stream) {
+    PlanParams p;
+    p.ctx = a.ctx_lens, p.fresh = a.new_lens, p.free_pages = a.free_pages, p.free_count = a.free_count;
+    p.table = a.page_table, p.lens = a.seq_lens, p.cu = a.cu_tokens, p.positions = a.positions, p.slots = a.slots;
+    p.free_left = a.free_left;
+    p.B = a.B, p.T = a.T, p.max_pages = a.max_pages, p.page_shift = a.page_shift, p.num_pages = a.num_pages;
+    p.free_size = a.free_size;
+    int grid = (a.T + kPlanTokens - 1) / kPlanTokens;
+    const int row_ctas = (a.B + 31) / 32;  // four rows per warp
+    if (grid < row_ctas) grid = row_ctas;
+    const size_t smem = (size_t)(2 * a.B + 1) * sizeof(int);
+    if (smem > 47 * 1024) {  // 48 KB without opting in
+        cudaError_t e = cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    chain_begin();
+    return launch_pdl(paged_plan_kernel, dim3((unsigned)grid), dim3(kPlanThreads), smem, stream, p);
+}
+
+// ---------------------------------------- head norm + rotary + paged write ---
+// For token t, head vector x and frequency i < D/2 with axis a(i), position p = positions[a(i), t]:
+//   n = x / sqrt(mean(x^2) + eps) * w
+//   y_i = n_i cos[p, i] - n_{i+D/2} sin[p, i],   y_{i+D/2} = n_{i+D/2} cos[p, i+D/2] + n_i sin[p, i+D/2]
+// in fp32 with one rounding, as the stand-alone operator of a decode step and the decode attention do.
+// What bounds it: HBM for prompts (every head is read and written once), latency for a handful of tokens.  A head is
+// D/8 lanes of 16 bytes, so a warp moves 32 * 16 bytes per access; the partner of a rotation sits D/16 lanes away (one
+// shuffle per element).  A warp keeps the cos and sin values of ONE token in registers for all the heads it walks; how many
+// that are (`steps`) follows from the number of tokens: one group of heads per warp while there are fewer warps than the
+// chip holds, more when the table rows would otherwise be fetched again for every group.
+struct PagedRopeParams {
+    const bf16* qkv;
+    long long ld;
+    const bf16 *qw, *kw, *cos, *sin;
+    const int *positions, *slots;
+    bf16 *K, *V, *q_out;
+    int T, H, NKV, S, axes, page_shift, steps, chunks;
+    long long n_slots;
+    float eps;
+    unsigned int* status;
+    unsigned char axis[128];  // axis of frequency i
+};
+
+template <int D>
+__global__ void __launch_bounds__(256) paged_qk_norm_rope_kernel(const __grid_constant__ PagedRopeParams p) {
+    constexpr int LPH = D / 8, HPW = 32 / LPH;  // lanes per head, heads per warp
+    pdl_open(1);
+    const int lane = threadIdx.x & 31;
+    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int t = (int)(unit / p.chunks), chunk = (int)(unit - (long long)t * p.chunks);
+    if (t >= p.T) return;
+    const int sub = lane & (LPH - 1);             // 16-byte piece of the head
+    const bool upper = sub >= LPH / 2;            // second half of the head
+    const int f0 = (sub & (LPH / 2 - 1)) * 8;     // first frequency of this lane
+    const int heads = p.H + 2 * p.NKV;
+
+    int pos[3];
+    bool real = true, inside = true;
+#pragma unroll
+    for (int a = 0; a < 3; ++a) {
+        pos[a] = a < p.axes ? __ldg(p.positions + (long long)a * p.T + t) : 0;
+        real = real && pos[a] >= 0;
+        inside = inside && pos[a] < p.S;
+    }
+    const int slot = __ldg(p.slots + t);
+    if (!real) return;  // a padded token: nothing is written
+    if (!inside) {
+        if (lane == 0) report_fault(p.status, FAULT_ROPE_POSITION);
+        return;
+    }
+    const bool cached = slot >= 0 && slot < p.n_slots;
+    if (slot >= p.n_slots && lane == 0) report_fault(p.status, FAULT_SLOT_RANGE);
+
+    // Table rows: the lane's 8 columns of every axis, then the axis of each frequency picks.
+    float c[8], s[8];
+#pragma unroll
+    for (int a = 0; a < 3; ++a) {
+        if (a < p.axes) {
+            const uint4 cv = __ldg(reinterpret_cast<const uint4*>(p.cos + (long long)pos[a] * D + sub * 8));
+            const uint4 sv = __ldg(reinterpret_cast<const uint4*>(p.sin + (long long)pos[a] * D + sub * 8));
+            const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (a == 0 || p.axis[f0 + e] == a) {
+                    c[e] = (e & 1) ? bf16_hi(cw[e / 2]) : bf16_lo(cw[e / 2]);
+                    s[e] = (e & 1) ? bf16_hi(sw[e / 2]) : bf16_lo(sw[e / 2]);
+                }
+        }
+    }
+    if (!upper) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = -s[e];
+    }
+    const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+    const uint4 qw = p.qw ? __ldg(reinterpret_cast<const uint4*>(p.qw) + sub) : one;
+    const uint4 kw = p.kw ? __ldg(reinterpret_cast<const uint4*>(p.kw) + sub) : one;
+    const long long page = slot >> p.page_shift, off = slot & ((1 << p.page_shift) - 1);
+
+    const int h0 = chunk * p.steps * HPW + lane / LPH;
+    const bf16* src = p.qkv + (long long)t * p.ld + (long long)h0 * D + sub * 8;
+    constexpr int U = 4;  // heads in flight per lane
+    for (int i = 0; i < p.steps; i += U) {
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + (i + u) * HPW;
+            x[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (i + u < p.steps && h < heads) x[u] = *reinterpret_cast<const uint4*>(src + (long long)(i + u) * HPW * D);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int h = h0 + (i + u) * HPW;
+            const bool live = i + u < p.steps && h < heads;
+            const bool is_v = h >= p.H + p.NKV, is_q = h < p.H;
+            const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+            float v[8], ssq = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (e & 1) ? bf16_hi(xw[e / 2]) : bf16_lo(xw[e / 2]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ssq += v[e] * v[e];
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+            const float r = 1.0f / sqrtf(ssq * (1.0f / D) + p.eps);
+            const uint4 wv = is_q ? qw : kw;
+            const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = v[e] * r * ((e & 1) ? bf16_hi(ww[e / 2]) : bf16_lo(ww[e / 2]));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float other = __shfl_xor_sync(0xffffffffu, v[e], LPH / 2);
+                y[e] = __fadd_rn(__fmul_rn(v[e], c[e]), __fmul_rn(other, s[e]));
+            }
+            uint4 out = x[u];
+            if (!is_v) out = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+            if (live && is_q)
+                *reinterpret_cast<uint4*>(p.q_out + ((long long)t * p.H + h) * D + sub * 8) = out;
+            else if (live && cached) {
+                bf16* pool = is_v ? p.V : p.K;
+                const int kh = h - p.H - (is_v ? p.NKV : 0);
+                *reinterpret_cast<uint4*>(pool + (((page * p.NKV + kh) << p.page_shift) + off) * D + sub * 8) = out;
+            }
+        }
+    }
+}
+
+cudaError_t launch_paged_qk_norm_rope(const PagedRopeArgs& a, cudaStream_t stream) {
+    PagedRopeParams p;
+    p.qkv = a.qkv, p.ld = a.ld, p.qw = a.qw, p.kw = a.kw, p.cos = a.cos, p.sin = a.sin;
+    p.positions = a.positions, p.slots = a.slots, p.K = a.K, p.V = a.V, p.q_out = a.q_out;
+    p.T = a.T, p.H = a.H, p.NKV = a.NKV, p.S = a.S, p.axes = a.axes, p.page_shift = a.page_shift;
+    p.n_slots = (long long)a.num_pages << a.page_shift;
+    p.eps = a.eps;
+    p.status = status_ptr();
+    if (!p.status) return cudaErrorUnknown;
+    for (int i = 0; i < 128; ++i) p.axis[i] = i < a.D / 2 ? a.axis_of_frequency[i] : 0;
+    const int per_warp = 32 / (a.D / 8), groups = (a.H + 2 * a.NKV + per_warp - 1) / per_warp;
+    const long long fill = (long long)sm_count() * 32;
+    p.steps = 1;
+    while (p.steps < 8 && (long long)a.T * ((groups + 2 * p.steps - 1) / (2 * p.steps)) >= fill) p.steps *= 2;
+    p.chunks = (groups + p.steps - 1) / p.steps;
+    const long long warps = (long long)a.T * p.chunks;
+    chain_begin();
+    if (a.D == 64) return launch_pdl(paged_qk_norm_rope_kernel<64>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
+    return launch_pdl(paged_qk_norm_rope_kernel<128>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
+}
+
+}  // namespace ezb

@@ -6,15 +6,19 @@ on the class and refuses duplicates with ``ValueError``; ``get_kernel`` raises
 ``KeyError`` naming the backends that do exist.  The reference wraps
 ``__call__`` in a TileLang cache-naming scope (registry.py:19-29); this package
 has no TileLang backend, so classes are stored unwrapped.
+
+Operators beyond the decode path carry a family name: ``list_ops()`` lists the
+decode operators, ``list_ops("prompt")`` those that take prompts.
 """
 
 from __future__ import annotations
 
 _REGISTRY: dict[tuple[str, str], type] = {}
+_FAMILY: dict[str, str] = {}  # operators outside the decode path
 
 
-def register_kernel(op_name: str, backend: str):
-    """Class decorator: make ``cls`` the ``backend`` implementation of ``op_name``."""
+def register_kernel(op_name: str, backend: str, family: str | None = None):
+    """Class decorator: make ``cls`` the ``backend`` implementation of ``op_name`` (of a ``family`` of its own)."""
 
     def decorator(cls):
         key = (op_name, backend)
@@ -24,6 +28,8 @@ def register_kernel(op_name: str, backend: str):
         cls.op_name = op_name
         cls.backend = backend
         _REGISTRY[key] = cls
+        if family is not None:
+            _FAMILY[op_name] = family
         return cls
 
     return decorator
@@ -43,5 +49,5 @@ def list_backends(op_name: str) -> list[str]:
     return [b for (name, b) in _REGISTRY if name == op_name]
 
 
-def list_ops() -> list[str]:
-    return sorted({name for (name, _) in _REGISTRY})
+def list_ops(family: str | None = None) -> list[str]:
+    return sorted({name for (name, _) in _REGISTRY if _FAMILY.get(name) == family})

@@ -316,6 +316,91 @@ int ezb_qwen3_decode_stack_paged(const void* hidden, void* out, const ezb_layer_
                                  int max_pages, int num_pages, void* workspace, size_t workspace_bytes, int B, int H, int I,
                                  int NH, int NKV, int D, float eps, ezb_stream_t stream);
 
+/* ---------------------------------------------------------------- prompts ---
+ * The operators that take prompts through the same model over the same page
+ * pools (the reference has decode steps only).  A step holds the tokens of B
+ * rows one behind the other; a row may bring a whole prompt, a piece of one, a
+ * single token or nothing:
+ *   ezb_paged_plan           page tables, positions and cache slots of the step
+ *   ezb_linear_bf16          projections with bias, activation, residual
+ *   ezb_paged_qk_norm_rope   head norm, rotary embedding, write into the pools
+ *   ezb_attn_prompt          causal attention over the pools
+ * Pools and tables are those of ezb_attn_decode_paged; a decode step can follow
+ * a prompt step on them without a copy.  All index arrays are device int32. */
+
+/* The plan of a step, on the device.  Row b has ctx_lens[b] cached and
+ * new_lens[b] new tokens (values below 0 count as 0).  Its first
+ * ceil(ctx / page_size) table entries are in use; the pages that the new tokens
+ * need behind them are taken from the free list free_pages[free_size], a stack of
+ * which the first *free_count entries are valid, from its end, row by row, and
+ * written into page_table [B, max_pages] (in place; other entries stay).
+ *   seq_lens [B]              ctx + new
+ *   cu_tokens [B + 1]         first token of each row; [B] = tokens in the step
+ *   positions, slots [max_tokens]   position in its row and page * page_size +
+ *                             offset of each token; -1 behind the last one
+ *   free_left [1]             free_count less the pages taken; negative when the
+ *                             list was too short by that many, whose table entries
+ *                             and slots are then -1
+ * Tokens beyond max_tokens are dropped (cu_tokens stops there); a token beyond the
+ * max_pages * page_size positions of its row gets slot -1, and seq_lens stops
+ * there; an id outside [0, num_pages) is written and used as -1.  Outputs must not
+ * overlap inputs.  B <= 8192. */
+int ezb_paged_plan(const int* ctx_lens, const int* new_lens, int* page_table, const int* free_pages, const int* free_count,
+                   int* seq_lens, int* cu_tokens, int* positions, int* slots, int* free_left, int B, int max_tokens, int max_pages,
+                   int page_size, int num_pages, int free_size, ezb_stream_t stream);
+
+/* Per-head RMSNorm (+ weight, null = unit) and rotary embedding of the q and k
+ * heads of T tokens, straight from the rows of a fused projection
+ * (qkv [T, ldqkv]: H q heads | NKV k heads | NKV v heads, D elements each); q goes to
+ * q_out [T, H, D], k and v to pool slot slots[t] (ezb_qk_norm_rope's arithmetic:
+ * fp32, one rounding).  Positions may have up to three axes (time, height, width of an
+ * image or video token): positions [axes, T], and frequency i < D/2 is turned by the
+ * position of its axis - with interleaved = 0 the first sections_host[0]
+ * frequencies belong to axis 0, the next sections_host[1] to axis 1, ...; with
+ * interleaved = 1 axis a > 0 has the frequencies a + axes * j, j < sections_host[a],
+ * and axis 0 the others.  The sections add up to D/2.  cos, sin [table_rows, D].
+ * A token with a negative position is padding: nothing is written for it.  A
+ * negative slot writes q only.  A position behind the tables (fault 0x301, nothing
+ * written) or a slot behind the pools (fault 0x303, q only) is recorded in the
+ * status word.  Two tokens with one slot leave either's k and v there.
+ * D in {64, 128}. */
+int ezb_paged_qk_norm_rope(const void* qkv, long long ldqkv, const void* qw_or_null, const void* kw_or_null, const void* cos,
+                           const void* sin, const int* positions, const int* slots, void* K_pool, void* V_pool, void* q_out, int T,
+                           int H, int NKV, int D, int table_rows, int axes, const int* sections_host, int interleaved, int page_size,
+                           int num_pages, float eps, ezb_stream_t stream);
+
+/* out[m, n] = act(sum_k X[m, k] W[n, k] + bias[n]) + residual[m, n] for any number
+ * of rows M: bf16 operands, everything behind the product in fp32, one rounding to bf16
+ * (or none: out_f32 = 1 stores fp32).  EZB_ACT_SWIGLU: W [2N, K] and bias [2N] hold
+ * the gate rows, then the up rows, and act is silu(gate) * up.  Rows of X, residual
+ * (bf16) and out may be further apart than they are long (ldx, ldres, ldout in
+ * elements; ldx a multiple of 8).  residual may be out itself.  K % 8 == 0.  The path,
+ * and with it the order of the sums, follows from M, N and K. */
+#define EZB_ACT_NONE 0
+#define EZB_ACT_SILU 1
+#define EZB_ACT_GELU 2 /* x/2 * (1 + erf(x / sqrt 2)) */
+#define EZB_ACT_RELU 3
+#define EZB_ACT_SWIGLU 4
+int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bias_or_null, const void* residual_or_null,
+                    long long ldres, void* out, long long ldout, int M, int N, int K, int activation, int out_f32, ezb_stream_t stream);
+
+/* Causal grouped-query attention of the step's tokens over the pools.  Row b holds
+ * tokens cu_tokens[b] .. cu_tokens[b+1] of Q [T, ldq] (H heads of D) and has
+ * seq_lens[b] valid keys, the last ones being those of its own tokens: its i-th of n
+ * tokens sees the keys 0 .. seq_lens[b] - n + i (none of them: zeros).  Rows of Out
+ * [T, ldo] that belong to no row of the batch are left as they were.  Keys behind
+ * seq_lens[b] are never used, whatever they hold; the values of a row's own keys must
+ * be finite (a masked key counts with weight 0, and 0 * inf is not 0).  Table entries
+ * outside [0, num_pages) inside a row's length read as zeros and record fault 0x302.
+ * cu_tokens is cut to [0, T], seq_lens to [0, max_pages * page_size].  Equal calls
+ * give equal bits; where a row's sums are cut may depend on the other rows.
+ * The workspace depends on D only; as everywhere it is zero-filled once and serves one
+ * stream at a time.  D in {64, 128}; H / NKV <= 128; page_size a power of two >= 64. */
+size_t ezb_attn_prompt_workspace_bytes(int D);
+int ezb_attn_prompt(const void* Q, long long ldq, const void* K_pool, const void* V_pool, const int* page_table, const int* seq_lens,
+                    const int* cu_tokens, void* Out, long long ldo, void* workspace, size_t workspace_bytes, int B, int T, int H, int NKV,
+                    int D, int max_pages, int page_size, int num_pages, ezb_stream_t stream);
+
 /* The stack of layers, tensor parallel with the exchange fused into the kernels:
  * ezb_qwen3_decode_stack on this rank's shards (as ezb_qwen3_decode_layer_tp_fused
  * takes them), one call for all layers.  A layer's second sum is folded into
