@@ -24,9 +24,10 @@
 
 namespace ezb {
 
-static constexpr int kApThreads = 384;  // warps 0-3 and 4-7: softmax of tile 0 / 1; 8: TMA; 9: MMA; 10 and 11 fill up their warpgroup
+static constexpr int kApThreads = 384;  // warps 0-3 and 4-7: softmax of tile 0 / 1; 8: TMA; 9: MMA; 10: deals out the work; 11 fills up its warpgroup
 static constexpr int kApStages = 5;     // ring of K and V tiles
 static constexpr int kApKeys = 128;     // keys per tile
+static constexpr int kApSegments = 4;   // ring of work descriptors
 static constexpr int kApUnitCost = 256;  // a unit's fixed cost in keys; at least 127, so that its last tile lies inside its cost
 static constexpr int kApMinShare = 256;  // keys below which a further CTA is not worth its merge
 
@@ -81,6 +82,27 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// Two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 // Descriptor of the B operand of P V: V is stored [key][64 elements] with the 128-byte swizzle, so the MMA's N runs along
 // the contiguous dimension; 64-element column blocks lie 16 KB apart, groups of eight keys 1 KB.
 template <int D>
@@ -121,27 +143,46 @@ struct ApCursor {
     long long x0;  // where the unit starts on the line
     ApRow row;
 };
+// What the warps of a CTA have to know about the part of a unit that is theirs.
 struct ApSegment {
-    int tokens, first;    // tokens of the unit, its first token within the row
-    int extent, tiles;    // keys that any of its queries sees, in tiles of 128
-    int ks, ke;           // tiles of this CTA
-    bool dual, whole;     // at most 128 rows; nothing cut
+    int cnt;            // tiles of 128 keys of this CTA (0: a unit without keys), or -1: no more segments
+    int tiles, ks;      // tiles of the unit, first one of this CTA
+    int dual;           // the unit has at most 128 rows
+    int extent;         // keys that any of its queries sees
+    int token, tokens;  // first token (in Q and Out), tokens
+    int sees;           // keys that the first token sees (below 1: none); every further token sees one more
+    int row, head;      // batch row, kv head
+    int clear;          // the last V tile straddles the end of the row's keys
+    int slot;           // where a part of it goes
+    int c0, c1;         // first and last CTA with tiles of it
+    long long x0;       // its start on the line
 };
 __device__ __forceinline__ int ap_tile_at(long long x, long long x0, int tiles) {
     const long long k = (x - x0) >> 7;
     return x <= x0 ? 0 : (k < tiles ? (int)k : tiles);
 }
-// The unit under the cursor as CTA share [lo, hi) sees it; false when none of its tiles belongs to the share.
-__device__ __forceinline__ bool ap_segment(const ApParams& p, const ApCursor& c, long long lo, long long hi, ApSegment& s) {
-    const int u = 2 * p.tpt;
-    s.first = c.j * u;
-    s.tokens = min(u, c.row.n - s.first);
-    s.extent = max(0, c.row.len - (c.row.n - s.first - s.tokens));
+// The unit under the cursor as CTA `cta` with share [lo, hi) sees it; false when none of its tiles belongs to the share.
+__device__ __forceinline__ bool ap_segment(const ApParams& p, const ApLine& line, const ApCursor& c, int cta, long long lo, long long hi,
+                                           ApSegment& s) {
+    const int u = 2 * p.tpt, first = c.j * u;
+    s.tokens = min(u, c.row.n - first);
+    s.extent = max(0, c.row.len - (c.row.n - first - s.tokens));
     s.tiles = (s.extent + kApKeys - 1) / kApKeys;
-    s.ks = ap_tile_at(lo, c.x0, s.tiles), s.ke = ap_tile_at(hi, c.x0, s.tiles);
+    s.ks = ap_tile_at(lo, c.x0, s.tiles);
+    s.cnt = ap_tile_at(hi, c.x0, s.tiles) - s.ks;
+    if (s.tiles ? s.cnt == 0 : lo > c.x0) return false;  // a unit without keys belongs to the share in which it starts
     s.dual = s.tokens <= p.tpt;
-    s.whole = s.ke - s.ks == s.tiles;
-    return s.tiles ? s.ks < s.ke : lo <= c.x0;  // a unit without keys belongs to the share in which it starts
+    s.token = c.row.q0 + first;
+    s.sees = c.row.len - c.row.n + first + 1;
+    s.row = c.b, s.head = c.h;
+    s.clear = ((s.extent + 63) & ~63) > c.row.len && (s.extent & 63);
+    s.x0 = c.x0;
+    s.slot = 2 * cta + (c.x0 >= lo ? 1 : 0);  // 2 * cta: a unit that an earlier CTA began
+    s.c0 = s.c1 = cta;
+    // (a unit may start in one share and have all its tiles in the next: its start is no whole tile away)
+    while (s.c0 > 0 && ap_share(line, s.c0) > c.x0) --s.c0;
+    while (s.c1 + 1 < line.ctas && ap_tile_at(ap_share(line, s.c1 + 1), c.x0, s.tiles) < s.tiles) ++s.c1;
+    return true;
 }
 // Next unit; false at the end of the batch.
 __device__ __forceinline__ bool ap_advance(const ApParams& p, ApCursor& c) {
@@ -170,10 +211,11 @@ struct ApTail {
     uint64_t full[kApStages], empty[kApStages];
     uint64_t q_full, q_empty, fix;
     uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+    uint64_t seg_full[kApSegments], seg_empty[kApSegments];
+    ApSegment seg[kApSegments];
     uint32_t tmem;
     int abort_flag;
     int last;  // this CTA joins the parts of the unit
-    ApLine line;
     ApCursor start;
     long long warp_sum[kApThreads / 32];
     int list[2 * 160];  // parts of a unit in the order of its keys: 2 * slot + tile, or -1
@@ -202,6 +244,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
             mbar_init(smem_u32(&t.s_full[i]), 1), mbar_init(smem_u32(&t.o_full[i]), 1);
             mbar_init(smem_u32(&t.p_full[i]), 4), mbar_init(smem_u32(&t.o_empty[i]), 4);  // one arrival per warp
         }
+        for (int i = 0; i < kApSegments; ++i)
+            mbar_init(smem_u32(&t.seg_full[i]), 1), mbar_init(smem_u32(&t.seg_empty[i]), 10);  // warps that read it
         t.abort_flag = 0;
         mbar_fence_init();
     }
@@ -281,321 +325,358 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
     tc_fence_after();
     const uint32_t tmem = t.tmem;
     const uint32_t sm_q = smem_u32(smem), sm_ring = sm_q + L::kRing;
-    // A thread holds a row of scores: 384 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72.
-    if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
 
-    if (!idle) {
-        ApCursor cur = t.start;
-        ApSegment seg;
-        bool more = true;
-        if (warp == 8) {
-            // ------------------------------------------------------------ TMA producer
-            int it = 0, n_q = 0, n_fix = 0;  // ring tiles, query loads, repaired tiles so far
-            for (; more && cur.x0 < hi && !*abort_flag; more = ap_advance(p, cur)) {
-                if (!ap_segment(p, cur, lo, hi, seg) || seg.tiles == 0) continue;
-                const int cnt = seg.ke - seg.ks;
-                const int* table = p.table + (long long)cur.b * p.max_pages;
-                const bool clear_tail = ((seg.extent + 63) & ~63) > cur.row.len && (seg.extent & 63);
-                if (!mbar_wait_bounded(smem_u32(&t.q_empty), (uint32_t)((n_q & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+    // The next work descriptor (all lanes of a warp); it is read in place and given back with `release`.
+    int n_seg = 0;
+    auto next_segment = [&]() -> const ApSegment* {
+        const int i = n_seg % kApSegments;
+        if (!mbar_wait_bounded(smem_u32(&t.seg_full[i]), (uint32_t)((n_seg / kApSegments) & 1), abort_flag, p.status, FAULT_PROMPT_WAIT))
+            return nullptr;
+        return t.seg[i].cnt < 0 ? nullptr : &t.seg[i];
+    };
+    auto release = [&]() {
+        mbar_arrive(smem_u32(&t.seg_empty[n_seg % kApSegments]));
+        ++n_seg;
+    };
+
+    // A softmax thread holds a row of scores: 384 threads x 168 registers at launch = 2 x 128 x 192 + 128 x 120.
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    if (idle) {
+    } else if (warp == 10) {
+        // ------------------------------------------------------------ work descriptors
+        if (lane == 0) {
+            ApCursor cur = t.start;
+            for (bool more = true;; more = more && ap_advance(p, cur)) {
+                const bool end = !more || cur.x0 >= hi;
+                ApSegment s;
+                s.cnt = -1;
+                if (!end && !ap_segment(p, line, cur, cta, lo, hi, s)) continue;
+                const int i = n_seg % kApSegments;
+                if (!mbar_wait_bounded(smem_u32(&t.seg_empty[i]), (uint32_t)(((n_seg / kApSegments) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+                t.seg[i] = s;
+                mbar_arrive(smem_u32(&t.seg_full[i]));
+                ++n_seg;
+                if (end) break;
+            }
+        }
+    } else if (warp == 8) {
+        // ------------------------------------------------------------ TMA producer
+        int it = 0, n_q = 0, n_fix = 0;  // ring tiles, query loads, repaired tiles so far
+        while (const ApSegment* sp = next_segment()) {
+            const ApSegment seg = *sp;
+            __syncwarp();
+            if (lane == 0) release();
+            else ++n_seg;
+            if (seg.cnt == 0) continue;
+            const int* table = p.table + (long long)seg.row * p.max_pages;
+            if (!mbar_wait_bounded(smem_u32(&t.q_empty), (uint32_t)((n_q & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+            if (elect_one()) {
+                const uint32_t bar = smem_u32(&t.q_full);
+                const int tiles_q = seg.dual ? 1 : 2;
+                mbar_arrive_expect_tx(bar, (uint32_t)(p.tpt * p.G * 128 * BLOCKS * tiles_q));
+                for (int m = 0; m < tiles_q; ++m)
+#pragma unroll
+                    for (int k = 0; k < BLOCKS; ++k)
+                        tma_load_3d(sm_q + m * L::kTile + k * 16384, &mapQ, k * 64, seg.head * p.G, seg.token + m * p.tpt, bar);
+            }
+            __syncwarp();
+            ++n_q;
+            int ids = 0, ids_from = -16;  // lane i: pool page of key block (ids_from * 2 + i), 64 keys each
+            // K and V tiles in the order of their use: K(0) V(0) K(1) V(1) ..., or K(0) K(1) V(0) K(2) V(1) ... (dual)
+            const int ahead = seg.dual ? 2 : 1, lead = min(ahead, seg.cnt);
+#pragma unroll 1
+            for (int i = 0; i < 2 * seg.cnt && !*abort_flag; ++i) {
+                int v = 0, k = i;
+                if (i >= lead) {
+                    const int o = i - lead;  // V(0) K(ahead) V(1) K(ahead + 1) ... then the last V
+                    const int pairs = seg.cnt - lead;
+                    if (o < 2 * pairs) v = !(o & 1), k = (o >> 1) + (v ? 0 : ahead);
+                    else v = 1, k = pairs + (o - 2 * pairs);
+                }
+                k += seg.ks;
+                if (k < ids_from || k >= ids_from + 16) {
+                    ids_from = k;
+                    const long long key = ((long long)k * 2 + lane) * 64;
+                    ids = p.num_pages;  // out of range: zeros
+                    if (key < seg.extent) {
+                        const int id = __ldg(table + (key >> p.page_shift));
+                        if (id >= 0 && id < p.num_pages) ids = id;
+                        else report_fault(p.status, FAULT_PAGE_RANGE);
+                    }
+                }
+                const int stage = it % kApStages;
+                if (!mbar_wait_bounded(smem_u32(&t.empty[stage]), (uint32_t)(((it / kApStages) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+                const int id0 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2), id1 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2 + 1);
+                const bool repair = v && seg.clear && k == seg.tiles - 1;
+                const uint32_t dst = sm_ring + stage * L::kTile, bar = smem_u32(repair ? &t.fix : &t.full[stage]);
                 if (elect_one()) {
-                    const uint32_t bar = smem_u32(&t.q_full), bytes = (uint32_t)(p.tpt * p.G * 128 * BLOCKS);
-                    const int tiles_q = seg.dual ? 1 : 2;
-                    mbar_arrive_expect_tx(bar, bytes * tiles_q);
-                    for (int m = 0; m < tiles_q; ++m)
-                        for (int k = 0; k < BLOCKS; ++k)
-                            tma_load_3d(sm_q + m * L::kTile + k * 16384, &mapQ, k * 64, cur.h * p.G, cur.row.q0 + seg.first + m * p.tpt, bar);
+                    const CUtensorMap* map = v ? &mapV : &mapK;
+                    const int mask = (1 << p.page_shift) - 1, y0 = (k * kApKeys) & mask, y1 = (k * kApKeys + 64) & mask;
+                    mbar_arrive_expect_tx(bar, L::kTile);
+#pragma unroll
+                    for (int c = 0; c < BLOCKS; ++c) {
+                        tma_load_3d(dst + c * 16384, map, c * 64, y0, id0 * p.NKV + seg.head, bar);
+                        tma_load_3d(dst + c * 16384 + 8192, map, c * 64, y1, id1 * p.NKV + seg.head, bar);
+                    }
                 }
                 __syncwarp();
-                ++n_q;
-                int ids = 0, ids_from = -16;  // lane i: pool page of key block (ids_from * 2 + i), 64 keys each
-                // the tile of K (v = 0) or V (v = 1) number k of the unit
-                auto load = [&](int k, int v) {
-                    if (k < ids_from || k >= ids_from + 16) {
-                        ids_from = k;
-                        const long long key = ((long long)k * 2 + lane) * 64;
-                        ids = p.num_pages;  // out of range: zeros
-                        if (key < seg.extent) {
-                            const int id = __ldg(table + (key >> p.page_shift));
-                            if (id >= 0 && id < p.num_pages) ids = id;
-                            else report_fault(p.status, FAULT_PAGE_RANGE);
-                        }
-                    }
-                    const int stage = it % kApStages;
-                    if (!mbar_wait_bounded(smem_u32(&t.empty[stage]), (uint32_t)(((it / kApStages) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT))
-                        return;
-                    const int id0 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2), id1 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2 + 1);
-                    const bool repair = v && clear_tail && k == seg.tiles - 1;
-                    const uint32_t dst = sm_ring + stage * L::kTile, bar = smem_u32(repair ? &t.fix : &t.full[stage]);
-                    if (elect_one()) {
-                        const CUtensorMap* map = v ? &mapV : &mapK;
-                        const int mask = (1 << p.page_shift) - 1, y0 = (k * kApKeys) & mask, y1 = (k * kApKeys + 64) & mask;
-                        mbar_arrive_expect_tx(bar, L::kTile);
-#pragma unroll
-                        for (int c = 0; c < BLOCKS; ++c) {
-                            tma_load_3d(dst + c * 16384, map, c * 64, y0, id0 * p.NKV + cur.h, bar);
-                            tma_load_3d(dst + c * 16384 + 8192, map, c * 64, y1, id1 * p.NKV + cur.h, bar);
-                        }
-                    }
+                ++it;
+                if (repair) {
+                    // rows behind the last key of the block that straddles it: P is zero there, and V has to be
+                    mbar_wait_bounded(bar, (uint32_t)(n_fix & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    ++n_fix;
+                    const int r0 = seg.extent - k * kApKeys, bytes = (((r0 + 63) & ~63) - r0) * 128;  // extent is no multiple of 64 here
+                    for (int c = 0; c < BLOCKS; ++c)
+                        for (int o = lane * 16; o < bytes; o += 512)
+                            *reinterpret_cast<uint4*>(smem + L::kRing + stage * L::kTile + c * 16384 + r0 * 128 + o) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_async_shared();
                     __syncwarp();
-                    ++it;
-                    if (repair) {
-                        // rows behind the last key of the block that straddles it: P is zero there, and V has to be
-                        mbar_wait_bounded(bar, (uint32_t)(n_fix & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
-                        ++n_fix;
-                        const int r0 = seg.extent - k * kApKeys, r1 = (r0 + 63) & ~63;  // extent is no multiple of 64 here
-                        for (int i = lane; i < (r1 - r0) * 8 * BLOCKS; i += 32) {
-                            const int c = i / ((r1 - r0) * 8), o = i - c * (r1 - r0) * 8;
-                            *reinterpret_cast<uint4*>(smem + L::kRing + stage * L::kTile + c * 16384 + r0 * 128 + o * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        }
-                        fence_async_shared();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&t.full[stage]));
-                    }
-                };
-                const int ahead = seg.dual ? 2 : 1;  // K tiles in front of the V tile they belong to
-                for (int i = 0; i < ahead && i < cnt; ++i) load(seg.ks + i, 0);
-                for (int i = 0; i < cnt && !*abort_flag; ++i) {
-                    load(seg.ks + i, 1);
-                    if (i + ahead < cnt) load(seg.ks + i + ahead, 0);
+                    if (lane == 0) mbar_arrive(smem_u32(&t.full[stage]));
                 }
             }
-            if (*abort_flag) {  // nothing may still be landing in this CTA's shared memory when it exits
-                const long long t0 = clock64();
-                while (clock64() - t0 < kWaitLimitCycles / 100) {}
-            }
-        } else if (warp == 9) {
-            // ------------------------------------------------------------ MMA issuer
-            if (elect_one()) {
-                int it = 0, n_q = 0, n_tile[2] = {0, 0}, n_unit[2] = {0, 0};
-                auto wait = [&](uint64_t* bar, int parity) {
-                    const bool ok = mbar_wait_bounded(smem_u32(bar), (uint32_t)parity, abort_flag, p.status, FAULT_PROMPT_WAIT);
-                    tc_fence_after();
-                    return ok;
-                };
-                auto wait_stage = [&](int i) { return wait(&t.full[i % kApStages], (i / kApStages) & 1); };
-                auto scores = [&](int m, int q_tile, int i) {  // S[m] = Q K^T
-                    const uint64_t a = umma_desc_sw128(sm_q + q_tile * L::kTile), b = umma_desc_sw128(sm_ring + (i % kApStages) * L::kTile);
+        }
+        if (*abort_flag) {  // nothing may still be landing in this CTA's shared memory when it exits
+            const long long t0 = clock64();
+            while (clock64() - t0 < kWaitLimitCycles / 100) {}
+        }
+    } else if (warp == 9) {
+        // ------------------------------------------------------------ MMA issuer
+        if (elect_one()) {
+            int it = 0, n_q = 0;
+            uint32_t tiles_seen = 0, units_seen = 0;  // bit m: parity of the tiles / units of warpgroup m so far
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                const bool ok = mbar_wait_bounded(smem_u32(bar), parity, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                tc_fence_after();
+                return ok;
+            };
+            auto wait_stage = [&](int i) { return wait(&t.full[i % kApStages], (uint32_t)((i / kApStages) & 1)); };
+            auto scores = [&](int m, int q_tile, int i) {  // S[m] = Q K^T
+                const uint64_t a = umma_desc_sw128(sm_q + q_tile * L::kTile), b = umma_desc_sw128(sm_ring + (i % kApStages) * L::kTile);
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const int off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-                        tc_mma_bf16(tmem + m * 128, a + off, b + off, IDESC_QK, k > 0);
-                    }
-                    tc_commit(smem_u32(&t.s_full[m]));
-                };
-                auto values = [&](int m, int i, bool fresh) {  // O[m] (+)= P V
-                    const uint64_t b = umma_desc_sw128_mn<D>(sm_ring + (i % kApStages) * L::kTile);
+                for (int k = 0; k < D / 16; ++k) {
+                    const int off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+                    tc_mma_bf16(tmem + m * 128, a + off, b + off, IDESC_QK, k > 0);
+                }
+                tc_commit(smem_u32(&t.s_full[m]));
+            };
+            auto values = [&](int m, int i, bool fresh) {  // O[m] (+)= P V
+                const uint64_t b = umma_desc_sw128_mn<D>(sm_ring + (i % kApStages) * L::kTile);
 #pragma unroll
-                    for (int k = 0; k < kApKeys / 16; ++k)
-                        tc_mma_bf16_ts(tmem + 256 + m * D, tmem + m * 128 + k * 8, b + k * (2048 >> 4), IDESC_PV, !(fresh && k == 0));
-                };
-                for (; more && cur.x0 < hi && !*abort_flag; more = ap_advance(p, cur)) {
-                    if (!ap_segment(p, cur, lo, hi, seg) || seg.tiles == 0) continue;
-                    const int cnt = seg.ke - seg.ks;
-                    if (!wait(&t.q_full, n_q & 1)) break;
-                    ++n_q;
-                    if (!seg.dual) {
-                        // K(0) V(0) K(1) V(1) ... in the ring, each for both tiles
-                        if (!wait_stage(it)) break;
-                        scores(0, 0, it), scores(1, 1, it);
-                        tc_commit(smem_u32(&t.empty[it % kApStages]));
-                        ++it;
-                        if (cnt == 1) tc_commit(smem_u32(&t.q_empty));
-                        for (int i = 0; i < cnt && !*abort_flag; ++i) {
-                            const int v = it, k = it + 1;
-                            const bool next = i + 1 < cnt;
+                for (int k = 0; k < kApKeys / 16; ++k)
+                    tc_mma_bf16_ts(tmem + 256 + m * D, tmem + m * 128 + k * 8, b + k * (2048 >> 4), IDESC_PV, !(fresh && k == 0));
+            };
+            auto free_stage = [&](int i) { tc_commit(smem_u32(&t.empty[i % kApStages])); };
+            // P[m] is there, and for the first tile of a unit O[m] has been drained
+            auto wait_probabilities = [&](int m, bool fresh) {
+                if (!wait(&t.p_full[m], (tiles_seen >> m) & 1u)) return false;
+                tiles_seen ^= 1u << m;
+                if (fresh) {
+                    if (!wait(&t.o_empty[m], ((units_seen >> m) & 1u) ^ 1u)) return false;
+                    units_seen ^= 1u << m;
+                }
+                return true;
+            };
+            while (const ApSegment* sp = next_segment()) {
+                const int cnt = sp->cnt, dual = sp->dual;
+                release();
+                if (cnt == 0) continue;
+                if (!wait(&t.q_full, (uint32_t)(n_q & 1))) break;
+                ++n_q;
+                if (!dual) {
+                    // every K and V tile serves both tiles of queries
+                    if (!wait_stage(it)) break;
+                    scores(0, 0, it);
+                    scores(1, 1, it);
+                    free_stage(it);
+                    ++it;
+                    if (cnt == 1) tc_commit(smem_u32(&t.q_empty));
+#pragma unroll 1
+                    for (int i = 0; i < cnt && !*abort_flag; ++i) {
+                        const bool next = i + 1 < cnt;
 #pragma unroll
-                            for (int m = 0; m < 2; ++m) {
-                                if (!wait(&t.p_full[m], n_tile[m] & 1)) break;
-                                ++n_tile[m];
-                                if (i == 0) {
-                                    if (!wait(&t.o_empty[m], (n_unit[m] & 1) ^ 1)) break;
-                                    ++n_unit[m];
-                                }
-                                if (m == 0 && !wait_stage(v)) break;
-                                values(m, v, i == 0);
-                                if (m == 1) tc_commit(smem_u32(&t.empty[v % kApStages]));
-                                if (next) {
-                                    if (m == 0 && !wait_stage(k)) break;
-                                    scores(m, m, k);
-                                    if (m == 1) {
-                                        tc_commit(smem_u32(&t.empty[k % kApStages]));
-                                        if (i + 2 == cnt) tc_commit(smem_u32(&t.q_empty));
-                                    }
-                                } else {
-                                    tc_commit(smem_u32(&t.o_full[m]));
-                                }
-                            }
-                            it += next ? 2 : 1;
-                        }
-                    } else {
-                        // K(0) K(1) V(0) K(2) V(1) K(3) ...: tile i of the keys belongs to warpgroup i & 1
-                        for (int i = 0; i < 2 && i < cnt; ++i) {
-                            if (!wait_stage(it)) break;
-                            scores(i, 0, it);
-                            tc_commit(smem_u32(&t.empty[it % kApStages]));
-                            ++it;
-                        }
-                        if (cnt <= 2) tc_commit(smem_u32(&t.q_empty));
-                        for (int i = 0; i < cnt && !*abort_flag; ++i) {
-                            const int m = i & 1;
-                            int& tiles = n_tile[m];
-                            if (!wait(&t.p_full[m], tiles & 1)) break;
-                            ++tiles;
-                            if (i < 2) {
-                                if (!wait(&t.o_empty[m], (n_unit[m] & 1) ^ 1)) break;
-                                ++n_unit[m];
-                            }
-                            if (!wait_stage(it)) break;
-                            values(m, it, i < 2);
-                            tc_commit(smem_u32(&t.empty[it % kApStages]));
-                            ++it;
-                            if (i + 2 < cnt) {
-                                if (!wait_stage(it)) break;
-                                scores(m, 0, it);
-                                tc_commit(smem_u32(&t.empty[it % kApStages]));
-                                ++it;
-                                if (i + 3 == cnt) tc_commit(smem_u32(&t.q_empty));
+                        for (int m = 0; m < 2; ++m) {
+                            if (!wait_probabilities(m, i == 0)) break;
+                            if (m == 0 && !wait_stage(it)) break;
+                            values(m, it, i == 0);
+                            if (m == 1) free_stage(it);
+                            if (next) {
+                                if (m == 0 && !wait_stage(it + 1)) break;
+                                scores(m, m, it + 1);
+                                if (m == 1) free_stage(it + 1);
                             } else {
                                 tc_commit(smem_u32(&t.o_full[m]));
                             }
                         }
+                        if (i + 2 == cnt) tc_commit(smem_u32(&t.q_empty));
+                        it += next ? 2 : 1;
+                    }
+                } else {
+                    // tile i of the keys belongs to warpgroup i & 1
+#pragma unroll 1
+                    for (int i = 0; i < 2 && i < cnt; ++i) {
+                        if (!wait_stage(it)) break;
+                        scores(i, 0, it);
+                        free_stage(it);
+                        ++it;
+                    }
+                    if (cnt <= 2) tc_commit(smem_u32(&t.q_empty));
+#pragma unroll 1
+                    for (int i = 0; i < cnt && !*abort_flag; ++i) {
+                        const int m = i & 1;
+                        if (!wait_probabilities(m, i < 2)) break;
+                        if (!wait_stage(it)) break;
+                        values(m, it, i < 2);
+                        free_stage(it);
+                        ++it;
+                        if (i + 2 < cnt) {
+                            if (!wait_stage(it)) break;
+                            scores(m, 0, it);
+                            free_stage(it);
+                            ++it;
+                            if (i + 3 == cnt) tc_commit(smem_u32(&t.q_empty));
+                        } else {
+                            tc_commit(smem_u32(&t.o_full[m]));
+                        }
                     }
                 }
             }
-        } else if (warp < 8) {
-            // ------------------------------------------------------------ softmax, one row per thread
-            const int m = warp >> 2;                                    // tile
-            const int r = (warp & 3) * 32 + lane;                       // row of the tile
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t t_s = tmem + lanes + m * 128, t_o = tmem + lanes + 256 + m * D;
-            const int r_tok = r / p.G, r_head = r - r_tok * p.G;
-            int n_tile = 0, n_unit = 0;
-            for (; more && cur.x0 < hi; more = ap_advance(p, cur)) {
-                if (!ap_segment(p, cur, lo, hi, seg)) continue;
-                const int cnt = seg.ke - seg.ks;
-                const int tok0 = seg.first + (seg.dual ? 0 : m * p.tpt);  // first token of this tile within the row
-                const int tok = tok0 + r_tok;
-                const bool live = r_tok < p.tpt && tok < seg.first + seg.tokens;
-                // keys that this query sees; for the tile: what all of its queries see
-                const int limit = live ? max(0, cur.row.len - (cur.row.n - 1 - tok)) : 0;
-                const int all_see = cur.row.len - (cur.row.n - 1 - tok0);
-                const int my0 = seg.dual ? m : 0, step = seg.dual ? 2 : 1;
-                const int mine = seg.dual ? (cnt + 1 - m) / 2 : cnt;
-                float mx = -INFINITY, sum = 0.f;
-                for (int i = my0; i < cnt; i += step) {
-                    const int key0 = (seg.ks + i) * kApKeys;
-                    mbar_wait_bounded(smem_u32(&t.s_full[m]), (uint32_t)(n_tile & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
-                    ++n_tile;
-                    tc_fence_after();
-                    float s[kApKeys];
+        }
+    }
+    } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if (!idle) {
+        // ------------------------------------------------------------ softmax, one row per thread
+        const int m = warp >> 2;                                    // tile
+        const int r = (warp & 3) * 32 + lane;                       // row of the tile
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + m * 128, t_o = tmem + lanes + 256 + m * D;
+        const int r_tok = r / p.G, r_head = r - r_tok * p.G;
+        uint32_t n_tile = 0, n_unit = 0;
+        while (const ApSegment* sp = next_segment()) {
+            const ApSegment& seg = *sp;  // stays in shared memory until the end of the segment
+            const int cnt = seg.cnt, dual = seg.dual;
+            const int first = dual ? 0 : m * p.tpt, tok = first + r_tok;  // within the unit
+            const bool live = r_tok < p.tpt && tok < seg.tokens;
+            // keys that this query sees, and that all queries of the tile see, counted from the CTA's first key
+            const int from = seg.ks * kApKeys;
+            const int limit = live ? seg.sees + tok - from : 0, all_see = seg.sees + first - from;
+            const int my0 = dual ? m : 0, step = dual ? 2 : 1;
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+            for (int i = my0; i < cnt; i += step) {
+                const int key0 = i * kApKeys;
+                mbar_wait_bounded(smem_u32(&t.s_full[m]), n_tile & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                ++n_tile;
+                tc_fence_after();
+                float s[kApKeys];
 #pragma unroll
-                    for (int c = 0; c < kApKeys; c += 32) tmem_ld32(t_s + c, s + c);
-                    tmem_ld_wait();
-                    if (key0 + kApKeys > all_see) {
+                for (int c = 0; c < kApKeys; c += 32) tmem_ld32(t_s + c, s + c);
+                tmem_ld_wait();
+                if (key0 + kApKeys > all_see) {
 #pragma unroll
-                        for (int c = 0; c < kApKeys; ++c)
-                            if (key0 + c >= limit) s[c] = -INFINITY;
-                    }
-                    float top = s[0];
+                    for (int c = 0; c < kApKeys; ++c)
+                        if (key0 + c >= limit) s[c] = -INFINITY;
+                }
+                float top4[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int c = 1; c < kApKeys; ++c) top = fmaxf(top, s[c]);
-                    if (i == my0) {
-                        mx = top;
-                    } else {
-                        // all keys so far masked: nothing has been summed, and the factor is exp2(-inf) = 0
-                        const float higher = fmaxf(mx, top);
-                        const bool grow = (higher - mx) * p.scale_log2 > 8.f;
-                        if (__any_sync(0xffffffffu, grow)) {
-                            const float f = grow ? exp2_approx((mx - higher) * p.scale_log2) : 1.f;
-                            if (grow) mx = higher;
-                            sum *= f;
+                for (int c = 4; c < kApKeys; c += 8) {
 #pragma unroll
-                            for (int c = 0; c < D; c += 32) {
-                                float o[32];
-                                tmem_ld32(t_o + c, o);
-                                tmem_ld_wait();
-                                uint32_t w[32];
+                    for (int e = 0; e < 4; ++e) top4[e] = c + 4 + e < kApKeys ? max3(top4[e], s[c + e], s[c + 4 + e]) : fmaxf(top4[e], s[c + e]);
+                }
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                if (i == my0) {
+                    mx = top;
+                } else {
+                    // all keys so far masked: nothing has been summed, and the factor is exp2(-inf) = 0
+                    const float higher = fmaxf(mx, top);
+                    const bool grow = (higher - mx) * p.scale_log2 > 8.f;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? exp2_approx((mx - higher) * p.scale_log2) : 1.f;
+                        if (grow) mx = higher;
+                        sum *= f;
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            uint32_t w[16];
+                            tmem_ld16(t_o + c, o);
+                            tmem_ld_wait();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-                                tmem_st16(t_o + c, w);
-                                tmem_st16(t_o + c + 16, w + 16);
-                            }
-                            tmem_st_wait();
+                            for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
+                            tmem_st16(t_o + c, w);
                         }
                     }
-                    const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
-                    float add[4] = {0.f, 0.f, 0.f, 0.f};
+                }
+                const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+                float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(-shift, -shift);
 #pragma unroll
-                    for (int c = 0; c < kApKeys; c += 32) {
-                        uint32_t w[16];
+                for (int c = 0; c < kApKeys; c += 32) {
+                    uint32_t w[16];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float a = exp2_approx(fmaf(s[c + 2 * e], p.scale_log2, -shift));
-                            const float b = exp2_approx(fmaf(s[c + 2 * e + 1], p.scale_log2, -shift));
-                            add[(2 * e) & 3] += a, add[(2 * e + 1) & 3] += b;
-                            w[e] = pack_bf16(a, b);
-                        }
-                        tmem_st16(t_s + c / 2, w);
+                    for (int e = 0; e < 16; ++e) {
+                        float2 x = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2);
+                        x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
+                        add[e & 1] = add2(add[e & 1], x);
+                        w[e] = pack_bf16(x.x, x.y);
                     }
-                    sum += (add[0] + add[1]) + (add[2] + add[3]);
-                    tmem_st_wait();
+                    tmem_st16(t_s + c / 2, w);
+                }
+                sum += (add[0].x + add[1].x) + (add[0].y + add[1].y);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&t.p_full[m]));
+            }
+            // ---- end of the segment
+            const bool mine = my0 < cnt, whole = cnt == seg.tiles;
+            if (mine) {
+                mbar_wait_bounded(smem_u32(&t.o_full[m]), n_unit & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                ++n_unit;
+                tc_fence_after();
+            }
+            if (whole && (!dual || cnt <= 1)) {
+                // a query that sees no key gives zero; the second tile of a single block of keys has no rows
+                const bool store = live && !(dual && m == 1) && !*abort_flag;
+                const float inv = limit > 0 ? 1.0f / sum : 0.f;
+                bf16* out = p.Out + (long long)(seg.token + tok) * p.ldo + (long long)(seg.head * p.G + r_head) * D;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    float o[16];
+                    if (mine) {
+                        tmem_ld16(t_o + c, o);
+                        tmem_ld_wait();
+                    }
+                    uint32_t w[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) w[q] = limit > 0 ? pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
+                    if (store) {
+                        *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
+                    __syncwarp();
+                }
+                if (mine) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&t.p_full[m]));
+                    if (lane == 0) mbar_arrive(smem_u32(&t.o_empty[m]));
                 }
-                // ---- end of the segment
-                const bool direct = seg.tiles == 0 || (seg.whole && (!seg.dual || cnt == 1));
-                if (mine > 0) {
-                    mbar_wait_bounded(smem_u32(&t.o_full[m]), (uint32_t)(n_unit & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
-                    ++n_unit;
-                    tc_fence_after();
-                }
-                if (direct) {
-                    if (seg.dual && m == 1) continue;  // tile 0 holds all rows
-                    const float inv = 1.0f / sum;
-                    bf16* out = p.Out + (long long)(cur.row.q0 + tok) * p.ldo + (long long)(cur.h * p.G + r_head) * D;
-#pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        if (mine > 0) {
-                            tmem_ld32(t_o + c, o);
-                            tmem_ld_wait();
-                        }
-                        if (live && !*abort_flag) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 8) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int q = 0; q < 4; ++q)  // a query that sees no key gives zero
-                                    w[q] = limit == 0 ? 0u : pack_bf16(o[e + 2 * q] * inv, o[e + 2 * q + 1] * inv);
-                                *reinterpret_cast<uint4*>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                        }
-                    }
-                    if (mine > 0) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&t.o_empty[m]));
-                    }
-                    continue;
-                }
-                // A part: slot 2 * cta holds the unit that the CTA in front began, 2 * cta + 1 one that starts here
-                const int slot = 2 * cta + (cur.x0 >= lo ? 1 : 0);
+            } else {
                 constexpr long long kPart = (long long)(D + 2) * 128;
-                if (mine > 0) {
-                    float* part = p.parts + (slot * 2 + m) * kPart;
+                if (mine) {
+                    float* part = p.parts + (seg.slot * 2 + m) * kPart;
                     if (live) __stcg(part + (long long)D * 128 + r, mx), __stcg(part + (long long)(D + 1) * 128 + r, sum);
-#pragma unroll
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        tmem_ld32(t_o + c, o);
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        float o[16];
+                        tmem_ld16(t_o + c, o);
                         tmem_ld_wait();
                         if (live) {
 #pragma unroll
-                            for (int e = 0; e < 32; e += 4)
+                            for (int e = 0; e < 16; e += 4)
                                 __stcg(reinterpret_cast<float4*>(part) + (c + e) / 4 * 128 + r, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
                         }
+                        __syncwarp();
                     }
                     tc_fence_before();
                     __syncwarp();
@@ -603,36 +684,29 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                 }
                 __threadfence();
                 named_bar_sync(1, 256);
-                // the share in which the unit starts, and the last one with keys of it
-                int c0 = (int)(cur.x0 * line.ctas / line.total), c1;
-                while (c0 > 0 && ap_share(line, c0) > cur.x0) --c0;
-                while (ap_share(line, c0 + 1) <= cur.x0) ++c0;
                 if (tid == 0) {
                     // One counter per share: of the units that start in it only the last can be cut.  (The others have to leave
                     // it alone: the next CTA may already have added its part of that last one.)
                     t.last = 1;
-                    if (!seg.whole) {
-                        t.last = atomicAdd(p.count + c0, (unsigned)cnt) + (unsigned)cnt == (unsigned)seg.tiles;
-                        if (t.last) p.count[c0] = 0u;
+                    if (!whole) {
+                        t.last = atomicAdd(p.count + seg.c0, (unsigned)cnt) + (unsigned)cnt == (unsigned)seg.tiles;
+                        if (t.last) p.count[seg.c0] = 0u;
                     }
                 }
-                c1 = c0;
-                while (c1 + 1 < line.ctas && ap_tile_at(ap_share(line, c1 + 1), cur.x0, seg.tiles) < seg.tiles) ++c1;
+                const int c0 = seg.c0, c1 = seg.c1;
                 for (int c = c0 + tid; c <= c1; c += 256) {
-                    const int a = ap_tile_at(ap_share(line, c), cur.x0, seg.tiles), z = ap_tile_at(ap_share(line, c + 1), cur.x0, seg.tiles);
+                    const int a = ap_tile_at(ap_share(line, c), seg.x0, seg.tiles), z = ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles);
                     const int sl = 2 * (2 * c + (c == c0 ? 1 : 0));
                     t.list[2 * (c - c0)] = a < z ? sl : -1;
-                    t.list[2 * (c - c0) + 1] = seg.dual && z - a > 1 ? sl + 1 : -1;
+                    t.list[2 * (c - c0) + 1] = dual && z - a > 1 ? sl + 1 : -1;
                 }
                 named_bar_sync(1, 256);
                 if (t.last && !*abort_flag) {
                     __threadfence();
-                    const int n_list = 2 * (c1 - c0 + 1), rows = seg.tokens * p.G;
-                    // dual: all rows in every part; else tile q of row / (tpt * G), which is the second of a pair of parts
-                    const int per_tile = p.tpt * p.G;
+                    const int n_list = 2 * (c1 - c0 + 1), rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
                     for (int i = tid; i < rows * (D / 4); i += 256) {
                         const int row = i % rows, c = i / rows;
-                        const int q = row / per_tile, rr = row - q * per_tile;
+                        const int q = row / per_tile, rr = row - q * per_tile;  // tile of the pair (dual: always 0) and row in it
                         float top = -INFINITY;
                         for (int k = 0; k < n_list; ++k) {
                             const int id = t.list[k];
@@ -650,17 +724,20 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                             all += w * __ldcg(part + (long long)(D + 1) * 128 + rr);
                             acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
                         }
-                        const int token = seg.first + row / p.G, head = row % p.G;
+                        const int token = row / p.G, head = row - token * p.G;
                         const float inv = 1.0f / all;
                         uint2 w = make_uint2(0u, 0u);  // a query that sees no key
-                        if (cur.row.len - (cur.row.n - 1 - token) > 0)
-                            w = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-                        *reinterpret_cast<uint2*>(p.Out + (long long)(cur.row.q0 + token) * p.ldo + (long long)(cur.h * p.G + head) * D + c * 4) = w;
+                        if (seg.sees + token > 0) w = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+                        *reinterpret_cast<uint2*>(p.Out + (long long)(seg.token + token) * p.ldo + (long long)(seg.head * p.G + head) * D + c * 4) = w;
                     }
                 }
                 named_bar_sync(1, 256);  // the list and the flag are free again
             }
+            __syncwarp();
+            if (lane == 0) release();
+            else ++n_seg;
         }
+    }
     }
     __syncwarp();
     tc_fence_before();
