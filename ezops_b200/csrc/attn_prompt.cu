@@ -29,6 +29,7 @@ static constexpr int kApStages = 5;     // ring of K and V tiles
 static constexpr int kApKeys = 128;     // keys per tile
 static constexpr int kApSegments = 4;   // ring of work descriptors
 static constexpr int kApUnitCost = 256;  // a unit's fixed cost in keys; at least 127, so that its last tile lies inside its cost
+static constexpr int kApWhole = 4;      // units of at most so many tiles are never cut
 static constexpr int kApMinShare = 256;  // keys below which a further CTA is not worth its merge
 
 struct ApParams {
@@ -157,9 +158,13 @@ struct ApSegment {
     int c0, c1;         // first and last CTA with tiles of it
     long long x0;       // its start on the line
 };
+// The tile of the unit that starts at x0 at which place x of the line cuts it: short units are not cut, and no piece is
+// shorter than two tiles (a part costs a trip through the workspace).
 __device__ __forceinline__ int ap_tile_at(long long x, long long x0, int tiles) {
-    const long long k = (x - x0) >> 7;
-    return x <= x0 ? 0 : (k < tiles ? (int)k : tiles);
+    if (x <= x0) return 0;
+    const int k = (x - x0) >> 7 < tiles ? (int)((x - x0) >> 7) : tiles;
+    if (tiles <= kApWhole) return 2 * k >= tiles ? tiles : 0;
+    return k < 2 ? 0 : (k > tiles - 2 ? tiles : k);
 }
 // The unit under the cursor as CTA `cta` with share [lo, hi) sees it; false when none of its tiles belongs to the share.
 __device__ __forceinline__ bool ap_segment(const ApParams& p, const ApLine& line, const ApCursor& c, int cta, long long lo, long long hi,
@@ -221,6 +226,59 @@ struct ApTail {
     int list[2 * 160];  // parts of a unit in the order of its keys: 2 * slot + tile, or -1
 };
 static_assert(sizeof(ApTail) <= 2048, "tail of the shared memory");
+
+// Joins the parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by 256 threads.  Not
+// inlined: its registers would be taken from the loop over the keys.
+template <int D>
+__device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const int* list, int tid) {
+    constexpr long long kPart = (long long)(D + 2) * 128;
+    // A thread keeps one row of the unit and every (256 / rows)-th group of four columns of it; rows rounded
+    // up to a power of two.  Eight groups are on their way at a time.
+    const int n_list = 2 * (seg.c1 - seg.c0 + 1), rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
+    const int log_rows = rows > 1 ? 32 - __clz(rows - 1) : 0, row = tid & ((1 << log_rows) - 1);
+    const int stride = 256 >> log_rows;
+    if (row < rows) {
+        const int q = row / per_tile, rr = row - q * per_tile;  // tile of the pair (dual: always 0) and row in it
+        const float* stat = p.parts + q * kPart + (long long)D * 128 + rr;
+        float top = -INFINITY, all = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < n_list; ++k)
+            if (list[k] >= 0) top = fmaxf(top, __ldcg(stat + list[k] * kPart));
+        const int token = row / p.G, head = row - token * p.G;
+        const bool any = seg.sees + token > 0;  // else the query sees no key
+        bf16* out = p.Out + (long long)(seg.token + token) * p.ldo + (long long)(seg.head * p.G + head) * D;
+#pragma unroll 1
+        for (int g0 = tid >> log_rows; g0 < D / 4; g0 += 8 * stride) {
+            float4 acc[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            all = 0.f;
+#pragma unroll 1
+            for (int k = 0; k < n_list; ++k) {
+                const int id = list[k];
+                if (id < 0) continue;
+                const float4* part = reinterpret_cast<const float4*>(p.parts + (id + q) * kPart) + rr;
+                float4 o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (g0 + e * stride < D / 4) o[e] = __ldcg(part + (g0 + e * stride) * 128);
+                const float pm = __ldcg(stat + id * kPart), ps = __ldcg(stat + id * kPart + 128);
+                const float w = pm == -INFINITY ? 0.f : exp2_approx((pm - top) * p.scale_log2);
+                all += w * ps;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (g0 + e * stride < D / 4)
+                        acc[e].x += w * o[e].x, acc[e].y += w * o[e].y, acc[e].z += w * o[e].z, acc[e].w += w * o[e].w;
+            }
+            const float inv = 1.0f / all;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (g0 + e * stride < D / 4)
+                    *reinterpret_cast<uint2*>(out + (g0 + e * stride) * 4) =
+                        any ? make_uint2(pack_bf16(acc[e].x * inv, acc[e].y * inv), pack_bf16(acc[e].z * inv, acc[e].w * inv)) : make_uint2(0u, 0u);
+        }
+    }
+}
 
 template <int D>
 __global__ void __launch_bounds__(kApThreads, 1)
@@ -703,33 +761,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                 named_bar_sync(1, 256);
                 if (t.last && !*abort_flag) {
                     __threadfence();
-                    const int n_list = 2 * (c1 - c0 + 1), rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
-                    for (int i = tid; i < rows * (D / 4); i += 256) {
-                        const int row = i % rows, c = i / rows;
-                        const int q = row / per_tile, rr = row - q * per_tile;  // tile of the pair (dual: always 0) and row in it
-                        float top = -INFINITY;
-                        for (int k = 0; k < n_list; ++k) {
-                            const int id = t.list[k];
-                            if (id >= 0) top = fmaxf(top, __ldcg(p.parts + (id + q) * kPart + (long long)D * 128 + rr));
-                        }
-                        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                        float all = 0.f;
-                        for (int k = 0; k < n_list; ++k) {
-                            const int id = t.list[k];
-                            if (id < 0) continue;
-                            const float* part = p.parts + (id + q) * kPart;
-                            const float pm = __ldcg(part + (long long)D * 128 + rr);
-                            const float w = pm == -INFINITY ? 0.f : exp2_approx((pm - top) * p.scale_log2);
-                            const float4 o = __ldcg(reinterpret_cast<const float4*>(part) + c * 128 + rr);
-                            all += w * __ldcg(part + (long long)(D + 1) * 128 + rr);
-                            acc.x += w * o.x, acc.y += w * o.y, acc.z += w * o.z, acc.w += w * o.w;
-                        }
-                        const int token = row / p.G, head = row - token * p.G;
-                        const float inv = 1.0f / all;
-                        uint2 w = make_uint2(0u, 0u);  // a query that sees no key
-                        if (seg.sees + token > 0) w = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-                        *reinterpret_cast<uint2*>(p.Out + (long long)(seg.token + token) * p.ldo + (long long)(seg.head * p.G + head) * D + c * 4) = w;
-                    }
+                    ap_join<D>(p, seg, t.list, tid);
                 }
                 named_bar_sync(1, 256);  // the list and the flag are free again
             }
