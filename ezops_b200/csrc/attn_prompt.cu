@@ -215,7 +215,7 @@ struct ApSmem {
 struct ApTail {
     uint64_t full[kApStages], empty[kApStages];
     uint64_t q_full, q_empty, fix;
-    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], turn[2];
     uint64_t seg_full[kApSegments], seg_empty[kApSegments];
     ApSegment seg[kApSegments];
     uint32_t tmem;
@@ -301,6 +301,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&t.s_full[i]), 1), mbar_init(smem_u32(&t.o_full[i]), 1);
             mbar_init(smem_u32(&t.p_full[i]), 4), mbar_init(smem_u32(&t.o_empty[i]), 4);  // one arrival per warp
+            mbar_init(smem_u32(&t.turn[i]), 4);
         }
         for (int i = 0; i < kApSegments; ++i)
             mbar_init(smem_u32(&t.seg_full[i]), 1), mbar_init(smem_u32(&t.seg_empty[i]), 10);  // warps that read it
@@ -610,7 +611,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lanes + m * 128, t_o = tmem + lanes + 256 + m * D;
         const int r_tok = r / p.G, r_head = r - r_tok * p.G;
-        uint32_t n_tile = 0, n_unit = 0;
+        uint32_t n_tile = 0, n_unit = 0, n_turn = 0;
         while (const ApSegment* sp = next_segment()) {
             const ApSegment& seg = *sp;  // stays in shared memory until the end of the segment
             const int cnt = seg.cnt, dual = seg.dual;
@@ -666,6 +667,12 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                     }
                 }
                 const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+                // The warpgroups take turns: side by side they would both exponentiate at half speed and then both wait for
+                // the tensor cores.
+                if (!dual) {
+                    mbar_wait_bounded(smem_u32(&t.turn[m]), (n_turn & 1u) ^ (m == 0 ? 1u : 0u), abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    ++n_turn;
+                }
                 float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(-shift, -shift);
 #pragma unroll
@@ -679,6 +686,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                         w[e] = pack_bf16(x.x, x.y);
                     }
                     tmem_st16(t_s + c / 2, w);
+                }
+                if (!dual) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&t.turn[1 - m]));
                 }
                 sum += (add[0].x + add[1].x) + (add[0].y + add[1].y);
                 tmem_st_wait();
