@@ -50,11 +50,22 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Operand descriptors as halves: the low word holds the address (and the column block stride), the high word is one constant
+// for all 128-byte-swizzled tiles (see umma_desc_sw128), so that only 32 bits a tile have to be kept.
+static constexpr uint32_t kApDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t ap_desc(uint32_t smem_addr) { return (smem_addr & 0x3FFFFu) >> 4; }
+__device__ __forceinline__ void ap_mma_ss(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_low), "r"(b_low), "r"(idesc), "r"(kApDescHigh), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void ap_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_low), "r"(idesc), "r"(kApDescHigh), "r"(accumulate)
         : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -104,13 +115,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-// Descriptor of the B operand of P V: V is stored [key][64 elements] with the 128-byte swizzle, so the MMA's N runs along
-// the contiguous dimension; 64-element column blocks lie 16 KB apart, groups of eight keys 1 KB.
-template <int D>
-__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr) {
-    return umma_desc_sw128(smem_addr) | (D > 64 ? (uint64_t)(16384u >> 4) << 16 : 0ull);
-}
-
 // ---- the line of work ----------------------------------------------------------
 // A unit: 2 * tpt consecutive tokens of a row for one kv head.
 struct ApRow {
@@ -184,9 +188,11 @@ __device__ __forceinline__ bool ap_segment(const ApParams& p, const ApLine& line
     s.x0 = c.x0;
     s.slot = 2 * cta + (c.x0 >= lo ? 1 : 0);  // 2 * cta: a unit that an earlier CTA began
     s.c0 = s.c1 = cta;
-    // (a unit may start in one share and have all its tiles in the next: its start is no whole tile away)
-    while (s.c0 > 0 && ap_share(line, s.c0) > c.x0) --s.c0;
-    while (s.c1 + 1 < line.ctas && ap_tile_at(ap_share(line, s.c1 + 1), c.x0, s.tiles) < s.tiles) ++s.c1;
+    // (a unit may start in one share and have all its tiles in the next)
+    if (c.x0 < lo)
+        while (s.c0 > 0 && ap_share(line, s.c0) > c.x0) --s.c0;
+    if (s.ks + s.cnt < s.tiles)
+        while (s.c1 + 1 < line.ctas && ap_tile_at(ap_share(line, s.c1 + 1), c.x0, s.tiles) < s.tiles) ++s.c1;
     return true;
 }
 // Next unit; false at the end of the batch.
@@ -215,7 +221,7 @@ struct ApSmem {
 struct ApTail {
     uint64_t full[kApStages], empty[kApStages];
     uint64_t q_full, q_empty, fix;
-    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], turn[2];
+    uint64_t s_full[2], p_full[2], o_full[2], o_empty[2], turn[2], h_full[2];
     uint64_t seg_full[kApSegments], seg_empty[kApSegments];
     ApSegment seg[kApSegments];
     uint32_t tmem;
@@ -223,60 +229,67 @@ struct ApTail {
     int last;  // this CTA joins the parts of the unit
     ApCursor start;
     long long warp_sum[kApThreads / 32];
-    int list[2 * 160];  // parts of a unit in the order of its keys: 2 * slot + tile, or -1
+    int parts;
+    int list[2 * 160];  // parts of a unit in the order of its keys: 2 * slot + tile
 };
 static_assert(sizeof(ApTail) <= 2048, "tail of the shared memory");
 
-// Joins the parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by 256 threads.  Not
-// inlined: its registers would be taken from the loop over the keys.
+// Joins the n parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by the 256 softmax
+// threads.  A thread keeps one row of the unit (rows rounded up to a power of two) and every (256 / rows)-th group of four
+// columns of it; what it loads of two parts at a time is on its way together.  Not inlined: its registers would be taken from
+// the loop over the keys.
 template <int D>
-__device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const int* list, int tid) {
+__device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const int* list, int n, int tid) {
     constexpr long long kPart = (long long)(D + 2) * 128;
-    // A thread keeps one row of the unit and every (256 / rows)-th group of four columns of it; rows rounded
-    // up to a power of two.  Eight groups are on their way at a time.
-    const int n_list = 2 * (seg.c1 - seg.c0 + 1), rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
-    const int log_rows = rows > 1 ? 32 - __clz(rows - 1) : 0, row = tid & ((1 << log_rows) - 1);
-    const int stride = 256 >> log_rows;
-    if (row < rows) {
-        const int q = row / per_tile, rr = row - q * per_tile;  // tile of the pair (dual: always 0) and row in it
-        const float* stat = p.parts + q * kPart + (long long)D * 128 + rr;
-        float top = -INFINITY, all = 0.f;
+    constexpr int W = 8;  // groups of columns at a time
+    const int rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
+    const int log_rows = rows > 1 ? 32 - __clz(rows - 1) : 0, row = tid & ((1 << log_rows) - 1), stride = 256 >> log_rows;
+    if (row >= rows) return;
+    const int q = row / per_tile, rr = row - q * per_tile;  // tile of the pair (one of keys: always 0) and row in it
+    const float* base = p.parts + q * kPart;
+    const float* stat = base + (long long)D * 128 + rr;
+    float top = -INFINITY, all = 0.f;
 #pragma unroll 4
-        for (int k = 0; k < n_list; ++k)
-            if (list[k] >= 0) top = fmaxf(top, __ldcg(stat + list[k] * kPart));
-        const int token = row / p.G, head = row - token * p.G;
-        const bool any = seg.sees + token > 0;  // else the query sees no key
-        bf16* out = p.Out + (long long)(seg.token + token) * p.ldo + (long long)(seg.head * p.G + head) * D;
+    for (int k = 0; k < n; ++k) top = fmaxf(top, __ldcg(stat + list[k] * kPart));
+    const int token = row / p.G, head = row - token * p.G;
+    const bool any = seg.sees + token > 0;  // else the query sees no key
+    bf16* out = p.Out + (long long)(seg.token + token) * p.ldo + (long long)(seg.head * p.G + head) * D;
 #pragma unroll 1
-        for (int g0 = tid >> log_rows; g0 < D / 4; g0 += 8 * stride) {
-            float4 acc[8];
+    for (int g0 = tid >> log_rows; g0 < D / 4; g0 += W * stride) {
+        float4 acc[W];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-            all = 0.f;
+        for (int e = 0; e < W; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        all = 0.f;
 #pragma unroll 1
-            for (int k = 0; k < n_list; ++k) {
-                const int id = list[k];
-                if (id < 0) continue;
-                const float4* part = reinterpret_cast<const float4*>(p.parts + (id + q) * kPart) + rr;
-                float4 o[8];
+        for (int k = 0; k < n; k += 2) {
+            float4 o[2][W];
+            float w[2], ps[2];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (g0 + e * stride < D / 4) o[e] = __ldcg(part + (g0 + e * stride) * 128);
-                const float pm = __ldcg(stat + id * kPart), ps = __ldcg(stat + id * kPart + 128);
-                const float w = pm == -INFINITY ? 0.f : exp2_approx((pm - top) * p.scale_log2);
-                all += w * ps;
+            for (int u = 0; u < 2; ++u) {
+                const long long at = list[min(k + u, n - 1)] * kPart;
+                const float4* part = reinterpret_cast<const float4*>(base + at) + rr;
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (g0 + e * stride < D / 4)
-                        acc[e].x += w * o[e].x, acc[e].y += w * o[e].y, acc[e].z += w * o[e].z, acc[e].w += w * o[e].w;
+                for (int e = 0; e < W; ++e)
+                    if (g0 + e * stride < D / 4) o[u][e] = __ldcg(part + (g0 + e * stride) * 128);
+                w[u] = __ldcg(stat + at), ps[u] = __ldcg(stat + at + 128);
             }
-            const float inv = 1.0f / all;
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (g0 + e * stride < D / 4)
-                    *reinterpret_cast<uint2*>(out + (g0 + e * stride) * 4) =
-                        any ? make_uint2(pack_bf16(acc[e].x * inv, acc[e].y * inv), pack_bf16(acc[e].z * inv, acc[e].w * inv)) : make_uint2(0u, 0u);
+            for (int u = 0; u < 2; ++u) {
+                const float f = w[u] == -INFINITY || k + u >= n ? 0.f : exp2_approx((w[u] - top) * p.scale_log2);
+                if (f == 0.f) continue;  // nothing of this part counts (its sums may be NaN only if f is not 0)
+                all += f * ps[u];
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    if (g0 + e * stride < D / 4)
+                        acc[e].x += f * o[u][e].x, acc[e].y += f * o[u][e].y, acc[e].z += f * o[u][e].z, acc[e].w += f * o[u][e].w;
+            }
         }
+        const float inv = 1.0f / all;
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+            if (g0 + e * stride < D / 4)
+                *reinterpret_cast<uint2*>(out + (g0 + e * stride) * 4) =
+                    any ? make_uint2(pack_bf16(acc[e].x * inv, acc[e].y * inv), pack_bf16(acc[e].z * inv, acc[e].w * inv)) : make_uint2(0u, 0u);
     }
 }
 
@@ -301,7 +314,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&t.s_full[i]), 1), mbar_init(smem_u32(&t.o_full[i]), 1);
             mbar_init(smem_u32(&t.p_full[i]), 4), mbar_init(smem_u32(&t.o_empty[i]), 4);  // one arrival per warp
-            mbar_init(smem_u32(&t.turn[i]), 4);
+            mbar_init(smem_u32(&t.turn[i]), 4), mbar_init(smem_u32(&t.h_full[i]), 4);
         }
         for (int i = 0; i < kApSegments; ++i)
             mbar_init(smem_u32(&t.seg_full[i]), 1), mbar_init(smem_u32(&t.seg_empty[i]), 10);  // warps that read it
@@ -398,9 +411,9 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         ++n_seg;
     };
 
-    // A softmax thread holds a row of scores: 384 threads x 168 registers at launch = 2 x 128 x 192 + 128 x 120.
+    // A softmax thread holds a row of scores: 384 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72.
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (idle) {
     } else if (warp == 10) {
         // ------------------------------------------------------------ work descriptors
@@ -510,30 +523,37 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                 return ok;
             };
             auto wait_stage = [&](int i) { return wait(&t.full[i % kApStages], (uint32_t)((i / kApStages) & 1)); };
+            const uint32_t q_low = ap_desc(sm_q), ring_low = ap_desc(sm_ring);
             auto scores = [&](int m, int q_tile, int i) {  // S[m] = Q K^T
-                const uint64_t a = umma_desc_sw128(sm_q + q_tile * L::kTile), b = umma_desc_sw128(sm_ring + (i % kApStages) * L::kTile);
+                const uint32_t a = q_low + q_tile * (L::kTile >> 4), b = ring_low + (i % kApStages) * (L::kTile >> 4);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const int off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-                    tc_mma_bf16(tmem + m * 128, a + off, b + off, IDESC_QK, k > 0);
+                    ap_mma_ss(tmem + m * 128, a + off, b + off, IDESC_QK, k > 0);
                 }
                 tc_commit(smem_u32(&t.s_full[m]));
             };
-            auto values = [&](int m, int i, bool fresh) {  // O[m] (+)= P V
-                const uint64_t b = umma_desc_sw128_mn<D>(sm_ring + (i % kApStages) * L::kTile);
+            // O[m] (+)= P V for one half of the keys.  V is stored [key][64 elements], so the MMA's N runs along the contiguous
+            // dimension; 64-element column blocks lie 16 KB apart (the stride in the descriptor), groups of eight keys 1 KB.
+            auto values = [&](int m, int i, bool fresh, int half) {
+                const uint32_t b = (ring_low + (i % kApStages) * (L::kTile >> 4) + half * (8192 >> 4)) | (D > 64 ? (16384u >> 4) << 16 : 0u);
 #pragma unroll
-                for (int k = 0; k < kApKeys / 16; ++k)
-                    tc_mma_bf16_ts(tmem + 256 + m * D, tmem + m * 128 + k * 8, b + k * (2048 >> 4), IDESC_PV, !(fresh && k == 0));
+                for (int k = 0; k < kApKeys / 32; ++k)
+                    ap_mma_ts(tmem + 256 + m * D, tmem + m * 128 + half * 32 + k * 8, b + k * (2048 >> 4), IDESC_PV, !(fresh && k == 0));
             };
             auto free_stage = [&](int i) { tc_commit(smem_u32(&t.empty[i % kApStages])); };
-            // P[m] is there, and for the first tile of a unit O[m] has been drained
-            auto wait_probabilities = [&](int m, bool fresh) {
-                if (!wait(&t.p_full[m], (tiles_seen >> m) & 1u)) return false;
-                tiles_seen ^= 1u << m;
+            // O[m] (+)= P[m] V as the halves of P come; for the first tile of a unit O[m] has to be drained first
+            auto add_values = [&](int m, int i, bool fresh, bool wait_v) {
+                if (!wait(&t.h_full[m], (tiles_seen >> m) & 1u)) return false;
                 if (fresh) {
                     if (!wait(&t.o_empty[m], ((units_seen >> m) & 1u) ^ 1u)) return false;
                     units_seen ^= 1u << m;
                 }
+                if (wait_v && !wait_stage(i)) return false;
+                values(m, i, fresh, 0);
+                if (!wait(&t.p_full[m], (tiles_seen >> m) & 1u)) return false;
+                tiles_seen ^= 1u << m;
+                values(m, i, false, 1);
                 return true;
             };
             while (const ApSegment* sp = next_segment()) {
@@ -555,9 +575,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                         const bool next = i + 1 < cnt;
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
-                            if (!wait_probabilities(m, i == 0)) break;
-                            if (m == 0 && !wait_stage(it)) break;
-                            values(m, it, i == 0);
+                            if (!add_values(m, it, i == 0, m == 0)) break;
                             if (m == 1) free_stage(it);
                             if (next) {
                                 if (m == 0 && !wait_stage(it + 1)) break;
@@ -583,9 +601,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
 #pragma unroll 1
                     for (int i = 0; i < cnt && !*abort_flag; ++i) {
                         const int m = i & 1;
-                        if (!wait_probabilities(m, i < 2)) break;
-                        if (!wait_stage(it)) break;
-                        values(m, it, i < 2);
+                        if (!add_values(m, it, i < 2, true)) break;
                         free_stage(it);
                         ++it;
                         if (i + 2 < cnt) {
@@ -603,7 +619,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         }
     }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     if (!idle) {
         // ------------------------------------------------------------ softmax, one row per thread
         const int m = warp >> 2;                                    // tile
@@ -686,10 +702,16 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                         w[e] = pack_bf16(x.x, x.y);
                     }
                     tmem_st16(t_s + c / 2, w);
-                }
-                if (!dual) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&t.turn[1 - m]));
+                    if (c == 32) {  // half of P is there: its products may start
+                        tmem_st_wait();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&t.h_full[m]));
+                    }
+                    if (c == 64 && !dual) {  // the rest of this tile and the start of the other one fill each other's gaps
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&t.turn[1 - m]));
+                    }
                 }
                 sum += (add[0].x + add[1].x) + (add[0].y + add[1].y);
                 tmem_st_wait();
@@ -762,17 +784,28 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                         if (t.last) p.count[seg.c0] = 0u;
                     }
                 }
-                const int c0 = seg.c0, c1 = seg.c1;
-                for (int c = c0 + tid; c <= c1; c += 256) {
-                    const int a = ap_tile_at(ap_share(line, c), seg.x0, seg.tiles), z = ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles);
-                    const int sl = 2 * (2 * c + (c == c0 ? 1 : 0));
-                    t.list[2 * (c - c0)] = a < z ? sl : -1;
-                    t.list[2 * (c - c0) + 1] = dual && z - a > 1 ? sl + 1 : -1;
+                if (warp == 0) {
+                    // the parts that there are, in the order of the keys: of every CTA from c0 to c1, dual: of both warpgroups
+                    int n = 0;
+                    for (int c0 = seg.c0; c0 <= seg.c1; c0 += 32) {
+                        const int c = c0 + lane;
+                        int tiles = 0;
+                        if (c <= seg.c1)
+                            tiles = whole ? (c == cta ? cnt : 0)
+                                          : ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles) - ap_tile_at(ap_share(line, c), seg.x0, seg.tiles);
+                        const uint32_t one = __ballot_sync(0xffffffffu, tiles > 0), two = __ballot_sync(0xffffffffu, dual && tiles > 1);
+                        const uint32_t below = (1u << lane) - 1u;
+                        const int at = n + __popc(one & below) + __popc(two & below), slot = 2 * (2 * c + (c == seg.c0 ? 1 : 0));
+                        if (tiles > 0) t.list[at] = slot;
+                        if (dual && tiles > 1) t.list[at + 1] = slot + 1;
+                        n += __popc(one) + __popc(two);
+                    }
+                    if (lane == 0) t.parts = n;
                 }
                 named_bar_sync(1, 256);
                 if (t.last && !*abort_flag) {
                     __threadfence();
-                    ap_join<D>(p, seg, t.list, tid);
+                    ap_join<D>(p, seg, t.list, t.parts, tid);
                 }
                 named_bar_sync(1, 256);  // the list and the flag are free again
             }
