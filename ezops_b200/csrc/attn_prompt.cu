@@ -39,6 +39,7 @@ struct ApParams {
     float* parts;        // [2 * grid slots][2 tiles][D + 2][128] fp32
     unsigned int* count;  // [grid], zero between calls
     int B, T, H, NKV, G, tpt, max_pages, page_shift, num_pages;
+    int out32;  // rows of Out start at 32-byte boundaries
     float scale_log2;  // log2(e) / sqrt(D)
     unsigned int* status;
 };
@@ -49,6 +50,19 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
+}
+__device__ __forceinline__ void store32(void* dst, const uint32_t (&w)[8]) {  // 32 bytes at a 32-byte boundary: a whole sector
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+__device__ __forceinline__ void store_row16(bf16* dst, const uint32_t (&w)[8], bool whole_sector) {  // 16 elements
+    if (whole_sector) {
+        store32(dst, w);
+    } else {
+        reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
 }
 // Operand descriptors as halves: the low word holds the address (and the column block stride), the high word is one constant
 // for all 128-byte-swizzled tiles (see umma_desc_sw128), so that only 32 bits a tile have to be kept.
@@ -235,31 +249,31 @@ struct ApTail {
 static_assert(sizeof(ApTail) <= 2048, "tail of the shared memory");
 
 // Joins the n parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by the 256 softmax
-// threads.  A thread keeps one row of the unit (rows rounded up to a power of two) and every (256 / rows)-th group of four
-// columns of it; what it loads of two parts at a time is on its way together.  Not inlined: its registers would be taken from
-// the loop over the keys.
-template <int D>
+// threads.  A thread keeps one row of the unit (rows rounded up to a power of two) and D / (256 / rows) neighbouring columns of
+// it, 16 at a time (4 when there are few rows); what it loads of two parts is on its way together.  Not inlined: its registers
+// would be taken from the loop over the keys.
+template <int D, int W>  // W groups of four columns at a time
 __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const int* list, int n, int tid) {
     constexpr long long kPart = (long long)(D + 2) * 128;
-    constexpr int W = 8;  // groups of columns at a time
     const int rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
-    const int log_rows = rows > 1 ? 32 - __clz(rows - 1) : 0, row = tid & ((1 << log_rows) - 1), stride = 256 >> log_rows;
+    const int log_rows = rows > 1 ? 32 - __clz(rows - 1) : 0, row = tid & ((1 << log_rows) - 1), share = 256 >> log_rows;
     if (row >= rows) return;
     const int q = row / per_tile, rr = row - q * per_tile;  // tile of the pair (one of keys: always 0) and row in it
     const float* base = p.parts + q * kPart;
     const float* stat = base + (long long)D * 128 + rr;
-    float top = -INFINITY, all = 0.f;
+    float top = -INFINITY;
 #pragma unroll 4
     for (int k = 0; k < n; ++k) top = fmaxf(top, __ldcg(stat + list[k] * kPart));
     const int token = row / p.G, head = row - token * p.G;
     const bool any = seg.sees + token > 0;  // else the query sees no key
     bf16* out = p.Out + (long long)(seg.token + token) * p.ldo + (long long)(seg.head * p.G + head) * D;
+    const int per = max(W, D / 4 / share);  // groups of this thread
 #pragma unroll 1
-    for (int g0 = tid >> log_rows; g0 < D / 4; g0 += W * stride) {
+    for (int g0 = (tid >> log_rows) * per, g1 = min(g0 + per, D / 4); g0 < g1; g0 += W) {
         float4 acc[W];
 #pragma unroll
         for (int e = 0; e < W; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-        all = 0.f;
+        float all = 0.f;
 #pragma unroll 1
         for (int k = 0; k < n; k += 2) {
             float4 o[2][W];
@@ -269,27 +283,26 @@ __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, co
                 const long long at = list[min(k + u, n - 1)] * kPart;
                 const float4* part = reinterpret_cast<const float4*>(base + at) + rr;
 #pragma unroll
-                for (int e = 0; e < W; ++e)
-                    if (g0 + e * stride < D / 4) o[u][e] = __ldcg(part + (g0 + e * stride) * 128);
+                for (int e = 0; e < W; ++e) o[u][e] = __ldcg(part + (g0 + e) * 128);
                 w[u] = __ldcg(stat + at), ps[u] = __ldcg(stat + at + 128);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const float f = w[u] == -INFINITY || k + u >= n ? 0.f : exp2_approx((w[u] - top) * p.scale_log2);
-                if (f == 0.f) continue;  // nothing of this part counts (its sums may be NaN only if f is not 0)
                 all += f * ps[u];
 #pragma unroll
-                for (int e = 0; e < W; ++e)
-                    if (g0 + e * stride < D / 4)
-                        acc[e].x += f * o[u][e].x, acc[e].y += f * o[u][e].y, acc[e].z += f * o[u][e].z, acc[e].w += f * o[u][e].w;
+                for (int e = 0; e < W; ++e) acc[e].x += f * o[u][e].x, acc[e].y += f * o[u][e].y, acc[e].z += f * o[u][e].z, acc[e].w += f * o[u][e].w;
             }
         }
         const float inv = 1.0f / all;
+        uint32_t w[2 * W];
 #pragma unroll
-        for (int e = 0; e < W; ++e)
-            if (g0 + e * stride < D / 4)
-                *reinterpret_cast<uint2*>(out + (g0 + e * stride) * 4) =
-                    any ? make_uint2(pack_bf16(acc[e].x * inv, acc[e].y * inv), pack_bf16(acc[e].z * inv, acc[e].w * inv)) : make_uint2(0u, 0u);
+        for (int e = 0; e < W; ++e) {
+            w[2 * e] = any ? pack_bf16(acc[e].x * inv, acc[e].y * inv) : 0u;
+            w[2 * e + 1] = any ? pack_bf16(acc[e].z * inv, acc[e].w * inv) : 0u;
+        }
+        if constexpr (W == 4) store_row16(out + g0 * 4, w, p.out32);
+        else *reinterpret_cast<uint2*>(out + g0 * 4) = make_uint2(w[0], w[1]);
     }
 }
 
@@ -741,10 +754,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                     uint32_t w[8];
 #pragma unroll
                     for (int q = 0; q < 8; ++q) w[q] = limit > 0 ? pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
-                    if (store) {
-                        *reinterpret_cast<uint4*>(out + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4*>(out + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
+                    if (store) store_row16(out + c, w, p.out32);
                     __syncwarp();
                 }
                 if (mine) {
@@ -805,7 +815,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                 named_bar_sync(1, 256);
                 if (t.last && !*abort_flag) {
                     __threadfence();
-                    ap_join<D>(p, seg, t.list, t.parts, tid);
+                    if (seg.tokens * p.G > 32) ap_join<D, 4>(p, seg, t.list, t.parts, tid);
+                    else ap_join<D, 1>(p, seg, t.list, t.parts, tid);
                 }
                 named_bar_sync(1, 256);  // the list and the flag are free again
             }
@@ -865,6 +876,7 @@ cudaError_t launch_attn_prompt(const AttnPromptArgs& a, cudaStream_t stream) {
     p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + kApMaxGrid * 4);
     p.B = a.B, p.T = a.T, p.H = a.H, p.NKV = a.NKV, p.G = a.H / a.NKV, p.tpt = 128 / p.G;
     p.max_pages = a.max_pages, p.page_shift = a.page_shift, p.num_pages = a.num_pages;
+    p.out32 = (reinterpret_cast<uintptr_t>(a.Out) & 31u) == 0 && a.ldo % 16 == 0;
     p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)a.D));
     p.status = status_ptr();
     if (!p.status) return cudaErrorUnknown;
