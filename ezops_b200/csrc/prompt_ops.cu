@@ -164,12 +164,19 @@ struct PagedRopeParams {
     unsigned char axis[128];  // axis of frequency i
 };
 
+static constexpr int kRopeSteps = 8;  // heads per lane
+__device__ __forceinline__ uint4 ld_stream16(const bf16* p) {  // read once
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 template <int D>
-__global__ void __launch_bounds__(256) paged_qk_norm_rope_kernel(const __grid_constant__ PagedRopeParams p) {
+__global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_constant__ PagedRopeParams p) {
     constexpr int LPH = D / 8, HPW = 32 / LPH;  // lanes per head, heads per warp
     pdl_open(1);
     const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int t = (int)(unit / p.chunks), chunk = (int)(unit - (long long)t * p.chunks);
     if (t >= p.T) return;
     const int sub = lane & (LPH - 1);             // 16-byte piece of the head
@@ -177,6 +184,13 @@ __global__ void __launch_bounds__(256) paged_qk_norm_rope_kernel(const __grid_co
     const int f0 = (sub & (LPH / 2 - 1)) * 8;     // first frequency of this lane
     const int heads = p.H + 2 * p.NKV;
 
+    // Everything that does not depend on the position is requested together with it: the heads, the weights, the slot.
+    const int h0 = chunk * p.steps * HPW + lane / LPH;
+    const bf16* src = p.qkv + (long long)t * p.ld + (long long)h0 * D + sub * 8;
+    uint4 x[kRopeSteps];
+#pragma unroll
+    for (int u = 0; u < kRopeSteps; ++u)
+        if (u < p.steps && h0 + u * HPW < heads) x[u] = ld_stream16(src + u * HPW * D);
     int pos[3];
     bool real = true, inside = true;
 #pragma unroll
@@ -186,6 +200,9 @@ __global__ void __launch_bounds__(256) paged_qk_norm_rope_kernel(const __grid_co
         inside = inside && pos[a] < p.S;
     }
     const int slot = __ldg(p.slots + t);
+    const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
+    const uint4 qw = p.qw ? __ldg(reinterpret_cast<const uint4*>(p.qw) + sub) : one;
+    const uint4 kw = p.kw ? __ldg(reinterpret_cast<const uint4*>(p.kw) + sub) : one;
     if (!real) return;  // a padded token: nothing is written
     if (!inside) {
         if (lane == 0) report_fault(p.status, FAULT_ROPE_POSITION);
@@ -196,45 +213,36 @@ __global__ void __launch_bounds__(256) paged_qk_norm_rope_kernel(const __grid_co
 
     // Table rows: the lane's 8 columns of every axis, then the axis of each frequency picks.
     float c[8], s[8];
+    if (chunk * p.steps * HPW < p.H + p.NKV) {  // a warp with v heads only copies
 #pragma unroll
-    for (int a = 0; a < 3; ++a) {
-        if (a < p.axes) {
-            const uint4 cv = __ldg(reinterpret_cast<const uint4*>(p.cos + (long long)pos[a] * D + sub * 8));
-            const uint4 sv = __ldg(reinterpret_cast<const uint4*>(p.sin + (long long)pos[a] * D + sub * 8));
-            const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+        for (int a = 0; a < 3; ++a) {
+            if (a < p.axes) {
+                const uint4 cv = __ldg(reinterpret_cast<const uint4*>(p.cos + (long long)pos[a] * D + sub * 8));
+                const uint4 sv = __ldg(reinterpret_cast<const uint4*>(p.sin + (long long)pos[a] * D + sub * 8));
+                const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (a == 0 || p.axis[f0 + e] == a) {
-                    c[e] = (e & 1) ? bf16_hi(cw[e / 2]) : bf16_lo(cw[e / 2]);
-                    s[e] = (e & 1) ? bf16_hi(sw[e / 2]) : bf16_lo(sw[e / 2]);
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (a == 0 || p.axis[f0 + e] == a) {
+                        c[e] = (e & 1) ? bf16_hi(cw[e / 2]) : bf16_lo(cw[e / 2]);
+                        s[e] = (e & 1) ? bf16_hi(sw[e / 2]) : bf16_lo(sw[e / 2]);
+                    }
+            }
+        }
+        if (!upper) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = -s[e];
         }
     }
-    if (!upper) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = -s[e];
-    }
-    const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-    const uint4 qw = p.qw ? __ldg(reinterpret_cast<const uint4*>(p.qw) + sub) : one;
-    const uint4 kw = p.kw ? __ldg(reinterpret_cast<const uint4*>(p.kw) + sub) : one;
     const long long page = slot >> p.page_shift, off = slot & ((1 << p.page_shift) - 1);
-
-    const int h0 = chunk * p.steps * HPW + lane / LPH;
-    const bf16* src = p.qkv + (long long)t * p.ld + (long long)h0 * D + sub * 8;
-    constexpr int U = 4;  // heads in flight per lane
-    for (int i = 0; i < p.steps; i += U) {
-        uint4 x[U];
+    bf16* q_row = p.q_out + (long long)t * p.H * D + sub * 8;
+    const long long kv_row = ((page * p.NKV) << p.page_shift) + off;  // + kv head * page size
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + (i + u) * HPW;
-            x[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (i + u < p.steps && h < heads) x[u] = *reinterpret_cast<const uint4*>(src + (long long)(i + u) * HPW * D);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = h0 + (i + u) * HPW;
-            const bool live = i + u < p.steps && h < heads;
-            const bool is_v = h >= p.H + p.NKV, is_q = h < p.H;
+    for (int u = 0; u < kRopeSteps; ++u) {
+        if (u >= p.steps) break;
+        const int h = h0 + u * HPW;
+        const bool live = h < heads, is_v = h >= p.H + p.NKV, is_q = h < p.H;
+        uint4 out = x[u];
+        if ((chunk * p.steps + u) * HPW < p.H + p.NKV) {  // the same for the whole warp
             const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
             float v[8], ssq = 0.f;
 #pragma unroll
@@ -254,15 +262,13 @@ __global__ void __launch_bounds__(256) paged_qk_norm_rope_kernel(const __grid_co
                 const float other = __shfl_xor_sync(0xffffffffu, v[e], LPH / 2);
                 y[e] = __fadd_rn(__fmul_rn(v[e], c[e]), __fmul_rn(other, s[e]));
             }
-            uint4 out = x[u];
             if (!is_v) out = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-            if (live && is_q)
-                *reinterpret_cast<uint4*>(p.q_out + ((long long)t * p.H + h) * D + sub * 8) = out;
-            else if (live && cached) {
-                bf16* pool = is_v ? p.V : p.K;
-                const int kh = h - p.H - (is_v ? p.NKV : 0);
-                *reinterpret_cast<uint4*>(pool + (((page * p.NKV + kh) << p.page_shift) + off) * D + sub * 8) = out;
-            }
+        }
+        if (live && is_q) {
+            *reinterpret_cast<uint4*>(q_row + (long long)h * D) = out;
+        } else if (live && cached) {
+            const long long row = kv_row + ((long long)(h - p.H - (is_v ? p.NKV : 0)) << p.page_shift);
+            *reinterpret_cast<uint4*>((is_v ? p.V : p.K) + row * D + sub * 8) = out;
         }
     }
 }
@@ -280,12 +286,12 @@ cudaError_t launch_paged_qk_norm_rope(const PagedRopeArgs& a, cudaStream_t strea
     const int per_warp = 32 / (a.D / 8), groups = (a.H + 2 * a.NKV + per_warp - 1) / per_warp;
     const long long fill = (long long)sm_count() * 32;
     p.steps = 1;
-    while (p.steps < 8 && (long long)a.T * ((groups + 2 * p.steps - 1) / (2 * p.steps)) >= fill) p.steps *= 2;
+    while (p.steps < kRopeSteps && (long long)a.T * ((groups + 2 * p.steps - 1) / (2 * p.steps)) >= fill) p.steps *= 2;
     p.chunks = (groups + p.steps - 1) / p.steps;
     const long long warps = (long long)a.T * p.chunks;
     chain_begin();
-    if (a.D == 64) return launch_pdl(paged_qk_norm_rope_kernel<64>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
-    return launch_pdl(paged_qk_norm_rope_kernel<128>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, stream, p);
+    if (a.D == 64) return launch_pdl(paged_qk_norm_rope_kernel<64>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p);
+    return launch_pdl(paged_qk_norm_rope_kernel<128>, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, stream, p);
 }
 
 }  // namespace ezb
