@@ -28,7 +28,7 @@ struct LtParams {
     long long ldres, ldout;
     int M, N, kblocks;
     int tiles_m, tiles_n, stages, act, out_f32;
-    int vec_out, vec_res, vec_bias;  // rows allow 16-byte accesses
+    int vec_out, vec_res, vec_bias;  // rows start at 32-byte (out) or 16-byte boundaries
     unsigned int* status;
 };
 
@@ -76,20 +76,20 @@ struct LtSmem {
     static constexpr int kBytes = 1024 + kStages * kStage + kTail;
 };
 
-// Result rows leave in pieces of 16 columns per thread (32 or 64 contiguous bytes).
+// W bf16 values, as they are; beyond `left` zeros.
 template <int W>
-__device__ __forceinline__ void load_bf16(const bf16* src, int left, int vec, float (&v)[W]) {
+__device__ __forceinline__ void load_packed(const bf16* src, int left, int vec, uint32_t (&w)[W / 2]) {
     if (vec && left >= W) {
 #pragma unroll
-        for (int e = 0; e < W; e += 8) {
-            const uint4 q = __ldg(reinterpret_cast<const uint4*>(src + e));
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[e + 2 * i] = bf16_lo(w[i]), v[e + 2 * i + 1] = bf16_hi(w[i]);
+        for (int e = 0; e < W / 2; e += 4) {
+            const uint4 q = *reinterpret_cast<const uint4*>(src + 2 * e);
+            w[e] = q.x, w[e + 1] = q.y, w[e + 2] = q.z, w[e + 3] = q.w;
         }
     } else {
+        const unsigned short* raw = reinterpret_cast<const unsigned short*>(src);
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = e < left ? __bfloat162float(src[e]) : 0.f;
+        for (int e = 0; e < W / 2; ++e)
+            w[e] = (2 * e < left ? raw[2 * e] : 0u) | (2 * e + 1 < left ? (uint32_t)raw[2 * e + 1] << 16 : 0u);
     }
 }
 
@@ -175,6 +175,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             }
         }
     } else {
+        // A warp of the quarter of rows that it may read; W columns at a time.  What the residual stream holds there is requested
+        // one step ahead (the first step: before the products are complete), or its latency would be paid once per step.
+        constexpr int W = 32;
         const int q = warp & 3, row = q * 32 + lane;
         int n = 0;
         for (int i = blockIdx.x >> 1; i < n_tiles; i += n_clusters, ++n) {
@@ -185,62 +188,71 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             const bool live_row = m < p.M;
             const int n0 = tn * UNITS;
             const int cols = min(UNITS, p.N - n0);
+            const bf16* res_row = p.residual ? p.residual + (long long)m * p.ldres + n0 : nullptr;
+            uint32_t ahead[W / 2];  // residual values of the next step, packed
+            if (res_row && live_row) load_packed<W>(res_row, cols, p.vec_res, ahead);
             mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             tc_fence_after();
             const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * BN;
-            constexpr int W = 16;  // columns at a time
 #pragma unroll 1
             for (int c = 0; c < cols; c += W) {
-                float v[W], up[W];
-                tmem_ld16(t + c, v);
-                if (PAIR) tmem_ld16(t + UNITS + c, up);
+                float v[W], up[PAIR ? W : 1];
+                tmem_ld32(t + c, v);
+                if constexpr (PAIR) tmem_ld32(t + UNITS + c, up);
                 const int left = cols - c, col = n0 + c;
-                float res[W];
-                if (p.residual && live_row) load_bf16<W>(p.residual + (long long)m * p.ldres + col, left, p.vec_res, res);
+                uint32_t res[W / 2];
+                if (res_row) {
+#pragma unroll
+                    for (int e = 0; e < W / 2; ++e) res[e] = ahead[e];
+                    if (live_row && left > W) load_packed<W>(res_row + c + W, left - W, p.vec_res, ahead);
+                }
                 tmem_ld_wait();
                 if (live_row && !*abort_flag) {
                     if (p.bias) {
-                        float b[W];
-                        load_bf16<W>(p.bias + col, left, p.vec_bias, b);
-    #pragma unroll
-                        for (int e = 0; e < W; ++e) v[e] += b[e];
-                        if (PAIR) {
-                            load_bf16<W>(p.bias + p.N + col, left, p.vec_bias, b);
-    #pragma unroll
-                            for (int e = 0; e < W; ++e) up[e] += b[e];
+                        uint32_t b[W / 2];
+                        load_packed<W>(p.bias + col, left, p.vec_bias, b);
+#pragma unroll
+                        for (int e = 0; e < W; ++e) v[e] += (e & 1) ? bf16_hi(b[e / 2]) : bf16_lo(b[e / 2]);
+                        if constexpr (PAIR) {
+                            load_packed<W>(p.bias + p.N + col, left, p.vec_bias, b);
+#pragma unroll
+                            for (int e = 0; e < W; ++e) up[e] += (e & 1) ? bf16_hi(b[e / 2]) : bf16_lo(b[e / 2]);
                         }
                     }
-                    if (PAIR) {
-    #pragma unroll
+                    if constexpr (PAIR) {
+#pragma unroll
                         for (int e = 0; e < W; ++e) v[e] = silu_f32(v[e]) * up[e];
                     } else if (p.act != ACT_NONE) {
-    #pragma unroll
+#pragma unroll
                         for (int e = 0; e < W; ++e) v[e] = linear_act(v[e], p.act);
                     }
-                    if (p.residual) {
-    #pragma unroll
-                        for (int e = 0; e < W; ++e) v[e] += res[e];
+                    if (res_row) {
+#pragma unroll
+                        for (int e = 0; e < W; ++e) v[e] += (e & 1) ? bf16_hi(res[e / 2]) : bf16_lo(res[e / 2]);
                     }
                     const long long o = (long long)m * p.ldout + col;
                     if (p.out_f32) {
                         float* dst = static_cast<float*>(p.out) + o;
                         if (p.vec_out && left >= W) {
-    #pragma unroll
-                            for (int e = 0; e < W; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+#pragma unroll
+                            for (int e = 0; e < W; e += 8) store32(dst + e, reinterpret_cast<const uint32_t(&)[8]>(v[e]));
                         } else {
-    #pragma unroll
+#pragma unroll
                             for (int e = 0; e < W; ++e)
                                 if (e < left) dst[e] = v[e];
                         }
                     } else {
                         bf16* dst = static_cast<bf16*>(p.out) + o;
                         if (p.vec_out && left >= W) {
-    #pragma unroll
-                            for (int e = 0; e < W; e += 8)
-                                *reinterpret_cast<uint4*>(dst + e) =
-                                    make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]), pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
+#pragma unroll
+                            for (int e = 0; e < W; e += 16) {
+                                uint32_t w[8];
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) w[k] = pack_bf16(v[e + 2 * k], v[e + 2 * k + 1]);
+                                store32(dst + e, w);
+                            }
                         } else {
-    #pragma unroll
+#pragma unroll
                             for (int e = 0; e < W; ++e)
                                 if (e < left) dst[e] = __float2bfloat16_rn(v[e]);
                         }
@@ -297,8 +309,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
     p.bias = a.bias, p.residual = a.residual, p.out = a.out, p.ldres = a.ldres, p.ldout = a.ldout;
     p.M = a.M, p.N = a.N, p.kblocks = (a.K + kLtBlockK - 1) / kLtBlockK;
     p.act = a.act, p.out_f32 = a.out_f32;
-    const int per16 = a.out_f32 ? 4 : 8;
-    p.vec_out = aligned16(a.out) && a.ldout % per16 == 0;
+    p.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.ldout % (a.out_f32 ? 8 : 16) == 0;
     p.vec_res = a.residual && aligned16(a.residual) && a.ldres % 8 == 0;
     p.vec_bias = a.bias && aligned16(a.bias) && (a.act != ACT_SWIGLU || a.N % 8 == 0);
     p.status = status_ptr();

@@ -147,8 +147,8 @@ cudaError_t launch_paged_plan(const PlanArgs& a, cudaStream_t stream) {
 //   y_i = n_i cos[p, i] - n_{i+D/2} sin[p, i],   y_{i+D/2} = n_{i+D/2} cos[p, i+D/2] + n_i sin[p, i+D/2]
 // in fp32 with one rounding, as the stand-alone operator of a decode step and the decode attention do.
 // What bounds it: HBM for prompts (every head is read and written once), latency for a handful of tokens.  A head is
-// D/8 lanes of 16 bytes, so a warp moves 32 * 16 bytes per access; the partner of a rotation sits D/16 lanes away (one
-// shuffle per element).  A warp keeps the cos and sin values of ONE token in registers for all the heads it walks; how many
+// D/8 lanes, each with four elements of its first half and their partners in the second, so that a rotation stays inside a
+// lane, and two elements share an instruction.  A warp keeps the cos and sin values of ONE token in registers for all the heads it walks; how many
 // that are (`steps`) follows from the number of tokens: one group of heads per warp while there are fewer warps than the
 // chip holds, more when the table rows would otherwise be fetched again for every group.
 struct PagedRopeParams {
@@ -165,9 +165,9 @@ struct PagedRopeParams {
 };
 
 static constexpr int kRopeSteps = 8;  // heads per lane
-__device__ __forceinline__ uint4 ld_stream16(const bf16* p) {  // read once
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+__device__ __forceinline__ uint2 ld_stream8(const bf16* p) {  // read once
+    uint2 v;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
     return v;
 }
 
@@ -179,18 +179,16 @@ __global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_co
     const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
     const int t = (int)(unit / p.chunks), chunk = (int)(unit - (long long)t * p.chunks);
     if (t >= p.T) return;
-    const int sub = lane & (LPH - 1);             // 16-byte piece of the head
-    const bool upper = sub >= LPH / 2;            // second half of the head
-    const int f0 = (sub & (LPH / 2 - 1)) * 8;     // first frequency of this lane
+    const int f0 = (lane & (LPH - 1)) * 4;  // first frequency of this lane: it holds the elements f0.. and D/2 + f0..
     const int heads = p.H + 2 * p.NKV;
 
     // Everything that does not depend on the position is requested together with it: the heads, the weights, the slot.
     const int h0 = chunk * p.steps * HPW + lane / LPH;
-    const bf16* src = p.qkv + (long long)t * p.ld + (long long)h0 * D + sub * 8;
-    uint4 x[kRopeSteps];
+    const bf16* src = p.qkv + (long long)t * p.ld + (long long)h0 * D + f0;
+    uint2 lo[kRopeSteps], hi[kRopeSteps];
 #pragma unroll
     for (int u = 0; u < kRopeSteps; ++u)
-        if (u < p.steps && h0 + u * HPW < heads) x[u] = ld_stream16(src + u * HPW * D);
+        if (u < p.steps && h0 + u * HPW < heads) lo[u] = ld_stream8(src + u * HPW * D), hi[u] = ld_stream8(src + u * HPW * D + D / 2);
     int pos[3];
     bool real = true, inside = true;
 #pragma unroll
@@ -200,9 +198,9 @@ __global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_co
         inside = inside && pos[a] < p.S;
     }
     const int slot = __ldg(p.slots + t);
-    const uint4 one = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-    const uint4 qw = p.qw ? __ldg(reinterpret_cast<const uint4*>(p.qw) + sub) : one;
-    const uint4 kw = p.kw ? __ldg(reinterpret_cast<const uint4*>(p.kw) + sub) : one;
+    const uint2 one = make_uint2(0x3f803f80u, 0x3f803f80u);
+    auto weights = [&](const bf16* w, int at) { return w ? __ldg(reinterpret_cast<const uint2*>(w + at)) : one; };
+    const uint2 qw1 = weights(p.qw, f0), qw2 = weights(p.qw, D / 2 + f0), kw1 = weights(p.kw, f0), kw2 = weights(p.kw, D / 2 + f0);
     if (!real) return;  // a padded token: nothing is written
     if (!inside) {
         if (lane == 0) report_fault(p.status, FAULT_ROPE_POSITION);
@@ -211,64 +209,67 @@ __global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_co
     const bool cached = slot >= 0 && slot < p.n_slots;
     if (slot >= p.n_slots && lane == 0) report_fault(p.status, FAULT_SLOT_RANGE);
 
-    // Table rows: the lane's 8 columns of every axis, then the axis of each frequency picks.
-    float c[8], s[8];
+    // Table rows: the lane's columns of every axis, then the axis of each frequency picks.  [0]: first half, [1]: second half.
+    auto unpack = [](const uint2& v, float2 (&x)[2]) {
+        x[0] = make_float2(bf16_lo(v.x), bf16_hi(v.x)), x[1] = make_float2(bf16_lo(v.y), bf16_hi(v.y));
+    };
+    float2 c1[2], c2[2], s1[2], s2[2];
     if (chunk * p.steps * HPW < p.H + p.NKV) {  // a warp with v heads only copies
 #pragma unroll
         for (int a = 0; a < 3; ++a) {
             if (a < p.axes) {
-                const uint4 cv = __ldg(reinterpret_cast<const uint4*>(p.cos + (long long)pos[a] * D + sub * 8));
-                const uint4 sv = __ldg(reinterpret_cast<const uint4*>(p.sin + (long long)pos[a] * D + sub * 8));
-                const uint32_t cw[4] = {cv.x, cv.y, cv.z, cv.w}, sw[4] = {sv.x, sv.y, sv.z, sv.w};
+                const bf16 *cr = p.cos + (long long)pos[a] * D + f0, *sr = p.sin + (long long)pos[a] * D + f0;
+                float2 x[4][2];
+                unpack(__ldg(reinterpret_cast<const uint2*>(cr)), x[0]), unpack(__ldg(reinterpret_cast<const uint2*>(cr + D / 2)), x[1]);
+                unpack(__ldg(reinterpret_cast<const uint2*>(sr)), x[2]), unpack(__ldg(reinterpret_cast<const uint2*>(sr + D / 2)), x[3]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (a == 0 || p.axis[f0 + e] == a) {
-                        c[e] = (e & 1) ? bf16_hi(cw[e / 2]) : bf16_lo(cw[e / 2]);
-                        s[e] = (e & 1) ? bf16_hi(sw[e / 2]) : bf16_lo(sw[e / 2]);
-                    }
+                for (int e = 0; e < 2; ++e) {
+                    if (a == 0 || p.axis[f0 + 2 * e] == a) c1[e].x = x[0][e].x, c2[e].x = x[1][e].x, s1[e].x = -x[2][e].x, s2[e].x = x[3][e].x;
+                    if (a == 0 || p.axis[f0 + 2 * e + 1] == a) c1[e].y = x[0][e].y, c2[e].y = x[1][e].y, s1[e].y = -x[2][e].y, s2[e].y = x[3][e].y;
+                }
             }
-        }
-        if (!upper) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = -s[e];
         }
     }
     const long long page = slot >> p.page_shift, off = slot & ((1 << p.page_shift) - 1);
-    bf16* q_row = p.q_out + (long long)t * p.H * D + sub * 8;
+    bf16* q_row = p.q_out + (long long)t * p.H * D + f0;
     const long long kv_row = ((page * p.NKV) << p.page_shift) + off;  // + kv head * page size
 #pragma unroll
     for (int u = 0; u < kRopeSteps; ++u) {
         if (u >= p.steps) break;
         const int h = h0 + u * HPW;
         const bool live = h < heads, is_v = h >= p.H + p.NKV, is_q = h < p.H;
-        uint4 out = x[u];
+        uint2 out1 = lo[u], out2 = hi[u];
         if ((chunk * p.steps + u) * HPW < p.H + p.NKV) {  // the same for the whole warp
-            const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-            float v[8], ssq = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (e & 1) ? bf16_hi(xw[e / 2]) : bf16_lo(xw[e / 2]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ssq += v[e] * v[e];
+            float2 a[2], b[2], w1[2], w2[2];
+            unpack(lo[u], a), unpack(hi[u], b);
+            unpack(is_q ? qw1 : kw1, w1), unpack(is_q ? qw2 : kw2, w2);
+            float2 sq = mul2(a[0], a[0]);
+            sq = fma2(a[1], a[1], sq), sq = fma2(b[0], b[0], sq), sq = fma2(b[1], b[1], sq);
+            float ssq = sq.x + sq.y;
 #pragma unroll
             for (int o = LPH / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-            const float r = 1.0f / sqrtf(ssq * (1.0f / D) + p.eps);
-            const uint4 wv = is_q ? qw : kw;
-            const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
-            float y[8];
+            const float r = rsqrtf(ssq * (1.0f / D) + p.eps);
+            const float2 r2 = make_float2(r, r);
+            float2 y1[2], y2[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = v[e] * r * ((e & 1) ? bf16_hi(ww[e / 2]) : bf16_lo(ww[e / 2]));
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float other = __shfl_xor_sync(0xffffffffu, v[e], LPH / 2);
-                y[e] = __fadd_rn(__fmul_rn(v[e], c[e]), __fmul_rn(other, s[e]));
+            for (int e = 0; e < 2; ++e) {
+                const float2 n1 = mul2(mul2(a[e], r2), w1[e]), n2 = mul2(mul2(b[e], r2), w2[e]);
+                y1[e] = add2(mul2(n1, c1[e]), mul2(n2, s1[e]));
+                y2[e] = add2(mul2(n2, c2[e]), mul2(n1, s2[e]));
             }
-            if (!is_v) out = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+            if (!is_v) {
+                out1 = make_uint2(pack_bf16(y1[0].x, y1[0].y), pack_bf16(y1[1].x, y1[1].y));
+                out2 = make_uint2(pack_bf16(y2[0].x, y2[0].y), pack_bf16(y2[1].x, y2[1].y));
+            }
         }
-        if (live && is_q) {
-            *reinterpret_cast<uint4*>(q_row + (long long)h * D) = out;
-        } else if (live && cached) {
+        bf16* dst = q_row + (long long)h * D;
+        if (!is_q) {
             const long long row = kv_row + ((long long)(h - p.H - (is_v ? p.NKV : 0)) << p.page_shift);
-            *reinterpret_cast<uint4*>((is_v ? p.V : p.K) + row * D + sub * 8) = out;
+            dst = (is_v ? p.V : p.K) + row * D + f0;
+        }
+        if (live && (is_q || cached)) {
+            *reinterpret_cast<uint2*>(dst) = out1;
+            *reinterpret_cast<uint2*>(dst + D / 2) = out2;
         }
     }
 }
