@@ -161,10 +161,10 @@ struct PagedRopeParams {
     long long n_slots;
     float eps;
     unsigned int* status;
-    unsigned char axis[128];  // axis of frequency i
+    alignas(4) unsigned char axis[64];  // axis of frequency i
 };
 
-static constexpr int kRopeSteps = 8;  // heads per lane
+static constexpr int kRopeBatch = 4;  // heads in flight per lane
 __device__ __forceinline__ uint2 ld_stream8(const bf16* p) {  // read once
     uint2 v;
     asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
@@ -172,7 +172,7 @@ __device__ __forceinline__ uint2 ld_stream8(const bf16* p) {  // read once
 }
 
 template <int D>
-__global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_constant__ PagedRopeParams p) {
+__global__ void __launch_bounds__(128, 7) paged_qk_norm_rope_kernel(const __grid_constant__ PagedRopeParams p) {
     constexpr int LPH = D / 8, HPW = 32 / LPH;  // lanes per head, heads per warp
     pdl_open(1);
     const int lane = threadIdx.x & 31;
@@ -185,10 +185,14 @@ __global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_co
     // Everything that does not depend on the position is requested together with it: the heads, the weights, the slot.
     const int h0 = chunk * p.steps * HPW + lane / LPH;
     const bf16* src = p.qkv + (long long)t * p.ld + (long long)h0 * D + f0;
-    uint2 lo[kRopeSteps], hi[kRopeSteps];
+    uint2 lo[kRopeBatch], hi[kRopeBatch];
+    auto load = [&](int i) {
 #pragma unroll
-    for (int u = 0; u < kRopeSteps; ++u)
-        if (u < p.steps && h0 + u * HPW < heads) lo[u] = ld_stream8(src + u * HPW * D), hi[u] = ld_stream8(src + u * HPW * D + D / 2);
+        for (int u = 0; u < kRopeBatch; ++u)
+            if (i + u < p.steps && h0 + (i + u) * HPW < heads)
+                lo[u] = ld_stream8(src + (long long)(i + u) * HPW * D), hi[u] = ld_stream8(src + (long long)(i + u) * HPW * D + D / 2);
+    };
+    load(0);
     int pos[3];
     bool real = true, inside = true;
 #pragma unroll
@@ -209,37 +213,45 @@ __global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_co
     const bool cached = slot >= 0 && slot < p.n_slots;
     if (slot >= p.n_slots && lane == 0) report_fault(p.status, FAULT_SLOT_RANGE);
 
-    // Table rows: the lane's columns of every axis, then the axis of each frequency picks.  [0]: first half, [1]: second half.
+    // Table rows: the lane's columns of every axis; the axis of each frequency picks, 16 bits at a time.
     auto unpack = [](const uint2& v, float2 (&x)[2]) {
         x[0] = make_float2(bf16_lo(v.x), bf16_hi(v.x)), x[1] = make_float2(bf16_lo(v.y), bf16_hi(v.y));
     };
     float2 c1[2], c2[2], s1[2], s2[2];
     if (chunk * p.steps * HPW < p.H + p.NKV) {  // a warp with v heads only copies
+        const uint32_t axes4 = *reinterpret_cast<const uint32_t*>(p.axis + f0);
+        uint2 row[4];  // cos of the first and second half, sin of the first and second half
 #pragma unroll
         for (int a = 0; a < 3; ++a) {
             if (a < p.axes) {
                 const bf16 *cr = p.cos + (long long)pos[a] * D + f0, *sr = p.sin + (long long)pos[a] * D + f0;
-                float2 x[4][2];
-                unpack(__ldg(reinterpret_cast<const uint2*>(cr)), x[0]), unpack(__ldg(reinterpret_cast<const uint2*>(cr + D / 2)), x[1]);
-                unpack(__ldg(reinterpret_cast<const uint2*>(sr)), x[2]), unpack(__ldg(reinterpret_cast<const uint2*>(sr + D / 2)), x[3]);
+                const uint2 x[4] = {__ldg(reinterpret_cast<const uint2*>(cr)), __ldg(reinterpret_cast<const uint2*>(cr + D / 2)),
+                                    __ldg(reinterpret_cast<const uint2*>(sr)), __ldg(reinterpret_cast<const uint2*>(sr + D / 2))};
+                auto half = [&](int i) { return ((axes4 >> (8 * i)) & 255u) == (uint32_t)a ? 0xffffu : 0u; };
+                const uint32_t m0 = a ? half(0) | half(1) << 16 : ~0u, m1 = a ? half(2) | half(3) << 16 : ~0u;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if (a == 0 || p.axis[f0 + 2 * e] == a) c1[e].x = x[0][e].x, c2[e].x = x[1][e].x, s1[e].x = -x[2][e].x, s2[e].x = x[3][e].x;
-                    if (a == 0 || p.axis[f0 + 2 * e + 1] == a) c1[e].y = x[0][e].y, c2[e].y = x[1][e].y, s1[e].y = -x[2][e].y, s2[e].y = x[3][e].y;
+                for (int i = 0; i < 4; ++i) {
+                    row[i].x = a ? (row[i].x & ~m0) | (x[i].x & m0) : x[i].x;
+                    row[i].y = a ? (row[i].y & ~m1) | (x[i].y & m1) : x[i].y;
                 }
             }
         }
+        row[2].x ^= 0x80008000u, row[2].y ^= 0x80008000u;
+        unpack(row[0], c1), unpack(row[1], c2), unpack(row[2], s1), unpack(row[3], s2);
     }
     const long long page = slot >> p.page_shift, off = slot & ((1 << p.page_shift) - 1);
     bf16* q_row = p.q_out + (long long)t * p.H * D + f0;
     const long long kv_row = ((page * p.NKV) << p.page_shift) + off;  // + kv head * page size
+#pragma unroll 1
+    for (int i = 0; i < p.steps; i += kRopeBatch) {
+    if (i > 0) load(i);
 #pragma unroll
-    for (int u = 0; u < kRopeSteps; ++u) {
-        if (u >= p.steps) break;
-        const int h = h0 + u * HPW;
+    for (int u = 0; u < kRopeBatch; ++u) {
+        if (i + u >= p.steps) break;
+        const int h = h0 + (i + u) * HPW;
         const bool live = h < heads, is_v = h >= p.H + p.NKV, is_q = h < p.H;
         uint2 out1 = lo[u], out2 = hi[u];
-        if ((chunk * p.steps + u) * HPW < p.H + p.NKV) {  // the same for the whole warp
+        if ((chunk * p.steps + i + u) * HPW < p.H + p.NKV) {  // the same for the whole warp
             float2 a[2], b[2], w1[2], w2[2];
             unpack(lo[u], a), unpack(hi[u], b);
             unpack(is_q ? qw1 : kw1, w1), unpack(is_q ? qw2 : kw2, w2);
@@ -272,6 +284,7 @@ __global__ void __launch_bounds__(128) paged_qk_norm_rope_kernel(const __grid_co
             *reinterpret_cast<uint2*>(dst + D / 2) = out2;
         }
     }
+    }
 }
 
 cudaError_t launch_paged_qk_norm_rope(const PagedRopeArgs& a, cudaStream_t stream) {
@@ -283,11 +296,11 @@ cudaError_t launch_paged_qk_norm_rope(const PagedRopeArgs& a, cudaStream_t strea
     p.eps = a.eps;
     p.status = status_ptr();
     if (!p.status) return cudaErrorUnknown;
-    for (int i = 0; i < 128; ++i) p.axis[i] = i < a.D / 2 ? a.axis_of_frequency[i] : 0;
+    for (int i = 0; i < 64; ++i) p.axis[i] = i < a.D / 2 ? a.axis_of_frequency[i] : 0;
     const int per_warp = 32 / (a.D / 8), groups = (a.H + 2 * a.NKV + per_warp - 1) / per_warp;
     const long long fill = (long long)sm_count() * 32;
     p.steps = 1;
-    while (p.steps < kRopeSteps && (long long)a.T * ((groups + 2 * p.steps - 1) / (2 * p.steps)) >= fill) p.steps *= 2;
+    while (p.steps < groups && (long long)a.T * ((groups + 2 * p.steps - 1) / (2 * p.steps)) >= fill) p.steps *= 2;
     p.chunks = (groups + p.steps - 1) / p.steps;
     const long long warps = (long long)a.T * p.chunks;
     chain_begin();
