@@ -19,6 +19,8 @@
 // and PV (D = 128) and 1024 cycles of the MUFU, twice per step; for single tokens the bytes of the caches.
 // Keys behind a row's last one, entries outside the pools and everything masked are never added: K there is masked after
 // the product, V is zero (out-of-range TMA boxes, or cleared in shared memory where a box straddles the end).
+#include <atomic>
+
 #include "prompt.h"
 #include "tc.cuh"
 
@@ -828,8 +830,8 @@ static cudaError_t launch_attn_prompt_d(const AttnPromptArgs& a, const ApParams&
     if (!encode_3d(&mq, a.Q, D, a.H, a.T, D, a.ldq, p.G, p.tpt) || !encode_3d(&mk, a.K, D, P, z, D, P * D, 64, 1) ||
         !encode_3d(&mv, a.V, D, P, z, D, P * D, 64, 1))
         return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ApSmem<D>::kBytes);
-    if (e != cudaSuccess) return e;
+    static std::atomic<bool> configured[64];
+    if (cudaError_t e = allow_smem_once(attn_prompt_kernel<D>, ApSmem<D>::kBytes, configured)) return e;
     chain_begin();
     return launch_pdl(attn_prompt_kernel<D>, dim3((unsigned)attn_prompt_grid()), dim3(kApThreads), ApSmem<D>::kBytes, stream, mq, mk, mv, p);
 }

@@ -12,6 +12,8 @@
 // leave clusters without work (linear_plan).
 // What bounds it: the tensor cores (and from a few hundred rows down the weights' bytes).
 // Few rows: the kernel of the batched decode projections (gemm_tc.cu) with this epilogue.
+#include <atomic>
+
 #include "prompt.h"
 #include "tc.cuh"
 
@@ -294,8 +296,8 @@ static cudaError_t launch_linear_tile(const LinearArgs& a, LtParams& p, cudaStre
     if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, 128) || !encode_rows(&w0, a.W, a.N, a.K, a.K, BN / 2) ||
         !encode_rows(&w1, PAIR ? a.W + (long long)a.N * a.K : a.W, a.N, a.K, a.K, BN / 2))
         return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(linear_tc_kernel<BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, LtSmem<BN>::kBytes);
-    if (e != cudaSuccess) return e;
+    static std::atomic<bool> configured[64];
+    if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR>, LtSmem<BN>::kBytes, configured)) return e;
     p.tiles_m = (a.M + 255) / 256, p.tiles_n = (a.N + UNITS - 1) / UNITS;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     const int clusters = (int)(tiles < sm_count() / 2 ? tiles : sm_count() / 2);

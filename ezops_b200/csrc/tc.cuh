@@ -4,6 +4,8 @@
 
 #include <cuda.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ezb {
@@ -173,6 +175,18 @@ inline EncodeTiledFn encode_fn() {
             fn = reinterpret_cast<EncodeTiledFn>(ptr);
     }
     return fn;
+}
+
+// Opts a kernel in to `bytes` of dynamic shared memory, once per device.
+template <typename K>
+inline cudaError_t allow_smem_once(K kernel, int bytes, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    const bool keep = dev >= 0 && dev < 64;
+    if (keep && done[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    if (keep) done[dev].store(true, std::memory_order_relaxed);
+    return cudaSuccess;
 }
 
 }  // namespace ezb

@@ -10,34 +10,53 @@ import torch
 from .. import _lib
 from ..registry import register_kernel
 from .base_kernel import BaseKernel
-from .sm100 import _BF16, _current_device, _require, _stream, _zeros_bytes
+from .sm100 import _BF16, _current_device, _raw_stream, _zeros_bytes
 
 _I32 = torch.int32
 
 
-def _require_rows(t: torch.Tensor, name: str, shape, dtype=_BF16) -> int:
-    """As ``_require``, but rows (the first dimension) may lie further apart; returns their distance in elements."""
+# A step is a few short kernels, so the host's share counts (see sm100.py): a call asks everything about its tensors in one
+# expression (0.2 us a tensor) and looks for what is wrong only when it fails.  Launches go to the current device's current
+# stream, so tensors of another device are refused.
+def _whole(t: torch.Tensor, shape, dtype, device: int) -> bool:
+    return t.get_device() == device and t.dtype is dtype and t.shape == shape and t.is_contiguous()
+
+
+def _rows(t: torch.Tensor, shape, dtype, device: int) -> bool:
+    """As ``_whole``, but rows (the first dimension) may lie further apart."""
+    return (t.get_device() == device and t.dtype is dtype and t.shape == shape and t.numel() > 0
+            and (t.is_contiguous() or t[0].is_contiguous()))
+
+
+def _device(t: torch.Tensor, name: str) -> int:
+    """The current device, if there is one."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.numel() == 0:
-        raise ValueError(f"{name} is empty")
-    if t.is_contiguous():
-        return t.numel() // t.shape[0]
-    if not t[0].is_contiguous():
-        raise ValueError(f"{name} must be contiguous within a row")
-    return t.stride(0)
+    return _current_device()
 
 
-def _require_here(*tensors) -> None:
-    """Launches go to the current device's current stream: tensors of another device do not belong there."""
-    here = _current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"tensors are on {t.device}, but the current device is cuda:{here} (use torch.cuda.device)")
+def _refuse(checks, device: int):
+    """Raises for the first of ``checks`` - (name, tensor, shape, dtype, rows may lie apart) - that does not hold."""
+    for name, t, shape, dtype, apart in checks:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if t.get_device() != device:
+            raise ValueError(f"{name} is on {t.device}, but the current device is cuda:{device} (use torch.cuda.device)")
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+        if t.numel() == 0:
+            raise ValueError(f"{name} is empty")
+        if not t.is_contiguous() and not (apart and t[0].is_contiguous()):
+            raise ValueError(f"{name} must be contiguous" + (" within a row" if apart else ""))
+
+
+def _distance(t: torch.Tensor) -> int:
+    """Elements from one row to the next."""
+    return t.numel() // t.shape[0] if t.is_contiguous() else t.stride(0)
 
 
 def _ptr(t):
@@ -50,22 +69,27 @@ class PagedPlanSm100Kernel(BaseKernel):
         if batch > 8192:
             raise ValueError(f"batch ({batch}) must be at most 8192")
         self.sizes = (batch, max_tokens, max_pages, page_size, num_pages)
-        self._in = (("ctx_lens", (batch,)), ("new_lens", (batch,)), ("page_table", (batch, max_pages)))
-        self._out = (("seq_lens", (batch,)), ("cu_tokens", (batch + 1,)), ("positions", (max_tokens,)), ("slots", (max_tokens,)),
-                     ("free_count", (1,)))
-        self._lib = _lib.load()
+        self._rows, self._table, self._cu, self._tokens, self._one = (batch,), (batch, max_pages), (batch + 1,), (max_tokens,), (1,)
+        self._entry = _lib.load().ezb_paged_plan
 
     def __call__(self, ctx_lens, new_lens, page_table, free_pages, free_count, out) -> None:
-        for (name, shape), t in zip(self._in, (ctx_lens, new_lens, page_table)):
-            _require(t, name, shape, _I32)
-        _require(free_pages, "free_pages", (free_pages.numel(),), _I32)
-        _require(free_count, "free_count", (1,), _I32)
-        for (name, shape), t in zip(self._out, out):
-            _require(t, f"out.{name}", shape, _I32)
-        _require_here(ctx_lens, new_lens, page_table, free_pages, free_count, *out)
-        _lib.check(self._lib.ezb_paged_plan(
-            ctx_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-            *(t.data_ptr() for t in out), *self.sizes, free_pages.numel(), _stream()))
+        dev, rows, tokens, one = _device(ctx_lens, "ctx_lens"), self._rows, self._tokens, self._one
+        lens, cu, positions, slots, left = out
+        free = (free_pages.numel(),)
+        if not (_whole(ctx_lens, rows, _I32, dev) and _whole(new_lens, rows, _I32, dev) and _whole(page_table, self._table, _I32, dev)
+                and _whole(free_pages, free, _I32, dev) and _whole(free_count, one, _I32, dev) and _whole(lens, rows, _I32, dev)
+                and _whole(cu, self._cu, _I32, dev) and _whole(positions, tokens, _I32, dev) and _whole(slots, tokens, _I32, dev)
+                and _whole(left, one, _I32, dev) and free[0] > 0):
+            _refuse([(n, t, shape, _I32, False) for n, t, shape in (
+                ("ctx_lens", ctx_lens, rows), ("new_lens", new_lens, rows), ("page_table", page_table, self._table),
+                ("free_pages", free_pages, free), ("free_count", free_count, one), ("out.seq_lens", lens, rows),
+                ("out.cu_tokens", cu, self._cu), ("out.positions", positions, tokens), ("out.slots", slots, tokens),
+                ("out.free_count", left, one))], dev)
+        rc = self._entry(ctx_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+                         lens.data_ptr(), cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), left.data_ptr(), *self.sizes, free[0],
+                         _raw_stream(dev))
+        if rc:
+            _lib.check(rc)
 
 
 @register_kernel("paged_qk_norm_rope", "cuda", family="prompt")
@@ -73,33 +97,36 @@ class PagedQkNormRopeSm100Kernel(BaseKernel):
     rms_eps = 1e-6
 
     def __init__(self, num_heads, head_dim, max_positions, page_size, num_pages, num_kv_heads=None, sections=None, interleaved=False):
-        self.H, self.D, self.S, self.P, self.pages = num_heads, head_dim, max_positions, page_size, num_pages
-        self.NKV = num_heads if num_kv_heads is None else num_kv_heads
-        self.sections = (head_dim // 2,) if sections is None else tuple(sections)
-        self.interleaved = int(interleaved)
-        self._sections = (ctypes.c_int * len(self.sections))(*self.sections)
-        self._lib = _lib.load()
+        NKV = num_heads if num_kv_heads is None else num_kv_heads
+        self.H, self.D = num_heads, head_dim
+        sections = (head_dim // 2,) if sections is None else tuple(sections)
+        self.axes = len(sections)
+        self._sections = (ctypes.c_int * self.axes)(*sections)
+        self._width, self._w, self._table = (num_heads + 2 * NKV) * head_dim, (head_dim,), (max_positions, head_dim)
+        self._pool = (num_pages, NKV, page_size, head_dim)
+        self._sizes = (num_heads, NKV, head_dim, max_positions, self.axes, self._sections, int(interleaved), page_size, num_pages, self.rms_eps)
+        self._entry = _lib.load().ezb_paged_qk_norm_rope
 
     def __call__(self, qkv, q_norm_w, k_norm_w, cos, sin, positions, slots, K_pool, V_pool, out=None):
-        T, H, NKV, D, axes = qkv.shape[0], self.H, self.NKV, self.D, len(self.sections)
-        ld = _require_rows(qkv, "qkv", (T, (H + 2 * NKV) * D))
-        for name, t in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
-            if t is not None:
-                _require(t, name, (D,))
-        _require(cos, "cos", (self.S, D)); _require(sin, "sin", (self.S, D))
-        _require(positions, "positions", (T,) if axes == 1 and positions.dim() == 1 else (axes, T), _I32)
-        _require(slots, "slots", (T,), _I32)
-        pool = (self.pages, NKV, self.P, D)
-        _require(K_pool, "K_pool", pool); _require(V_pool, "V_pool", pool)
+        dev, T, w, table, pool = _device(qkv, "qkv"), qkv.shape[0], self._w, self._table, self._pool
+        row = (T, self._width)
         if out is None:
-            out = torch.empty(T, H, D, dtype=_BF16, device=qkv.device)
-        else:
-            _require(out, "out", (T, H, D))
-        _require_here(qkv, q_norm_w, k_norm_w, cos, sin, positions, slots, K_pool, V_pool, out)
-        _lib.check(self._lib.ezb_paged_qk_norm_rope(
-            qkv.data_ptr(), ld, _ptr(q_norm_w), _ptr(k_norm_w), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-            K_pool.data_ptr(), V_pool.data_ptr(), out.data_ptr(), T, H, NKV, D, self.S, axes, self._sections, self.interleaved, self.P,
-            self.pages, self.rms_eps, _stream()))
+            out = torch.empty(T, self.H, self.D, dtype=_BF16, device=qkv.device)
+        where = (T,) if self.axes == 1 and positions.dim() == 1 else (self.axes, T)
+        heads = (T, self.H, self.D)
+        if not (_rows(qkv, row, _BF16, dev) and (q_norm_w is None or _whole(q_norm_w, w, _BF16, dev))
+                and (k_norm_w is None or _whole(k_norm_w, w, _BF16, dev)) and _whole(cos, table, _BF16, dev)
+                and _whole(sin, table, _BF16, dev) and _whole(positions, where, _I32, dev) and _whole(slots, (T,), _I32, dev)
+                and _whole(K_pool, pool, _BF16, dev) and _whole(V_pool, pool, _BF16, dev) and _whole(out, heads, _BF16, dev)):
+            _refuse([("qkv", qkv, row, _BF16, True), ("q_norm_w", q_norm_w, w, _BF16, False), ("k_norm_w", k_norm_w, w, _BF16, False),
+                     ("cos", cos, table, _BF16, False), ("sin", sin, table, _BF16, False), ("positions", positions, where, _I32, False),
+                     ("slots", slots, (T,), _I32, False), ("K_pool", K_pool, pool, _BF16, False), ("V_pool", V_pool, pool, _BF16, False),
+                     ("out", out, heads, _BF16, False)], dev)
+        rc = self._entry(qkv.data_ptr(), _distance(qkv), _ptr(q_norm_w), _ptr(k_norm_w), cos.data_ptr(), sin.data_ptr(),
+                         positions.data_ptr(), slots.data_ptr(), K_pool.data_ptr(), V_pool.data_ptr(), out.data_ptr(), T, *self._sizes,
+                         _raw_stream(dev))
+        if rc:
+            _lib.check(rc)
         return out
 
 
@@ -111,22 +138,23 @@ class LinearSm100Kernel(BaseKernel):
         if in_features % 8:
             raise ValueError(f"in_features ({in_features}) must be divisible by 8")
         self.N, self.K, self.out_dtype, self.act = out_features, in_features, out_dtype, ACTIVATIONS[activation]
-        self.rows = out_features * (2 if activation == "swiglu" else 1)
-        self._lib = _lib.load()
+        rows = out_features * (2 if activation == "swiglu" else 1)
+        self._w, self._bias = (rows, in_features), (rows,)
+        self._f32 = int(out_dtype == torch.float32)
+        self._entry = _lib.load().ezb_linear_bf16
 
     def __call__(self, X, W, bias=None, residual=None, out=None):
-        M, N, K = X.shape[0], self.N, self.K
-        ldx = _require_rows(X, "X", (M, K))
-        _require(W, "W", (self.rows, K))
-        if bias is not None:
-            _require(bias, "bias", (self.rows,))
-        ldres = N if residual is None else _require_rows(residual, "residual", (M, N))
+        dev, M, N, K = _device(X, "X"), X.shape[0], self.N, self.K
         if out is None:
             out = torch.empty(M, N, dtype=self.out_dtype, device=X.device)
-        ldout = _require_rows(out, "out", (M, N), self.out_dtype)
-        _require_here(X, W, bias, residual, out)
-        _lib.check(self._lib.ezb_linear_bf16(X.data_ptr(), ldx, W.data_ptr(), _ptr(bias), _ptr(residual), ldres, out.data_ptr(), ldout,
-                                             M, N, K, self.act, int(self.out_dtype == torch.float32), _stream()))
+        if not (_rows(X, (M, K), _BF16, dev) and _whole(W, self._w, _BF16, dev) and (bias is None or _whole(bias, self._bias, _BF16, dev))
+                and (residual is None or _rows(residual, (M, N), _BF16, dev)) and _rows(out, (M, N), self.out_dtype, dev)):
+            _refuse([("X", X, (M, K), _BF16, True), ("W", W, self._w, _BF16, False), ("bias", bias, self._bias, _BF16, False),
+                     ("residual", residual, (M, N), _BF16, True), ("out", out, (M, N), self.out_dtype, True)], dev)
+        rc = self._entry(X.data_ptr(), _distance(X), W.data_ptr(), _ptr(bias), _ptr(residual), N if residual is None else _distance(residual),
+                         out.data_ptr(), _distance(out), M, N, K, self.act, self._f32, _raw_stream(dev))
+        if rc:
+            _lib.check(rc)
         return out
 
 
@@ -137,8 +165,10 @@ class AttnPromptSm100Kernel(BaseKernel):
     def __init__(self, batch, num_heads, head_dim, max_pages, page_size, num_kv_heads=None):
         self.B, self.H, self.D, self.max_pages, self.P = batch, num_heads, head_dim, max_pages, page_size
         self.NKV = num_heads if num_kv_heads is None else num_kv_heads
+        self._table, self._lens, self._cu = (batch, max_pages), (batch,), (batch + 1,)
         self._ws = None
         self._lib = _lib.load()
+        self._entry = self._lib.ezb_attn_prompt
 
     def workspace(self, device):
         if self._ws is None or self._ws.device != device:
@@ -146,19 +176,20 @@ class AttnPromptSm100Kernel(BaseKernel):
         return self._ws
 
     def __call__(self, Q, K_pool, V_pool, page_table, seq_lens, cu_tokens, out=None):
-        T, H, NKV, D = Q.shape[0], self.H, self.NKV, self.D
-        ldq = _require_rows(Q, "Q", (T, H, D))
-        for name, t in (("K_pool", K_pool), ("V_pool", V_pool)):
-            _require(t, name, (K_pool.shape[0], NKV, self.P, D))
-        _require(page_table, "page_table", (self.B, self.max_pages), _I32)
-        _require(seq_lens, "seq_lens", (self.B,), _I32)
-        _require(cu_tokens, "cu_tokens", (self.B + 1,), _I32)
+        dev, T, H, D = _device(Q, "Q"), Q.shape[0], self.H, self.D
+        heads, pool = (T, H, D), (K_pool.shape[0], self.NKV, self.P, D)
         if out is None:
             out = torch.empty(T, H, D, dtype=_BF16, device=Q.device)
-        ldo = _require_rows(out, "out", (T, H, D))
-        _require_here(Q, K_pool, V_pool, page_table, seq_lens, cu_tokens, out)
+        if not (_rows(Q, heads, _BF16, dev) and _whole(K_pool, pool, _BF16, dev) and _whole(V_pool, pool, _BF16, dev)
+                and _whole(page_table, self._table, _I32, dev) and _whole(seq_lens, self._lens, _I32, dev)
+                and _whole(cu_tokens, self._cu, _I32, dev) and _rows(out, heads, _BF16, dev)):
+            _refuse([("Q", Q, heads, _BF16, True), ("K_pool", K_pool, pool, _BF16, False), ("V_pool", V_pool, pool, _BF16, False),
+                     ("page_table", page_table, self._table, _I32, False), ("seq_lens", seq_lens, self._lens, _I32, False),
+                     ("cu_tokens", cu_tokens, self._cu, _I32, False), ("out", out, heads, _BF16, True)], dev)
         ws = self.workspace(Q.device)
-        _lib.check(self._lib.ezb_attn_prompt(
-            Q.data_ptr(), ldq, K_pool.data_ptr(), V_pool.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(), cu_tokens.data_ptr(),
-            out.data_ptr(), ldo, ws.data_ptr(), ws.numel(), self.B, T, H, NKV, D, self.max_pages, self.P, K_pool.shape[0], _stream()))
+        rc = self._entry(Q.data_ptr(), _distance(Q), K_pool.data_ptr(), V_pool.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
+                         cu_tokens.data_ptr(), out.data_ptr(), _distance(out), ws.data_ptr(), ws.numel(), self.B, T, H, self.NKV, D,
+                         self.max_pages, self.P, pool[0], _raw_stream(dev))
+        if rc:
+            _lib.check(rc)
         return out
