@@ -295,9 +295,43 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
             mbar_wait_bounded(smem_u32(&acc_full[acc]), (uint32_t)((i >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             if (i == 0) trace_mark(trec, 4);
             tc_fence_after();
-            if (i > 0)  // the previous tile's parts have been read, here and by the CTAs they were sent to
+            const bool straight = EXT && C == 1 && !p.pair;  // no parts, see below
+            if (i > 0 && !straight)  // the previous tile's parts have been read, here and by the CTAs they were sent to
                 mbar_wait_bounded_cluster(smem_u32(recv_free), (uint32_t)((i - 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             const uint32_t t_addr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * NB + b_half);
+            if constexpr (EXT) {
+                // Nothing to add up and no partner row: a warp's lanes hold 32 neighbouring outputs of a batch column, so the
+                // columns go from tensor memory straight to the result, 128 bytes (64 in bf16) at a time.
+                if (straight) {
+                    const int n_own = tile * p.units + row;
+                    const bool own = row < p.units && n_own < p.N && !*abort_flag;
+                    const float bias = p.bias && own ? __bfloat162float(p.bias[n_own]) : 0.f;
+#pragma unroll 1
+                    for (int c = 0; c < HC; c += 8) {
+                        if (b_half + c >= p.B) break;
+                        float v[8], r8[8];
+                        tmem_ld8(t_addr + (uint32_t)c, v);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            r8[e] = p.residual && own && b_half + c + e < p.B ? __bfloat162float(p.residual[(long long)(b_half + c + e) * p.ldres + n_own]) : 0.f;
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            if (own && b_half + c + e < p.B) {
+                                const float x = linear_act(v[e] + bias, p.act) + r8[e];
+                                const long long o = (long long)(b_half + c + e) * p.ldout + n_own;
+                                if (p.out_f32) static_cast<float*>(p.out)[o] = x;
+                                else static_cast<bf16*>(p.out)[o] = __float2bfloat16_rn(x);
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&acc_empty[acc]));
+                    continue;
+                }
+            }
             float* dst = mine + (size_t)b_half * RS + row;
             const int b_left = p.B - b_half;
             if constexpr (HC == 8) {
