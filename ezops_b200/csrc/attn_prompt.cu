@@ -619,6 +619,15 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
             const int limit = live ? seg.sees + tok - from : 0, all_see = seg.sees + first - from;
             const int my0 = dual ? m : 0, step = dual ? 2 : 1;
             float mx = -INFINITY, sum = 0.f;
+            auto row_max = [](const float (&s)[kApKeys]) {
+                float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int c = 4; c < kApKeys; c += 8) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = c + 4 + e < kApKeys ? max3(top[e], s[c + e], s[c + 4 + e]) : fmaxf(top[e], s[c + e]);
+                }
+                return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            };
 #pragma unroll 1
             for (int i = my0; i < cnt; i += step) {
                 const int key0 = i * kApKeys;
@@ -634,61 +643,70 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                     for (int c = 0; c < kApKeys; ++c)
                         if (key0 + c >= limit) s[c] = -INFINITY;
                 }
-                float top4[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int c = 4; c < kApKeys; c += 8) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) top4[e] = c + 4 + e < kApKeys ? max3(top4[e], s[c + e], s[c + 4 + e]) : fmaxf(top4[e], s[c + e]);
-                }
-                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-                if (i == my0) {
-                    mx = top;
-                } else {
-                    // all keys so far masked: nothing has been summed, and the factor is exp2(-inf) = 0
-                    const float higher = fmaxf(mx, top);
-                    const bool grow = (higher - mx) * p.scale_log2 > 8.f;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float f = grow ? exp2_approx((mx - higher) * p.scale_log2) : 1.f;
-                        if (grow) mx = higher;
-                        sum *= f;
-#pragma unroll 1
-                        for (int c = 0; c < D; c += 16) {
-                            float o[16];
-                            uint32_t w[16];
-                            tmem_ld16(t_o + c, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(o[e] * f);
-                            tmem_st16(t_o + c, w);
-                        }
-                    }
-                }
-                const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
-                // The warpgroups take turns: side by side they would both exponentiate at half speed and then both wait for
+                if (i == my0) mx = row_max(s);
+                // The tiles take turns: side by side they would both exponentiate at half speed and then both wait for
                 // the tensor cores.
                 if (!dual) {
                     mbar_wait_bounded(smem_u32(&t.turn[m]), (n_turn & 1u) ^ (m == 0 ? 1u : 0u), abort_flag, p.status, FAULT_PROMPT_WAIT);
                     ++n_turn;
                 }
-                float2 add[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2), shift2 = make_float2(-shift, -shift);
+                // The first half is exponentiated against the maximum of the blocks before, while this block's is being found: it
+                // hardly ever matters (the comment at the top), and the search costs nothing next to the MUFU.
+                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+                float2 add[2];
+                uint32_t w[32];
+                auto first_half = [&]() {
+                    const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+                    const float2 shift2 = make_float2(-shift, -shift);
+                    add[0] = add[1] = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int c = 0; c < kApKeys; c += 32) {
-                    uint32_t w[16];
+                    for (int e = 0; e < 32; ++e) {
+                        float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), scale2, shift2);
+                        x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
+                        add[e & 1] = add2(add[e & 1], x);
+                        w[e] = pack_bf16(x.x, x.y);
+                    }
+                };
+                first_half();
+                const float higher = fmaxf(mx, row_max(s));
+                // all keys so far masked: nothing has been summed, and the factor is exp2(-inf) = 0
+                const bool grow = (higher - mx) * p.scale_log2 > 8.f;
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float f = grow ? exp2_approx((mx - higher) * p.scale_log2) : 1.f;
+                    if (grow) mx = higher;
+                    sum *= f;
+                    if (i != my0) {
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            uint32_t u[16];
+                            tmem_ld16(t_o + c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
+                            tmem_st16(t_o + c, u);
+                        }
+                    }
+                    first_half();
+                }
+                tmem_st16(t_s, w), tmem_st16(t_s + 16, w + 16);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&t.h_full[m]));  // half of P is there: its products may start
+                const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+                const float2 shift2 = make_float2(-shift, -shift);
+#pragma unroll
+                for (int c = kApKeys / 2; c < kApKeys; c += 32) {
+                    uint32_t v[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         float2 x = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2);
                         x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
                         add[e & 1] = add2(add[e & 1], x);
-                        w[e] = pack_bf16(x.x, x.y);
+                        v[e] = pack_bf16(x.x, x.y);
                     }
-                    tmem_st16(t_s + c / 2, w);
-                    if (c == 32) {  // half of P is there: its products may start
-                        tmem_st_wait();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&t.h_full[m]));
-                    }
+                    tmem_st16(t_s + c / 2, v);
                     if (c == 64 && !dual) {  // the rest of this tile and the start of the other one fill each other's gaps
                         __syncwarp();
                         if (lane == 0) mbar_arrive(smem_u32(&t.turn[1 - m]));
