@@ -209,22 +209,28 @@ struct ApTail {
     uint32_t tmem;
     int abort_flag;
     int last;  // this CTA joins the parts of the unit
-    ApCursor start;
-    long long warp_sum[kApThreads / 32];
     int parts;
-    int list[2 * 160];  // parts of a unit in the order of its keys: 2 * slot + tile
+    short list[160];  // parts of a unit in the order of its keys: twice their slot
+    union {
+        struct {
+            ApCursor start;  // where the CTA's share starts
+            long long warp_sum[kApThreads / 32];
+        };
+        float stat[2][128];  // later: maxima and sums of warpgroup 1 on their way to warpgroup 0
+    };
 };
 static_assert(sizeof(ApTail) <= 2048, "tail of the shared memory");
 
-// Joins the n parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by the 256 softmax
-// threads.  A thread keeps one row of the unit (rows rounded up to a power of two) and D / (256 / rows) neighbouring columns of
+// Joins the n parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by the softmax
+// threads that wrote them.  A thread keeps one row of the unit (rows rounded up to a power of two) and D / (threads / rows)
+// neighbouring columns of
 // it, 16 at a time (4 when there are few rows); what it loads of two parts is on its way together.  Not inlined: its registers
 // would be taken from the loop over the keys.
 template <int D, int W>  // W groups of four columns at a time
-__device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const int* list, int n, int tid) {
+__device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const short* list, int n, int tid, int threads) {
     constexpr long long kPart = (long long)(D + 2) * 128;
     const int rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
-    const int log_rows = rows > 1 ? 32 - __clz(rows - 1) : 0, row = tid & ((1 << log_rows) - 1), share = 256 >> log_rows;
+    const int log_rows = rows > 1 ? 32 - __clz(rows - 1) : 0, row = tid & ((1 << log_rows) - 1), share = threads >> log_rows;
     if (row >= rows) return;
     const int q = row / per_tile, rr = row - q * per_tile;  // tile of the pair (one of keys: always 0) and row in it
     const float* base = p.parts + q * kPart;
@@ -608,7 +614,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lanes + m * 128, t_o = tmem + lanes + 256 + m * D;
         const int r_tok = r / p.G, r_head = r - r_tok * p.G;
-        uint32_t n_tile = 0, n_unit = 0, n_turn = 0;
+        uint32_t n_tile = 0, n_unit = 0, n_turn = 0, n_other = 0;  // n_other: units of warpgroup 1, as warpgroup 0 counts them
         while (const ApSegment* sp = next_segment()) {
             const ApSegment& seg = *sp;  // stays in shared memory until the end of the segment
             const int cnt = seg.cnt, dual = seg.dual;
@@ -719,45 +725,76 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                 if (lane == 0) mbar_arrive(smem_u32(&t.p_full[m]));
             }
             // ---- end of the segment
-            const bool mine = my0 < cnt, whole = cnt == seg.tiles;
+            const bool mine = my0 < cnt, whole = cnt == seg.tiles, two = dual && cnt > 1;
             if (mine) {
                 mbar_wait_bounded(smem_u32(&t.o_full[m]), n_unit & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
                 ++n_unit;
                 tc_fence_after();
             }
-            if (whole && (!dual || cnt <= 1)) {
-                // a query that sees no key gives zero; the second tile of a single block of keys has no rows
-                const bool store = live && !(dual && m == 1) && !*abort_flag;
-                const float inv = limit > 0 ? 1.0f / sum : 0.f;
-                bf16* out = p.Out + (long long)(seg.token + tok) * p.ldo + (long long)(seg.head * p.G + r_head) * D;
-#pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                    float o[16];
-                    if (mine) {
-                        tmem_ld16(t_o + c, o);
+            // Two sums over the same rows meet here: warpgroup 0 reads the other one's O from tensor memory (the same lanes).
+            float w0 = 1.f, w1 = 0.f;
+            bool writes = true;
+            if (dual) {
+                if (two && m == 1) t.stat[0][r] = mx, t.stat[1][r] = sum;
+                named_bar_sync(1, 256);
+                writes = m == 0;
+                if (two && m == 0) {
+                    mbar_wait_bounded(smem_u32(&t.o_full[1]), n_other & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    tc_fence_after();
+                    const float mx1 = t.stat[0][r], top = fmaxf(mx, mx1);
+                    w0 = mx == -INFINITY ? 0.f : exp2_approx((mx - top) * p.scale_log2);
+                    w1 = mx1 == -INFINITY ? 0.f : exp2_approx((mx1 - top) * p.scale_log2);
+                    sum = w0 * sum + w1 * t.stat[1][r];
+                    mx = top;
+                }
+            }
+            if (two || (!dual && cnt > 0)) ++n_other;
+            if (writes) {
+                // 16 columns of the row's O; the other warpgroup's lie D columns behind
+                auto columns = [&](int c, float (&o)[16]) {
+                    tmem_ld16(t_o + c, o);
+                    if (two) {
+                        float o1[16];
+                        tmem_ld16(t_o + D + c, o1);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) o[e] = w0 * o[e] + w1 * o1[e];
+                    } else {
                         tmem_ld_wait();
                     }
-                    uint32_t w[8];
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) w[q] = limit > 0 ? pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
-                    if (store) store_row16(out + c, w, p.out32);
-                    __syncwarp();
-                }
-                if (mine) {
+                };
+                auto drained = [&]() {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&t.o_empty[m]));
-                }
-            } else {
-                constexpr long long kPart = (long long)(D + 2) * 128;
-                if (mine) {
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&t.o_empty[m]));
+                        if (two) mbar_arrive(smem_u32(&t.o_empty[1]));
+                    }
+                };
+                if (whole) {
+                    const bool store = live && !*abort_flag;
+                    const float inv = 1.0f / sum;
+                    bf16* out = p.Out + (long long)(seg.token + tok) * p.ldo + (long long)(seg.head * p.G + r_head) * D;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {
+                        float o[16];
+                        if (mine) columns(c, o);
+                        uint32_t w[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q)  // a query that sees no key gives zero
+                            w[q] = limit > 0 ? pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
+                        if (store) store_row16(out + c, w, p.out32);
+                        __syncwarp();
+                    }
+                    if (mine) drained();
+                } else {
+                    constexpr long long kPart = (long long)(D + 2) * 128;
                     float* part = p.parts + (seg.slot * 2 + m) * kPart;
                     if (live) __stcg(part + (long long)D * 128 + r, mx), __stcg(part + (long long)(D + 1) * 128 + r, sum);
 #pragma unroll 1
                     for (int c = 0; c < D; c += 16) {
                         float o[16];
-                        tmem_ld16(t_o + c, o);
-                        tmem_ld_wait();
+                        columns(c, o);
                         if (live) {
 #pragma unroll
                             for (int e = 0; e < 16; e += 4)
@@ -765,46 +802,35 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                         }
                         __syncwarp();
                     }
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&t.o_empty[m]));
-                }
-                __threadfence();
-                named_bar_sync(1, 256);
-                if (tid == 0) {
-                    // One counter per share: of the units that start in it only the last can be cut.  (The others have to leave
-                    // it alone: the next CTA may already have added its part of that last one.)
-                    t.last = 1;
-                    if (!whole) {
+                    drained();
+                    const int writers = dual ? 128 : 256;
+                    named_bar_sync(dual ? 2 : 1, writers);  // behind it thread 0 speaks for all
+                    if (tid == 0) {
+                        // One counter per share: of the units that start in it only the last can be cut.
+                        __threadfence();
                         t.last = atomicAdd(p.count + seg.c0, (unsigned)cnt) + (unsigned)cnt == (unsigned)seg.tiles;
                         if (t.last) p.count[seg.c0] = 0u;
+                        __threadfence();
                     }
-                }
-                if (warp == 0) {
-                    // the parts that there are, in the order of the keys: of every CTA from c0 to c1, dual: of both warpgroups
-                    int n = 0;
-                    for (int c0 = seg.c0; c0 <= seg.c1; c0 += 32) {
-                        const int c = c0 + lane;
-                        int tiles = 0;
-                        if (c <= seg.c1)
-                            tiles = whole ? (c == cta ? cnt : 0)
-                                          : ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles) - ap_tile_at(ap_share(line, c), seg.x0, seg.tiles);
-                        const uint32_t one = __ballot_sync(0xffffffffu, tiles > 0), two = __ballot_sync(0xffffffffu, dual && tiles > 1);
-                        const uint32_t below = (1u << lane) - 1u;
-                        const int at = n + __popc(one & below) + __popc(two & below), slot = 2 * (2 * c + (c == seg.c0 ? 1 : 0));
-                        if (tiles > 0) t.list[at] = slot;
-                        if (dual && tiles > 1) t.list[at + 1] = slot + 1;
-                        n += __popc(one) + __popc(two);
+                    if (warp == 1) {
+                        // meanwhile the parts that there are, in the order of the keys
+                        int n = 0;
+                        for (int c0 = seg.c0; c0 <= seg.c1; c0 += 32) {
+                            const int c = c0 + lane;
+                            const bool has = c <= seg.c1 && ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles) > ap_tile_at(ap_share(line, c), seg.x0, seg.tiles);
+                            const uint32_t all = __ballot_sync(0xffffffffu, has);
+                            if (has) t.list[n + __popc(all & ((1u << lane) - 1u))] = (short)(2 * (2 * c + (c == seg.c0 ? 1 : 0)));
+                            n += __popc(all);
+                        }
+                        if (lane == 0) t.parts = n;
                     }
-                    if (lane == 0) t.parts = n;
+                    named_bar_sync(dual ? 2 : 1, writers);
+                    if (t.last && !*abort_flag) {
+                        if (seg.tokens * p.G > 8) ap_join<D, 4>(p, seg, t.list, t.parts, tid, writers);
+                        else ap_join<D, 1>(p, seg, t.list, t.parts, tid, writers);
+                    }
+                    named_bar_sync(dual ? 2 : 1, writers);  // the list and the flag are free again
                 }
-                named_bar_sync(1, 256);
-                if (t.last && !*abort_flag) {
-                    __threadfence();
-                    if (seg.tokens * p.G > 32) ap_join<D, 4>(p, seg, t.list, t.parts, tid);
-                    else ap_join<D, 1>(p, seg, t.list, t.parts, tid);
-                }
-                named_bar_sync(1, 256);  // the list and the flag are free again
             }
             __syncwarp();
             if (lane == 0) release();
