@@ -659,9 +659,9 @@ static cudaError_t launch_tc_instance(const GemvArgs& a, const bf16* x, long lon
     while (p.cols_pad < p.cpc) p.cols_pad *= 2;
     alignas(64) CUtensorMap m0, m1, mx;
     if (EXT) {  // called with ever new activation buffers: descriptors are encoded (1 us) instead of filling up the table
-        if (!encode_map(&m0, a.W0, a.N, a.K, a.ldw, p.units) || !encode_map(&m1, p.pair ? a.W1 : a.W0, a.N, a.K, a.ldw, p.units) ||
-            !encode_map(&mx, x, a.B, a.K, ldx, NB))
-            return cudaErrorInvalidValue;
+        if (!encode_map(&m0, a.W0, a.N, a.K, a.ldw, p.units) || !encode_map(&mx, x, a.B, a.K, ldx, NB)) return cudaErrorInvalidValue;
+        m1 = m0;
+        if (p.pair && !encode_map(&m1, a.W1, a.N, a.K, a.ldw, p.units)) return cudaErrorInvalidValue;
         return launch_pdl_cluster(kernel, dim3((unsigned)clusters << p.log2c), dim3(kTcThreads), 1 << p.log2c, smem, stream, m0, m1, mx, p);
     }
     if (!make_map(&m0, a.W0, a.N, a.K, a.ldw, p.units)) return cudaErrorInvalidValue;

@@ -6,7 +6,7 @@
 // (tcgen05.mma.cta_group::2: each CTA holds half of x's rows and half of W's, and 128 x BN of the result in its tensor
 // memory), so each operand byte that enters an SM is used by two.  One elected thread per CTA fills a ring of 64-element
 // K blocks by TMA (both CTAs' bytes are counted on the first CTA's barrier), one thread of the first CTA issues the MMAs,
-// four warps of each CTA drain one of two accumulators while the next tile is multiplied: bias, activation, residual and
+// eight warps of each CTA drain one of two accumulators while the next tile is multiplied: bias, activation, residual and
 // rounding happen there, in registers.  Grid: one CTA per SM, tiles in groups of kLinearGroup row tiles so that the x and W
 // tiles in flight stay in L2.  BN = 256 reads least per product; narrower tiles (128, 64) are taken when the wide ones would
 // leave clusters without work (linear_plan).
@@ -19,7 +19,7 @@
 
 namespace ezb {
 
-static constexpr int kLtThreads = 192;  // TMA warp, MMA warp, four epilogue warps
+static constexpr int kLtThreads = 320;  // TMA warp, MMA warp, eight epilogue warps
 static constexpr int kLtBlockK = 64;
 static constexpr int kLtMaxStages = 12;
 static constexpr int kLtGroup = 8;  // row tiles per group of the tile order
@@ -117,7 +117,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
 
     if (tid == 0) {
         for (int s = 0; s < L::kStages; ++s) mbar_init(smem_u32(&full[s]), 1), mbar_init(smem_u32(&empty[s]), 1);
-        for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&acc_full[a]), 1), mbar_init(smem_u32(&acc_empty[a]), 8);  // warps of both CTAs
+        for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&acc_full[a]), 1), mbar_init(smem_u32(&acc_empty[a]), 16);  // warps of both CTAs
         *abort_flag = 0;
         mbar_fence_init();
     }
@@ -181,6 +181,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         // one step ahead (the first step: before the products are complete), or its latency would be paid once per step.
         constexpr int W = 32;
         const int q = warp & 3, row = q * 32 + lane;
+        const int c0 = ((warp - 2) >> 2) * W;  // two warps share a quarter: every other step each
         int n = 0;
         for (int i = blockIdx.x >> 1; i < n_tiles; i += n_clusters, ++n) {
             int tm, tn;
@@ -192,12 +193,12 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             const int cols = min(UNITS, p.N - n0);
             const bf16* res_row = p.residual ? p.residual + (long long)m * p.ldres + n0 : nullptr;
             uint32_t ahead[W / 2];  // residual values of the next step, packed
-            if (res_row && live_row) load_packed<W>(res_row, cols, p.vec_res, ahead);
+            if (res_row && live_row && cols > c0) load_packed<W>(res_row + c0, cols - c0, p.vec_res, ahead);
             mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             tc_fence_after();
             const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * BN;
 #pragma unroll 1
-            for (int c = 0; c < cols; c += W) {
+            for (int c = c0; c < cols; c += 2 * W) {
                 float v[W], up[PAIR ? W : 1];
                 tmem_ld32(t + c, v);
                 if constexpr (PAIR) tmem_ld32(t + UNITS + c, up);
@@ -206,7 +207,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                 if (res_row) {
 #pragma unroll
                     for (int e = 0; e < W / 2; ++e) res[e] = ahead[e];
-                    if (live_row && left > W) load_packed<W>(res_row + c + W, left - W, p.vec_res, ahead);
+                    if (live_row && left > 2 * W) load_packed<W>(res_row + c + 2 * W, left - 2 * W, p.vec_res, ahead);
                 }
                 tmem_ld_wait();
                 if (live_row && !*abort_flag) {
@@ -293,9 +294,9 @@ template <int BN, bool PAIR>
 static cudaError_t launch_linear_tile(const LinearArgs& a, LtParams& p, cudaStream_t stream) {
     constexpr int UNITS = PAIR ? BN / 2 : BN;
     alignas(64) CUtensorMap mx, w0, w1;
-    if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, 128) || !encode_rows(&w0, a.W, a.N, a.K, a.K, BN / 2) ||
-        !encode_rows(&w1, PAIR ? a.W + (long long)a.N * a.K : a.W, a.N, a.K, a.K, BN / 2))
-        return cudaErrorInvalidValue;
+    if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, 128) || !encode_rows(&w0, a.W, a.N, a.K, a.K, BN / 2)) return cudaErrorInvalidValue;
+    if (!PAIR) w1 = w0;
+    else if (!encode_rows(&w1, a.W + (long long)a.N * a.K, a.N, a.K, a.K, BN / 2)) return cudaErrorInvalidValue;
     static std::atomic<bool> configured[64];
     if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR>, LtSmem<BN>::kBytes, configured)) return e;
     p.tiles_m = (a.M + 255) / 256, p.tiles_n = (a.N + UNITS - 1) / UNITS;

@@ -55,9 +55,9 @@ class LinearOp(Op):
                                                          residual=self.residual, out_dtype=out_dtype)
 
     def forward(self, X, W, bias=None, residual=None, out=None):
-        for name, given, expected in (("bias", bias, self.bias), ("residual", residual, self.residual)):
-            if (given is not None) != expected:
-                raise ValueError(f"the operator was made {'with' if expected else 'without'} a {name}")
+        if (bias is None) is self.bias or (residual is None) is self.residual:
+            name, expected = ("bias", self.bias) if (bias is None) is self.bias else ("residual", self.residual)
+            raise ValueError(f"the operator was made {'with' if expected else 'without'} a {name}")
         return self._kernel(X, W, bias, residual, out)
 
     def check(self, actual, expected) -> bool:
