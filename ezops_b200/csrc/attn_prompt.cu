@@ -47,6 +47,7 @@ struct ApParams {
 };
 
 // ---- wrappers -----------------------------------------------------------------
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
@@ -120,10 +121,13 @@ __device__ __forceinline__ long long ap_unit_start(const ApParams& p, const ApRo
 }
 
 struct ApLine {
-    long long total;
+    long long total, share;
     int ctas;  // CTAs that take a share
 };
-__device__ __forceinline__ long long ap_share(const ApLine& l, int c) { return l.total * c / l.ctas; }
+__device__ __forceinline__ long long ap_share(const ApLine& l, int c) {  // where CTA c's share starts
+    const long long x = l.share * c;
+    return x < l.total ? x : l.total;
+}
 
 struct ApCursor {
     int b, h, j;
@@ -177,18 +181,22 @@ __device__ __forceinline__ bool ap_segment(const ApParams& p, const ApLine& line
         while (s.c1 + 1 < line.ctas && ap_tile_at(ap_share(line, s.c1 + 1), c.x0, s.tiles) < s.tiles) ++s.c1;
     return true;
 }
-// Next unit; false at the end of the batch.
-__device__ __forceinline__ bool ap_advance(const ApParams& p, ApCursor& c) {
+// Next unit; false at the end of the batch.  Called by a whole warp: rows without tokens are passed over 32 at a time.
+__device__ __forceinline__ bool ap_advance(const ApParams& p, ApCursor& c, int lane) {
     c.x0 += c.row.per_unit + (long long)(c.j + 1) * 2 * p.tpt;
     if (++c.j < c.row.units) return true;
     c.j = 0;
     if (++c.h < p.NKV) return true;
     c.h = 0;
-    do {
-        if (++c.b >= p.B) return false;
-        c.row = ap_row(p, c.b);
-    } while (c.row.units == 0);
-    return true;
+    for (int b = c.b + 1; b < p.B; b += 32) {
+        const uint32_t some = __ballot_sync(0xffffffffu, b + lane < p.B && ap_row(p, min(b + lane, p.B - 1)).units > 0);
+        if (some) {
+            c.b = b + __ffs(some) - 1;
+            c.row = ap_row(p, c.b);
+            return true;
+        }
+    }
+    return false;
 }
 
 template <int D>
@@ -208,7 +216,8 @@ struct ApTail {
     ApSegment seg[kApSegments];
     uint32_t tmem;
     int abort_flag;
-    int last;  // this CTA joins the parts of the unit
+    int published;  // descriptors in all, once they are all there (before: -1)
+    int last;       // this CTA joins the parts of the unit
     int parts;
     short list[160];  // parts of a unit in the order of its keys: twice their slot
     union {
@@ -224,7 +233,7 @@ static_assert(sizeof(ApTail) <= 2048, "tail of the shared memory");
 // Joins the n parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by the softmax
 // threads that wrote them.  A thread keeps one row of the unit (rows rounded up to a power of two) and D / (threads / rows)
 // neighbouring columns of
-// it, 16 at a time (4 when there are few rows); what it loads of two parts is on its way together.  Not inlined: its registers
+// it, 32 at a time (4 when there are few rows); what it loads of two parts is on its way together.  Not inlined: its registers
 // would be taken from the loop over the keys.
 template <int D, int W>  // W groups of four columns at a time
 __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const short* list, int n, int tid, int threads) {
@@ -275,8 +284,10 @@ __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, co
             w[2 * e] = any ? pack_bf16(acc[e].x * inv, acc[e].y * inv) : 0u;
             w[2 * e + 1] = any ? pack_bf16(acc[e].z * inv, acc[e].w * inv) : 0u;
         }
-        if constexpr (W == 4) store_row16(out + g0 * 4, w, p.out32);
-        else *reinterpret_cast<uint2*>(out + g0 * 4) = make_uint2(w[0], w[1]);
+        if constexpr (W > 1) {
+#pragma unroll
+            for (int e = 0; e < W / 4; ++e) store_row16(out + (g0 + 4 * e) * 4, reinterpret_cast<const uint32_t(&)[8]>(w[8 * e]), p.out32);
+        } else *reinterpret_cast<uint2*>(out + g0 * 4) = make_uint2(w[0], w[1]);
     }
 }
 
@@ -305,8 +316,11 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         }
         for (int i = 0; i < kApSegments; ++i)
             mbar_init(smem_u32(&t.seg_full[i]), 1), mbar_init(smem_u32(&t.seg_empty[i]), 10);  // warps that read it
-        t.abort_flag = 0;
+        t.abort_flag = 0, t.published = -1;
         mbar_fence_init();
+    }
+    if (tid == 32) {
+        prefetch_map(&mapQ), prefetch_map(&mapK), prefetch_map(&mapV);
     }
     pdl_open(1);
 
@@ -332,8 +346,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
         return before + s - v;
     };
     long long total = 0, first_cost = 0, first_prefix = 0;
+    ApRow first_row = {};  // of the first rows, one per thread: all there are, mostly
+    if (tid < p.B) first_row = ap_row(p, tid);
     for (int b0 = 0; b0 < p.B; b0 += kApThreads) {
-        const long long v = row_cost(b0 + tid);
+        const long long v = b0 == 0 ? first_row.head_cost * p.NKV : row_cost(b0 + tid);
         long long sum;
         const long long pre = chunk_scan(v, sum);
         if (b0 == 0) first_cost = v, first_prefix = pre;
@@ -341,10 +357,9 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
     }
     ApLine line;
     line.total = total;
-    {
-        const long long want = total / kApMinShare;
-        line.ctas = want < 1 ? 1 : (want < gridDim.x ? (int)want : (int)gridDim.x);
-    }
+    line.share = (total + gridDim.x - 1) / gridDim.x;
+    if (line.share < kApMinShare) line.share = kApMinShare;
+    line.ctas = (int)min((long long)gridDim.x, (total + line.share - 1) / line.share);
     const bool idle = total == 0 || cta >= line.ctas;
     const long long lo = idle ? 0 : ap_share(line, cta), hi = idle ? 0 : ap_share(line, cta + 1);
     if (!idle) {
@@ -359,8 +374,10 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
             if (v > 0 && x <= lo && lo < x + v) {
                 ApCursor c;
                 c.b = b0 + tid;
-                c.row = ap_row(p, c.b);
-                c.h = (int)((lo - x) / c.row.head_cost);
+                c.row = b0 == 0 ? first_row : ap_row(p, c.b);
+                c.h = (int)((float)(lo - x) / (float)c.row.head_cost);  // at most one off, below
+                if (c.h >= p.NKV || c.h * c.row.head_cost > lo - x) --c.h;
+                else if ((c.h + 1) * c.row.head_cost <= lo - x) ++c.h;
                 const long long rem = (lo - x) - c.h * c.row.head_cost;
                 int a = 0, z = c.row.units;  // last unit that starts at or before rem
                 while (z - a > 1) {
@@ -389,8 +406,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
     int n_seg = 0;
     auto next_segment = [&]() -> const ApSegment* {
         const int i = n_seg % kApSegments;
-        if (!mbar_wait_bounded(smem_u32(&t.seg_full[i]), (uint32_t)((n_seg / kApSegments) & 1), abort_flag, p.status, FAULT_PROMPT_WAIT))
-            return nullptr;
+        if (!mbar_wait_bounded(smem_u32(&t.seg_full[i]), (uint32_t)((n_seg / kApSegments) & 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) {
+            // Some wait has run out.  Warps that meet at barriers have to leave behind the same descriptor: the last one there is.
+            const long long t0 = clock64();
+            while (*(volatile int*)&t.published < 0)
+                if (clock64() - t0 > kWaitLimitCycles) return nullptr;
+            if (n_seg >= *(volatile int*)&t.published) return nullptr;
+        }
         return t.seg[i].cnt < 0 ? nullptr : &t.seg[i];
     };
     auto release = [&]() {
@@ -404,21 +426,24 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
     if (idle) {
     } else if (warp == 10) {
         // ------------------------------------------------------------ work descriptors
-        if (lane == 0) {
-            ApCursor cur = t.start;
-            for (bool more = true;; more = more && ap_advance(p, cur)) {
-                const bool end = !more || cur.x0 >= hi;
-                ApSegment s;
-                s.cnt = -1;
-                if (!end && !ap_segment(p, line, cur, cta, lo, hi, s)) continue;
-                const int i = n_seg % kApSegments;
-                if (!mbar_wait_bounded(smem_u32(&t.seg_empty[i]), (uint32_t)(((n_seg / kApSegments) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+        ApCursor cur = t.start;
+        for (bool more = true;; more = more && ap_advance(p, cur, lane)) {
+            const bool end = !more || cur.x0 >= hi;
+            ApSegment s;
+            s.cnt = -1;
+            if (!end && !ap_segment(p, line, cur, cta, lo, hi, s)) continue;
+            const int i = n_seg % kApSegments;
+            if (!mbar_wait_bounded(smem_u32(&t.seg_empty[i]), (uint32_t)(((n_seg / kApSegments) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+            if (lane == 0) {
                 t.seg[i] = s;
                 mbar_arrive(smem_u32(&t.seg_full[i]));
-                ++n_seg;
-                if (end) break;
             }
+            __syncwarp();
+            ++n_seg;
+            if (end) break;
         }
+        __threadfence_block();
+        if (lane == 0) *(volatile int*)&t.published = n_seg;
     } else if (warp == 8) {
         // ------------------------------------------------------------ TMA producer
         int it = 0, n_q = 0, n_fix = 0;  // ring tiles, query loads, repaired tiles so far
@@ -826,7 +851,7 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                     }
                     named_bar_sync(dual ? 2 : 1, writers);
                     if (t.last && !*abort_flag) {
-                        if (seg.tokens * p.G > 8) ap_join<D, 4>(p, seg, t.list, t.parts, tid, writers);
+                        if (seg.tokens * p.G > 16) ap_join<D, 8>(p, seg, t.list, t.parts, tid, writers);
                         else ap_join<D, 1>(p, seg, t.list, t.parts, tid, writers);
                     }
                     named_bar_sync(dual ? 2 : 1, writers);  // the list and the flag are free again

@@ -257,6 +257,16 @@ def test_linear_many_tiles(M, N, K, act):
     linear_case(M, N, K, act, residual=act is None)
 
 
+@pytest.mark.parametrize("M", [1, 17, 64])
+@pytest.mark.parametrize("out_dtype", [BF16, torch.float32])
+def test_linear_few_rows_many_tiles(M, out_dtype):
+    """Several rounds of tiles per CTA, tiles cut along K and not, results that are no multiple of a tile."""
+    linear_case(M, 60001, 64, bias=True, residual=True, out_dtype=out_dtype)
+    linear_case(M, 30000, 200, act="silu", out_dtype=out_dtype)
+    linear_case(M, 20008, 136, act="swiglu", bias=True, out_dtype=out_dtype)
+    linear_case(M, 520, 8192, bias=True, out_dtype=out_dtype)
+
+
 @pytest.mark.parametrize("M", [3, 500])
 def test_linear_strides_and_in_place_residual(M):
     N, K = 200, 136
@@ -456,6 +466,21 @@ def test_attn_many_rows(B, low, high):
     new = torch.randint(low, high + 1, (B,), generator=g).tolist()
     ctx = torch.randint(0, 200, (B,), generator=g).tolist()
     attn_case(new, ctx, 4, 2, 64, 64)
+
+
+def test_attn_few_tokens_among_many_empty_rows():
+    B = 5000
+    new, ctx = [0] * B, [0] * B
+    for b, (n, c) in {3: (40, 0), 4: (1, 500), 777: (200, 100), 4095: (1, 0), 4999: (70, 64)}.items():
+        new[b], ctx[b] = n, c
+    attn_case(new, ctx, 8, 2, 128, 64)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_attn_one_long_row_for_many_ctas(D):
+    """A few queries behind a long context: every CTA has a part of the same unit, odd counts of blocks in each."""
+    for new, ctx in ([2], [30000]), ([33], [9999]), ([1, 1], [12800, 128 * 37 - 1]), ([40, 1], [5000, 63]):
+        attn_case(new, ctx, 8, 1, D, 128)
 
 
 def test_attn_long_rows_are_cut_and_joined():
