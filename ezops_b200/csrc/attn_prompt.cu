@@ -232,10 +232,9 @@ static_assert(sizeof(ApTail) <= 2048, "tail of the shared memory");
 
 // Joins the n parts of a unit: out = sum_k w_k O_k / sum_k w_k sum_k with w_k = exp2(scale (max_k - max)), by the softmax
 // threads that wrote them.  A thread keeps one row of the unit (rows rounded up to a power of two) and D / (threads / rows)
-// neighbouring columns of
-// it, 32 at a time (4 when there are few rows); what it loads of two parts is on its way together.  Not inlined: its registers
-// would be taken from the loop over the keys.
-template <int D, int W>  // W groups of four columns at a time
+// neighbouring columns of it, 4 W at a time; what it loads of U parts is on its way together.  Not inlined: its registers would
+// be taken from the loop over the keys.
+template <int D, int W, int U>
 __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, const short* list, int n, int tid, int threads) {
     constexpr long long kPart = (long long)(D + 2) * 128;
     const int rows = seg.tokens * p.G, per_tile = p.tpt * p.G;
@@ -245,12 +244,12 @@ __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, co
     const float* base = p.parts + q * kPart;
     const float* stat = base + (long long)D * 128 + rr;
     float top = -INFINITY;
-#pragma unroll 4
+#pragma unroll 8
     for (int k = 0; k < n; ++k) top = fmaxf(top, __ldcg(stat + list[k] * kPart));
     const int token = row / p.G, head = row - token * p.G;
     const bool any = seg.sees + token > 0;  // else the query sees no key
     bf16* out = p.Out + (long long)(seg.token + token) * p.ldo + (long long)(seg.head * p.G + head) * D;
-    const int per = max(W, D / 4 / share);  // groups of this thread
+    const int per = max(W, D / 4 / share);  // groups of four columns of this thread
 #pragma unroll 1
     for (int g0 = (tid >> log_rows) * per, g1 = min(g0 + per, D / 4); g0 < g1; g0 += W) {
         float4 acc[W];
@@ -258,11 +257,11 @@ __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, co
         for (int e = 0; e < W; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
         float all = 0.f;
 #pragma unroll 1
-        for (int k = 0; k < n; k += 2) {
-            float4 o[2][W];
-            float w[2], ps[2];
+        for (int k = 0; k < n; k += U) {
+            float4 o[U][W];
+            float w[U], ps[U];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const long long at = list[min(k + u, n - 1)] * kPart;
                 const float4* part = reinterpret_cast<const float4*>(base + at) + rr;
 #pragma unroll
@@ -270,7 +269,7 @@ __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, co
                 w[u] = __ldcg(stat + at), ps[u] = __ldcg(stat + at + 128);
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < U; ++u) {
                 const float f = w[u] == -INFINITY || k + u >= n ? 0.f : exp2_approx((w[u] - top) * p.scale_log2);
                 all += f * ps[u];
 #pragma unroll
@@ -287,7 +286,9 @@ __device__ __noinline__ void ap_join(const ApParams& p, const ApSegment& seg, co
         if constexpr (W > 1) {
 #pragma unroll
             for (int e = 0; e < W / 4; ++e) store_row16(out + (g0 + 4 * e) * 4, reinterpret_cast<const uint32_t(&)[8]>(w[8 * e]), p.out32);
-        } else *reinterpret_cast<uint2*>(out + g0 * 4) = make_uint2(w[0], w[1]);
+        } else {
+            *reinterpret_cast<uint2*>(out + g0 * 4) = make_uint2(w[0], w[1]);
+        }
     }
 }
 
@@ -851,8 +852,9 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                     }
                     named_bar_sync(dual ? 2 : 1, writers);
                     if (t.last && !*abort_flag) {
-                        if (seg.tokens * p.G > 16) ap_join<D, 8>(p, seg, t.list, t.parts, tid, writers);
-                        else ap_join<D, 1>(p, seg, t.list, t.parts, tid, writers);
+                        if (seg.tokens * p.G > 32) ap_join<D, 8, 2>(p, seg, t.list, t.parts, tid, writers);
+                        else if (seg.tokens * p.G > 8) ap_join<D, 4, 4>(p, seg, t.list, t.parts, tid, writers);
+                        else ap_join<D, 1, 8>(p, seg, t.list, t.parts, tid, writers);
                     }
                     named_bar_sync(dual ? 2 : 1, writers);  // the list and the flag are free again
                 }

@@ -30,7 +30,8 @@ struct LtParams {
     long long ldres, ldout;
     int M, N, kblocks;
     int tiles_m, tiles_n, stages, act, out_f32;
-    int vec_out, vec_res, vec_bias;  // rows start at 32-byte (out) or 16-byte boundaries
+    int rows_aligned;  // rows of out start at 32-byte, of residual at 16-byte boundaries
+    int vec_bias;      // so does bias
     unsigned int* status;
 };
 
@@ -74,8 +75,10 @@ struct LtSmem {
     static constexpr int kB = BN / 2 * kLtBlockK * 2;     // this CTA's rows of W
     static constexpr int kStage = kA + kB;
     static constexpr int kTail = 1024;
-    static constexpr int kStages = (232448 - 1024 - kTail) / kStage < kLtMaxStages ? (232448 - 1024 - kTail) / kStage : kLtMaxStages;
-    static constexpr int kBytes = 1024 + kStages * kStage + kTail;
+    static constexpr int kTurn = 8 * 32 * 33 * 4;         // a 32 x 32 block of each epilogue warp
+    static constexpr int kRoom = 232448 - 1024 - kTail - kTurn;
+    static constexpr int kStages = kRoom / kStage < kLtMaxStages ? kRoom / kStage : kLtMaxStages;
+    static constexpr int kBytes = 1024 + kStages * kStage + kTurn + kTail;
 };
 
 // W bf16 values, as they are; beyond `left` zeros.
@@ -105,7 +108,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     extern __shared__ unsigned char lt_raw[];
     const uint32_t raw = smem_u32(lt_raw);
     unsigned char* smem = lt_raw + (((raw + 1023u) & ~1023u) - raw);
-    unsigned char* tail = smem + L::kStages * L::kStage;
+    unsigned char* tail = smem + L::kStages * L::kStage + L::kTurn;
     uint64_t* full = reinterpret_cast<uint64_t*>(tail);
     uint64_t* empty = full + kLtMaxStages;
     uint64_t* acc_full = empty + kLtMaxStages;
@@ -181,6 +184,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         // one step ahead (the first step: before the products are complete), or its latency would be paid once per step.
         constexpr int W = 32;
         const int q = warp & 3, row = q * 32 + lane;
+        float* turn = reinterpret_cast<float*>(smem + L::kStages * L::kStage) + (warp - 2) * 32 * (W + 1);
         const int c0 = ((warp - 2) >> 2) * W;  // two warps share a quarter: every other step each
         int n = 0;
         for (int i = blockIdx.x >> 1; i < n_tiles; i += n_clusters, ++n) {
@@ -191,9 +195,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             const bool live_row = m < p.M;
             const int n0 = tn * UNITS;
             const int cols = min(UNITS, p.N - n0);
-            const bf16* res_row = p.residual ? p.residual + (long long)m * p.ldres + n0 : nullptr;
+            const bf16* res_row = p.residual && p.rows_aligned ? p.residual + (long long)m * p.ldres + n0 : nullptr;
             uint32_t ahead[W / 2];  // residual values of the next step, packed
-            if (res_row && live_row && cols > c0) load_packed<W>(res_row + c0, cols - c0, p.vec_res, ahead);
+            if (res_row && live_row && cols - c0 >= W) load_packed<W>(res_row + c0, W, 1, ahead);
             mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             tc_fence_after();
             const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * BN;
@@ -207,10 +211,11 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                 if (res_row) {
 #pragma unroll
                     for (int e = 0; e < W / 2; ++e) res[e] = ahead[e];
-                    if (live_row && left > 2 * W) load_packed<W>(res_row + c + 2 * W, left - 2 * W, p.vec_res, ahead);
+                    if (live_row && left >= 3 * W) load_packed<W>(res_row + c + 2 * W, W, 1, ahead);
                 }
                 tmem_ld_wait();
-                if (live_row && !*abort_flag) {
+                const bool fine = !__any_sync(0xffffffffu, *abort_flag);
+                if (live_row && fine) {
                     if (p.bias) {
                         uint32_t b[W / 2];
                         load_packed<W>(p.bias + col, left, p.vec_bias, b);
@@ -229,35 +234,41 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
 #pragma unroll
                         for (int e = 0; e < W; ++e) v[e] = linear_act(v[e], p.act);
                     }
-                    if (res_row) {
+                    if (p.rows_aligned && left >= W) {
+                        if (res_row) {
 #pragma unroll
-                        for (int e = 0; e < W; ++e) v[e] += (e & 1) ? bf16_hi(res[e / 2]) : bf16_lo(res[e / 2]);
-                    }
-                    const long long o = (long long)m * p.ldout + col;
-                    if (p.out_f32) {
-                        float* dst = static_cast<float*>(p.out) + o;
-                        if (p.vec_out && left >= W) {
-#pragma unroll
-                            for (int e = 0; e < W; e += 8) store32(dst + e, reinterpret_cast<const uint32_t(&)[8]>(v[e]));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < W; ++e)
-                                if (e < left) dst[e] = v[e];
+                            for (int e = 0; e < W; ++e) v[e] += (e & 1) ? bf16_hi(res[e / 2]) : bf16_lo(res[e / 2]);
                         }
-                    } else {
-                        bf16* dst = static_cast<bf16*>(p.out) + o;
-                        if (p.vec_out && left >= W) {
+                        const long long o = (long long)m * p.ldout + col;
+                        if (p.out_f32) {
+#pragma unroll
+                            for (int e = 0; e < W; e += 8) store32(static_cast<float*>(p.out) + o + e, reinterpret_cast<const uint32_t(&)[8]>(v[e]));
+                        } else {
 #pragma unroll
                             for (int e = 0; e < W; e += 16) {
                                 uint32_t w[8];
 #pragma unroll
                                 for (int k = 0; k < 8; ++k) w[k] = pack_bf16(v[e + 2 * k], v[e + 2 * k + 1]);
-                                store32(dst + e, w);
+                                store32(static_cast<bf16*>(p.out) + o + e, w);
                             }
-                        } else {
+                        }
+                    }
+                }
+                if (!(p.rows_aligned && left >= W) && fine) {
+                    // Rows that start anywhere, or the last columns: the 32 x 32 block turns in shared memory, and a lane has a column.
 #pragma unroll
-                            for (int e = 0; e < W; ++e)
-                                if (e < left) dst[e] = __float2bfloat16_rn(v[e]);
+                    for (int e = 0; e < W; ++e) turn[lane * (W + 1) + e] = v[e];
+                    __syncwarp();
+                    const int rows = min(32, p.M - (m - lane));
+                    if (lane < left) {
+                        const bf16* res_col = p.residual ? p.residual + (long long)(m - lane) * p.ldres + col + lane : nullptr;
+                        const long long o = (long long)(m - lane) * p.ldout + col + lane;
+#pragma unroll 4
+                        for (int r = 0; r < rows; ++r) {
+                            float x = turn[r * (W + 1) + lane];
+                            if (res_col) x += __bfloat162float(res_col[r * p.ldres]);
+                            if (p.out_f32) static_cast<float*>(p.out)[o + r * p.ldout] = x;
+                            else static_cast<bf16*>(p.out)[o + r * p.ldout] = __float2bfloat16_rn(x);
                         }
                     }
                 }
@@ -312,8 +323,8 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
     p.bias = a.bias, p.residual = a.residual, p.out = a.out, p.ldres = a.ldres, p.ldout = a.ldout;
     p.M = a.M, p.N = a.N, p.kblocks = (a.K + kLtBlockK - 1) / kLtBlockK;
     p.act = a.act, p.out_f32 = a.out_f32;
-    p.vec_out = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.ldout % (a.out_f32 ? 8 : 16) == 0;
-    p.vec_res = a.residual && aligned16(a.residual) && a.ldres % 8 == 0;
+    p.rows_aligned = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0 && a.ldout % (a.out_f32 ? 8 : 16) == 0 &&
+                     (!a.residual || (aligned16(a.residual) && a.ldres % 8 == 0));
     p.vec_bias = a.bias && aligned16(a.bias) && (a.act != ACT_SWIGLU || a.N % 8 == 0);
     p.status = status_ptr();
     if (!p.status) return cudaErrorUnknown;
