@@ -316,9 +316,12 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                             r8[e] = p.residual && own && b_half + c + e < p.B ? __bfloat162float(p.residual[(long long)(b_half + c + e) * p.ldres + n_own]) : 0.f;
                         tmem_ld_wait();
 #pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += bias;
+                        linear_act(v, p.act);
+#pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             if (own && b_half + c + e < p.B) {
-                                const float x = linear_act(v[e] + bias, p.act) + r8[e];
+                                const float x = v[e] + r8[e];
                                 const long long o = (long long)(b_half + c + e) * p.ldout + n_own;
                                 if (p.out_f32) static_cast<float*>(p.out)[o] = x;
                                 else static_cast<bf16*>(p.out)[o] = __float2bfloat16_rn(x);
@@ -397,11 +400,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                         if (p.pair) gather(col, frow + p.half_rows, up);
                         if (p.residual && col != cg) fetch_residual(col);
 #pragma unroll
+                        for (int u = 0; u < CU; ++u) v[u] += b0;
+                        linear_act(v, p.act);
+#pragma unroll
                         for (int u = 0; u < CU; ++u) {
                             const int c = col + u * groups;
                             if (c < n_cols) {
-                                float x = v[u] + b0;
-                                x = p.pair ? silu_f32(x) * (up[u] + b1) : linear_act(x, p.act);
+                                float x = p.pair ? silu_fast(v[u]) * (up[u] + b1) : v[u];
                                 if (p.residual) x += res[u];
                                 const long long o = (long long)(b_first + c) * p.ldout + n;
                                 if (p.out_f32) static_cast<float*>(p.out)[o] = x;

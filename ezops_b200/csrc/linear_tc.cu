@@ -22,6 +22,7 @@ namespace ezb {
 static constexpr int kLtThreads = 320;  // TMA warp, MMA warp, eight epilogue warps
 static constexpr int kLtBlockK = 64;
 static constexpr int kLtMaxStages = 12;
+static constexpr int kLtCountBytes = 4096;  // counters in front of the parts
 static constexpr int kLtGroup = 8;  // row tiles per group of the tile order
 
 struct LtParams {
@@ -32,7 +33,36 @@ struct LtParams {
     int tiles_m, tiles_n, stages, act, out_f32;
     int rows_aligned;  // rows of out start at 32-byte, of residual at 16-byte boundaries
     int vec_bias;      // so does bias
+    // Tiles from sk_first on are cut: their kblocks form one line, and every cluster takes the same length of it.
+    int sk_first;
+    int sk_units, sk_share;  // k blocks on the line, and of a cluster
+    float* parts;         // [2 * clusters slots][2 CTAs][BN][128] fp32
+    unsigned int* count;  // [clusters][2 CTAs], zero between calls
     unsigned int* status;
+};
+// Where cluster c's length of the line starts.
+__device__ __forceinline__ int lt_share(const LtParams& p, int c) { return min(p.sk_units, c * p.sk_share); }
+// What a cluster works off: first its pieces of cut tiles, then whole tiles.
+struct LtWork {
+    int x, end;        // on the line
+    int next;          // whole tile
+    int tile, k0, k1;  // the piece: k blocks of a tile
+    bool part;
+    __device__ __forceinline__ void start(const LtParams& p, int cluster) {
+        x = lt_share(p, cluster), end = lt_share(p, cluster + 1), next = cluster;
+    }
+    __device__ __forceinline__ bool step(const LtParams& p, int clusters) {
+        if (x < end) {
+            const int t = x / p.kblocks, first = t * p.kblocks;
+            tile = p.sk_first + t, k0 = x - first, k1 = min(end - first, p.kblocks);
+            x = first + k1;
+            part = k1 - k0 < p.kblocks;
+            return true;
+        }
+        if (next >= p.sk_first) return false;
+        tile = next, next += clusters, k0 = 0, k1 = p.kblocks, part = false;
+        return true;
+    }
 };
 
 // ---- cta_group::2 wrappers ------------------------------------------------------
@@ -115,6 +145,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* last = abort_flag + 1;  // this CTA joins the parts of its rows of a tile
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int rank = (int)cluster_rank();
 
@@ -135,7 +166,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     const uint32_t tmem = *tmem_slot;
     pdl_open(1);
 
-    const int n_tiles = p.tiles_m * p.tiles_n, n_clusters = gridDim.x >> 1;
+    const int n_clusters = gridDim.x >> 1, cluster = blockIdx.x >> 1;
+    LtWork work;
+    work.start(p, cluster);
     auto tile_at = [&](int i, int& m, int& n) {  // groups of kLtGroup row tiles, column tile by column tile
         const int per = kLtGroup * p.tiles_n, g = i / per, rows = min(kLtGroup, p.tiles_m - g * kLtGroup), r = i - g * per;
         m = g * kLtGroup + r % rows, n = r / rows;
@@ -143,13 +176,13 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     if (warp == 0) {
         if (elect_one()) {
             int it = 0;
-            for (int i = blockIdx.x >> 1; i < n_tiles && !*abort_flag; i += n_clusters) {
+            while (!*abort_flag && work.step(p, n_clusters)) {
                 int tm, tn;
-                tile_at(i, tm, tn);
+                tile_at(work.tile, tm, tn);
                 const int y_x = tm * 256 + rank * 128;
                 const CUtensorMap* mapB = PAIR && rank ? &mapW1 : &mapW0;  // SwiGLU: the second CTA brings the up rows
                 const int y_w = PAIR ? tn * UNITS : tn * BN + rank * (BN / 2);
-                for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+                for (int kb = work.k0; kb < work.k1; ++kb, ++it) {
                     const int s = it % L::kStages;
                     if (!mbar_wait_bounded(smem_u32(&empty[s]), (uint32_t)(((it / L::kStages) & 1) ^ 1), abort_flag, p.status, FAULT_GEMV_EMPTY_WAIT)) break;
                     const uint32_t bar = smem_u32(&full[s]), a = smem_u32(smem) + s * L::kStage;
@@ -162,18 +195,18 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
             int it = 0, n = 0;
-            for (int i = blockIdx.x >> 1; i < n_tiles && !*abort_flag; i += n_clusters, ++n) {
+            for (; !*abort_flag && work.step(p, n_clusters); ++n) {
                 const int acc = n & 1;
                 if (!mbar_wait_bounded_cluster(smem_u32(&acc_empty[acc]), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, p.status, FAULT_TC_ACC_WAIT)) break;
                 tc_fence_after();
-                for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
+                for (int kb = work.k0; kb < work.k1; ++kb, ++it) {
                     const int s = it % L::kStages;
                     if (!mbar_wait_bounded_cluster(smem_u32(&full[s]), (uint32_t)((it / L::kStages) & 1), abort_flag, p.status, FAULT_GEMV_FULL_WAIT)) break;
                     tc_fence_after();
                     const uint32_t a = smem_u32(smem) + s * L::kStage;
                     const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + L::kA);
 #pragma unroll
-                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * BN, ad + 2 * k, bd + 2 * k, IDESC, kb > 0 || k > 0);
+                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * BN, ad + 2 * k, bd + 2 * k, IDESC, kb > work.k0 || k > 0);
                     tc_commit_pair(smem_u32(&empty[s]));
                 }
                 tc_commit_pair(smem_u32(&acc_full[acc]));
@@ -186,10 +219,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         const int q = warp & 3, row = q * 32 + lane;
         float* turn = reinterpret_cast<float*>(smem + L::kStages * L::kStage) + (warp - 2) * 32 * (W + 1);
         const int c0 = ((warp - 2) >> 2) * W;  // two warps share a quarter: every other step each
-        int n = 0;
-        for (int i = blockIdx.x >> 1; i < n_tiles; i += n_clusters, ++n) {
+        for (int n = 0; work.step(p, n_clusters); ++n) {
             int tm, tn;
-            tile_at(i, tm, tn);
+            tile_at(work.tile, tm, tn);
             const int acc = n & 1;
             const int m = tm * 256 + rank * 128 + row;
             const bool live_row = m < p.M;
@@ -201,11 +233,68 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             tc_fence_after();
             const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * BN;
+            auto drained = [&]() {
+                __syncwarp();
+                tc_fence_before();
+                if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[acc]), 0));
+            };
+            // A part: into the workspace, [group of four columns][row]; who adds the last one of a tile joins them in the order of K.
+            int first = cluster, n_parts = 0;  // the clusters first .. first + n_parts - 1 have one
+            auto part_of = [&](int c) {
+                return reinterpret_cast<const float4*>(p.parts) + ((long long)((2 * c + (c == first ? 1 : 0)) * 2 + rank) * (BN / 4)) * 128 + row;
+            };
+            if (work.part) {
+                const int tile0 = (work.tile - p.sk_first) * p.kblocks, tile1 = tile0 + p.kblocks;
+                while (first > 0 && lt_share(p, first) > tile0) --first;
+                int end = cluster + 1;
+                while (end < n_clusters && lt_share(p, end) < tile1) ++end;
+                n_parts = end - first;
+                float4* mine = const_cast<float4*>(part_of(cluster));
+#pragma unroll 1
+                for (int c = c0; c < BN; c += 2 * W) {
+                    float v[W];
+                    tmem_ld32(t + c, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < W; e += 4) __stcg(mine + (c + e) / 4 * 128, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
+                }
+                drained();
+                named_bar_sync(1, kLtThreads - 64);  // behind it one thread speaks for all
+                if (tid == 64) {
+                    __threadfence();
+                    unsigned int* count = p.count + 2 * first + rank;  // one tile at most is cut that starts in a cluster's length
+                    const unsigned int done = atomicAdd(count, (unsigned)(work.k1 - work.k0)) + (unsigned)(work.k1 - work.k0);
+                    *last = done == (unsigned)p.kblocks;
+                    if (*last) *count = 0u;
+                    __threadfence();
+                }
+                named_bar_sync(1, kLtThreads - 64);
+                const bool join = *last;
+                named_bar_sync(1, kLtThreads - 64);  // the flag is free again
+                if (!join) continue;
+            }
+            auto columns = [&](int at, float* v) {  // W sums of this row
+                if (!work.part) {
+                    tmem_ld32(t + at, v);
+                    return;
+                }
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[e] = 0.f;
+#pragma unroll 1
+                for (int i = 0; i < n_parts; ++i) {
+                    const float4* part = part_of(first + i) + at / 4 * 128;
+#pragma unroll
+                    for (int e = 0; e < W; e += 4) {
+                        const float4 x = __ldcg(part + e / 4 * 128);
+                        v[e] += x.x, v[e + 1] += x.y, v[e + 2] += x.z, v[e + 3] += x.w;
+                    }
+                }
+            };
 #pragma unroll 1
             for (int c = c0; c < cols; c += 2 * W) {
                 float v[W], up[PAIR ? W : 1];
-                tmem_ld32(t + c, v);
-                if constexpr (PAIR) tmem_ld32(t + UNITS + c, up);
+                columns(c, v);
+                if constexpr (PAIR) columns(UNITS + c, up);
                 const int left = cols - c, col = n0 + c;
                 uint32_t res[W / 2];
                 if (res_row) {
@@ -229,10 +318,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                     }
                     if constexpr (PAIR) {
 #pragma unroll
-                        for (int e = 0; e < W; ++e) v[e] = silu_f32(v[e]) * up[e];
+                        for (int e = 0; e < W; ++e) v[e] = silu_fast(v[e]) * up[e];
                     } else if (p.act != ACT_NONE) {
-#pragma unroll
-                        for (int e = 0; e < W; ++e) v[e] = linear_act(v[e], p.act);
+                        linear_act(v, p.act);
                     }
                     if (p.rows_aligned && left >= W) {
                         if (res_row) {
@@ -263,20 +351,24 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                     if (lane < left) {
                         const bf16* res_col = p.residual ? p.residual + (long long)(m - lane) * p.ldres + col + lane : nullptr;
                         const long long o = (long long)(m - lane) * p.ldout + col + lane;
-#pragma unroll 4
-                        for (int r = 0; r < rows; ++r) {
-                            float x = turn[r * (W + 1) + lane];
-                            if (res_col) x += __bfloat162float(res_col[r * p.ldres]);
-                            if (p.out_f32) static_cast<float*>(p.out)[o + r * p.ldout] = x;
-                            else static_cast<bf16*>(p.out)[o + r * p.ldout] = __float2bfloat16_rn(x);
+#pragma unroll 1
+                        for (int r0 = 0; r0 < rows; r0 += 16) {
+                            float x[16];  // 16 rows on their way at a time
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) x[r] = res_col && r0 + r < rows ? __bfloat162float(res_col[(r0 + r) * p.ldres]) : 0.f;
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) {
+                                if (r0 + r >= rows) break;
+                                const float y = turn[(r0 + r) * (W + 1) + lane] + x[r];
+                                if (p.out_f32) static_cast<float*>(p.out)[o + (r0 + r) * p.ldout] = y;
+                                else static_cast<bf16*>(p.out)[o + (r0 + r) * p.ldout] = __float2bfloat16_rn(y);
+                            }
                         }
                     }
                 }
                 __syncwarp();
             }
-            __syncwarp();
-            tc_fence_before();
-            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[acc]), 0));
+            if (!work.part) drained();
         }
     }
     __syncwarp();
@@ -301,8 +393,48 @@ static bool encode_rows(CUtensorMap* map, const bf16* base, long long rows, long
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The width of the tiles, and whether they are cut along K.  A k block of a tile costs a cluster what its two SMs need to bring the
+// operands in (measured 520, 490 and 410 cycles for 256, 128 and 64 columns), so the widest tile that leaves no more rounds is
+// taken.  Few outputs behind a long K (a router's scores, 44 columns of 555 rows, K = 5544) would be left to a handful of
+// clusters: there up to kLtMostParts of them share a tile (24.4 -> 14.4 us).  Wider or shorter products are not cut: writing the
+// parts and joining them in one SM takes longer than the clusters are idle (N = 4096, K = 4096: 256 rows 13.6 us on whole tiles,
+// 29.3 cut; 138 rows of 176 outputs, K = 2248: 12.5 and 17.1; 3383 rows of 64, K = 4984, 14 tiles: 21.7 and 18.7 to 25).
+struct LtPlan {
+    int bn, clusters, sk_tiles;
+};
+static constexpr int kLtMinBlocks = 8;   // k blocks below which a further cluster does not pay
+static constexpr int kLtMostParts = 8;
+static constexpr int kLtCutTiles = 8;    // most tiles that are cut
+static constexpr int kLtCutBlocks = 64;  // fewest k blocks of a tile that is
+static LtPlan linear_plan(int M, int N, int K, int act, bool cut) {
+    const long long rows = act == ACT_SWIGLU ? 2ll * N : N, tm = (M + 255) / 256, kb = (K + kLtBlockK - 1) / kLtBlockK, most = sm_count() / 2;
+    const int widths[3] = {256, 128, 64};
+    const double block[3] = {520., 490., 410.};
+    LtPlan best = {256, 1, 0};
+    double least = -1.;
+    for (int i = 0; i < 3; ++i) {
+        const long long tiles = tm * ((rows + widths[i] - 1) / widths[i]);
+        const double cost = (double)((tiles + most - 1) / most) * (double)kb * block[i];
+        if (least < 0. || cost < least) least = cost, best = {widths[i], (int)(tiles < most ? tiles : most), 0};
+    }
+    if (cut && best.bn == 64 && best.clusters <= kLtCutTiles && kb >= kLtCutBlocks) {
+        long long clusters = (long long)best.clusters * kLtMostParts, by_blocks = best.clusters * kb / kLtMinBlocks;
+        if (clusters > by_blocks) clusters = by_blocks;
+        if (clusters > most) clusters = most;
+        best.sk_tiles = best.clusters, best.clusters = (int)clusters;
+    }
+    return best;
+}
+
+size_t linear_workspace_bytes(int M, int N, int K, int act) {
+    if (M <= kLinearFewRows) return 0;
+    const LtPlan plan = linear_plan(M, N, K, act, true);
+    // one size for all, so that an operator's workspace never has to grow under a captured graph
+    return plan.sk_tiles ? (size_t)kLtCountBytes + (size_t)(sm_count() / 2) * 4 * 256 * 128 * sizeof(float) : 0;
+}
+
 template <int BN, bool PAIR>
-static cudaError_t launch_linear_tile(const LinearArgs& a, LtParams& p, cudaStream_t stream) {
+static cudaError_t launch_linear_tile(const LinearArgs& a, const LtPlan& plan, LtParams& p, cudaStream_t stream) {
     constexpr int UNITS = PAIR ? BN / 2 : BN;
     alignas(64) CUtensorMap mx, w0, w1;
     if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, 128) || !encode_rows(&w0, a.W, a.N, a.K, a.K, BN / 2)) return cudaErrorInvalidValue;
@@ -311,10 +443,10 @@ static cudaError_t launch_linear_tile(const LinearArgs& a, LtParams& p, cudaStre
     static std::atomic<bool> configured[64];
     if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR>, LtSmem<BN>::kBytes, configured)) return e;
     p.tiles_m = (a.M + 255) / 256, p.tiles_n = (a.N + UNITS - 1) / UNITS;
-    const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    const int clusters = (int)(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
+    p.sk_first = p.tiles_m * p.tiles_n - plan.sk_tiles, p.sk_units = plan.sk_tiles * p.kblocks;
+    p.sk_share = (p.sk_units + plan.clusters - 1) / plan.clusters;
     chain_begin();
-    return launch_pdl_cluster(linear_tc_kernel<BN, PAIR>, dim3(2u * clusters), dim3(kLtThreads), 2, LtSmem<BN>::kBytes, stream, mx, w0, w1, p);
+    return launch_pdl_cluster(linear_tc_kernel<BN, PAIR>, dim3(2u * plan.clusters), dim3(kLtThreads), 2, LtSmem<BN>::kBytes, stream, mx, w0, w1, p);
 }
 
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
@@ -328,17 +460,13 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
     p.vec_bias = a.bias && aligned16(a.bias) && (a.act != ACT_SWIGLU || a.N % 8 == 0);
     p.status = status_ptr();
     if (!p.status) return cudaErrorUnknown;
-    // The width of a tile: rounds of tiles over the clusters times what a tile of that width costs.
+    const LtPlan plan = linear_plan(a.M, a.N, a.K, a.act, a.workspace != nullptr);
+    p.count = static_cast<unsigned int*>(a.workspace);
+    p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + kLtCountBytes);
     const bool pair = a.act == ACT_SWIGLU;
-    const long long rows = pair ? 2ll * a.N : a.N, tm = (a.M + 255) / 256, clusters = sm_count() / 2;
-    auto cost = [&](int bn, double per_block) {
-        const long long tiles = tm * ((rows + bn - 1) / bn);
-        return (double)((tiles + clusters - 1) / clusters) * per_block;
-    };
-    const double c256 = cost(256, 256.), c128 = cost(128, 160.), c64 = cost(64, 110.);
-    if (c256 <= c128 && c256 <= c64) return pair ? launch_linear_tile<256, true>(a, p, stream) : launch_linear_tile<256, false>(a, p, stream);
-    if (c128 <= c64) return pair ? launch_linear_tile<128, true>(a, p, stream) : launch_linear_tile<128, false>(a, p, stream);
-    return pair ? launch_linear_tile<64, true>(a, p, stream) : launch_linear_tile<64, false>(a, p, stream);
+    if (plan.bn == 256) return pair ? launch_linear_tile<256, true>(a, plan, p, stream) : launch_linear_tile<256, false>(a, plan, p, stream);
+    if (plan.bn == 128) return pair ? launch_linear_tile<128, true>(a, plan, p, stream) : launch_linear_tile<128, false>(a, plan, p, stream);
+    return pair ? launch_linear_tile<64, true>(a, plan, p, stream) : launch_linear_tile<64, false>(a, plan, p, stream);
 }
 
 }  // namespace ezb

@@ -134,7 +134,7 @@ def test_attention_reference_query_by_query():
 def test_c_entries_refuse_without_a_gpu():
     lib, P = _lib.load(), ctypes.c_void_p
     a, b, c, odd = P(0x100000), P(0x2000000), P(0x4000000), P(0x4000002)
-    bad, shape, ws = _lib.EZB_ERR_INVALID_ARGUMENT, _lib.EZB_ERR_UNSUPPORTED_SHAPE, _lib.EZB_ERR_WORKSPACE
+    bad, shape, none = _lib.EZB_ERR_INVALID_ARGUMENT, _lib.EZB_ERR_UNSUPPORTED_SHAPE, _lib.EZB_ERR_WORKSPACE
 
     def plan(*sizes, out=c, ctx=a):
         outs = [P(out.value + 0x100000 * i) for i in range(5)]
@@ -158,9 +158,9 @@ def test_c_entries_refuse_without_a_gpu():
     assert rope(ld=500) == bad and rope(ld=516) == bad and rope(qkv=odd) == bad and rope(out=a) == bad
     assert rope(pages=1 << 25) == shape
 
-    def linear(M=4, N=8, K=16, X=a, ldx=None, W=b, bias=None, res=None, ldres=None, out=c, ldout=None, act=0, f32=0):
+    def linear(M=4, N=8, K=16, X=a, ldx=None, W=b, bias=None, res=None, ldres=None, out=c, ldout=None, act=0, f32=0, ws=None, size=0):
         return lib.ezb_linear_bf16(X, K if ldx is None else ldx, W, bias, res, N if ldres is None else ldres, out,
-                                   N if ldout is None else ldout, M, N, K, act, f32, None)
+                                   N if ldout is None else ldout, ws, size, M, N, K, act, f32, None)
 
     assert linear(M=0) == bad and linear(K=12) == shape and linear(act=5) == bad and linear(act=-1) == bad
     assert linear(X=odd) == bad and linear(W=odd) == bad and linear(ldx=8) == bad and linear(ldx=20) == bad and linear(ldout=7) == bad
@@ -169,6 +169,11 @@ def test_c_entries_refuse_without_a_gpu():
     assert linear(res=P(0x4000010)) == bad and linear(res=c, ldres=9) == bad and linear(res=c, f32=1) == bad
     assert b"overlaps residual" in lib.ezb_last_error_message()
     assert linear(M=1 << 30, N=1 << 30) == shape
+    need = lib.ezb_linear_workspace_bytes(100, 8, 8192, 0)
+    assert need > 0 and lib.ezb_linear_workspace_bytes(64, 8, 8192, 0) == 0 and lib.ezb_linear_workspace_bytes(0, 8, 8192, 0) == 0
+    far = P(0x40000000)
+    assert linear(M=100, K=8192, out=far, ws=P(0x80000000), size=need - 1) == _lib.EZB_ERR_WORKSPACE
+    assert linear(M=100, K=8192, out=far, ws=P(0x80000004), size=need) == _lib.EZB_ERR_WORKSPACE
 
     def attn(B=2, T=8, H=4, NKV=2, D=64, max_pages=4, page=64, pages=9, Q=a, ldq=256, out=c, ldo=256, w=b, size=1 << 30):
         return lib.ezb_attn_prompt(Q, ldq, b, b, b, b, b, out, ldo, w, size, B, T, H, NKV, D, max_pages, page, pages, None)
@@ -176,6 +181,6 @@ def test_c_entries_refuse_without_a_gpu():
     assert attn(B=0) == bad and attn(T=0) == bad and attn(D=32) == shape and attn(NKV=3) == shape and attn(page=32) == shape
     assert attn(H=258, ldq=1 << 15, ldo=1 << 15, NKV=2) == shape
     assert attn(ldq=255) == bad and attn(ldq=260) == bad and attn(ldo=128) == bad and attn(Q=odd) == bad and attn(out=odd) == bad
-    assert attn(out=a) == bad and attn(w=None) == ws and attn(size=100) == ws
+    assert attn(out=a) == bad and attn(w=None) == none and attn(size=100) == none
     assert attn(max_pages=1 << 25) == shape
     assert lib.ezb_attn_prompt_workspace_bytes(96) == 0
