@@ -30,7 +30,7 @@ struct LtParams {
     void* out;
     long long ldres, ldout;
     int M, N, kblocks;
-    int tiles_m, tiles_n, stages, act, out_f32;
+    int tiles_a, tiles_b, act, out_f32;  // tiles along A's and B's rows
     int rows_aligned;  // rows of out start at 32-byte, of residual at 16-byte boundaries
     int vec_bias;      // so does bias
     // Tiles from sk_first on are cut: their kblocks form one line, and every cluster takes the same length of it.
@@ -99,13 +99,14 @@ __device__ __forceinline__ void cluster_sync_full() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-template <int BN>
+template <int BN, bool PAIR, bool SWAP>
 struct LtSmem {
-    static constexpr int kA = 128 * kLtBlockK * 2;        // this CTA's rows of x
-    static constexpr int kB = BN / 2 * kLtBlockK * 2;     // this CTA's rows of W
+    static constexpr int kARows = 128 * kLtBlockK * 2;
+    static constexpr int kA = (PAIR && SWAP ? 2 : 1) * kARows;  // this CTA's rows of A; SwiGLU, swapped: gate rows | up rows
+    static constexpr int kB = BN / 2 * kLtBlockK * 2;           // and of B
     static constexpr int kStage = kA + kB;
     static constexpr int kTail = 1024;
-    static constexpr int kTurn = 8 * 32 * 33 * 4;         // a 32 x 32 block of each epilogue warp
+    static constexpr int kTurn = SWAP ? 0 : 8 * 32 * 33 * 4;    // a 32 x 32 block of each epilogue warp
     static constexpr int kRoom = 232448 - 1024 - kTail - kTurn;
     static constexpr int kStages = kRoom / kStage < kLtMaxStages ? kRoom / kStage : kLtMaxStages;
     static constexpr int kBytes = 1024 + kStages * kStage + kTurn + kTail;
@@ -128,13 +129,15 @@ __device__ __forceinline__ void load_packed(const bf16* src, int left, int vec, 
     }
 }
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool SWAP>
 __global__ void __launch_bounds__(kLtThreads, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW0,
                  const __grid_constant__ CUtensorMap mapW1, const __grid_constant__ LtParams p) {
-    using L = LtSmem<BN>;
+    using L = LtSmem<BN, PAIR, SWAP>;
     constexpr uint32_t IDESC = umma_idesc_bf16(256, BN);
-    constexpr int UNITS = PAIR ? BN / 2 : BN;  // output columns of a tile
+    constexpr int UNITS = PAIR && !SWAP ? BN / 2 : BN;  // output columns of a tile; swapped: rows
+    constexpr int ACC = PAIR && SWAP ? 2 * BN : BN;     // columns of tensor memory of a tile
+    static_assert(2 * ACC <= 512);
     extern __shared__ unsigned char lt_raw[];
     const uint32_t raw = smem_u32(lt_raw);
     unsigned char* smem = lt_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -156,7 +159,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         mbar_fence_init();
     }
     if (warp == 1) {
-        tmem_alloc_pair(smem_u32(tmem_slot), 2 * BN);
+        tmem_alloc_pair(smem_u32(tmem_slot), 2 * ACC);
         tmem_relinquish_pair();
     }
     tc_fence_before();
@@ -169,8 +172,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     const int n_clusters = gridDim.x >> 1, cluster = blockIdx.x >> 1;
     LtWork work;
     work.start(p, cluster);
-    auto tile_at = [&](int i, int& m, int& n) {  // groups of kLtGroup row tiles, column tile by column tile
-        const int per = kLtGroup * p.tiles_n, g = i / per, rows = min(kLtGroup, p.tiles_m - g * kLtGroup), r = i - g * per;
+    auto tile_at = [&](int i, int& m, int& n) {  // groups of kLtGroup tiles along A, tile by tile along B
+        const int per = kLtGroup * p.tiles_b, g = i / per, rows = min(kLtGroup, p.tiles_a - g * kLtGroup), r = i - g * per;
         m = g * kLtGroup + r % rows, n = r / rows;
     };
     if (warp == 0) {
@@ -179,16 +182,18 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             while (!*abort_flag && work.step(p, n_clusters)) {
                 int tm, tn;
                 tile_at(work.tile, tm, tn);
-                const int y_x = tm * 256 + rank * 128;
-                const CUtensorMap* mapB = PAIR && rank ? &mapW1 : &mapW0;  // SwiGLU: the second CTA brings the up rows
-                const int y_w = PAIR ? tn * UNITS : tn * BN + rank * (BN / 2);
+                const int y_a = tm * 256 + rank * 128;
+                // SwiGLU: the second CTA brings the up rows
+                const CUtensorMap *mapA = SWAP ? &mapW0 : &mapX, *mapB = SWAP ? &mapX : PAIR && rank ? &mapW1 : &mapW0;
+                const int y_b = PAIR && !SWAP ? tn * UNITS : tn * BN + rank * (BN / 2);
                 for (int kb = work.k0; kb < work.k1; ++kb, ++it) {
                     const int s = it % L::kStages;
                     if (!mbar_wait_bounded(smem_u32(&empty[s]), (uint32_t)(((it / L::kStages) & 1) ^ 1), abort_flag, p.status, FAULT_GEMV_EMPTY_WAIT)) break;
                     const uint32_t bar = smem_u32(&full[s]), a = smem_u32(smem) + s * L::kStage;
                     if (rank == 0) mbar_arrive_expect_tx(bar, 2 * L::kStage);
-                    tma_load_2d_pair(a, &mapX, kb * kLtBlockK, y_x, bar);
-                    tma_load_2d_pair(a + L::kA, mapB, kb * kLtBlockK, y_w, bar);
+                    tma_load_2d_pair(a, mapA, kb * kLtBlockK, y_a, bar);
+                    if constexpr (PAIR && SWAP) tma_load_2d_pair(a + L::kARows, &mapW1, kb * kLtBlockK, y_a, bar);
+                    tma_load_2d_pair(a + L::kA, mapB, kb * kLtBlockK, y_b, bar);
                 }
             }
         }
@@ -206,11 +211,83 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                     const uint32_t a = smem_u32(smem) + s * L::kStage;
                     const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + L::kA);
 #pragma unroll
-                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * BN, ad + 2 * k, bd + 2 * k, IDESC, kb > work.k0 || k > 0);
+                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * ACC, ad + 2 * k, bd + 2 * k, IDESC, kb > work.k0 || k > 0);
+                    if constexpr (PAIR && SWAP) {
+                        const uint64_t ud = umma_desc_sw128(a + L::kARows);
+#pragma unroll
+                        for (int k = 0; k < kLtBlockK / 16; ++k)
+                            tc_mma_bf16_pair(tmem + acc * ACC + BN, ud + 2 * k, bd + 2 * k, IDESC, kb > work.k0 || k > 0);
+                    }
                     tc_commit_pair(smem_u32(&empty[s]));
                 }
                 tc_commit_pair(smem_u32(&acc_full[acc]));
             }
+        }
+    } else if constexpr (SWAP) {
+        // A lane has an output column and walks rows of it, W at a time: a warp's loads and stores run along the rows of the
+        // output, wherever those start.  The residual is requested a step ahead.
+        constexpr int W = 32;
+        const int q = warp & 3, c0 = ((warp - 2) >> 2) * W;
+        for (int n = 0; work.step(p, n_clusters); ++n) {
+            int ta, tb;
+            tile_at(work.tile, ta, tb);
+            const int acc = n & 1, n0 = ta * 256 + rank * 128 + q * 32, col = n0 + lane, m0 = tb * BN;
+            const int rows = n0 < p.N ? min(BN, p.M - m0) : 0;
+            const bool live = col < p.N;
+            const bf16* res_col = p.residual && live ? p.residual + (long long)m0 * p.ldres + col : nullptr;
+            const float bias = p.bias && live ? __bfloat162float(p.bias[col]) : 0.f;
+            const float bias_up = PAIR && p.bias && live ? __bfloat162float(p.bias[p.N + col]) : 0.f;
+            unsigned short res[W];
+            auto request = [&](int c) {
+                if (!res_col) return;
+                const unsigned short* src = reinterpret_cast<const unsigned short*>(res_col + (long long)c * p.ldres);
+#pragma unroll
+                for (int e = 0; e < W; ++e) res[e] = c + e < rows ? src[e * p.ldres] : 0;
+            };
+            request(c0);
+            mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
+            tc_fence_after();
+            const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * ACC;
+#pragma unroll 1
+            for (int c = c0; c < rows; c += 2 * W) {
+                float v[W], up[PAIR ? W : 1];
+                tmem_ld32(t + c, v);
+                if constexpr (PAIR) tmem_ld32(t + BN + c, up);
+                tmem_ld_wait();
+                const bool fine = !__any_sync(0xffffffffu, *abort_flag);
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[e] += bias;
+                if constexpr (PAIR) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) v[e] = silu_fast(v[e]) * (up[e] + bias_up);
+                } else if (p.act != ACT_NONE) {
+                    linear_act(v, p.act);
+                }
+                if (res_col) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) v[e] += __uint_as_float((uint32_t)res[e] << 16);
+                    request(c + 2 * W);
+                }
+                if (live && fine) {
+                    const long long o = (long long)(m0 + c) * p.ldout + col;
+                    auto store = [&](auto* dst, auto round) {
+                        if (rows - c >= W) {
+#pragma unroll
+                            for (int e = 0; e < W; ++e) dst[e * p.ldout] = round(v[e]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < W; ++e)
+                                if (c + e < rows) dst[e * p.ldout] = round(v[e]);
+                        }
+                    };
+                    if (p.out_f32) store(static_cast<float*>(p.out) + o, [](float x) { return x; });
+                    else store(static_cast<bf16*>(p.out) + o, [](float x) { return __float2bfloat16_rn(x); });
+                }
+                __syncwarp();
+            }
+            __syncwarp();
+            tc_fence_before();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[acc]), 0));
         }
     } else {
         // A warp of the quarter of rows that it may read; W columns at a time.  What the residual stream holds there is requested
@@ -232,7 +309,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             if (res_row && live_row && cols - c0 >= W) load_packed<W>(res_row + c0, W, 1, ahead);
             mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             tc_fence_after();
-            const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * BN;
+            const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * ACC;
             auto drained = [&]() {
                 __syncwarp();
                 tc_fence_before();
@@ -354,14 +431,25 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
 #pragma unroll 1
                         for (int r0 = 0; r0 < rows; r0 += 16) {
                             float x[16];  // 16 rows on their way at a time
+                            if (res_col) {
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) x[r] = res_col && r0 + r < rows ? __bfloat162float(res_col[(r0 + r) * p.ldres]) : 0.f;
+                                for (int r = 0; r < 16; ++r) x[r] = r0 + r < rows ? __bfloat162float(__ldg(res_col + (r0 + r) * p.ldres)) : 0.f;
+                            } else {
 #pragma unroll
-                            for (int r = 0; r < 16; ++r) {
-                                if (r0 + r >= rows) break;
-                                const float y = turn[(r0 + r) * (W + 1) + lane] + x[r];
-                                if (p.out_f32) static_cast<float*>(p.out)[o + (r0 + r) * p.ldout] = y;
-                                else static_cast<bf16*>(p.out)[o + (r0 + r) * p.ldout] = __float2bfloat16_rn(y);
+                                for (int r = 0; r < 16; ++r) x[r] = 0.f;
+                            }
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) x[r] += turn[(r0 + r) * (W + 1) + lane];
+                            if (p.out_f32) {
+                                float* dst = static_cast<float*>(p.out) + o + r0 * p.ldout;
+#pragma unroll
+                                for (int r = 0; r < 16; ++r)
+                                    if (r0 + r < rows) dst[r * p.ldout] = x[r];
+                            } else {
+                                bf16* dst = static_cast<bf16*>(p.out) + o + r0 * p.ldout;
+#pragma unroll
+                                for (int r = 0; r < 16; ++r)
+                                    if (r0 + r < rows) dst[r * p.ldout] = __float2bfloat16_rn(x[r]);
                             }
                         }
                     }
@@ -378,7 +466,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     cluster_sync_full();  // nothing is written to or signalled in a CTA that has left
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc_pair(tmem, 2 * BN);
+        tmem_dealloc_pair(tmem, 2 * ACC);
     }
 }
 
@@ -401,52 +489,71 @@ static bool encode_rows(CUtensorMap* map, const bf16* base, long long rows, long
 // 29.3 cut; 138 rows of 176 outputs, K = 2248: 12.5 and 17.1; 3383 rows of 64, K = 4984, 14 tiles: 21.7 and 18.7 to 25).
 struct LtPlan {
     int bn, clusters, sk_tiles;
+    bool swap;
 };
 static constexpr int kLtMinBlocks = 8;   // k blocks below which a further cluster does not pay
 static constexpr int kLtMostParts = 8;
 static constexpr int kLtCutTiles = 8;    // most tiles that are cut
 static constexpr int kLtCutBlocks = 64;  // fewest k blocks of a tile that is
-static LtPlan linear_plan(int M, int N, int K, int act, bool cut) {
-    const long long rows = act == ACT_SWIGLU ? 2ll * N : N, tm = (M + 255) / 256, kb = (K + kLtBlockK - 1) / kLtBlockK, most = sm_count() / 2;
+static LtPlan linear_plan(int M, int N, int K, int act, bool cut, bool aligned) {
+    const long long kb = (K + kLtBlockK - 1) / kLtBlockK, most = sm_count() / 2;
     const int widths[3] = {256, 128, 64};
     const double block[3] = {520., 490., 410.};
-    LtPlan best = {256, 1, 0};
-    double least = -1.;
-    for (int i = 0; i < 3; ++i) {
-        const long long tiles = tm * ((rows + widths[i] - 1) / widths[i]);
-        const double cost = (double)((tiles + most - 1) / most) * (double)kb * block[i];
-        if (least < 0. || cost < least) least = cost, best = {widths[i], (int)(tiles < most ? tiles : most), 0};
-    }
+    auto whole = [&](long long a_rows, long long b_rows, int widest) {
+        LtPlan best = {256, 1, 0, false};
+        double least = -1.;
+        for (int i = widest; i < 3; ++i) {
+            const long long tiles = (a_rows + 255) / 256 * ((b_rows + widths[i] - 1) / widths[i]);
+            const double cost = (double)((tiles + most - 1) / most) * (double)kb * block[i];
+            if (least < 0. || cost < least) least = cost, best = {widths[i], (int)(tiles < most ? tiles : most), 0, false};
+        }
+        return best;
+    };
+    LtPlan best = whole(M, act == ACT_SWIGLU ? 2ll * N : N, 0);
     if (cut && best.bn == 64 && best.clusters <= kLtCutTiles && kb >= kLtCutBlocks) {
         long long clusters = (long long)best.clusters * kLtMostParts, by_blocks = best.clusters * kb / kLtMinBlocks;
         if (clusters > by_blocks) clusters = by_blocks;
         if (clusters > most) clusters = most;
         best.sk_tiles = best.clusters, best.clusters = (int)clusters;
+    } else if (!aligned) {
+        best = whole(N, M, act == ACT_SWIGLU ? 1 : 0);
+        best.swap = true;
     }
     return best;
 }
 
 size_t linear_workspace_bytes(int M, int N, int K, int act) {
     if (M <= kLinearFewRows) return 0;
-    const LtPlan plan = linear_plan(M, N, K, act, true);
+    const LtPlan plan = linear_plan(M, N, K, act, true, true);
     // one size for all, so that an operator's workspace never has to grow under a captured graph
     return plan.sk_tiles ? (size_t)kLtCountBytes + (size_t)(sm_count() / 2) * 4 * 256 * 128 * sizeof(float) : 0;
 }
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool SWAP>
 static cudaError_t launch_linear_tile(const LinearArgs& a, const LtPlan& plan, LtParams& p, cudaStream_t stream) {
-    constexpr int UNITS = PAIR ? BN / 2 : BN;
+    constexpr int UNITS = PAIR && !SWAP ? BN / 2 : BN, kBytes = LtSmem<BN, PAIR, SWAP>::kBytes;
     alignas(64) CUtensorMap mx, w0, w1;
-    if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, 128) || !encode_rows(&w0, a.W, a.N, a.K, a.K, BN / 2)) return cudaErrorInvalidValue;
+    const int box_x = SWAP ? BN / 2 : 128, box_w = SWAP ? 128 : BN / 2;
+    if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, box_x) || !encode_rows(&w0, a.W, a.N, a.K, a.K, box_w)) return cudaErrorInvalidValue;
     if (!PAIR) w1 = w0;
-    else if (!encode_rows(&w1, a.W + (long long)a.N * a.K, a.N, a.K, a.K, BN / 2)) return cudaErrorInvalidValue;
+    else if (!encode_rows(&w1, a.W + (long long)a.N * a.K, a.N, a.K, a.K, box_w)) return cudaErrorInvalidValue;
     static std::atomic<bool> configured[64];
-    if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR>, LtSmem<BN>::kBytes, configured)) return e;
-    p.tiles_m = (a.M + 255) / 256, p.tiles_n = (a.N + UNITS - 1) / UNITS;
-    p.sk_first = p.tiles_m * p.tiles_n - plan.sk_tiles, p.sk_units = plan.sk_tiles * p.kblocks;
+    if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR, SWAP>, kBytes, configured)) return e;
+    p.tiles_a = ((SWAP ? a.N : a.M) + 255) / 256, p.tiles_b = ((SWAP ? a.M : a.N) + UNITS - 1) / UNITS;
+    p.sk_first = p.tiles_a * p.tiles_b - plan.sk_tiles, p.sk_units = plan.sk_tiles * p.kblocks;
     p.sk_share = (p.sk_units + plan.clusters - 1) / plan.clusters;
     chain_begin();
-    return launch_pdl_cluster(linear_tc_kernel<BN, PAIR>, dim3(2u * plan.clusters), dim3(kLtThreads), 2, LtSmem<BN>::kBytes, stream, mx, w0, w1, p);
+    return launch_pdl_cluster(linear_tc_kernel<BN, PAIR, SWAP>, dim3(2u * plan.clusters), dim3(kLtThreads), 2, kBytes, stream, mx, w0, w1, p);
+}
+template <bool PAIR>
+static cudaError_t launch_linear_form(const LinearArgs& a, const LtPlan& plan, LtParams& p, cudaStream_t stream) {
+    if (plan.swap) {
+        if constexpr (!PAIR)
+            if (plan.bn == 256) return launch_linear_tile<256, PAIR, true>(a, plan, p, stream);
+        return plan.bn == 128 ? launch_linear_tile<128, PAIR, true>(a, plan, p, stream) : launch_linear_tile<64, PAIR, true>(a, plan, p, stream);
+    }
+    if (plan.bn == 256) return launch_linear_tile<256, PAIR, false>(a, plan, p, stream);
+    return plan.bn == 128 ? launch_linear_tile<128, PAIR, false>(a, plan, p, stream) : launch_linear_tile<64, PAIR, false>(a, plan, p, stream);
 }
 
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
@@ -460,13 +567,10 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
     p.vec_bias = a.bias && aligned16(a.bias) && (a.act != ACT_SWIGLU || a.N % 8 == 0);
     p.status = status_ptr();
     if (!p.status) return cudaErrorUnknown;
-    const LtPlan plan = linear_plan(a.M, a.N, a.K, a.act, a.workspace != nullptr);
+    const LtPlan plan = linear_plan(a.M, a.N, a.K, a.act, a.workspace != nullptr, p.rows_aligned);
     p.count = static_cast<unsigned int*>(a.workspace);
     p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + kLtCountBytes);
-    const bool pair = a.act == ACT_SWIGLU;
-    if (plan.bn == 256) return pair ? launch_linear_tile<256, true>(a, plan, p, stream) : launch_linear_tile<256, false>(a, plan, p, stream);
-    if (plan.bn == 128) return pair ? launch_linear_tile<128, true>(a, plan, p, stream) : launch_linear_tile<128, false>(a, plan, p, stream);
-    return pair ? launch_linear_tile<64, true>(a, plan, p, stream) : launch_linear_tile<64, false>(a, plan, p, stream);
+    return a.act == ACT_SWIGLU ? launch_linear_form<true>(a, plan, p, stream) : launch_linear_form<false>(a, plan, p, stream);
 }
 
 }  // namespace ezb
