@@ -5,18 +5,27 @@
 // Tile: the G heads of a group are packed next to each other, so 128 rows of an MMA are floor(128/G) tokens x G heads and
 // every key and value is read once per group.  A unit of work is 256 such rows (two tiles, two softmax warpgroups) of one
 // (row, kv head); it walks the keys 128 at a time.  Scores S (fp32) live in tensor memory, one thread owns a whole row of
-// them: running maximum and sum without a shuffle.  P is written back over S in bf16 and is the MMA's A operand from tensor
-// memory; O (fp32) stays there too.  2 x (128 + D) columns of the 512.  While one warpgroup exponentiates, the other tile's
-// products run.  The output is rescaled only when a row's maximum has grown by more than 2^8 since the last time (the
-// result does not depend on which maximum is subtracted; sums and P stay far inside their ranges).
-// A unit with at most 128 rows (single tokens, the end of a prompt) uses the second tile for every other block of keys.
+// them: running maximum and sum without a shuffle.  P is written back over S in bf16 (relative error 2^-8 of a weight, the
+// sum keeps the unrounded one) and is the MMA's A operand from tensor memory, in two halves so that the products of the first
+// start under the exponentials of the second; O (fp32) stays there too.  2 x (128 + D) columns of the 512.  The two warpgroups
+// take turns: while one exponentiates, the other tile's products run.  The output is rescaled only when a row's maximum has
+// grown by more than 2^8 since the last time (the result does not depend on which maximum is subtracted; sums and P stay far
+// inside their ranges), so the first half of a block is exponentiated before its maximum is known.
+// A unit with at most 128 rows (single tokens, the end of a prompt) uses the second warpgroup for every other block of keys;
+// the halves meet in tensor memory.
 //
 // Work is dealt out on the device, since the lengths are there: all units form one line, weighted by their keys, and CTA c
 // takes the c-th equal share; a unit that is cut leaves (max, sum, O) parts in the workspace, and the CTA that finishes its
-// last part joins them in the order of the keys (equal calls give equal bits).
+// last part joins them in the order of the keys (equal calls give equal bits).  Units of up to kApWhole tiles stay whole: a part
+// costs a trip through the workspace (short prompts of 14 heads of 64: 37.7 -> 17.6 us).
 //
 // What bounds it: for prompts the exponentials and the products together - 128 x 128 scores take 512 cycles each for QK^T
-// and PV (D = 128) and 1024 cycles of the MUFU, twice per step; for single tokens the bytes of the caches.
+// and PV (D = 128) and 1024 cycles of the MUFU, twice per step.  8192 tokens, 32/8 heads of 128: 437 to 505 us, 1090 to 1260
+// TFLOP/s of the products that the mask leaves (the MMAs alone in this order 355 to 370 us); 8 prompts of 65 to 600 tokens
+// behind 300 to 7400: 235 to 255 us; 8192 tokens of D = 64: 380 us, of which 240 are exponentials.  For single tokens the bytes
+// of the caches: 32 of them over 1000 to 8100 keys 103 to 112 us, 5.5 to 5.9 TB/s.
+// Measured and left out: a polynomial in place of part of the exponentials, 512 softmax threads, P handed over at 75 %, blocks of
+// 64 keys (+12 % for QK^T), a third block of scores beside O of 64 columns (3 %): no gain that carries its code.
 // Keys behind a row's last one, entries outside the pools and everything masked are never added: K there is masked after
 // the product, V is zero (out-of-range TMA boxes, or cleared in shared memory where a box straddles the end).
 #include <atomic>
@@ -423,447 +432,447 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
 
     // A softmax thread holds a row of scores: 384 threads x 168 registers at launch = 2 x 128 x 216 + 128 x 72.
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (idle) {
-    } else if (warp == 10) {
-        // ------------------------------------------------------------ work descriptors
-        ApCursor cur = t.start;
-        for (bool more = true;; more = more && ap_advance(p, cur, lane)) {
-            const bool end = !more || cur.x0 >= hi;
-            ApSegment s;
-            s.cnt = -1;
-            if (!end && !ap_segment(p, line, cur, cta, lo, hi, s)) continue;
-            const int i = n_seg % kApSegments;
-            if (!mbar_wait_bounded(smem_u32(&t.seg_empty[i]), (uint32_t)(((n_seg / kApSegments) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
-            if (lane == 0) {
-                t.seg[i] = s;
-                mbar_arrive(smem_u32(&t.seg_full[i]));
-            }
-            __syncwarp();
-            ++n_seg;
-            if (end) break;
-        }
-        __threadfence_block();
-        if (lane == 0) *(volatile int*)&t.published = n_seg;
-    } else if (warp == 8) {
-        // ------------------------------------------------------------ TMA producer
-        int it = 0, n_q = 0, n_fix = 0;  // ring tiles, query loads, repaired tiles so far
-        while (const ApSegment* sp = next_segment()) {
-            const ApSegment seg = *sp;
-            __syncwarp();
-            if (lane == 0) release();
-            else ++n_seg;
-            if (seg.cnt == 0) continue;
-            const int* table = p.table + (long long)seg.row * p.max_pages;
-            if (!mbar_wait_bounded(smem_u32(&t.q_empty), (uint32_t)((n_q & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
-            if (elect_one()) {
-                const uint32_t bar = smem_u32(&t.q_full);
-                const int tiles_q = seg.dual ? 1 : 2;
-                mbar_arrive_expect_tx(bar, (uint32_t)(p.tpt * p.G * 128 * BLOCKS * tiles_q));
-                for (int m = 0; m < tiles_q; ++m)
-#pragma unroll
-                    for (int k = 0; k < BLOCKS; ++k)
-                        tma_load_3d(sm_q + m * L::kTile + k * 16384, &mapQ, k * 64, seg.head * p.G, seg.token + m * p.tpt, bar);
-            }
-            __syncwarp();
-            ++n_q;
-            int ids = 0, ids_from = -16;  // lane i: pool page of key block (ids_from * 2 + i), 64 keys each
-            // K and V tiles in the order of their use: K(0) V(0) K(1) V(1) ..., or K(0) K(1) V(0) K(2) V(1) ... (dual)
-            const int ahead = seg.dual ? 2 : 1, lead = min(ahead, seg.cnt);
-#pragma unroll 1
-            for (int i = 0; i < 2 * seg.cnt && !*abort_flag; ++i) {
-                int v = 0, k = i;
-                if (i >= lead) {
-                    const int o = i - lead;  // V(0) K(ahead) V(1) K(ahead + 1) ... then the last V
-                    const int pairs = seg.cnt - lead;
-                    if (o < 2 * pairs) v = !(o & 1), k = (o >> 1) + (v ? 0 : ahead);
-                    else v = 1, k = pairs + (o - 2 * pairs);
-                }
-                k += seg.ks;
-                if (k < ids_from || k >= ids_from + 16) {
-                    ids_from = k;
-                    const long long key = ((long long)k * 2 + lane) * 64;
-                    ids = p.num_pages;  // out of range: zeros
-                    if (key < seg.extent) {
-                        const int id = __ldg(table + (key >> p.page_shift));
-                        if (id >= 0 && id < p.num_pages) ids = id;
-                        else report_fault(p.status, FAULT_PAGE_RANGE);
-                    }
-                }
-                const int stage = it % kApStages;
-                if (!mbar_wait_bounded(smem_u32(&t.empty[stage]), (uint32_t)(((it / kApStages) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
-                const int id0 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2), id1 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2 + 1);
-                const bool repair = v && seg.clear && k == seg.tiles - 1;
-                const uint32_t dst = sm_ring + stage * L::kTile, bar = smem_u32(repair ? &t.fix : &t.full[stage]);
-                if (elect_one()) {
-                    const CUtensorMap* map = v ? &mapV : &mapK;
-                    const int mask = (1 << p.page_shift) - 1, y0 = (k * kApKeys) & mask, y1 = (k * kApKeys + 64) & mask;
-                    mbar_arrive_expect_tx(bar, L::kTile);
-#pragma unroll
-                    for (int c = 0; c < BLOCKS; ++c) {
-                        tma_load_3d(dst + c * 16384, map, c * 64, y0, id0 * p.NKV + seg.head, bar);
-                        tma_load_3d(dst + c * 16384 + 8192, map, c * 64, y1, id1 * p.NKV + seg.head, bar);
-                    }
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (idle) {
+        } else if (warp == 10) {
+            // ------------------------------------------------------------ work descriptors
+            ApCursor cur = t.start;
+            for (bool more = true;; more = more && ap_advance(p, cur, lane)) {
+                const bool end = !more || cur.x0 >= hi;
+                ApSegment s;
+                s.cnt = -1;
+                if (!end && !ap_segment(p, line, cur, cta, lo, hi, s)) continue;
+                const int i = n_seg % kApSegments;
+                if (!mbar_wait_bounded(smem_u32(&t.seg_empty[i]), (uint32_t)(((n_seg / kApSegments) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+                if (lane == 0) {
+                    t.seg[i] = s;
+                    mbar_arrive(smem_u32(&t.seg_full[i]));
                 }
                 __syncwarp();
-                ++it;
-                if (repair) {
-                    // rows behind the last key of the block that straddles it: P is zero there, and V has to be
-                    mbar_wait_bounded(bar, (uint32_t)(n_fix & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
-                    ++n_fix;
-                    const int r0 = seg.extent - k * kApKeys, bytes = (((r0 + 63) & ~63) - r0) * 128;  // extent is no multiple of 64 here
-                    for (int c = 0; c < BLOCKS; ++c)
-                        for (int o = lane * 16; o < bytes; o += 512)
-                            *reinterpret_cast<uint4*>(smem + L::kRing + stage * L::kTile + c * 16384 + r0 * 128 + o) = make_uint4(0u, 0u, 0u, 0u);
-                    fence_async_shared();
+                ++n_seg;
+                if (end) break;
+            }
+            __threadfence_block();
+            if (lane == 0) *(volatile int*)&t.published = n_seg;
+        } else if (warp == 8) {
+            // ------------------------------------------------------------ TMA producer
+            int it = 0, n_q = 0, n_fix = 0;  // ring tiles, query loads, repaired tiles so far
+            while (const ApSegment* sp = next_segment()) {
+                const ApSegment seg = *sp;
+                __syncwarp();
+                if (lane == 0) release();
+                else ++n_seg;
+                if (seg.cnt == 0) continue;
+                const int* table = p.table + (long long)seg.row * p.max_pages;
+                if (!mbar_wait_bounded(smem_u32(&t.q_empty), (uint32_t)((n_q & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+                if (elect_one()) {
+                    const uint32_t bar = smem_u32(&t.q_full);
+                    const int tiles_q = seg.dual ? 1 : 2;
+                    mbar_arrive_expect_tx(bar, (uint32_t)(p.tpt * p.G * 128 * BLOCKS * tiles_q));
+                    for (int m = 0; m < tiles_q; ++m)
+#pragma unroll
+                        for (int k = 0; k < BLOCKS; ++k)
+                            tma_load_3d(sm_q + m * L::kTile + k * 16384, &mapQ, k * 64, seg.head * p.G, seg.token + m * p.tpt, bar);
+                }
+                __syncwarp();
+                ++n_q;
+                int ids = 0, ids_from = -16;  // lane i: pool page of key block (ids_from * 2 + i), 64 keys each
+                // K and V tiles in the order of their use: K(0) V(0) K(1) V(1) ..., or K(0) K(1) V(0) K(2) V(1) ... (dual)
+                const int ahead = seg.dual ? 2 : 1, lead = min(ahead, seg.cnt);
+#pragma unroll 1
+                for (int i = 0; i < 2 * seg.cnt && !*abort_flag; ++i) {
+                    int v = 0, k = i;
+                    if (i >= lead) {
+                        const int o = i - lead;  // V(0) K(ahead) V(1) K(ahead + 1) ... then the last V
+                        const int pairs = seg.cnt - lead;
+                        if (o < 2 * pairs) v = !(o & 1), k = (o >> 1) + (v ? 0 : ahead);
+                        else v = 1, k = pairs + (o - 2 * pairs);
+                    }
+                    k += seg.ks;
+                    if (k < ids_from || k >= ids_from + 16) {
+                        ids_from = k;
+                        const long long key = ((long long)k * 2 + lane) * 64;
+                        ids = p.num_pages;  // out of range: zeros
+                        if (key < seg.extent) {
+                            const int id = __ldg(table + (key >> p.page_shift));
+                            if (id >= 0 && id < p.num_pages) ids = id;
+                            else report_fault(p.status, FAULT_PAGE_RANGE);
+                        }
+                    }
+                    const int stage = it % kApStages;
+                    if (!mbar_wait_bounded(smem_u32(&t.empty[stage]), (uint32_t)(((it / kApStages) & 1) ^ 1), abort_flag, p.status, FAULT_PROMPT_WAIT)) break;
+                    const int id0 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2), id1 = __shfl_sync(0xffffffffu, ids, (k - ids_from) * 2 + 1);
+                    const bool repair = v && seg.clear && k == seg.tiles - 1;
+                    const uint32_t dst = sm_ring + stage * L::kTile, bar = smem_u32(repair ? &t.fix : &t.full[stage]);
+                    if (elect_one()) {
+                        const CUtensorMap* map = v ? &mapV : &mapK;
+                        const int mask = (1 << p.page_shift) - 1, y0 = (k * kApKeys) & mask, y1 = (k * kApKeys + 64) & mask;
+                        mbar_arrive_expect_tx(bar, L::kTile);
+#pragma unroll
+                        for (int c = 0; c < BLOCKS; ++c) {
+                            tma_load_3d(dst + c * 16384, map, c * 64, y0, id0 * p.NKV + seg.head, bar);
+                            tma_load_3d(dst + c * 16384 + 8192, map, c * 64, y1, id1 * p.NKV + seg.head, bar);
+                        }
+                    }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&t.full[stage]));
+                    ++it;
+                    if (repair) {
+                        // rows behind the last key of the block that straddles it: P is zero there, and V has to be
+                        mbar_wait_bounded(bar, (uint32_t)(n_fix & 1), abort_flag, p.status, FAULT_PROMPT_WAIT);
+                        ++n_fix;
+                        const int r0 = seg.extent - k * kApKeys, bytes = (((r0 + 63) & ~63) - r0) * 128;  // extent is no multiple of 64 here
+                        for (int c = 0; c < BLOCKS; ++c)
+                            for (int o = lane * 16; o < bytes; o += 512)
+                                *reinterpret_cast<uint4*>(smem + L::kRing + stage * L::kTile + c * 16384 + r0 * 128 + o) = make_uint4(0u, 0u, 0u, 0u);
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&t.full[stage]));
+                    }
                 }
             }
-        }
-        if (*abort_flag) {  // nothing may still be landing in this CTA's shared memory when it exits
-            const long long t0 = clock64();
-            while (clock64() - t0 < kWaitLimitCycles / 100) {}
-        }
-    } else if (warp == 9) {
-        // ------------------------------------------------------------ MMA issuer
-        if (elect_one()) {
-            int it = 0, n_q = 0;
-            uint32_t tiles_seen = 0, units_seen = 0;  // bit m: parity of the tiles / units of warpgroup m so far
-            auto wait = [&](uint64_t* bar, uint32_t parity) {
-                const bool ok = mbar_wait_bounded(smem_u32(bar), parity, abort_flag, p.status, FAULT_PROMPT_WAIT);
-                tc_fence_after();
-                return ok;
-            };
-            auto wait_stage = [&](int i) { return wait(&t.full[i % kApStages], (uint32_t)((i / kApStages) & 1)); };
-            const uint32_t q_low = ap_desc(sm_q), ring_low = ap_desc(sm_ring);
-            auto scores = [&](int m, int q_tile, int i) {  // S[m] = Q K^T
-                const uint32_t a = q_low + q_tile * (L::kTile >> 4), b = ring_low + (i % kApStages) * (L::kTile >> 4);
+            if (*abort_flag) {  // nothing may still be landing in this CTA's shared memory when it exits
+                const long long t0 = clock64();
+                while (clock64() - t0 < kWaitLimitCycles / 100) {}
+            }
+        } else if (warp == 9) {
+            // ------------------------------------------------------------ MMA issuer
+            if (elect_one()) {
+                int it = 0, n_q = 0;
+                uint32_t tiles_seen = 0, units_seen = 0;  // bit m: parity of the tiles / units of warpgroup m so far
+                auto wait = [&](uint64_t* bar, uint32_t parity) {
+                    const bool ok = mbar_wait_bounded(smem_u32(bar), parity, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    tc_fence_after();
+                    return ok;
+                };
+                auto wait_stage = [&](int i) { return wait(&t.full[i % kApStages], (uint32_t)((i / kApStages) & 1)); };
+                const uint32_t q_low = ap_desc(sm_q), ring_low = ap_desc(sm_ring);
+                auto scores = [&](int m, int q_tile, int i) {  // S[m] = Q K^T
+                    const uint32_t a = q_low + q_tile * (L::kTile >> 4), b = ring_low + (i % kApStages) * (L::kTile >> 4);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const int off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
-                    ap_mma_ss(tmem + m * 128, a + off, b + off, IDESC_QK, k > 0);
-                }
-                tc_commit(smem_u32(&t.s_full[m]));
-            };
-            // O[m] (+)= P V for one half of the keys.  V is stored [key][64 elements], so the MMA's N runs along the contiguous
-            // dimension; 64-element column blocks lie 16 KB apart (the stride in the descriptor), groups of eight keys 1 KB.
-            auto values = [&](int m, int i, bool fresh, int half) {
-                const uint32_t b = (ring_low + (i % kApStages) * (L::kTile >> 4) + half * (8192 >> 4)) | (D > 64 ? (16384u >> 4) << 16 : 0u);
+                    for (int k = 0; k < D / 16; ++k) {
+                        const int off = (k >> 2) * (16384 >> 4) + (k & 3) * 2;
+                        ap_mma_ss(tmem + m * 128, a + off, b + off, IDESC_QK, k > 0);
+                    }
+                    tc_commit(smem_u32(&t.s_full[m]));
+                };
+                // O[m] (+)= P V for one half of the keys.  V is stored [key][64 elements], so the MMA's N runs along the contiguous
+                // dimension; 64-element column blocks lie 16 KB apart (the stride in the descriptor), groups of eight keys 1 KB.
+                auto values = [&](int m, int i, bool fresh, int half) {
+                    const uint32_t b = (ring_low + (i % kApStages) * (L::kTile >> 4) + half * (8192 >> 4)) | (D > 64 ? (16384u >> 4) << 16 : 0u);
 #pragma unroll
-                for (int k = 0; k < kApKeys / 32; ++k)
-                    ap_mma_ts(tmem + 256 + m * D, tmem + m * 128 + half * 32 + k * 8, b + k * (2048 >> 4), IDESC_PV, !(fresh && k == 0));
-            };
-            auto free_stage = [&](int i) { tc_commit(smem_u32(&t.empty[i % kApStages])); };
-            // O[m] (+)= P[m] V as the halves of P come; for the first tile of a unit O[m] has to be drained first
-            auto add_values = [&](int m, int i, bool fresh, bool wait_v) {
-                if (!wait(&t.h_full[m], (tiles_seen >> m) & 1u)) return false;
-                if (fresh) {
-                    if (!wait(&t.o_empty[m], ((units_seen >> m) & 1u) ^ 1u)) return false;
-                    units_seen ^= 1u << m;
-                }
-                if (wait_v && !wait_stage(i)) return false;
-                values(m, i, fresh, 0);
-                if (!wait(&t.p_full[m], (tiles_seen >> m) & 1u)) return false;
-                tiles_seen ^= 1u << m;
-                values(m, i, false, 1);
-                return true;
-            };
-            while (const ApSegment* sp = next_segment()) {
-                const int cnt = sp->cnt, dual = sp->dual;
-                release();
-                if (cnt == 0) continue;
-                if (!wait(&t.q_full, (uint32_t)(n_q & 1))) break;
-                ++n_q;
-                if (!dual) {
-                    // every K and V tile serves both tiles of queries
-                    if (!wait_stage(it)) break;
-                    scores(0, 0, it);
-                    scores(1, 1, it);
-                    free_stage(it);
-                    ++it;
-                    if (cnt == 1) tc_commit(smem_u32(&t.q_empty));
+                    for (int k = 0; k < kApKeys / 32; ++k)
+                        ap_mma_ts(tmem + 256 + m * D, tmem + m * 128 + half * 32 + k * 8, b + k * (2048 >> 4), IDESC_PV, !(fresh && k == 0));
+                };
+                auto free_stage = [&](int i) { tc_commit(smem_u32(&t.empty[i % kApStages])); };
+                // O[m] (+)= P[m] V as the halves of P come; for the first tile of a unit O[m] has to be drained first
+                auto add_values = [&](int m, int i, bool fresh, bool wait_v) {
+                    if (!wait(&t.h_full[m], (tiles_seen >> m) & 1u)) return false;
+                    if (fresh) {
+                        if (!wait(&t.o_empty[m], ((units_seen >> m) & 1u) ^ 1u)) return false;
+                        units_seen ^= 1u << m;
+                    }
+                    if (wait_v && !wait_stage(i)) return false;
+                    values(m, i, fresh, 0);
+                    if (!wait(&t.p_full[m], (tiles_seen >> m) & 1u)) return false;
+                    tiles_seen ^= 1u << m;
+                    values(m, i, false, 1);
+                    return true;
+                };
+                while (const ApSegment* sp = next_segment()) {
+                    const int cnt = sp->cnt, dual = sp->dual;
+                    release();
+                    if (cnt == 0) continue;
+                    if (!wait(&t.q_full, (uint32_t)(n_q & 1))) break;
+                    ++n_q;
+                    if (!dual) {
+                        // every K and V tile serves both tiles of queries
+                        if (!wait_stage(it)) break;
+                        scores(0, 0, it);
+                        scores(1, 1, it);
+                        free_stage(it);
+                        ++it;
+                        if (cnt == 1) tc_commit(smem_u32(&t.q_empty));
 #pragma unroll 1
-                    for (int i = 0; i < cnt && !*abort_flag; ++i) {
-                        const bool next = i + 1 < cnt;
+                        for (int i = 0; i < cnt && !*abort_flag; ++i) {
+                            const bool next = i + 1 < cnt;
 #pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            if (!add_values(m, it, i == 0, m == 0)) break;
-                            if (m == 1) free_stage(it);
-                            if (next) {
-                                if (m == 0 && !wait_stage(it + 1)) break;
-                                scores(m, m, it + 1);
-                                if (m == 1) free_stage(it + 1);
+                            for (int m = 0; m < 2; ++m) {
+                                if (!add_values(m, it, i == 0, m == 0)) break;
+                                if (m == 1) free_stage(it);
+                                if (next) {
+                                    if (m == 0 && !wait_stage(it + 1)) break;
+                                    scores(m, m, it + 1);
+                                    if (m == 1) free_stage(it + 1);
+                                } else {
+                                    tc_commit(smem_u32(&t.o_full[m]));
+                                }
+                            }
+                            if (i + 2 == cnt) tc_commit(smem_u32(&t.q_empty));
+                            it += next ? 2 : 1;
+                        }
+                    } else {
+                        // tile i of the keys belongs to warpgroup i & 1
+#pragma unroll 1
+                        for (int i = 0; i < 2 && i < cnt; ++i) {
+                            if (!wait_stage(it)) break;
+                            scores(i, 0, it);
+                            free_stage(it);
+                            ++it;
+                        }
+                        if (cnt <= 2) tc_commit(smem_u32(&t.q_empty));
+#pragma unroll 1
+                        for (int i = 0; i < cnt && !*abort_flag; ++i) {
+                            const int m = i & 1;
+                            if (!add_values(m, it, i < 2, true)) break;
+                            free_stage(it);
+                            ++it;
+                            if (i + 2 < cnt) {
+                                if (!wait_stage(it)) break;
+                                scores(m, 0, it);
+                                free_stage(it);
+                                ++it;
+                                if (i + 3 == cnt) tc_commit(smem_u32(&t.q_empty));
                             } else {
                                 tc_commit(smem_u32(&t.o_full[m]));
                             }
                         }
-                        if (i + 2 == cnt) tc_commit(smem_u32(&t.q_empty));
-                        it += next ? 2 : 1;
-                    }
-                } else {
-                    // tile i of the keys belongs to warpgroup i & 1
-#pragma unroll 1
-                    for (int i = 0; i < 2 && i < cnt; ++i) {
-                        if (!wait_stage(it)) break;
-                        scores(i, 0, it);
-                        free_stage(it);
-                        ++it;
-                    }
-                    if (cnt <= 2) tc_commit(smem_u32(&t.q_empty));
-#pragma unroll 1
-                    for (int i = 0; i < cnt && !*abort_flag; ++i) {
-                        const int m = i & 1;
-                        if (!add_values(m, it, i < 2, true)) break;
-                        free_stage(it);
-                        ++it;
-                        if (i + 2 < cnt) {
-                            if (!wait_stage(it)) break;
-                            scores(m, 0, it);
-                            free_stage(it);
-                            ++it;
-                            if (i + 3 == cnt) tc_commit(smem_u32(&t.q_empty));
-                        } else {
-                            tc_commit(smem_u32(&t.o_full[m]));
-                        }
                     }
                 }
             }
         }
-    }
     } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    if (!idle) {
-        // ------------------------------------------------------------ softmax, one row per thread
-        const int m = warp >> 2;                                    // tile
-        const int r = (warp & 3) * 32 + lane;                       // row of the tile
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + lanes + m * 128, t_o = tmem + lanes + 256 + m * D;
-        const int r_tok = r / p.G, r_head = r - r_tok * p.G;
-        uint32_t n_tile = 0, n_unit = 0, n_turn = 0, n_other = 0;  // n_other: units of warpgroup 1, as warpgroup 0 counts them
-        while (const ApSegment* sp = next_segment()) {
-            const ApSegment& seg = *sp;  // stays in shared memory until the end of the segment
-            const int cnt = seg.cnt, dual = seg.dual;
-            const int first = dual ? 0 : m * p.tpt, tok = first + r_tok;  // within the unit
-            const bool live = r_tok < p.tpt && tok < seg.tokens;
-            // keys that this query sees, and that all queries of the tile see, counted from the CTA's first key
-            const int from = seg.ks * kApKeys;
-            const int limit = live ? seg.sees + tok - from : 0, all_see = seg.sees + first - from;
-            const int my0 = dual ? m : 0, step = dual ? 2 : 1;
-            float mx = -INFINITY, sum = 0.f;
-            auto row_max = [](const float (&s)[kApKeys]) {
-                float top[4] = {s[0], s[1], s[2], s[3]};
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        if (!idle) {
+            // ------------------------------------------------------------ softmax, one row per thread
+            const int m = warp >> 2;                                    // tile
+            const int r = (warp & 3) * 32 + lane;                       // row of the tile
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t t_s = tmem + lanes + m * 128, t_o = tmem + lanes + 256 + m * D;
+            const int r_tok = r / p.G, r_head = r - r_tok * p.G;
+            uint32_t n_tile = 0, n_unit = 0, n_turn = 0, n_other = 0;  // n_other: units of warpgroup 1, as warpgroup 0 counts them
+            while (const ApSegment* sp = next_segment()) {
+                const ApSegment& seg = *sp;  // stays in shared memory until the end of the segment
+                const int cnt = seg.cnt, dual = seg.dual;
+                const int first = dual ? 0 : m * p.tpt, tok = first + r_tok;  // within the unit
+                const bool live = r_tok < p.tpt && tok < seg.tokens;
+                // keys that this query sees, and that all queries of the tile see, counted from the CTA's first key
+                const int from = seg.ks * kApKeys;
+                const int limit = live ? seg.sees + tok - from : 0, all_see = seg.sees + first - from;
+                const int my0 = dual ? m : 0, step = dual ? 2 : 1;
+                float mx = -INFINITY, sum = 0.f;
+                auto row_max = [](const float (&s)[kApKeys]) {
+                    float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int c = 4; c < kApKeys; c += 8) {
+                    for (int c = 4; c < kApKeys; c += 8) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top[e] = c + 4 + e < kApKeys ? max3(top[e], s[c + e], s[c + 4 + e]) : fmaxf(top[e], s[c + e]);
-                }
-                return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            };
+                        for (int e = 0; e < 4; ++e) top[e] = c + 4 + e < kApKeys ? max3(top[e], s[c + e], s[c + 4 + e]) : fmaxf(top[e], s[c + e]);
+                    }
+                    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                };
 #pragma unroll 1
-            for (int i = my0; i < cnt; i += step) {
-                const int key0 = i * kApKeys;
-                mbar_wait_bounded(smem_u32(&t.s_full[m]), n_tile & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
-                ++n_tile;
-                tc_fence_after();
-                float s[kApKeys];
+                for (int i = my0; i < cnt; i += step) {
+                    const int key0 = i * kApKeys;
+                    mbar_wait_bounded(smem_u32(&t.s_full[m]), n_tile & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    ++n_tile;
+                    tc_fence_after();
+                    float s[kApKeys];
 #pragma unroll
-                for (int c = 0; c < kApKeys; c += 32) tmem_ld32(t_s + c, s + c);
-                tmem_ld_wait();
-                if (key0 + kApKeys > all_see) {
+                    for (int c = 0; c < kApKeys; c += 32) tmem_ld32(t_s + c, s + c);
+                    tmem_ld_wait();
+                    if (key0 + kApKeys > all_see) {
 #pragma unroll
-                    for (int c = 0; c < kApKeys; ++c)
-                        if (key0 + c >= limit) s[c] = -INFINITY;
-                }
-                if (i == my0) mx = row_max(s);
-                // The tiles take turns: side by side they would both exponentiate at half speed and then both wait for
-                // the tensor cores.
-                if (!dual) {
-                    mbar_wait_bounded(smem_u32(&t.turn[m]), (n_turn & 1u) ^ (m == 0 ? 1u : 0u), abort_flag, p.status, FAULT_PROMPT_WAIT);
-                    ++n_turn;
-                }
-                // The first half is exponentiated against the maximum of the blocks before, while this block's is being found: it
-                // hardly ever matters (the comment at the top), and the search costs nothing next to the MUFU.
-                const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
-                float2 add[2];
-                uint32_t w[32];
-                auto first_half = [&]() {
+                        for (int c = 0; c < kApKeys; ++c)
+                            if (key0 + c >= limit) s[c] = -INFINITY;
+                    }
+                    if (i == my0) mx = row_max(s);
+                    // The tiles take turns: side by side they would both exponentiate at half speed and then both wait for
+                    // the tensor cores.
+                    if (!dual) {
+                        mbar_wait_bounded(smem_u32(&t.turn[m]), (n_turn & 1u) ^ (m == 0 ? 1u : 0u), abort_flag, p.status, FAULT_PROMPT_WAIT);
+                        ++n_turn;
+                    }
+                    // The first half is exponentiated against the maximum of the blocks before, while this block's is being found: it
+                    // hardly ever matters (the comment at the top), and the search costs nothing next to the MUFU.
+                    const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+                    float2 add[2];
+                    uint32_t w[32];
+                    auto first_half = [&]() {
+                        const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
+                        const float2 shift2 = make_float2(-shift, -shift);
+                        add[0] = add[1] = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), scale2, shift2);
+                            x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
+                            add[e & 1] = add2(add[e & 1], x);
+                            w[e] = pack_bf16(x.x, x.y);
+                        }
+                    };
+                    first_half();
+                    const float higher = fmaxf(mx, row_max(s));
+                    // all keys so far masked: nothing has been summed, and the factor is exp2(-inf) = 0
+                    const bool grow = (higher - mx) * p.scale_log2 > 8.f;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? exp2_approx((mx - higher) * p.scale_log2) : 1.f;
+                        if (grow) mx = higher;
+                        sum *= f;
+                        if (i != my0) {
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                float o[16];
+                                uint32_t u[16];
+                                tmem_ld16(t_o + c, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
+                                tmem_st16(t_o + c, u);
+                            }
+                        }
+                        first_half();
+                    }
+                    tmem_st16(t_s, w), tmem_st16(t_s + 16, w + 16);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&t.h_full[m]));  // half of P is there: its products may start
                     const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
                     const float2 shift2 = make_float2(-shift, -shift);
-                    add[0] = add[1] = make_float2(0.f, 0.f);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), scale2, shift2);
-                        x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
-                        add[e & 1] = add2(add[e & 1], x);
-                        w[e] = pack_bf16(x.x, x.y);
+                    for (int c = kApKeys / 2; c < kApKeys; c += 32) {
+                        uint32_t v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            float2 x = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2);
+                            x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
+                            add[e & 1] = add2(add[e & 1], x);
+                            v[e] = pack_bf16(x.x, x.y);
+                        }
+                        tmem_st16(t_s + c / 2, v);
+                        if (c == 64 && !dual) {  // the rest of this tile and the start of the other one fill each other's gaps
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(smem_u32(&t.turn[1 - m]));
+                        }
                     }
-                };
-                first_half();
-                const float higher = fmaxf(mx, row_max(s));
-                // all keys so far masked: nothing has been summed, and the factor is exp2(-inf) = 0
-                const bool grow = (higher - mx) * p.scale_log2 > 8.f;
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? exp2_approx((mx - higher) * p.scale_log2) : 1.f;
-                    if (grow) mx = higher;
-                    sum *= f;
-                    if (i != my0) {
+                    sum += (add[0].x + add[1].x) + (add[0].y + add[1].y);
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&t.p_full[m]));
+                }
+                // ---- end of the segment
+                const bool mine = my0 < cnt, whole = cnt == seg.tiles, two = dual && cnt > 1;
+                if (mine) {
+                    mbar_wait_bounded(smem_u32(&t.o_full[m]), n_unit & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                    ++n_unit;
+                    tc_fence_after();
+                }
+                // Two sums over the same rows meet here: warpgroup 0 reads the other one's O from tensor memory (the same lanes).
+                float w0 = 1.f, w1 = 0.f;
+                bool writes = true;
+                if (dual) {
+                    if (two && m == 1) t.stat[0][r] = mx, t.stat[1][r] = sum;
+                    named_bar_sync(1, 256);
+                    writes = m == 0;
+                    if (two && m == 0) {
+                        mbar_wait_bounded(smem_u32(&t.o_full[1]), n_other & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
+                        tc_fence_after();
+                        const float mx1 = t.stat[0][r], top = fmaxf(mx, mx1);
+                        w0 = mx == -INFINITY ? 0.f : exp2_approx((mx - top) * p.scale_log2);
+                        w1 = mx1 == -INFINITY ? 0.f : exp2_approx((mx1 - top) * p.scale_log2);
+                        sum = w0 * sum + w1 * t.stat[1][r];
+                        mx = top;
+                    }
+                }
+                if (two || (!dual && cnt > 0)) ++n_other;
+                if (writes) {
+                    // 16 columns of the row's O; the other warpgroup's lie D columns behind
+                    auto columns = [&](int c, float (&o)[16]) {
+                        tmem_ld16(t_o + c, o);
+                        if (two) {
+                            float o1[16];
+                            tmem_ld16(t_o + D + c, o1);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = w0 * o[e] + w1 * o1[e];
+                        } else {
+                            tmem_ld_wait();
+                        }
+                    };
+                    auto drained = [&]() {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            mbar_arrive(smem_u32(&t.o_empty[m]));
+                            if (two) mbar_arrive(smem_u32(&t.o_empty[1]));
+                        }
+                    };
+                    if (whole) {
+                        const bool store = live && !*abort_flag;
+                        const float inv = 1.0f / sum;
+                        bf16* out = p.Out + (long long)(seg.token + tok) * p.ldo + (long long)(seg.head * p.G + r_head) * D;
 #pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
                             float o[16];
-                            uint32_t u[16];
-                            tmem_ld16(t_o + c, o);
-                            tmem_ld_wait();
+                            if (mine) columns(c, o);
+                            uint32_t w[8];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * f);
-                            tmem_st16(t_o + c, u);
+                            for (int q = 0; q < 8; ++q)  // a query that sees no key gives zero
+                                w[q] = limit > 0 ? pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
+                            if (store) store_row16(out + c, w, p.out32);
+                            __syncwarp();
                         }
-                    }
-                    first_half();
-                }
-                tmem_st16(t_s, w), tmem_st16(t_s + 16, w + 16);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&t.h_full[m]));  // half of P is there: its products may start
-                const float shift = mx == -INFINITY ? 0.f : mx * p.scale_log2;
-                const float2 shift2 = make_float2(-shift, -shift);
-#pragma unroll
-                for (int c = kApKeys / 2; c < kApKeys; c += 32) {
-                    uint32_t v[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float2 x = fma2(make_float2(s[c + 2 * e], s[c + 2 * e + 1]), scale2, shift2);
-                        x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
-                        add[e & 1] = add2(add[e & 1], x);
-                        v[e] = pack_bf16(x.x, x.y);
-                    }
-                    tmem_st16(t_s + c / 2, v);
-                    if (c == 64 && !dual) {  // the rest of this tile and the start of the other one fill each other's gaps
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(smem_u32(&t.turn[1 - m]));
-                    }
-                }
-                sum += (add[0].x + add[1].x) + (add[0].y + add[1].y);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&t.p_full[m]));
-            }
-            // ---- end of the segment
-            const bool mine = my0 < cnt, whole = cnt == seg.tiles, two = dual && cnt > 1;
-            if (mine) {
-                mbar_wait_bounded(smem_u32(&t.o_full[m]), n_unit & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
-                ++n_unit;
-                tc_fence_after();
-            }
-            // Two sums over the same rows meet here: warpgroup 0 reads the other one's O from tensor memory (the same lanes).
-            float w0 = 1.f, w1 = 0.f;
-            bool writes = true;
-            if (dual) {
-                if (two && m == 1) t.stat[0][r] = mx, t.stat[1][r] = sum;
-                named_bar_sync(1, 256);
-                writes = m == 0;
-                if (two && m == 0) {
-                    mbar_wait_bounded(smem_u32(&t.o_full[1]), n_other & 1u, abort_flag, p.status, FAULT_PROMPT_WAIT);
-                    tc_fence_after();
-                    const float mx1 = t.stat[0][r], top = fmaxf(mx, mx1);
-                    w0 = mx == -INFINITY ? 0.f : exp2_approx((mx - top) * p.scale_log2);
-                    w1 = mx1 == -INFINITY ? 0.f : exp2_approx((mx1 - top) * p.scale_log2);
-                    sum = w0 * sum + w1 * t.stat[1][r];
-                    mx = top;
-                }
-            }
-            if (two || (!dual && cnt > 0)) ++n_other;
-            if (writes) {
-                // 16 columns of the row's O; the other warpgroup's lie D columns behind
-                auto columns = [&](int c, float (&o)[16]) {
-                    tmem_ld16(t_o + c, o);
-                    if (two) {
-                        float o1[16];
-                        tmem_ld16(t_o + D + c, o1);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = w0 * o[e] + w1 * o1[e];
+                        if (mine) drained();
                     } else {
-                        tmem_ld_wait();
-                    }
-                };
-                auto drained = [&]() {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive(smem_u32(&t.o_empty[m]));
-                        if (two) mbar_arrive(smem_u32(&t.o_empty[1]));
-                    }
-                };
-                if (whole) {
-                    const bool store = live && !*abort_flag;
-                    const float inv = 1.0f / sum;
-                    bf16* out = p.Out + (long long)(seg.token + tok) * p.ldo + (long long)(seg.head * p.G + r_head) * D;
+                        constexpr long long kPart = (long long)(D + 2) * 128;
+                        float* part = p.parts + (seg.slot * 2 + m) * kPart;
+                        if (live) __stcg(part + (long long)D * 128 + r, mx), __stcg(part + (long long)(D + 1) * 128 + r, sum);
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {
-                        float o[16];
-                        if (mine) columns(c, o);
-                        uint32_t w[8];
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            columns(c, o);
+                            if (live) {
 #pragma unroll
-                        for (int q = 0; q < 8; ++q)  // a query that sees no key gives zero
-                            w[q] = limit > 0 ? pack_bf16(o[2 * q] * inv, o[2 * q + 1] * inv) : 0u;
-                        if (store) store_row16(out + c, w, p.out32);
-                        __syncwarp();
-                    }
-                    if (mine) drained();
-                } else {
-                    constexpr long long kPart = (long long)(D + 2) * 128;
-                    float* part = p.parts + (seg.slot * 2 + m) * kPart;
-                    if (live) __stcg(part + (long long)D * 128 + r, mx), __stcg(part + (long long)(D + 1) * 128 + r, sum);
-#pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {
-                        float o[16];
-                        columns(c, o);
-                        if (live) {
-#pragma unroll
-                            for (int e = 0; e < 16; e += 4)
-                                __stcg(reinterpret_cast<float4*>(part) + (c + e) / 4 * 128 + r, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                                for (int e = 0; e < 16; e += 4)
+                                    __stcg(reinterpret_cast<float4*>(part) + (c + e) / 4 * 128 + r, make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                            }
+                            __syncwarp();
                         }
-                        __syncwarp();
-                    }
-                    drained();
-                    const int writers = dual ? 128 : 256;
-                    named_bar_sync(dual ? 2 : 1, writers);  // behind it thread 0 speaks for all
-                    if (tid == 0) {
-                        // One counter per share: of the units that start in it only the last can be cut.
-                        __threadfence();
-                        t.last = atomicAdd(p.count + seg.c0, (unsigned)cnt) + (unsigned)cnt == (unsigned)seg.tiles;
-                        if (t.last) p.count[seg.c0] = 0u;
-                        __threadfence();
-                    }
-                    if (warp == 1) {
-                        // meanwhile the parts that there are, in the order of the keys
-                        int n = 0;
-                        for (int c0 = seg.c0; c0 <= seg.c1; c0 += 32) {
-                            const int c = c0 + lane;
-                            const bool has = c <= seg.c1 && ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles) > ap_tile_at(ap_share(line, c), seg.x0, seg.tiles);
-                            const uint32_t all = __ballot_sync(0xffffffffu, has);
-                            if (has) t.list[n + __popc(all & ((1u << lane) - 1u))] = (short)(2 * (2 * c + (c == seg.c0 ? 1 : 0)));
-                            n += __popc(all);
+                        drained();
+                        const int writers = dual ? 128 : 256;
+                        named_bar_sync(dual ? 2 : 1, writers);  // behind it thread 0 speaks for all
+                        if (tid == 0) {
+                            // One counter per share: of the units that start in it only the last can be cut.
+                            __threadfence();
+                            t.last = atomicAdd(p.count + seg.c0, (unsigned)cnt) + (unsigned)cnt == (unsigned)seg.tiles;
+                            if (t.last) p.count[seg.c0] = 0u;
+                            __threadfence();
                         }
-                        if (lane == 0) t.parts = n;
+                        if (warp == 1) {
+                            // meanwhile the parts that there are, in the order of the keys
+                            int n = 0;
+                            for (int c0 = seg.c0; c0 <= seg.c1; c0 += 32) {
+                                const int c = c0 + lane;
+                                const bool has = c <= seg.c1 && ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles) > ap_tile_at(ap_share(line, c), seg.x0, seg.tiles);
+                                const uint32_t all = __ballot_sync(0xffffffffu, has);
+                                if (has) t.list[n + __popc(all & ((1u << lane) - 1u))] = (short)(2 * (2 * c + (c == seg.c0 ? 1 : 0)));
+                                n += __popc(all);
+                            }
+                            if (lane == 0) t.parts = n;
+                        }
+                        named_bar_sync(dual ? 2 : 1, writers);
+                        if (t.last && !*abort_flag) {
+                            if (seg.tokens * p.G > 32) ap_join<D, 8, 2>(p, seg, t.list, t.parts, tid, writers);
+                            else if (seg.tokens * p.G > 8) ap_join<D, 4, 4>(p, seg, t.list, t.parts, tid, writers);
+                            else ap_join<D, 1, 8>(p, seg, t.list, t.parts, tid, writers);
+                        }
+                        named_bar_sync(dual ? 2 : 1, writers);  // the list and the flag are free again
                     }
-                    named_bar_sync(dual ? 2 : 1, writers);
-                    if (t.last && !*abort_flag) {
-                        if (seg.tokens * p.G > 32) ap_join<D, 8, 2>(p, seg, t.list, t.parts, tid, writers);
-                        else if (seg.tokens * p.G > 8) ap_join<D, 4, 4>(p, seg, t.list, t.parts, tid, writers);
-                        else ap_join<D, 1, 8>(p, seg, t.list, t.parts, tid, writers);
-                    }
-                    named_bar_sync(dual ? 2 : 1, writers);  // the list and the flag are free again
                 }
+                __syncwarp();
+                if (lane == 0) release();
+                else ++n_seg;
             }
-            __syncwarp();
-            if (lane == 0) release();
-            else ++n_seg;
         }
-    }
     }
     __syncwarp();
     tc_fence_before();

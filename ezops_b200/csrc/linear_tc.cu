@@ -2,16 +2,26 @@
 //   out[m, n] = act( sum_k x[m, k] W[n, k] + bias[n] ) + residual[m, n],            fp32 until the one rounding,
 //   SwiGLU: silu(gate + bias_g) * (up + bias_u) with W = [gate rows | up rows].
 //
-// More than kLinearFewRows rows: two CTAs of a cluster share a tile of 256 rows of x by BN rows of W
-// (tcgen05.mma.cta_group::2: each CTA holds half of x's rows and half of W's, and 128 x BN of the result in its tensor
-// memory), so each operand byte that enters an SM is used by two.  One elected thread per CTA fills a ring of 64-element
+// More than kLinearFewRows rows: two CTAs of a cluster share a tile of 256 rows of A by BN rows of B, A = x and B = W or the
+// other way round (tcgen05.mma.cta_group::2: each CTA holds half of both operands' rows, and 128 x BN of the result in its
+// tensor memory), so each operand byte that enters an SM is used by two.  One elected thread per CTA fills a ring of 64-element
 // K blocks by TMA (both CTAs' bytes are counted on the first CTA's barrier), one thread of the first CTA issues the MMAs,
 // eight warps of each CTA drain one of two accumulators while the next tile is multiplied: bias, activation, residual and
-// rounding happen there, in registers.  Grid: one CTA per SM, tiles in groups of kLinearGroup row tiles so that the x and W
+// rounding happen there, in registers.  Grid: one CTA per SM, tiles in groups of kLtGroup tiles along A so that the x and W
 // tiles in flight stay in L2.  BN = 256 reads least per product; narrower tiles (128, 64) are taken when the wide ones would
 // leave clusters without work (linear_plan).
-// What bounds it: the tensor cores (and from a few hundred rows down the weights' bytes).
-// Few rows: the kernel of the batched decode projections (gemm_tc.cu) with this epilogue.
+//   A = x: a lane of the epilogue has a row of the result and stores whole sectors of it.
+//   A = W: a lane has a column, and a warp's stores run along a row: for rows that start anywhere (a vocabulary or a number of
+// experts that is no multiple of 16, columns of a wider tensor), where a lane with a row would write parts of sectors, and for
+// up to kLtSwapRows rows, where half of a tile of 256 rows of x would be empty.  SwiGLU then has gate and up rows as two A
+// operands, two accumulators side by side.  Measured, A = x against A = W: 7404 x 17921, K = 96, gelu 422 and 184 us (with 17920
+// columns: 154 and 163); 4530 x 3350, K = 720, fp32 62 and 32; 104 x 22304, K = 7360 86 and 67; 128 rows of 4096 through SwiGLU to
+// 12288 61 to 67 and 50; 300 x 4096, K = 4096 15.2 to 16.6 and 16.0 to 16.9; 8192 x 4096, K = 4096 193 and 188 to 193.
+// What bounds it: the tensor cores where tiles fill the clusters evenly (4096 rows of 4096 through SwiGLU to 12288: 507 to 600 us
+// under the power cap, 1370 to 1630 TFLOP/s); else the operands' way from L2 (777 x 4096, K = 12288: 64 tiles on 74 clusters bring
+// 0.7 GB into the SMs in 72 us); from a few hundred rows down the weights' bytes (104 x 22304, K = 7360: 5.1 TB/s).
+// Few rows: the kernel of the batched decode projections (gemm_tc.cu) with this epilogue (17 x 6144, K = 4096: 10.3 us, 4.9 TB/s;
+// 64 x 151936, K = 1024 to fp32: 57 us, 6.1 TB/s).
 #include <atomic>
 
 #include "prompt.h"
@@ -495,6 +505,7 @@ static constexpr int kLtMinBlocks = 8;   // k blocks below which a further clust
 static constexpr int kLtMostParts = 8;
 static constexpr int kLtCutTiles = 8;    // most tiles that are cut
 static constexpr int kLtCutBlocks = 64;  // fewest k blocks of a tile that is
+static constexpr int kLtSwapRows = 128;  // rows of x up to which W's rows are A
 static LtPlan linear_plan(int M, int N, int K, int act, bool cut, bool aligned) {
     const long long kb = (K + kLtBlockK - 1) / kLtBlockK, most = sm_count() / 2;
     const int widths[3] = {256, 128, 64};
@@ -515,7 +526,7 @@ static LtPlan linear_plan(int M, int N, int K, int act, bool cut, bool aligned) 
         if (clusters > by_blocks) clusters = by_blocks;
         if (clusters > most) clusters = most;
         best.sk_tiles = best.clusters, best.clusters = (int)clusters;
-    } else if (!aligned) {
+    } else if (!aligned || M <= kLtSwapRows) {
         best = whole(N, M, act == ACT_SWIGLU ? 1 : 0);
         best.swap = true;
     }
