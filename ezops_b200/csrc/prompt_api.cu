@@ -190,4 +190,14 @@ int ezb_attn_prompt(const void* Q, long long ldq, const void* K_pool, const void
     return EZB_OK;
 }
 
+unsigned long long ezb_stream_capture_id(ezb_stream_t stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 }  // extern "C"

@@ -10,9 +10,10 @@ import torch
 from .. import _lib
 from ..registry import register_kernel
 from .base_kernel import BaseKernel
-from .sm100 import _BF16, _current_device, _raw_stream, _zeros_bytes
+from .sm100 import _BF16, _current_device, _raw_stream
 
 _I32 = torch.int32
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 # A step is a few short kernels, so the host's share counts (see sm100.py): a call asks everything about its tensors in one
@@ -61,6 +62,31 @@ def _distance(t: torch.Tensor) -> int:
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+class _Workspaces:
+    """The workspaces of one operator: one per device and stream, and one per stream of a graph capture, so that neither calls on
+    several streams nor graphs that are replayed side by side meet in one.  A captured call never uses an eager one's, nor the
+    other way round: the counters in front (all that has to be zero) are cleared where the memory is first used, in a graph
+    once per replay.  A capture's are dropped when the next one begins: they lie in its graph's own pool."""
+
+    _COUNTERS = 4096
+
+    def __init__(self, lib):
+        self._lib, self._eager, self._captured, self._capture = lib, {}, {}, 0
+
+    def get(self, nbytes: int, device: int, stream: int):
+        held = self._eager
+        if _capturing():
+            capture = self._lib.ezb_stream_capture_id(stream)
+            if capture != self._capture:
+                self._capture, self._captured = capture, {}
+            held = self._captured
+        ws = held.get((device, stream))
+        if ws is None:
+            ws = held[device, stream] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
+            ws[: self._COUNTERS].zero_()
+        return ws
 
 
 @register_kernel("paged_plan", "cuda", family="prompt")
@@ -132,7 +158,7 @@ class PagedQkNormRopeSm100Kernel(BaseKernel):
 
 @register_kernel("linear", "cuda", family="prompt")
 class LinearSm100Kernel(BaseKernel):
-    """Owns a workspace per device for the numbers of rows that have a use for one; one operator serves one stream at a time."""
+    """Owns workspaces (``_Workspaces``) for the numbers of rows that have a use for one."""
 
     def __init__(self, out_features, in_features, bias=False, activation=None, residual=False, out_dtype=_BF16):
         from ..ops.linear import ACTIVATIONS
@@ -146,16 +172,17 @@ class LinearSm100Kernel(BaseKernel):
         self._lib = _lib.load()
         self._entry = self._lib.ezb_linear_bf16
         self._need: dict[int, int] = {}  # rows -> workspace bytes
-        self._ws = None
+        self._spaces, self._ws = _Workspaces(self._lib), None
 
     def workspace(self, rows: int, device):
         """The workspace for so many rows, or None; it never has to grow."""
         need = self._need.get(rows)
         if need is None:
             need = self._need[rows] = self._lib.ezb_linear_workspace_bytes(rows, self.N, self.K, self.act)
-        if need and (self._ws is None or self._ws.device != device):
-            self._ws = _zeros_bytes(need, device)
-        return self._ws if need else None
+        if not need:
+            return None
+        self._ws = self._spaces.get(need, device.index, _raw_stream(device.index))
+        return self._ws
 
     def __call__(self, X, W, bias=None, residual=None, out=None):
         dev, M, N, K = _device(X, "X"), X.shape[0], self.N, self.K
@@ -176,20 +203,16 @@ class LinearSm100Kernel(BaseKernel):
 
 @register_kernel("attn_prompt", "cuda", family="prompt")
 class AttnPromptSm100Kernel(BaseKernel):
-    """Owns a workspace per device; one operator serves one stream at a time."""
+    """Owns workspaces (``_Workspaces``)."""
 
     def __init__(self, batch, num_heads, head_dim, max_pages, page_size, num_kv_heads=None):
         self.B, self.H, self.D, self.max_pages, self.P = batch, num_heads, head_dim, max_pages, page_size
         self.NKV = num_heads if num_kv_heads is None else num_kv_heads
         self._table, self._lens, self._cu = (batch, max_pages), (batch,), (batch + 1,)
-        self._ws = None
         self._lib = _lib.load()
         self._entry = self._lib.ezb_attn_prompt
-
-    def workspace(self, device):
-        if self._ws is None or self._ws.device != device:
-            self._ws = _zeros_bytes(self._lib.ezb_attn_prompt_workspace_bytes(self.D), device)
-        return self._ws
+        self._need = self._lib.ezb_attn_prompt_workspace_bytes(self.D)
+        self._spaces = _Workspaces(self._lib)
 
     def __call__(self, Q, K_pool, V_pool, page_table, seq_lens, cu_tokens, out=None):
         dev, T, H, D = _device(Q, "Q"), Q.shape[0], self.H, self.D
@@ -202,10 +225,11 @@ class AttnPromptSm100Kernel(BaseKernel):
             _refuse([("Q", Q, heads, _BF16, True), ("K_pool", K_pool, pool, _BF16, False), ("V_pool", V_pool, pool, _BF16, False),
                      ("page_table", page_table, self._table, _I32, False), ("seq_lens", seq_lens, self._lens, _I32, False),
                      ("cu_tokens", cu_tokens, self._cu, _I32, False), ("out", out, heads, _BF16, True)], dev)
-        ws = self.workspace(Q.device)
+        stream = _raw_stream(dev)
+        ws = self._spaces.get(self._need, dev, stream)
         rc = self._entry(Q.data_ptr(), _distance(Q), K_pool.data_ptr(), V_pool.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
                          cu_tokens.data_ptr(), out.data_ptr(), _distance(out), ws.data_ptr(), ws.numel(), self.B, T, H, self.NKV, D,
-                         self.max_pages, self.P, pool[0], _raw_stream(dev))
+                         self.max_pages, self.P, pool[0], stream)
         if rc:
             _lib.check(rc)
         return out

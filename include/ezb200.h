@@ -375,8 +375,8 @@ int ezb_paged_qk_norm_rope(const void* qkv, long long ldqkv, const void* qw_or_n
  * the gate rows, then the up rows, and act is silu(gate) * up.  Rows of X, residual
  * (bf16) and out may be further apart than they are long (ldx, ldres, ldout in
  * elements; ldx a multiple of 8).  residual may be out itself.  K % 8 == 0.  The path,
- * and with it the order of the sums, follows from M, N, K and whether there is a
- * workspace: with one, sizes whose tiles would leave part of the GPU idle have some
+ * and with it the order of the sums, follows from M, N, K, whether rows of out (32 bytes)
+ * and residual (16) start at their boundaries, and whether there is a workspace: with one, sizes whose tiles would leave part of the GPU idle have some
  * tiles cut along K (ezb_linear_workspace_bytes() > 0; without one they are slower).
  * Equal calls give equal bits.  activation is one of EZB_ACT_*. */
 #define EZB_ACT_NONE 0
@@ -400,8 +400,12 @@ int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bia
  * cu_tokens is cut to [0, T], seq_lens to [0, max_pages * page_size].  Equal calls
  * give equal bits; where a row's sums are cut may depend on the other rows.
  * The workspace depends on D only; as everywhere it is zero-filled once and serves one
- * stream at a time.  D in {64, 128}; H / NKV <= 128; page_size a power of two >= 64. */
+ * stream at a time; after a recorded wait that ran out (0x1xx) it has to be zero-filled
+ * again.  D in {64, 128}; H / NKV <= 128; page_size a power of two >= 64. */
 size_t ezb_attn_prompt_workspace_bytes(int D);
+/* Identity of the graph capture that `stream` takes part in, 0 when there is none: a
+ * binding that keeps workspaces gives a captured call one of its capture's. */
+unsigned long long ezb_stream_capture_id(ezb_stream_t stream);
 int ezb_attn_prompt(const void* Q, long long ldq, const void* K_pool, const void* V_pool, const int* page_table, const int* seq_lens,
                     const int* cu_tokens, void* Out, long long ldo, void* workspace, size_t workspace_bytes, int B, int T, int H, int NKV,
                     int D, int max_pages, int page_size, int num_pages, ezb_stream_t stream);

@@ -557,3 +557,120 @@ def test_linear_tiles_cut_along_k(M, N, K, act, out_dtype):
     assert (op._kernel._ws[:4096] == 0).all()  # the counters are ready for the next call
     op._kernel.workspace = lambda rows, device: None
     close(op(X, W, bias=b, residual=r), y, tol)
+
+
+@pytest.mark.parametrize("M,N,K,act", [(700, 1043, 200, "gelu"), (2500, 9001, 72, None), (190, 19494, 136, "relu"), (100, 5000, 520, "silu"),
+                                       (128, 640, 1000, None), (129, 6402, 264, "swiglu"), (1030, 5005, 80, "swiglu"), (66, 33, 64, "swiglu"),
+                                       (5000, 31, 72, "silu")])
+@pytest.mark.parametrize("out_dtype", [BF16, torch.float32])
+def test_linear_rows_that_start_anywhere(M, N, K, act, out_dtype):
+    """A lane per output column: one and several rounds of tiles of every width, last tiles of both kinds, pitches of any size."""
+    linear_case(M, N, K, act, True, True, out_dtype)
+    op = ez.LinearOp(M, N, K, backend="cuda", activation=act, residual=True, out_dtype=out_dtype)
+    torch.manual_seed(N)
+    X, W, _, r = op.gen_data()
+    y, tol = linear64(op, X, W, None, r)
+    wide_r = torch.full((M, N + 5), 9.0, device=DEV, dtype=BF16)
+    wide_r[:, 3 : 3 + N] = r
+    wide = torch.full((M, N + 9), 3.0, device=DEV, dtype=out_dtype)
+    out = wide[:, 4 : 4 + N]
+    op(X, W, residual=wide_r[:, 3 : 3 + N], out=out)
+    close(out, y, tol)
+    assert (wide[:, :4] == 3.0).all() and (wide[:, 4 + N :] == 3.0).all()
+
+
+def attn_rows(B, D, seed):
+    """An operator, its arguments and the result of a call that cuts units between CTAs."""
+    op = ez.AttnPromptOp(B, B, 8, D, 64, 64, num_kv_heads=2, backend="cuda")
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    Q = torch.randn(B, 8, D, generator=g, device=DEV).to(BF16)
+    K, V = (torch.randn(B * 64, 2, 64, D, generator=g, device=DEV).to(BF16) for _ in range(2))
+    table = torch.arange(B * 64, device=DEV, dtype=torch.int32).view(B, 64)
+    lens = torch.randint(2000, 4096, (B,), generator=g, device=DEV, dtype=torch.int32)
+    return op, [Q, K, V, table, lens, torch.arange(B + 1, device=DEV, dtype=torch.int32)]
+
+
+def test_attn_first_call_in_a_capture():
+    """A first call that is captured leaves nothing behind that a call outside of the graph would use, before or after a replay."""
+    op, args = attn_rows(3, 128, 1)
+    want = attn_rows(3, 128, 1)[0](*args)
+    out = torch.zeros_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op(*args, out=out)
+    assert torch.equal(op(*args), want)
+    for _ in range(2):
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, want)
+    assert torch.equal(op(*args), want)
+    lin = ez.LinearOp(555, 44, 5544, backend="cuda")
+    X, W, _, _ = lin.gen_data()
+    y = ez.LinearOp(555, 44, 5544, backend="cuda")(X, W)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        lin(X, W)
+    assert torch.equal(lin(X, W), y)
+
+
+def test_attn_streams_and_graphs_side_by_side():
+    """One operator on two streams at once, and two graphs of it replayed at once: each has a workspace of its own."""
+    op, args = attn_rows(2, 128, 2)
+    other = [a.clone() for a in args]
+    other[0] = -other[0]
+    want, want2 = op(*args), op(*other)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for a in (args, other):
+        out, graph = torch.zeros_like(want), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(8):
+                op(*a, out=out)
+        graphs.append(graph)
+        outs.append(out)
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], want) and torch.equal(outs[1], want2)
+    results = [[], []]
+    for _ in range(50):
+        for i, a in enumerate((args, other)):
+            with torch.cuda.stream(streams[i]):
+                results[i].append(op(*a))
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, want) for r in results[0]) and all(torch.equal(r, want2) for r in results[1])
+
+
+def test_pools_of_more_than_two_to_the_31_elements():
+    """The last pages of large pools give what the same pages of small ones give, bit for bit."""
+    NKV, page, D, pages = 8, 256, 128, 8300
+    K, V = (torch.zeros(pages, NKV, page, D, device=DEV, dtype=BF16) for _ in range(2))
+    assert K.numel() > 2**31
+    op, (Q, k, v, table, lens, cu), want = attn_case([40, 1], [300, 500], 32, NKV, D, page)
+    few = k.shape[0]
+    K[-few:], V[-few:] = k, v
+    far = torch.where(table >= 0, table + (pages - few), table)
+    assert torch.equal(op(Q, K, V, far, ints(*lens), ints(*cu)), want)
+    T = 50
+    small, large = (ez.PagedQkNormRopeOp(T, 32, D, 512, page, n, backend="cuda", num_kv_heads=NKV) for n in (few, pages))
+    qkv, qw, kw, cos, sin, positions, slots, k, v = small.gen_data()
+    K[-few:], V[-few:] = k, v
+    q = small(qkv, qw, kw, cos, sin, positions, slots, k, v)
+    far = torch.where(slots >= 0, slots + (pages - few) * page, slots)
+    assert torch.equal(large(qkv, qw, kw, cos, sin, positions, far, K, V), q)
+    assert torch.equal(K[-few:], k) and torch.equal(V[-few:], v)
+
+
+@pytest.mark.parametrize("N", [60000, 60001])
+def test_linear_results_of_more_than_two_to_the_31_elements(N):
+    M, K = 36000, 64
+    op = ez.LinearOp(M, N, K, backend="cuda", residual=True)
+    torch.manual_seed(N)
+    X, W = torch.randn(M, K, device=DEV).to(BF16), torch.randn(N, K, device=DEV).to(BF16)
+    r = torch.randn(M, N, device=DEV, dtype=BF16)
+    out = op(X, W, residual=r)
+    at = torch.tensor([0, 127, 128, 17000, 35791, 35792, 35999], device=DEV)  # 35791 * N is just below 2^31
+    y, tol = linear64(op, X[at], W, None, r[at])
+    close(out[at], y, tol)
