@@ -83,13 +83,24 @@ struct TcParams {
 // 2B layers above 488 -> 438 us, 28 layers of 0.6B at batch 4 1008 -> 858 us).
 // LINK: the instance for chains with the fused exchange: its epilogue can push fp32 results into the peers' inboxes (see
 // TpLink), and its waits start behind the gather of the kernel in front.
-// EXT: the instance for linear layers (LinearOp): bias, activation and residual in fp32, result in bf16 or fp32.
+// EXT: the instance for linear layers (LinearOp): bias, activation and residual in fp32, result in bf16 or fp32.  The tensor
+// cores cut their sums towards zero, 2^-24 a step on average and always the same way: a sum over K = 12800 ends 1.4e-5 short.
+// A result that is not rounded to bf16 therefore leaves them every kTcSegment k blocks and is added up, rounded to nearest, in
+// further columns of the tensor memory.
+static constexpr int kTcSegment = 8;
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(__float_as_uint(v[0])),
+                 "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])),
+                 "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7]))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 template <int NB, bool LINK, bool EXT>
 __global__ void __launch_bounds__(kTcThreads, 2)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant__ CUtensorMap mapW1,
                const __grid_constant__ CUtensorMap mapX, const TcParams p) {
     constexpr int B_BYTES = NB * kTcBlockK * 2;
-    constexpr int TMEM_COLS = (2 * NB < 32) ? 32 : 2 * NB;  // two accumulators, power of two >= 32
+    constexpr int TMEM_COLS = EXT ? 4 * NB : (2 * NB < 32) ? 32 : 2 * NB;  // two accumulators (EXT: and sums), power of two >= 32
     constexpr uint32_t IDESC = umma_idesc_bf16(kTcRows, NB);
 
     extern __shared__ unsigned char smem_raw[];
@@ -120,6 +131,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
     const int cluster = blockIdx.x >> p.log2c, n_clusters = gridDim.x >> p.log2c;
     const int kb0 = (int)((long long)KB * rank >> p.log2c), kb1 = (int)((long long)KB * (rank + 1) >> p.log2c);
     const int my_tiles = (p.tiles - cluster + n_clusters - 1) / n_clusters;
+    const int seg = EXT && p.out_f32 ? kTcSegment : KB;  // k blocks of an accumulator
 
     if (tid == 0) {
         for (int s = 0; s < NS; ++s) {
@@ -212,14 +224,15 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
             if (LINK) pdl_wait();
             int stage = 0;
             uint32_t full_parity = 0;
-            for (int i = 0; i < my_tiles && !(*abort_flag); ++i) {
-                const int acc = i & 1;
+            // (EXT: an iteration per segment, else per tile)
+            for (int i = 0, u = 0, k0 = kb0; i < my_tiles && !(*abort_flag); ++u) {
+                const int acc = u & 1, k1 = EXT ? min(k0 + seg, kb1) : kb1;
                 // wait until the epilogue has drained this accumulator (passes at once for its first use)
-                if (!mbar_wait_bounded(smem_u32(&acc_empty[acc]), (uint32_t)(((i >> 1) & 1) ^ 1), abort_flag, p.status, FAULT_TC_ACC_WAIT))
+                if (!mbar_wait_bounded(smem_u32(&acc_empty[acc]), (uint32_t)(((u >> 1) & 1) ^ 1), abort_flag, p.status, FAULT_TC_ACC_WAIT))
                     break;
                 tc_fence_after();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(acc * NB);
-                for (int kb = kb0; kb < kb1; ++kb) {
+                for (int kb = k0; kb < k1; ++kb) {
                     if (!mbar_wait_bounded(smem_u32(&full_bar[stage]), full_parity, abort_flag, p.status, FAULT_GEMV_FULL_WAIT))
                         break;
                     tc_fence_after();
@@ -230,11 +243,13 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                     // the shared memory holds, and the accumulator lanes they end up in are never read.
 #pragma unroll
                     for (int k = 0; k < kTcBlockK / 16; ++k)  // 32 bytes along K per MMA: +2 in the 16-byte address field
-                        tc_mma_bf16(d_tmem, adesc + 2 * k, bdesc + 2 * k, IDESC, (kb > kb0 || k > 0) ? 1u : 0u);
+                        tc_mma_bf16(d_tmem, adesc + 2 * k, bdesc + 2 * k, IDESC, (kb > k0 || k > 0) ? 1u : 0u);
                     tc_commit(smem_u32(&empty_bar[stage]));  // stage reusable once these MMAs have read it
                     if (++stage == NS) stage = 0, full_parity ^= 1;
                 }
                 tc_commit(smem_u32(&acc_full[acc]));
+                k0 = k1;
+                if (!EXT || k1 == kb1) ++i, k0 = kb0;
             }
         }
     } else {
@@ -274,9 +289,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
             }
             named_bar_sync(2, 32 * kTcEpiWarps);
         }
-        for (int i = 0; i < my_tiles; ++i) {
+        for (int i = 0, uses = 0; i < my_tiles; ++i, ++uses) {
             const int tile = cluster + i * n_clusters;
-            const int acc = i & 1;
             const int n = tile * p.units + frow;
             const bool live_row = frow < p.units && n < p.N;
             constexpr int CU = 4;  // columns in flight per thread
@@ -292,7 +306,32 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
             };
             if ((EXT ? p.residual != nullptr : p.epilogue == EPI_RESIDUAL) && live_row) fetch_residual(cg);
             const float next_w = (p.xw_out && live_row) ? __bfloat162float(p.next_norm_w[n]) : 0.f;
-            mbar_wait_bounded(smem_u32(&acc_full[acc]), (uint32_t)((i >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
+            const uint32_t t_sum = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(2 * NB + b_half);
+            bool summed = false;
+            if constexpr (EXT) {  // all segments but the last
+                for (int k = kb0; k + seg < kb1; k += seg, ++uses) {
+                    mbar_wait_bounded(smem_u32(&acc_full[uses & 1]), (uint32_t)((uses >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
+                    tc_fence_after();
+                    const uint32_t t = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)((uses & 1) * NB + b_half);
+#pragma unroll 1
+                    for (int c = 0; c < HC; c += 8) {
+                        float v[8], w[8];
+                        tmem_ld8(t + (uint32_t)c, v);
+                        if (summed) tmem_ld8(t_sum + (uint32_t)c, w);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = summed ? v[e] + w[e] : v[e];
+                        tmem_st8(t_sum + (uint32_t)c, v);
+                    }
+                    tmem_st_wait();
+                    summed = true;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&acc_empty[uses & 1]));
+                }
+            }
+            const int acc = (EXT ? uses : i) & 1;
+            mbar_wait_bounded(smem_u32(&acc_full[acc]), (uint32_t)(((EXT ? uses : i) >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
             if (i == 0) trace_mark(trec, 4);
             tc_fence_after();
             const bool straight = EXT && C == 1 && !p.pair;  // no parts, see below
@@ -314,9 +353,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
                             r8[e] = p.residual && own && b_half + c + e < p.B ? __bfloat162float(p.residual[(long long)(b_half + c + e) * p.ldres + n_own]) : 0.f;
+                        float w[8];
+                        if (summed) tmem_ld8(t_sum + (uint32_t)c, w);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += bias;
+                        for (int e = 0; e < 8; ++e) v[e] += (summed ? w[e] : 0.f) + bias;
                         linear_act(v, p.act);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
@@ -335,12 +376,20 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                     continue;
                 }
             }
+            auto add_sums = [&](int c, float* v) {
+                float w[8];
+                tmem_ld8(t_sum + (uint32_t)c, w);
+                tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += w[e];
+            };
             float* dst = mine + (size_t)b_half * RS + row;
             const int b_left = p.B - b_half;
             if constexpr (HC == 8) {
                 float v[8];
                 tmem_ld8(t_addr, v);
                 tmem_ld_wait();
+                if (EXT && summed) add_sums(0, v);
                 if (row < RS) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e, dst += RS)
@@ -352,6 +401,10 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                     float v[16];
                     tmem_ld16(t_addr + (uint32_t)c, v);
                     tmem_ld_wait();
+                    if (EXT && summed) {
+                        add_sums(c, v);
+                        add_sums(c + 8, v + 8);
+                    }
                     if (row < RS) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e, dst += RS)

@@ -20,6 +20,10 @@
 // What bounds it: the tensor cores where tiles fill the clusters evenly (4096 rows of 4096 through SwiGLU to 12288: 507 to 600 us
 // under the power cap, 1370 to 1630 TFLOP/s); else the operands' way from L2 (777 x 4096, K = 12288: 64 tiles on 74 clusters bring
 // 0.7 GB into the SMs in 72 us); from a few hundred rows down the weights' bytes (104 x 22304, K = 7360: 5.1 TB/s).
+// fp32 results of more than kLtSegment k blocks: the tensor cores cut their sums towards zero (gemm_tc.cu), so the sums leave them
+// every kLtSegment blocks and are added up, rounded to nearest, in the registers of the lane whose column it is (A = W); the relative
+// error is 4.8e-7 for any K (1.4e-5 at K = 12800 otherwise), and 8192 x 4096, K = 4096 takes 193 us instead of 191.  Rounded to
+// bf16 that error does not show.
 // Few rows: the kernel of the batched decode projections (gemm_tc.cu) with this epilogue (17 x 6144, K = 4096: 10.3 us, 4.9 TB/s;
 // 64 x 151936, K = 1024 to fp32: 57 us, 6.1 TB/s).
 #include <atomic>
@@ -33,6 +37,7 @@ static constexpr int kLtThreads = 320;  // TMA warp, MMA warp, eight epilogue wa
 static constexpr int kLtBlockK = 64;
 static constexpr int kLtMaxStages = 12;
 static constexpr int kLtCountBytes = 4096;  // counters in front of the parts
+static constexpr int kLtSegment = 8;  // k blocks of a sum that stays in the tensor cores, where the result is not rounded to bf16
 static constexpr int kLtGroup = 8;  // row tiles per group of the tile order
 
 struct LtParams {
@@ -139,7 +144,8 @@ __device__ __forceinline__ void load_packed(const bf16* src, int left, int vec, 
     }
 }
 
-template <int BN, bool PAIR, bool SWAP>
+// SEG: the products of kLtSegment k blocks at a time, added up in registers (fp32 results, swapped form).
+template <int BN, bool PAIR, bool SWAP, bool SEG>
 __global__ void __launch_bounds__(kLtThreads, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW0,
                  const __grid_constant__ CUtensorMap mapW1, const __grid_constant__ LtParams p) {
@@ -210,11 +216,12 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
             int it = 0, n = 0;
-            for (; !*abort_flag && work.step(p, n_clusters); ++n) {
+            for (bool more = work.step(p, n_clusters); more && !*abort_flag; ++n) {
                 const int acc = n & 1;
                 if (!mbar_wait_bounded_cluster(smem_u32(&acc_empty[acc]), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, p.status, FAULT_TC_ACC_WAIT)) break;
                 tc_fence_after();
-                for (int kb = work.k0; kb < work.k1; ++kb, ++it) {
+                const int k_end = SEG ? min(work.k0 + kLtSegment, work.k1) : work.k1;
+                for (int kb = work.k0; kb < k_end; ++kb, ++it) {
                     const int s = it % L::kStages;
                     if (!mbar_wait_bounded_cluster(smem_u32(&full[s]), (uint32_t)((it / L::kStages) & 1), abort_flag, p.status, FAULT_GEMV_FULL_WAIT)) break;
                     tc_fence_after();
@@ -231,17 +238,19 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                     tc_commit_pair(smem_u32(&empty[s]));
                 }
                 tc_commit_pair(smem_u32(&acc_full[acc]));
+                work.k0 = k_end;
+                if (!SEG || k_end == work.k1) more = work.step(p, n_clusters);
             }
         }
     } else if constexpr (SWAP) {
         // A lane has an output column and walks rows of it, W at a time: a warp's loads and stores run along the rows of the
         // output, wherever those start.  The residual is requested a step ahead.
-        constexpr int W = 32;
+        constexpr int W = SEG ? 16 : 32;
         const int q = warp & 3, c0 = ((warp - 2) >> 2) * W;
         for (int n = 0; work.step(p, n_clusters); ++n) {
             int ta, tb;
             tile_at(work.tile, ta, tb);
-            const int acc = n & 1, n0 = ta * 256 + rank * 128 + q * 32, col = n0 + lane, m0 = tb * BN;
+            const int n0 = ta * 256 + rank * 128 + q * 32, col = n0 + lane, m0 = tb * BN;
             const int rows = n0 < p.N ? min(BN, p.M - m0) : 0;
             const bool live = col < p.N;
             const bf16* res_col = p.residual && live ? p.residual + (long long)m0 * p.ldres + col : nullptr;
@@ -254,17 +263,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
 #pragma unroll
                 for (int e = 0; e < W; ++e) res[e] = c + e < rows ? src[e * p.ldres] : 0;
             };
-            request(c0);
-            mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
-            tc_fence_after();
-            const uint32_t t = tmem + ((uint32_t)(q * 32) << 16) + acc * ACC;
-#pragma unroll 1
-            for (int c = c0; c < rows; c += 2 * W) {
-                float v[W], up[PAIR ? W : 1];
-                tmem_ld32(t + c, v);
-                if constexpr (PAIR) tmem_ld32(t + BN + c, up);
-                tmem_ld_wait();
-                const bool fine = !__any_sync(0xffffffffu, *abort_flag);
+            auto finish = [&](int c, float (&v)[W], float (&up)[PAIR ? W : 1], bool fine) {
 #pragma unroll
                 for (int e = 0; e < W; ++e) v[e] += bias;
                 if constexpr (PAIR) {
@@ -276,7 +275,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                 if (res_col) {
 #pragma unroll
                     for (int e = 0; e < W; ++e) v[e] += __uint_as_float((uint32_t)res[e] << 16);
-                    request(c + 2 * W);
+                    if (!SEG) request(c + 2 * W);
                 }
                 if (live && fine) {
                     const long long o = (long long)(m0 + c) * p.ldout + col;
@@ -290,14 +289,76 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                                 if (c + e < rows) dst[e * p.ldout] = round(v[e]);
                         }
                     };
-                    if (p.out_f32) store(static_cast<float*>(p.out) + o, [](float x) { return x; });
+                    if (SEG || p.out_f32) store(static_cast<float*>(p.out) + o, [](float x) { return x; });
                     else store(static_cast<bf16*>(p.out) + o, [](float x) { return __float2bfloat16_rn(x); });
                 }
                 __syncwarp();
+            };
+            auto filled = [&]() {  // the accumulator's first column
+                const int acc = n & 1;
+                mbar_wait_bounded_cluster(smem_u32(&acc_full[acc]), (uint32_t)((n >> 1) & 1), abort_flag, p.status, FAULT_TC_ACC_WAIT);
+                tc_fence_after();
+                return tmem + ((uint32_t)(q * 32) << 16) + acc * ACC;
+            };
+            auto drained = [&]() {
+                __syncwarp();
+                tc_fence_before();
+                if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[n & 1]), 0));
+            };
+            if constexpr (SEG) {
+                constexpr int STEPS = BN / (2 * W);  // this warp's share: W columns of every 2 W
+                float sum[STEPS][W], sum_up[PAIR ? STEPS : 1][PAIR ? W : 1];
+#pragma unroll
+                for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        sum[j][e] = 0.f;
+                        if constexpr (PAIR) sum_up[j][e] = 0.f;
+                    }
+#pragma unroll 1
+                for (int k = work.k0; k < work.k1; k += kLtSegment) {
+                    const uint32_t t = filled();
+#pragma unroll
+                    for (int j = 0; j < STEPS; ++j) {
+                        const int c = c0 + j * 2 * W;
+                        if (c >= rows) break;
+                        float v[W];
+                        tmem_ld16(t + c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < W; ++e) sum[j][e] += v[e];
+                        if constexpr (PAIR) {
+                            tmem_ld16(t + BN + c, v);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int e = 0; e < W; ++e) sum_up[j][e] += v[e];
+                        }
+                    }
+                    drained();
+                    if (k + kLtSegment < work.k1) ++n;
+                }
+                const bool fine = !__any_sync(0xffffffffu, *abort_flag);
+#pragma unroll
+                for (int j = 0; j < STEPS; ++j) {
+                    const int c = c0 + j * 2 * W;
+                    if (c >= rows) break;
+                    request(c);
+                    if constexpr (PAIR) finish(c, sum[j], sum_up[j], fine);
+                    else finish(c, sum[j], sum_up[0], fine);
+                }
+            } else {
+                request(c0);
+                const uint32_t t = filled();
+#pragma unroll 1
+                for (int c = c0; c < rows; c += 2 * W) {
+                    float v[W], up[PAIR ? W : 1];
+                    tmem_ld32(t + c, v);
+                    if constexpr (PAIR) tmem_ld32(t + BN + c, up);
+                    tmem_ld_wait();
+                    finish(c, v, up, !__any_sync(0xffffffffu, *abort_flag));
+                }
+                drained();
             }
-            __syncwarp();
-            tc_fence_before();
-            if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[acc]), 0));
         }
     } else {
         // A warp of the quarter of rows that it may read; W columns at a time.  What the residual stream holds there is requested
@@ -499,48 +560,52 @@ static bool encode_rows(CUtensorMap* map, const bf16* base, long long rows, long
 // 29.3 cut; 138 rows of 176 outputs, K = 2248: 12.5 and 17.1; 3383 rows of 64, K = 4984, 14 tiles: 21.7 and 18.7 to 25).
 struct LtPlan {
     int bn, clusters, sk_tiles;
-    bool swap;
+    bool swap, seg;
 };
 static constexpr int kLtMinBlocks = 8;   // k blocks below which a further cluster does not pay
 static constexpr int kLtMostParts = 8;
 static constexpr int kLtCutTiles = 8;    // most tiles that are cut
 static constexpr int kLtCutBlocks = 64;  // fewest k blocks of a tile that is
 static constexpr int kLtSwapRows = 128;  // rows of x up to which W's rows are A
-static LtPlan linear_plan(int M, int N, int K, int act, bool cut, bool aligned) {
+static LtPlan linear_plan(int M, int N, int K, int act, bool cut, bool aligned, bool f32) {
     const long long kb = (K + kLtBlockK - 1) / kLtBlockK, most = sm_count() / 2;
     const int widths[3] = {256, 128, 64};
     const double block[3] = {520., 490., 410.};
     auto whole = [&](long long a_rows, long long b_rows, int widest) {
-        LtPlan best = {256, 1, 0, false};
+        LtPlan best = {256, 1, 0, false, false};
         double least = -1.;
         for (int i = widest; i < 3; ++i) {
             const long long tiles = (a_rows + 255) / 256 * ((b_rows + widths[i] - 1) / widths[i]);
             const double cost = (double)((tiles + most - 1) / most) * (double)kb * block[i];
-            if (least < 0. || cost < least) least = cost, best = {widths[i], (int)(tiles < most ? tiles : most), 0, false};
+            if (least < 0. || cost < least) least = cost, best = {widths[i], (int)(tiles < most ? tiles : most), 0, false, false};
         }
         return best;
     };
     LtPlan best = whole(M, act == ACT_SWIGLU ? 2ll * N : N, 0);
     if (cut && best.bn == 64 && best.clusters <= kLtCutTiles && kb >= kLtCutBlocks) {
-        long long clusters = (long long)best.clusters * kLtMostParts, by_blocks = best.clusters * kb / kLtMinBlocks;
-        if (clusters > by_blocks) clusters = by_blocks;
-        if (clusters > most) clusters = most;
-        best.sk_tiles = best.clusters, best.clusters = (int)clusters;
-    } else if (!aligned || M <= kLtSwapRows) {
+        const long long parts = f32 ? (kb + kLtSegment - 1) / kLtSegment : kLtMostParts;
+        long long clusters = best.clusters * parts, by_blocks = best.clusters * kb / kLtMinBlocks;
+        if (clusters > by_blocks && !f32) clusters = by_blocks;
+        if (clusters <= most || !f32) {
+            best.sk_tiles = best.clusters, best.clusters = (int)(clusters < most ? clusters : most);
+            return best;
+        }
+    }
+    if (!aligned || M <= kLtSwapRows || (f32 && kb > kLtSegment)) {
         best = whole(N, M, act == ACT_SWIGLU ? 1 : 0);
-        best.swap = true;
+        best.swap = true, best.seg = f32 && kb > kLtSegment;
     }
     return best;
 }
 
 size_t linear_workspace_bytes(int M, int N, int K, int act) {
     if (M <= kLinearFewRows) return 0;
-    const LtPlan plan = linear_plan(M, N, K, act, true, true);
+    const LtPlan plan = linear_plan(M, N, K, act, true, true, false);
     // one size for all, so that an operator's workspace never has to grow under a captured graph
     return plan.sk_tiles ? (size_t)kLtCountBytes + (size_t)(sm_count() / 2) * 4 * 256 * 128 * sizeof(float) : 0;
 }
 
-template <int BN, bool PAIR, bool SWAP>
+template <int BN, bool PAIR, bool SWAP, bool SEG = false>
 static cudaError_t launch_linear_tile(const LinearArgs& a, const LtPlan& plan, LtParams& p, cudaStream_t stream) {
     constexpr int UNITS = PAIR && !SWAP ? BN / 2 : BN, kBytes = LtSmem<BN, PAIR, SWAP>::kBytes;
     alignas(64) CUtensorMap mx, w0, w1;
@@ -549,15 +614,20 @@ static cudaError_t launch_linear_tile(const LinearArgs& a, const LtPlan& plan, L
     if (!PAIR) w1 = w0;
     else if (!encode_rows(&w1, a.W + (long long)a.N * a.K, a.N, a.K, a.K, box_w)) return cudaErrorInvalidValue;
     static std::atomic<bool> configured[64];
-    if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR, SWAP>, kBytes, configured)) return e;
+    if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR, SWAP, SEG>, kBytes, configured)) return e;
     p.tiles_a = ((SWAP ? a.N : a.M) + 255) / 256, p.tiles_b = ((SWAP ? a.M : a.N) + UNITS - 1) / UNITS;
     p.sk_first = p.tiles_a * p.tiles_b - plan.sk_tiles, p.sk_units = plan.sk_tiles * p.kblocks;
     p.sk_share = (p.sk_units + plan.clusters - 1) / plan.clusters;
     chain_begin();
-    return launch_pdl_cluster(linear_tc_kernel<BN, PAIR, SWAP>, dim3(2u * plan.clusters), dim3(kLtThreads), 2, kBytes, stream, mx, w0, w1, p);
+    return launch_pdl_cluster(linear_tc_kernel<BN, PAIR, SWAP, SEG>, dim3(2u * plan.clusters), dim3(kLtThreads), 2, kBytes, stream, mx, w0, w1, p);
 }
 template <bool PAIR>
 static cudaError_t launch_linear_form(const LinearArgs& a, const LtPlan& plan, LtParams& p, cudaStream_t stream) {
+    if (plan.seg) {
+        if constexpr (!PAIR)
+            if (plan.bn == 256) return launch_linear_tile<256, PAIR, true, true>(a, plan, p, stream);
+        return plan.bn == 128 ? launch_linear_tile<128, PAIR, true, true>(a, plan, p, stream) : launch_linear_tile<64, PAIR, true, true>(a, plan, p, stream);
+    }
     if (plan.swap) {
         if constexpr (!PAIR)
             if (plan.bn == 256) return launch_linear_tile<256, PAIR, true>(a, plan, p, stream);
@@ -578,7 +648,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
     p.vec_bias = a.bias && aligned16(a.bias) && (a.act != ACT_SWIGLU || a.N % 8 == 0);
     p.status = status_ptr();
     if (!p.status) return cudaErrorUnknown;
-    const LtPlan plan = linear_plan(a.M, a.N, a.K, a.act, a.workspace != nullptr, p.rows_aligned);
+    const LtPlan plan = linear_plan(a.M, a.N, a.K, a.act, a.workspace != nullptr, p.rows_aligned, a.out_f32);
     p.count = static_cast<unsigned int*>(a.workspace);
     p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + kLtCountBytes);
     return a.act == ACT_SWIGLU ? launch_linear_form<true>(a, plan, p, stream) : launch_linear_form<false>(a, plan, p, stream);

@@ -674,3 +674,18 @@ def test_linear_results_of_more_than_two_to_the_31_elements(N):
     at = torch.tensor([0, 127, 128, 17000, 35791, 35792, 35999], device=DEV)  # 35791 * N is just below 2^31
     y, tol = linear64(op, X[at], W, None, r[at])
     close(out[at], y, tol)
+
+
+@pytest.mark.parametrize("M", [5, 30, 64, 100, 129, 700])
+@pytest.mark.parametrize("N,K", [(600, 520), (600, 4096), (2000, 12800), (40, 12800), (20001, 2056)])
+def test_linear_fp32_results_keep_their_precision(M, N, K):
+    """Each of the 32 steps of a segment may cut 2^-23 of the sum so far (2^-24 on average), which grows like the root of the steps:
+    2/3 * 32 * 2^-24 of the segment, and segments err independently; plus a rounding per segment.  Sums that stay in the tensor
+    cores for all of K = 12800 are 1.4e-5 off."""
+    op = ez.LinearOp(M, N, K, backend="cuda", out_dtype=torch.float32)
+    torch.manual_seed(M + N + K)
+    X, W, _, _ = op.gen_data()
+    y = X.double() @ W.double().T
+    assert (op(X, W).double() - y).norm() <= (64 / 3 * 2**-24 + (K / 512) ** 0.5 * 2**-24) * y.norm()
+    for act in ("swiglu", "gelu"):
+        linear_case(M, min(N, 900) // 2, K, act, True, True, torch.float32)
