@@ -87,6 +87,7 @@ SIGNATURES = {
     "ezb_stream_capture_id": (ctypes.c_ulonglong, [c_void_p]),
     "ezb_attn_prompt_workspace_bytes": (c_size_t, [c_int]),
     "ezb_attn_prompt": (c_int, [c_void_p, c_longlong] + [c_void_p] * 6 + [c_longlong, c_void_p, c_size_t] + [c_int] * 8 + [c_void_p]),
+    **{f"ezb_{name}_packed": (c_int, [c_char_p]) for name in ("paged_plan", "paged_qk_norm_rope", "linear_bf16", "attn_prompt")},
     "ezb_vector_add_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_longlong, c_void_p]),
     "ezb_softmax_f32": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "ezb_reduce_workspace_bytes": (c_size_t, []),

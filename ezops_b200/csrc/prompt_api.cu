@@ -1,4 +1,8 @@
 // C entries of the prompt operators (declared in include/ezb200.h): argument checks, then one launch each.
+#include <cstring>
+#include <type_traits>
+#include <utility>
+
 #include "prompt.h"
 
 using namespace ezb;
@@ -28,6 +32,27 @@ bool overlap(const Rect& a, const Rect& b) {
 }
 
 constexpr int kMost = 1 << 30;  // sizes, positions and slots are 32-bit on the device
+
+// A call whose arguments are 64-bit words: pointers, sizes, and a float as its bits.
+template <class T>
+T from_word(long long w) {
+    if constexpr (std::is_pointer_v<T>) return reinterpret_cast<T>(static_cast<uintptr_t>(w));
+    else if constexpr (std::is_same_v<T, float>) {
+        const int bits = static_cast<int>(w);
+        float f;
+        memcpy(&f, &bits, sizeof(f));
+        return f;
+    } else return static_cast<T>(w);
+}
+template <class... A, size_t... I>
+int call_words(int (*f)(A...), const long long* w, std::index_sequence<I...>) {
+    return f(from_word<A>(w[I])...);
+}
+template <class... A>
+int call_packed(int (*f)(A...), const long long* w) {
+    EZB_REQUIRE(w, "null pointer");
+    return call_words(f, w, std::index_sequence_for<A...>{});
+}
 
 }  // namespace
 
@@ -199,5 +224,10 @@ unsigned long long ezb_stream_capture_id(ezb_stream_t stream) {
     }
     return status == cudaStreamCaptureStatusActive ? id : 0;
 }
+
+int ezb_paged_plan_packed(const long long* words) { return call_packed(ezb_paged_plan, words); }
+int ezb_paged_qk_norm_rope_packed(const long long* words) { return call_packed(ezb_paged_qk_norm_rope, words); }
+int ezb_linear_bf16_packed(const long long* words) { return call_packed(ezb_linear_bf16, words); }
+int ezb_attn_prompt_packed(const long long* words) { return call_packed(ezb_attn_prompt, words); }
 
 }  // extern "C"

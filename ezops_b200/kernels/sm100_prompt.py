@@ -4,6 +4,7 @@ tokens or rows per call, so the constructors hold what stays the same from step 
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -61,7 +62,14 @@ def _distance(t: torch.Tensor) -> int:
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
+
+
+def _packed(entry: str):
+    """The packed form of a C entry (its arguments as 64-bit words in one bytes object) and what packs them: ctypes converts one
+    argument instead of twenty."""
+    words = len(_lib.SIGNATURES[entry][1])
+    return getattr(_lib.load(), entry + "_packed"), struct.Struct(f"{words}q").pack
 
 
 class _Workspaces:
@@ -96,7 +104,7 @@ class PagedPlanSm100Kernel(BaseKernel):
             raise ValueError(f"batch ({batch}) must be at most 8192")
         self.sizes = (batch, max_tokens, max_pages, page_size, num_pages)
         self._rows, self._table, self._cu, self._tokens, self._one = (batch,), (batch, max_pages), (batch + 1,), (max_tokens,), (1,)
-        self._entry = _lib.load().ezb_paged_plan
+        self._entry, self._pack = _packed("ezb_paged_plan")
 
     def __call__(self, ctx_lens, new_lens, page_table, free_pages, free_count, out) -> None:
         dev, rows, tokens, one = _device(ctx_lens, "ctx_lens"), self._rows, self._tokens, self._one
@@ -111,9 +119,10 @@ class PagedPlanSm100Kernel(BaseKernel):
                 ("free_pages", free_pages, free), ("free_count", free_count, one), ("out.seq_lens", lens, rows),
                 ("out.cu_tokens", cu, self._cu), ("out.positions", positions, tokens), ("out.slots", slots, tokens),
                 ("out.free_count", left, one))], dev)
-        rc = self._entry(ctx_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
-                         lens.data_ptr(), cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), left.data_ptr(), *self.sizes, free[0],
-                         _raw_stream(dev))
+        rc = self._entry(self._pack(
+            ctx_lens.data_ptr(), new_lens.data_ptr(), page_table.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+            lens.data_ptr(), cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), left.data_ptr(), *self.sizes, free[0],
+            _raw_stream(dev)))
         if rc:
             _lib.check(rc)
 
@@ -130,8 +139,10 @@ class PagedQkNormRopeSm100Kernel(BaseKernel):
         self._sections = (ctypes.c_int * self.axes)(*sections)
         self._width, self._w, self._table = (num_heads + 2 * NKV) * head_dim, (head_dim,), (max_positions, head_dim)
         self._pool = (num_pages, NKV, page_size, head_dim)
-        self._sizes = (num_heads, NKV, head_dim, max_positions, self.axes, self._sections, int(interleaved), page_size, num_pages, self.rms_eps)
-        self._entry = _lib.load().ezb_paged_qk_norm_rope
+        eps = struct.unpack("i", struct.pack("f", self.rms_eps))[0]
+        self._sizes = (num_heads, NKV, head_dim, max_positions, self.axes, ctypes.addressof(self._sections), int(interleaved), page_size,
+                       num_pages, eps)
+        self._entry, self._pack = _packed("ezb_paged_qk_norm_rope")
 
     def __call__(self, qkv, q_norm_w, k_norm_w, cos, sin, positions, slots, K_pool, V_pool, out=None):
         dev, T, w, table, pool = _device(qkv, "qkv"), qkv.shape[0], self._w, self._table, self._pool
@@ -148,9 +159,9 @@ class PagedQkNormRopeSm100Kernel(BaseKernel):
                      ("cos", cos, table, _BF16, False), ("sin", sin, table, _BF16, False), ("positions", positions, where, _I32, False),
                      ("slots", slots, (T,), _I32, False), ("K_pool", K_pool, pool, _BF16, False), ("V_pool", V_pool, pool, _BF16, False),
                      ("out", out, heads, _BF16, False)], dev)
-        rc = self._entry(qkv.data_ptr(), _distance(qkv), _ptr(q_norm_w), _ptr(k_norm_w), cos.data_ptr(), sin.data_ptr(),
-                         positions.data_ptr(), slots.data_ptr(), K_pool.data_ptr(), V_pool.data_ptr(), out.data_ptr(), T, *self._sizes,
-                         _raw_stream(dev))
+        rc = self._entry(self._pack(
+            qkv.data_ptr(), _distance(qkv), _ptr(q_norm_w), _ptr(k_norm_w), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
+            slots.data_ptr(), K_pool.data_ptr(), V_pool.data_ptr(), out.data_ptr(), T, *self._sizes, _raw_stream(dev)))
         if rc:
             _lib.check(rc)
         return out
@@ -170,7 +181,7 @@ class LinearSm100Kernel(BaseKernel):
         self._w, self._bias = (rows, in_features), (rows,)
         self._f32 = int(out_dtype == torch.float32)
         self._lib = _lib.load()
-        self._entry = self._lib.ezb_linear_bf16
+        self._entry, self._pack = _packed("ezb_linear_bf16")
         self._need: dict[int, int] = {}  # rows -> workspace bytes
         self._spaces, self._ws = _Workspaces(self._lib), None
 
@@ -193,9 +204,9 @@ class LinearSm100Kernel(BaseKernel):
             _refuse([("X", X, (M, K), _BF16, True), ("W", W, self._w, _BF16, False), ("bias", bias, self._bias, _BF16, False),
                      ("residual", residual, (M, N), _BF16, True), ("out", out, (M, N), self.out_dtype, True)], dev)
         ws = self.workspace(M, X.device) if self._need.get(M) != 0 else None
-        rc = self._entry(X.data_ptr(), _distance(X), W.data_ptr(), _ptr(bias), _ptr(residual), N if residual is None else _distance(residual),
-                         out.data_ptr(), _distance(out), _ptr(ws), 0 if ws is None else ws.numel(), M, N, K, self.act, self._f32,
-                         _raw_stream(dev))
+        rc = self._entry(self._pack(
+            X.data_ptr(), _distance(X), W.data_ptr(), _ptr(bias), _ptr(residual), N if residual is None else _distance(residual),
+            out.data_ptr(), _distance(out), _ptr(ws), 0 if ws is None else ws.numel(), M, N, K, self.act, self._f32, _raw_stream(dev)))
         if rc:
             _lib.check(rc)
         return out
@@ -210,7 +221,7 @@ class AttnPromptSm100Kernel(BaseKernel):
         self.NKV = num_heads if num_kv_heads is None else num_kv_heads
         self._table, self._lens, self._cu = (batch, max_pages), (batch,), (batch + 1,)
         self._lib = _lib.load()
-        self._entry = self._lib.ezb_attn_prompt
+        self._entry, self._pack = _packed("ezb_attn_prompt")
         self._need = self._lib.ezb_attn_prompt_workspace_bytes(self.D)
         self._spaces = _Workspaces(self._lib)
 
@@ -227,9 +238,10 @@ class AttnPromptSm100Kernel(BaseKernel):
                      ("cu_tokens", cu_tokens, self._cu, _I32, False), ("out", out, heads, _BF16, True)], dev)
         stream = _raw_stream(dev)
         ws = self._spaces.get(self._need, dev, stream)
-        rc = self._entry(Q.data_ptr(), _distance(Q), K_pool.data_ptr(), V_pool.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
-                         cu_tokens.data_ptr(), out.data_ptr(), _distance(out), ws.data_ptr(), ws.numel(), self.B, T, H, self.NKV, D,
-                         self.max_pages, self.P, pool[0], stream)
+        rc = self._entry(self._pack(
+            Q.data_ptr(), _distance(Q), K_pool.data_ptr(), V_pool.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
+            cu_tokens.data_ptr(), out.data_ptr(), _distance(out), ws.data_ptr(), self._need, self.B, T, H, self.NKV, D, self.max_pages,
+            self.P, pool[0], stream))
         if rc:
             _lib.check(rc)
         return out

@@ -410,6 +410,13 @@ int ezb_attn_prompt(const void* Q, long long ldq, const void* K_pool, const void
                     const int* cu_tokens, void* Out, long long ldo, void* workspace, size_t workspace_bytes, int B, int T, int H, int NKV,
                     int D, int max_pages, int page_size, int num_pages, ezb_stream_t stream);
 
+/* The four calls above with their arguments, in their order, as 64-bit words (pointers, sizes, a float as
+ * its bits): for bindings to which every argument costs (Python's ctypes 2 us a call). */
+int ezb_paged_plan_packed(const long long* words);
+int ezb_paged_qk_norm_rope_packed(const long long* words);
+int ezb_linear_bf16_packed(const long long* words);
+int ezb_attn_prompt_packed(const long long* words);
+
 /* The stack of layers, tensor parallel with the exchange fused into the kernels:
  * ezb_qwen3_decode_stack on this rank's shards (as ezb_qwen3_decode_layer_tp_fused
  * takes them), one call for all layers.  A layer's second sum is folded into

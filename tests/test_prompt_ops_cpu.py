@@ -184,3 +184,25 @@ def test_c_entries_refuse_without_a_gpu():
     assert attn(out=a) == bad and attn(w=None) == none and attn(size=100) == none
     assert attn(max_pages=1 << 25) == shape
     assert lib.ezb_attn_prompt_workspace_bytes(96) == 0
+
+
+def test_packed_entries_are_the_same_calls():
+    """Words in the order of the arguments: pointers, negative sizes and a float arrive as they are."""
+    lib = _lib.load()
+    import struct
+
+    def same(name, *args):
+        words = [struct.unpack("i", struct.pack("f", a))[0] if isinstance(a, float) else 0 if a is None else a for a in args]
+        code = getattr(lib, name)(*args)
+        message = lib.ezb_last_error_message()
+        assert code < 0 and getattr(lib, name + "_packed")(struct.pack(f"{len(words)}q", *words)) == code
+        assert lib.ezb_last_error_message() == message
+        return message
+
+    p = 0x7F0012345600
+    assert b"null" in same("ezb_paged_plan", *[None] * 10, 2, 8, 4, 64, 8, 8, None)
+    assert b"8192" in same("ezb_paged_plan", *[p] * 10, 9000, 8, 4, 64, 8, 8, None)
+    assert b"positive" in same("ezb_linear_bf16", p, 64, p, None, None, 8, p, 8, None, 0, -3, 8, 64, 0, 0, None)
+    assert b"128 query" in same("ezb_attn_prompt", p, 1 << 40, p, p, p, p, p, p, 1 << 41, p, 1 << 33, 1, 1, 129, 1, 64, 1, 64, 1, None)
+    assert b"apart" in same("ezb_paged_qk_norm_rope", p, 8, None, None, *[p] * 7, 1, 8, 8, 64, 16, 1, p, 0, 64, 1, 1e-6, None)
+    assert lib.ezb_attn_prompt_packed(None) == lib.ezb_paged_plan(*[None] * 10, 2, 8, 4, 64, 8, 8, None)
