@@ -40,6 +40,9 @@ static constexpr int kApStages = 5;     // ring of K and V tiles
 static constexpr int kApKeys = 128;     // keys per tile
 static constexpr int kApSegments = 4;   // ring of work descriptors
 static constexpr int kApUnitCost = 256;  // a unit's fixed cost in keys; at least 127, so that its last tile lies inside its cost
+// Eighths that a unit of at most 128 rows costs less: half of the products, all of the bytes (32 rows of 1 to 100 tokens behind
+// 1000 to 8000 keys 222 -> 207 us, 2/8 212, 4/8 217; 8 of 65 to 600 238 -> 234).
+static constexpr int kApDualLess = 3;
 static constexpr int kApWhole = 4;      // units of at most so many tiles are never cut
 static constexpr int kApMinShare = 256;  // keys below which a further CTA is not worth its merge
 
@@ -111,7 +114,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // A unit: 2 * tpt consecutive tokens of a row for one kv head.
 struct ApRow {
     int q0, n, len, units;  // first token, tokens, valid keys
-    long long per_unit;     // cost of unit j: per_unit + (j + 1) * 2 * tpt
+    long long per_unit;     // cost of unit j: per_unit + (j + 1) * 2 * tpt,
+    long long less;         // less this for the last one, when it has one tile of queries
     long long head_cost;    // cost of all units of one head
 };
 __device__ __forceinline__ ApRow ap_row(const ApParams& p, int b) {
@@ -122,7 +126,8 @@ __device__ __forceinline__ ApRow ap_row(const ApParams& p, int b) {
     const int u = 2 * p.tpt;
     r.units = (r.n + u - 1) / u;
     r.per_unit = max(r.len - r.n, 0) + kApUnitCost;
-    r.head_cost = r.units * r.per_unit + (long long)u * r.units * (r.units + 1) / 2;
+    r.less = r.units && r.n - (r.units - 1) * u <= p.tpt ? (r.per_unit + (long long)r.units * u) * kApDualLess / 8 : 0;
+    r.head_cost = r.units * r.per_unit + (long long)u * r.units * (r.units + 1) / 2 - r.less;
     return r;
 }
 __device__ __forceinline__ long long ap_unit_start(const ApParams& p, const ApRow& r, int j) {  // inside its head
@@ -159,9 +164,10 @@ struct ApSegment {
 };
 // The tile of the unit that starts at x0 at which place x of the line cuts it: short units are not cut, and no piece is
 // shorter than two tiles (a part costs a trip through the workspace).
-__device__ __forceinline__ int ap_tile_at(long long x, long long x0, int tiles) {
+__device__ __forceinline__ int ap_tile_at(long long x, long long x0, int tiles, int dual) {
     if (x <= x0) return 0;
-    const int k = (x - x0) >> 7 < tiles ? (int)((x - x0) >> 7) : tiles;
+    const long long at = (dual ? (x - x0) * 8 / (8 - kApDualLess) : x - x0) >> 7;
+    const int k = at < tiles ? (int)at : tiles;
     if (tiles <= kApWhole) return 2 * k >= tiles ? tiles : 0;
     return k < 2 ? 0 : (k > tiles - 2 ? tiles : k);
 }
@@ -172,10 +178,10 @@ __device__ __forceinline__ bool ap_segment(const ApParams& p, const ApLine& line
     s.tokens = min(u, c.row.n - first);
     s.extent = max(0, c.row.len - (c.row.n - first - s.tokens));
     s.tiles = (s.extent + kApKeys - 1) / kApKeys;
-    s.ks = ap_tile_at(lo, c.x0, s.tiles);
-    s.cnt = ap_tile_at(hi, c.x0, s.tiles) - s.ks;
-    if (s.tiles ? s.cnt == 0 : lo > c.x0) return false;  // a unit without keys belongs to the share in which it starts
     s.dual = s.tokens <= p.tpt;
+    s.ks = ap_tile_at(lo, c.x0, s.tiles, s.dual);
+    s.cnt = ap_tile_at(hi, c.x0, s.tiles, s.dual) - s.ks;
+    if (s.tiles ? s.cnt == 0 : lo > c.x0) return false;  // a unit without keys belongs to the share in which it starts
     s.token = c.row.q0 + first;
     s.sees = c.row.len - c.row.n + first + 1;
     s.row = c.b, s.head = c.h;
@@ -187,13 +193,14 @@ __device__ __forceinline__ bool ap_segment(const ApParams& p, const ApLine& line
     if (c.x0 < lo)
         while (s.c0 > 0 && ap_share(line, s.c0) > c.x0) --s.c0;
     if (s.ks + s.cnt < s.tiles)
-        while (s.c1 + 1 < line.ctas && ap_tile_at(ap_share(line, s.c1 + 1), c.x0, s.tiles) < s.tiles) ++s.c1;
+        while (s.c1 + 1 < line.ctas && ap_tile_at(ap_share(line, s.c1 + 1), c.x0, s.tiles, s.dual) < s.tiles) ++s.c1;
     return true;
 }
 // Next unit; false at the end of the batch.  Called by a whole warp: rows without tokens are passed over 32 at a time.
 __device__ __forceinline__ bool ap_advance(const ApParams& p, ApCursor& c, int lane) {
     c.x0 += c.row.per_unit + (long long)(c.j + 1) * 2 * p.tpt;
     if (++c.j < c.row.units) return true;
+    c.x0 -= c.row.less;
     c.j = 0;
     if (++c.h < p.NKV) return true;
     c.h = 0;
@@ -852,7 +859,8 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
                             int n = 0;
                             for (int c0 = seg.c0; c0 <= seg.c1; c0 += 32) {
                                 const int c = c0 + lane;
-                                const bool has = c <= seg.c1 && ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles) > ap_tile_at(ap_share(line, c), seg.x0, seg.tiles);
+                                const bool has = c <= seg.c1 && ap_tile_at(ap_share(line, c + 1), seg.x0, seg.tiles, seg.dual) >
+                                                                    ap_tile_at(ap_share(line, c), seg.x0, seg.tiles, seg.dual);
                                 const uint32_t all = __ballot_sync(0xffffffffu, has);
                                 if (has) t.list[n + __popc(all & ((1u << lane) - 1u))] = (short)(2 * (2 * c + (c == seg.c0 ? 1 : 0)));
                                 n += __popc(all);
