@@ -20,9 +20,10 @@
 // costs a trip through the workspace (short prompts of 14 heads of 64: 37.7 -> 17.6 us).
 //
 // What bounds it: for prompts the exponentials and the products together - 128 x 128 scores take 512 cycles each for QK^T
-// and PV (D = 128) and 1024 cycles of the MUFU, twice per step.  8192 tokens, 32/8 heads of 128: 437 to 505 us, 1090 to 1260
-// TFLOP/s of the products that the mask leaves (the MMAs alone in this order 355 to 370 us); 8 prompts of 65 to 600 tokens
-// behind 300 to 7400: 235 to 255 us; 8192 tokens of D = 64: 380 us, of which 240 are exponentials.  For single tokens the bytes
+// and PV (D = 128) and 1024 cycles of the MUFU, twice per step.  8192 tokens, 32/8 heads of 128: 439 us, 1250
+// TFLOP/s of the products that the mask leaves (505 us at the 1.6 GHz of the power cap; the MMAs alone in this order 355 to 370
+// us); 8 prompts of 65 to 600 tokens behind 300 to 7400: 232 us (277 capped); 8192 tokens of D = 64: 380 us, of which 240 are
+// exponentials.  For single tokens the bytes
 // of the caches: 32 of them over 1000 to 8100 keys 103 to 112 us, 5.5 to 5.9 TB/s.
 // Measured and left out: a polynomial in place of part of the exponentials, 512 softmax threads, P handed over at 75 %, blocks of
 // 64 keys (+12 % for QK^T), a third block of scores beside O of 64 columns (3 %): no gain that carries its code.

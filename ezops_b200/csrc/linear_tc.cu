@@ -17,8 +17,8 @@
 // operands, two accumulators side by side.  Measured, A = x against A = W: 7404 x 17921, K = 96, gelu 422 and 184 us (with 17920
 // columns: 154 and 163); 4530 x 3350, K = 720, fp32 62 and 32; 104 x 22304, K = 7360 86 and 67; 128 rows of 4096 through SwiGLU to
 // 12288 61 to 67 and 50; 300 x 4096, K = 4096 15.2 to 16.6 and 16.0 to 16.9; 8192 x 4096, K = 4096 193 and 188 to 193.
-// What bounds it: the tensor cores where tiles fill the clusters evenly (4096 rows of 4096 through SwiGLU to 12288: 507 to 600 us
-// under the power cap, 1370 to 1630 TFLOP/s); else the operands' way from L2 (777 x 4096, K = 12288: 64 tiles on 74 clusters bring
+// What bounds it: the tensor cores where tiles fill the clusters evenly (4096 rows of 4096 through SwiGLU to 12288: 516 us,
+// 1600 TFLOP/s; 587 at the 1.3 GHz of the power cap); else the operands' way from L2 (777 x 4096, K = 12288: 64 tiles on 74 clusters bring
 // 0.7 GB into the SMs in 72 us); from a few hundred rows down the weights' bytes (104 x 22304, K = 7360: 5.1 TB/s).
 // fp32 results of more than kLtSegment k blocks: the tensor cores cut their sums towards zero (gemm_tc.cu), so the sums leave them
 // every kLtSegment blocks and are added up, rounded to nearest, in the registers of the lane whose column it is (A = W); the relative
