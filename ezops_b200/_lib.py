@@ -81,9 +81,8 @@ SIGNATURES = {
     "ezb_paged_plan": (c_int, [c_void_p] * 10 + [c_int] * 6 + [c_void_p]),
     "ezb_paged_qk_norm_rope": (c_int, [c_void_p, c_longlong] + [c_void_p] * 9 + [c_int] * 6 + [c_void_p] + [c_int] * 3
                                + [c_float, c_void_p]),
-    "ezb_linear_workspace_bytes": (c_size_t, [c_int] * 4),
-    "ezb_linear_bf16": (c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_size_t]
-                        + [c_int] * 5 + [c_void_p]),
+    "ezb_linear_bf16": (c_int, [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong, c_void_p, c_longlong] + [c_int] * 5
+                        + [c_void_p]),
     "ezb_stream_capture_id": (ctypes.c_ulonglong, [c_void_p]),
     "ezb_attn_prompt_workspace_bytes": (c_size_t, [c_int]),
     "ezb_attn_prompt": (c_int, [c_void_p, c_longlong] + [c_void_p] * 6 + [c_longlong, c_void_p, c_size_t] + [c_int] * 8 + [c_void_p]),

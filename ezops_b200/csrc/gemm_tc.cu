@@ -73,6 +73,7 @@ struct TcParams {
     // EXT instance: out = act(product + bias) + residual, one rounding
     const bf16* bias;  // [N], SwiGLU [2N] gate first, or null
     int act, out_f32;
+    int rows;  // of x: gridDim.y groups of B, the last one with what is left
 };
 
 // What bounds it: the weight stream.  A tile's parts meet in shared memory because the round trips of a reduction
@@ -126,6 +127,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int NS = p.nstages, KB = p.kblocks;
+    const int row0 = EXT ? (int)blockIdx.y * p.B : 0, B = EXT ? min(p.B, p.rows - row0) : p.B;  // rows of x
     const int C = 1 << p.log2c;
     const int rank = (int)cluster_rank();
     const int cluster = blockIdx.x >> p.log2c, n_clusters = gridDim.x >> p.log2c;
@@ -184,7 +186,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                 if (wkb == k_first) wt += n_clusters;
             };
             auto request_x = [&](int st) {
-                tma_load_2d(smem_u32(stages) + (uint32_t)st * stage_bytes + a_bytes, &mapX, xkb * kTcBlockK, 0, smem_u32(&full_bar[st]));
+                tma_load_2d(smem_u32(stages) + (uint32_t)st * stage_bytes + a_bytes, &mapX, xkb * kTcBlockK, row0, smem_u32(&full_bar[st]));
                 if (++xkb == kb1) xkb = kb0;
             };
             // weights do not depend on the kernel in front: request them before the dependency wait
@@ -260,7 +262,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
         constexpr int HC = NB / 2;         // two warps share a lane quarter: each drains half of the batch columns
         const int b_half = ((warp - 2) >> 2) * HC;
         const int cpc = p.cpc;  // batch columns per CTA of the cluster
-        auto cols_of = [&](int r) { return max(0, min(cpc, p.B - r * cpc)); };
+        auto cols_of = [&](int r) { return max(0, min(cpc, B - r * cpc)); };
         const int b_first = rank * cpc, n_cols = cols_of(rank);
         // the threads that finish a tile: a row (or pair) each, every `groups`-th column
         const int frow = p.pair ? (et & 63) : (et & 127);
@@ -297,7 +299,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
             // residual values of the first columns are fetched while the tile is still being multiplied
             float res[CU];
             auto fetch_residual = [&](int col) {
-                const bf16* src = p.residual + (long long)(b_first + col) * p.ldres + n;
+                const bf16* src = p.residual + (long long)(row0 + b_first + col) * p.ldres + n;
 #pragma unroll
                 for (int u = 0; u < CU; ++u) {
                     if (col + u * groups < n_cols) res[u] = __bfloat162float(*src);
@@ -347,12 +349,12 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                     const float bias = p.bias && own ? __bfloat162float(p.bias[n_own]) : 0.f;
 #pragma unroll 1
                     for (int c = 0; c < HC; c += 8) {
-                        if (b_half + c >= p.B) break;
+                        if (b_half + c >= B) break;
                         float v[8], r8[8];
                         tmem_ld8(t_addr + (uint32_t)c, v);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            r8[e] = p.residual && own && b_half + c + e < p.B ? __bfloat162float(p.residual[(long long)(b_half + c + e) * p.ldres + n_own]) : 0.f;
+                            r8[e] = p.residual && own && b_half + c + e < B ? __bfloat162float(p.residual[(long long)(row0 + b_half + c + e) * p.ldres + n_own]) : 0.f;
                         float w[8];
                         if (summed) tmem_ld8(t_sum + (uint32_t)c, w);
                         tmem_ld_wait();
@@ -361,9 +363,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                         linear_act(v, p.act);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            if (own && b_half + c + e < p.B) {
+                            if (own && b_half + c + e < B) {
                                 const float x = v[e] + r8[e];
-                                const long long o = (long long)(b_half + c + e) * p.ldout + n_own;
+                                const long long o = (long long)(row0 + b_half + c + e) * p.ldout + n_own;
                                 if (p.out_f32) static_cast<float*>(p.out)[o] = x;
                                 else static_cast<bf16*>(p.out)[o] = __float2bfloat16_rn(x);
                             }
@@ -384,7 +386,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                 for (int e = 0; e < 8; ++e) v[e] += w[e];
             };
             float* dst = mine + (size_t)b_half * RS + row;
-            const int b_left = p.B - b_half;
+            const int b_left = B - b_half;
             if constexpr (HC == 8) {
                 float v[8];
                 tmem_ld8(t_addr, v);
@@ -461,7 +463,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                             if (c < n_cols) {
                                 float x = p.pair ? silu_fast(v[u]) * (up[u] + b1) : v[u];
                                 if (p.residual) x += res[u];
-                                const long long o = (long long)(b_first + c) * p.ldout + n;
+                                const long long o = (long long)(row0 + b_first + c) * p.ldout + n;
                                 if (p.out_f32) static_cast<float*>(p.out)[o] = x;
                                 else static_cast<bf16*>(p.out)[o] = __float2bfloat16_rn(x);
                             }
@@ -653,13 +655,13 @@ static int tc_resident_clusters(int dev, int log2c, bool half) {
 // 0.6B o_proj 64.9 | 60.5 | 58.6 | 58.4).  A k-block costs 40 ns plus its bytes at a 148th of the HBM rate (never less
 // than 150 ns: waiting for a stage and issuing its MMAs, which read 128 rows of A whatever the tile holds).
 template <int NB, bool LINK, bool EXT>
-static bool tc_plan(TcParams& p, int dev, int& clusters, size_t& smem) {
+static bool tc_plan(TcParams& p, int dev, int groups, int& clusters, size_t& smem) {
     double best = 0.;
     for (int log2c = 0; (1 << log2c) <= kTcMaxCluster && (1 << log2c) <= p.kblocks; ++log2c) {
         const int C = 1 << log2c, max_units = p.pair ? kTcRows / 2 : kTcRows;
         const int cpc = (p.B + C - 1) / C, nk = (p.kblocks + C - 1) / C;
         for (int half = 0; half < 2; ++half) {
-            const int nc = tc_resident_clusters<NB, LINK, EXT>(dev, log2c, half != 0);
+            const int nc = tc_resident_clusters<NB, LINK, EXT>(dev, log2c, half != 0) / groups;
             if (nc < 1) continue;
             long long rounds = (p.N + (long long)nc * max_units - 1) / ((long long)nc * max_units);
             int units = (int)((p.N + nc * rounds - 1) / (nc * rounds));
@@ -710,17 +712,18 @@ static cudaError_t launch_tc_instance(const GemvArgs& a, const bf16* x, long lon
     }
     int clusters = 0;
     size_t smem = 0;
-    if (!tc_plan<NB, LINK, EXT>(p, dev, clusters, smem)) return cudaErrorInvalidConfiguration;
+    const int groups = EXT ? (p.rows + p.B - 1) / p.B : 1;
+    if (!tc_plan<NB, LINK, EXT>(p, dev, groups, clusters, smem)) return cudaErrorInvalidConfiguration;
     if (a.tiling && a.prologue != PRO_SCALED) a.tiling->units = p.units, a.tiling->tiles = p.tiles;
     p.first = chain_waits_first();
     p.cols_pad = 1;
     while (p.cols_pad < p.cpc) p.cols_pad *= 2;
     alignas(64) CUtensorMap m0, m1, mx;
     if (EXT) {  // called with ever new activation buffers: descriptors are encoded (1 us) instead of filling up the table
-        if (!encode_map(&m0, a.W0, a.N, a.K, a.ldw, p.units) || !encode_map(&mx, x, a.B, a.K, ldx, NB)) return cudaErrorInvalidValue;
+        if (!encode_map(&m0, a.W0, a.N, a.K, a.ldw, p.units) || !encode_map(&mx, x, p.rows, a.K, ldx, NB)) return cudaErrorInvalidValue;
         m1 = m0;
         if (p.pair && !encode_map(&m1, a.W1, a.N, a.K, a.ldw, p.units)) return cudaErrorInvalidValue;
-        return launch_pdl_cluster(kernel, dim3((unsigned)clusters << p.log2c), dim3(kTcThreads), 1 << p.log2c, smem, stream, m0, m1, mx, p);
+        return launch_pdl_cluster(kernel, dim3((unsigned)clusters << p.log2c, (unsigned)groups), dim3(kTcThreads), 1 << p.log2c, smem, stream, m0, m1, mx, p);
     }
     if (!make_map(&m0, a.W0, a.N, a.K, a.ldw, p.units)) return cudaErrorInvalidValue;
     if (!make_map(&m1, p.pair ? a.W1 : a.W0, a.N, a.K, a.ldw, p.units)) return cudaErrorInvalidValue;
@@ -747,7 +750,7 @@ cudaError_t launch_gemm_tc(const GemvArgs& a, const bf16* x, long long ldx, cuda
     if (a.prologue == PRO_SCALED) p.ssq_in = a.ssq, p.ssq_parts = a.tiling->parts();
     else if (a.ssq && a.epilogue == EPI_RESIDUAL) p.ssq_out = a.ssq, p.xw_out = a.next_norm_w ? a.xw_out : nullptr;
     p.link = a.link;
-    p.bias = nullptr, p.act = 0, p.out_f32 = 0;
+    p.bias = nullptr, p.act = 0, p.out_f32 = 0, p.rows = a.B;
     if (a.link.world > 0 && (a.link.gather_inbox >= 0 || pair)) return cudaErrorNotSupported;  // only the push side lives here
     const int NB = tc_batch_tile(a.B);
     if (a.link.world > 0 || a.behind_gather) {
@@ -764,12 +767,13 @@ cudaError_t launch_gemm_tc(const GemvArgs& a, const bf16* x, long long ldx, cuda
     }
 }
 
-cudaError_t launch_linear_few(const LinearArgs& l, cudaStream_t stream) {
+cudaError_t launch_linear_groups(const LinearArgs& l, cudaStream_t stream) {
     GemvArgs a;
     const bool pair = l.act == ACT_SWIGLU;
-    a.W0 = l.W, a.W1 = pair ? l.W + (long long)l.N * l.K : nullptr, a.ldw = l.K, a.N = l.N, a.K = l.K, a.B = l.M;
+    a.W0 = l.W, a.W1 = pair ? l.W + (long long)l.N * l.K : nullptr, a.ldw = l.K, a.N = l.N, a.K = l.K;
     TcParams p = {};
-    p.N = l.N, p.K = l.K, p.B = l.M;
+    const int groups = (l.M + kLinearGroupRows - 1) / kLinearGroupRows;
+    p.N = l.N, p.K = l.K, p.B = a.B = (l.M + groups - 1) / groups, p.rows = l.M;
     p.kblocks = (l.K + kTcBlockK - 1) / kTcBlockK;
     p.pair = pair ? 1 : 0;
     p.residual = l.residual, p.ldres = l.ldres;
@@ -780,7 +784,7 @@ cudaError_t launch_linear_few(const LinearArgs& l, cudaStream_t stream) {
     p.trace = trace_handle();
     p.link.push_inbox = p.link.gather_inbox = p.link.bump_inbox = -1;
     chain_begin();
-    switch (tc_batch_tile(l.M)) {
+    switch (tc_batch_tile(p.B)) {
         case 16: return launch_tc_instance<16, false, true>(a, l.x, l.ldx, p, stream);
         case 32: return launch_tc_instance<32, false, true>(a, l.x, l.ldx, p, stream);
         default: return launch_tc_instance<64, false, true>(a, l.x, l.ldx, p, stream);

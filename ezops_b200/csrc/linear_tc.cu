@@ -2,7 +2,7 @@
 //   out[m, n] = act( sum_k x[m, k] W[n, k] + bias[n] ) + residual[m, n],            fp32 until the one rounding,
 //   SwiGLU: silu(gate + bias_g) * (up + bias_u) with W = [gate rows | up rows].
 //
-// More than kLinearFewRows rows: two CTAs of a cluster share a tile of 256 rows of A by BN rows of B, A = x and B = W or the
+// Two CTAs of a cluster share a tile of 256 rows of A by BN rows of B, A = x and B = W or the
 // other way round (tcgen05.mma.cta_group::2: each CTA holds half of both operands' rows, and 128 x BN of the result in its
 // tensor memory), so each operand byte that enters an SM is used by two.  One elected thread per CTA fills a ring of 64-element
 // K blocks by TMA (both CTAs' bytes are counted on the first CTA's barrier), one thread of the first CTA issues the MMAs,
@@ -24,7 +24,7 @@
 // every kLtSegment blocks and are added up, rounded to nearest, in the registers of the lane whose column it is (A = W); the relative
 // error is 4.8e-7 for any K (1.4e-5 at K = 12800 otherwise), and 8192 x 4096, K = 4096 takes 193 us instead of 191.  Rounded to
 // bf16 that error does not show.
-// Few rows: the kernel of the batched decode projections (gemm_tc.cu) with this epilogue (17 x 6144, K = 4096: 10.3 us, 4.9 TB/s;
+// Few rows or few results (linear_in_groups): the kernel of the batched decode projections (gemm_tc.cu) with this epilogue (17 x 6144, K = 4096: 10.3 us, 4.9 TB/s;
 // 64 x 151936, K = 1024 to fp32: 57 us, 6.1 TB/s).
 #include <atomic>
 
@@ -36,7 +36,6 @@ namespace ezb {
 static constexpr int kLtThreads = 320;  // TMA warp, MMA warp, eight epilogue warps
 static constexpr int kLtBlockK = 64;
 static constexpr int kLtMaxStages = 12;
-static constexpr int kLtCountBytes = 4096;  // counters in front of the parts
 static constexpr int kLtSegment = 8;  // k blocks of a sum that stays in the tensor cores, where the result is not rounded to bf16
 static constexpr int kLtGroup = 8;  // row tiles per group of the tile order
 
@@ -48,38 +47,8 @@ struct LtParams {
     int tiles_a, tiles_b, act, out_f32;  // tiles along A's and B's rows
     int rows_aligned;  // rows of out start at 32-byte, of residual at 16-byte boundaries
     int vec_bias;      // so does bias
-    // Tiles from sk_first on are cut: their kblocks form one line, and every cluster takes the same length of it.
-    int sk_first;
-    int sk_units, sk_share;  // k blocks on the line, and of a cluster
-    float* parts;         // [2 * clusters slots][2 CTAs][BN][128] fp32
-    unsigned int* count;  // [clusters][2 CTAs], zero between calls
     unsigned int* status;
 };
-// Where cluster c's length of the line starts.
-__device__ __forceinline__ int lt_share(const LtParams& p, int c) { return min(p.sk_units, c * p.sk_share); }
-// What a cluster works off: first its pieces of cut tiles, then whole tiles.
-struct LtWork {
-    int x, end;        // on the line
-    int next;          // whole tile
-    int tile, k0, k1;  // the piece: k blocks of a tile
-    bool part;
-    __device__ __forceinline__ void start(const LtParams& p, int cluster) {
-        x = lt_share(p, cluster), end = lt_share(p, cluster + 1), next = cluster;
-    }
-    __device__ __forceinline__ bool step(const LtParams& p, int clusters) {
-        if (x < end) {
-            const int t = x / p.kblocks, first = t * p.kblocks;
-            tile = p.sk_first + t, k0 = x - first, k1 = min(end - first, p.kblocks);
-            x = first + k1;
-            part = k1 - k0 < p.kblocks;
-            return true;
-        }
-        if (next >= p.sk_first) return false;
-        tile = next, next += clusters, k0 = 0, k1 = p.kblocks, part = false;
-        return true;
-    }
-};
-
 // ---- cta_group::2 wrappers ------------------------------------------------------
 // The same barrier (or address) in the first CTA of the pair.
 __device__ __forceinline__ uint32_t pair_leader(uint32_t shared_addr) { return shared_addr & 0xFEFFFFFFu; }
@@ -164,7 +133,6 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     uint64_t* acc_empty = acc_full + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* last = abort_flag + 1;  // this CTA joins the parts of its rows of a tile
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int rank = (int)cluster_rank();
 
@@ -186,8 +154,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     pdl_open(1);
 
     const int n_clusters = gridDim.x >> 1, cluster = blockIdx.x >> 1;
-    LtWork work;
-    work.start(p, cluster);
+    const int n_tiles = p.tiles_a * p.tiles_b;
     auto tile_at = [&](int i, int& m, int& n) {  // groups of kLtGroup tiles along A, tile by tile along B
         const int per = kLtGroup * p.tiles_b, g = i / per, rows = min(kLtGroup, p.tiles_a - g * kLtGroup), r = i - g * per;
         m = g * kLtGroup + r % rows, n = r / rows;
@@ -195,14 +162,14 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
     if (warp == 0) {
         if (elect_one()) {
             int it = 0;
-            while (!*abort_flag && work.step(p, n_clusters)) {
+            for (int tile = cluster; tile < n_tiles && !*abort_flag; tile += n_clusters) {
                 int tm, tn;
-                tile_at(work.tile, tm, tn);
+                tile_at(tile, tm, tn);
                 const int y_a = tm * 256 + rank * 128;
                 // SwiGLU: the second CTA brings the up rows
                 const CUtensorMap *mapA = SWAP ? &mapW0 : &mapX, *mapB = SWAP ? &mapX : PAIR && rank ? &mapW1 : &mapW0;
                 const int y_b = PAIR && !SWAP ? tn * UNITS : tn * BN + rank * (BN / 2);
-                for (int kb = work.k0; kb < work.k1; ++kb, ++it) {
+                for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
                     const int s = it % L::kStages;
                     if (!mbar_wait_bounded(smem_u32(&empty[s]), (uint32_t)(((it / L::kStages) & 1) ^ 1), abort_flag, p.status, FAULT_GEMV_EMPTY_WAIT)) break;
                     const uint32_t bar = smem_u32(&full[s]), a = smem_u32(smem) + s * L::kStage;
@@ -215,31 +182,31 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         }
     } else if (warp == 1) {
         if (rank == 0 && elect_one()) {
-            int it = 0, n = 0;
-            for (bool more = work.step(p, n_clusters); more && !*abort_flag; ++n) {
+            int it = 0;
+            for (int tile = cluster, n = 0, k0 = 0; tile < n_tiles && !*abort_flag; ++n) {
                 const int acc = n & 1;
                 if (!mbar_wait_bounded_cluster(smem_u32(&acc_empty[acc]), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, p.status, FAULT_TC_ACC_WAIT)) break;
                 tc_fence_after();
-                const int k_end = SEG ? min(work.k0 + kLtSegment, work.k1) : work.k1;
-                for (int kb = work.k0; kb < k_end; ++kb, ++it) {
+                const int k1 = SEG ? min(k0 + kLtSegment, p.kblocks) : p.kblocks;
+                for (int kb = k0; kb < k1; ++kb, ++it) {
                     const int s = it % L::kStages;
                     if (!mbar_wait_bounded_cluster(smem_u32(&full[s]), (uint32_t)((it / L::kStages) & 1), abort_flag, p.status, FAULT_GEMV_FULL_WAIT)) break;
                     tc_fence_after();
                     const uint32_t a = smem_u32(smem) + s * L::kStage;
                     const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + L::kA);
 #pragma unroll
-                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * ACC, ad + 2 * k, bd + 2 * k, IDESC, kb > work.k0 || k > 0);
+                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * ACC, ad + 2 * k, bd + 2 * k, IDESC, kb > k0 || k > 0);
                     if constexpr (PAIR && SWAP) {
                         const uint64_t ud = umma_desc_sw128(a + L::kARows);
 #pragma unroll
                         for (int k = 0; k < kLtBlockK / 16; ++k)
-                            tc_mma_bf16_pair(tmem + acc * ACC + BN, ud + 2 * k, bd + 2 * k, IDESC, kb > work.k0 || k > 0);
+                            tc_mma_bf16_pair(tmem + acc * ACC + BN, ud + 2 * k, bd + 2 * k, IDESC, kb > k0 || k > 0);
                     }
                     tc_commit_pair(smem_u32(&empty[s]));
                 }
                 tc_commit_pair(smem_u32(&acc_full[acc]));
-                work.k0 = k_end;
-                if (!SEG || k_end == work.k1) more = work.step(p, n_clusters);
+                k0 = k1;
+                if (!SEG || k1 == p.kblocks) tile += n_clusters, k0 = 0;
             }
         }
     } else if constexpr (SWAP) {
@@ -247,9 +214,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         // output, wherever those start.  The residual is requested a step ahead.
         constexpr int W = SEG ? 16 : 32;
         const int q = warp & 3, c0 = ((warp - 2) >> 2) * W;
-        for (int n = 0; work.step(p, n_clusters); ++n) {
+        for (int tile = cluster, n = 0; tile < n_tiles; tile += n_clusters, ++n) {
             int ta, tb;
-            tile_at(work.tile, ta, tb);
+            tile_at(tile, ta, tb);
             const int n0 = ta * 256 + rank * 128 + q * 32, col = n0 + lane, m0 = tb * BN;
             const int rows = n0 < p.N ? min(BN, p.M - m0) : 0;
             const bool live = col < p.N;
@@ -316,7 +283,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                         if constexpr (PAIR) sum_up[j][e] = 0.f;
                     }
 #pragma unroll 1
-                for (int k = work.k0; k < work.k1; k += kLtSegment) {
+                for (int k = 0; k < p.kblocks; k += kLtSegment) {
                     const uint32_t t = filled();
 #pragma unroll
                     for (int j = 0; j < STEPS; ++j) {
@@ -335,7 +302,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                         }
                     }
                     drained();
-                    if (k + kLtSegment < work.k1) ++n;
+                    if (k + kLtSegment < p.kblocks) ++n;
                 }
                 const bool fine = !__any_sync(0xffffffffu, *abort_flag);
 #pragma unroll
@@ -367,9 +334,9 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         const int q = warp & 3, row = q * 32 + lane;
         float* turn = reinterpret_cast<float*>(smem + L::kStages * L::kStage) + (warp - 2) * 32 * (W + 1);
         const int c0 = ((warp - 2) >> 2) * W;  // two warps share a quarter: every other step each
-        for (int n = 0; work.step(p, n_clusters); ++n) {
+        for (int tile = cluster, n = 0; tile < n_tiles; tile += n_clusters, ++n) {
             int tm, tn;
-            tile_at(work.tile, tm, tn);
+            tile_at(tile, tm, tn);
             const int acc = n & 1;
             const int m = tm * 256 + rank * 128 + row;
             const bool live_row = m < p.M;
@@ -386,63 +353,11 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                 tc_fence_before();
                 if (lane == 0) mbar_arrive_cluster(map_to_rank(smem_u32(&acc_empty[acc]), 0));
             };
-            // A part: into the workspace, [group of four columns][row]; who adds the last one of a tile joins them in the order of K.
-            int first = cluster, n_parts = 0;  // the clusters first .. first + n_parts - 1 have one
-            auto part_of = [&](int c) {
-                return reinterpret_cast<const float4*>(p.parts) + ((long long)((2 * c + (c == first ? 1 : 0)) * 2 + rank) * (BN / 4)) * 128 + row;
-            };
-            if (work.part) {
-                const int tile0 = (work.tile - p.sk_first) * p.kblocks, tile1 = tile0 + p.kblocks;
-                while (first > 0 && lt_share(p, first) > tile0) --first;
-                int end = cluster + 1;
-                while (end < n_clusters && lt_share(p, end) < tile1) ++end;
-                n_parts = end - first;
-                float4* mine = const_cast<float4*>(part_of(cluster));
-#pragma unroll 1
-                for (int c = c0; c < BN; c += 2 * W) {
-                    float v[W];
-                    tmem_ld32(t + c, v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int e = 0; e < W; e += 4) __stcg(mine + (c + e) / 4 * 128, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]));
-                }
-                drained();
-                named_bar_sync(1, kLtThreads - 64);  // behind it one thread speaks for all
-                if (tid == 64) {
-                    __threadfence();
-                    unsigned int* count = p.count + 2 * first + rank;  // one tile at most is cut that starts in a cluster's length
-                    const unsigned int done = atomicAdd(count, (unsigned)(work.k1 - work.k0)) + (unsigned)(work.k1 - work.k0);
-                    *last = done == (unsigned)p.kblocks;
-                    if (*last) *count = 0u;
-                    __threadfence();
-                }
-                named_bar_sync(1, kLtThreads - 64);
-                const bool join = *last;
-                named_bar_sync(1, kLtThreads - 64);  // the flag is free again
-                if (!join) continue;
-            }
-            auto columns = [&](int at, float* v) {  // W sums of this row
-                if (!work.part) {
-                    tmem_ld32(t + at, v);
-                    return;
-                }
-#pragma unroll
-                for (int e = 0; e < W; ++e) v[e] = 0.f;
-#pragma unroll 1
-                for (int i = 0; i < n_parts; ++i) {
-                    const float4* part = part_of(first + i) + at / 4 * 128;
-#pragma unroll
-                    for (int e = 0; e < W; e += 4) {
-                        const float4 x = __ldcg(part + e / 4 * 128);
-                        v[e] += x.x, v[e + 1] += x.y, v[e + 2] += x.z, v[e + 3] += x.w;
-                    }
-                }
-            };
 #pragma unroll 1
             for (int c = c0; c < cols; c += 2 * W) {
                 float v[W], up[PAIR ? W : 1];
-                columns(c, v);
-                if constexpr (PAIR) columns(UNITS + c, up);
+                tmem_ld32(t + c, v);
+                if constexpr (PAIR) tmem_ld32(t + UNITS + c, up);
                 const int left = cols - c, col = n0 + c;
                 uint32_t res[W / 2];
                 if (res_row) {
@@ -527,7 +442,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                 }
                 __syncwarp();
             }
-            if (!work.part) drained();
+            drained();
         }
     }
     __syncwarp();
@@ -552,57 +467,39 @@ static bool encode_rows(CUtensorMap* map, const bf16* base, long long rows, long
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The width of the tiles, and whether they are cut along K.  A k block of a tile costs a cluster what its two SMs need to bring the
-// operands in (measured 520, 490 and 410 cycles for 256, 128 and 64 columns), so the widest tile that leaves no more rounds is
-// taken.  Few outputs behind a long K (a router's scores, 44 columns of 555 rows, K = 5544) would be left to a handful of
-// clusters: there up to kLtMostParts of them share a tile (24.4 -> 14.4 us).  Wider or shorter products are not cut: writing the
-// parts and joining them in one SM takes longer than the clusters are idle (N = 4096, K = 4096: 256 rows 13.6 us on whole tiles,
-// 29.3 cut; 138 rows of 176 outputs, K = 2248: 12.5 and 17.1; 3383 rows of 64, K = 4984, 14 tiles: 21.7 and 18.7 to 25).
+// The width of the tiles.  A k block of a tile costs a cluster what its two SMs need to bring the operands in (measured 520, 490
+// and 410 cycles for 256, 128 and 64 columns), so the widest tile that leaves no more rounds is taken.
 struct LtPlan {
-    int bn, clusters, sk_tiles;
+    int bn, clusters;
     bool swap, seg;
 };
-static constexpr int kLtMinBlocks = 8;   // k blocks below which a further cluster does not pay
-static constexpr int kLtMostParts = 8;
-static constexpr int kLtCutTiles = 8;    // most tiles that are cut
-static constexpr int kLtCutBlocks = 64;  // fewest k blocks of a tile that is
 static constexpr int kLtSwapRows = 128;  // rows of x up to which W's rows are A
-static LtPlan linear_plan(int M, int N, int K, int act, bool cut, bool aligned, bool f32) {
+static LtPlan linear_plan(int M, int N, int K, int act, bool aligned, bool f32) {
     const long long kb = (K + kLtBlockK - 1) / kLtBlockK, most = sm_count() / 2;
+    LtPlan best = {256, 1, false, f32 && kb > kLtSegment};
+    best.swap = !aligned || M <= kLtSwapRows || best.seg;
+    const bool pair = act == ACT_SWIGLU;
+    const long long a_rows = best.swap ? N : M, b_rows = best.swap ? M : pair ? 2ll * N : N;
     const int widths[3] = {256, 128, 64};
     const double block[3] = {520., 490., 410.};
-    auto whole = [&](long long a_rows, long long b_rows, int widest) {
-        LtPlan best = {256, 1, 0, false, false};
-        double least = -1.;
-        for (int i = widest; i < 3; ++i) {
-            const long long tiles = (a_rows + 255) / 256 * ((b_rows + widths[i] - 1) / widths[i]);
-            const double cost = (double)((tiles + most - 1) / most) * (double)kb * block[i];
-            if (least < 0. || cost < least) least = cost, best = {widths[i], (int)(tiles < most ? tiles : most), 0, false, false};
-        }
-        return best;
-    };
-    LtPlan best = whole(M, act == ACT_SWIGLU ? 2ll * N : N, 0);
-    if (cut && best.bn == 64 && best.clusters <= kLtCutTiles && kb >= kLtCutBlocks) {
-        const long long parts = f32 ? (kb + kLtSegment - 1) / kLtSegment : kLtMostParts;
-        long long clusters = best.clusters * parts, by_blocks = best.clusters * kb / kLtMinBlocks;
-        if (clusters > by_blocks && !f32) clusters = by_blocks;
-        if (clusters <= most || !f32) {
-            best.sk_tiles = best.clusters, best.clusters = (int)(clusters < most ? clusters : most);
-            return best;
-        }
-    }
-    if (!aligned || M <= kLtSwapRows || (f32 && kb > kLtSegment)) {
-        best = whole(N, M, act == ACT_SWIGLU ? 1 : 0);
-        best.swap = true, best.seg = f32 && kb > kLtSegment;
+    double least = -1.;
+    for (int i = best.swap && pair ? 1 : 0; i < 3; ++i) {
+        const long long tiles = (a_rows + 255) / 256 * ((b_rows + widths[i] - 1) / widths[i]);
+        const double cost = (double)((tiles + most - 1) / most) * (double)kb * block[i];
+        if (least < 0. || cost < least) least = cost, best.bn = widths[i], best.clusters = (int)(tiles < most ? tiles : most);
     }
     return best;
 }
 
-size_t linear_workspace_bytes(int M, int N, int K, int act) {
-    if (M <= kLinearFewRows) return 0;
-    const LtPlan plan = linear_plan(M, N, K, act, true, true, false);
-    // one size for all, so that an operator's workspace never has to grow under a captured graph
-    return plan.sk_tiles ? (size_t)kLtCountBytes + (size_t)(sm_count() / 2) * 4 * 256 * 128 * sizeof(float) : 0;
+// Few rows, or few results behind a long K, for which pairs of CTAs would leave most SMs idle: groups of 64 rows, each with the
+// weight cut along K over clusters that add their parts up in shared memory (us, pairs against groups: 128 x 64, K = 4096 10.3 and
+// 5.8; 128 x 515, K = 4600 20.8 and 7.3; 300 x 512, K = 2048 8.7 and 7.3, but 555 rows 8.6 and 10.0; 2048 x 128, K = 4096 13.3 and 9.0;
+// 400 x 128, K = 512 5.2 and 4.8, but 800 rows 5.2 and 5.7; 128 x 4096, K = 12288 32.6 and 28.4, K = 4096 14.3 and 15.0, K = 1024 6.8
+// and 9.3).
+static bool linear_in_groups(int M, int N, int K) {
+    const long long tiles = ((long long)M + kLinearGroupRows - 1) / kLinearGroupRows * ((N + 127ll) / 128);
+    if (((long long)M + kLinearGroupRows - 1) / kLinearGroupRows > sm_count()) return false;  // a cluster each at least
+    return M <= kLinearGroupRows || (tiles <= 64 && 60 * tiles <= K);
 }
 
 template <int BN, bool PAIR, bool SWAP, bool SEG = false>
@@ -616,8 +513,6 @@ static cudaError_t launch_linear_tile(const LinearArgs& a, const LtPlan& plan, L
     static std::atomic<bool> configured[64];
     if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR, SWAP, SEG>, kBytes, configured)) return e;
     p.tiles_a = ((SWAP ? a.N : a.M) + 255) / 256, p.tiles_b = ((SWAP ? a.M : a.N) + UNITS - 1) / UNITS;
-    p.sk_first = p.tiles_a * p.tiles_b - plan.sk_tiles, p.sk_units = plan.sk_tiles * p.kblocks;
-    p.sk_share = (p.sk_units + plan.clusters - 1) / plan.clusters;
     chain_begin();
     return launch_pdl_cluster(linear_tc_kernel<BN, PAIR, SWAP, SEG>, dim3(2u * plan.clusters), dim3(kLtThreads), 2, kBytes, stream, mx, w0, w1, p);
 }
@@ -638,7 +533,7 @@ static cudaError_t launch_linear_form(const LinearArgs& a, const LtPlan& plan, L
 }
 
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
-    if (a.M <= kLinearFewRows) return launch_linear_few(a, stream);
+    if (linear_in_groups(a.M, a.N, a.K)) return launch_linear_groups(a, stream);
     LtParams p;
     p.bias = a.bias, p.residual = a.residual, p.out = a.out, p.ldres = a.ldres, p.ldout = a.ldout;
     p.M = a.M, p.N = a.N, p.kblocks = (a.K + kLtBlockK - 1) / kLtBlockK;
@@ -648,9 +543,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
     p.vec_bias = a.bias && aligned16(a.bias) && (a.act != ACT_SWIGLU || a.N % 8 == 0);
     p.status = status_ptr();
     if (!p.status) return cudaErrorUnknown;
-    const LtPlan plan = linear_plan(a.M, a.N, a.K, a.act, a.workspace != nullptr, p.rows_aligned, a.out_f32);
-    p.count = static_cast<unsigned int*>(a.workspace);
-    p.parts = reinterpret_cast<float*>(static_cast<unsigned char*>(a.workspace) + kLtCountBytes);
+    const LtPlan plan = linear_plan(a.M, a.N, a.K, a.act, p.rows_aligned, a.out_f32);
     return a.act == ACT_SWIGLU ? launch_linear_form<true>(a, plan, p, stream) : launch_linear_form<false>(a, plan, p, stream);
 }
 

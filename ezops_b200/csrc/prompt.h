@@ -97,12 +97,10 @@ struct LinearArgs {
     void* out;
     long long ldx, ldres, ldout;
     int M, N, K, act, out_f32;
-    void* workspace;  // at least linear_workspace_bytes(), or null: no tile is cut along K
 };
-size_t linear_workspace_bytes(int M, int N, int K, int act);  // 0 when no tile is
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream);
-static constexpr int kLinearFewRows = 64;
-cudaError_t launch_linear_few(const LinearArgs& a, cudaStream_t stream);  // at most kLinearFewRows rows (gemm_tc.cu)
+static constexpr int kLinearGroupRows = 64;
+cudaError_t launch_linear_groups(const LinearArgs& a, cudaStream_t stream);  // groups of at most so many rows (gemm_tc.cu)
 
 struct AttnPromptArgs {
     const bf16 *Q, *K, *V;

@@ -140,14 +140,8 @@ int ezb_paged_qk_norm_rope(const void* qkv, long long ldqkv, const void* qw_or_n
     return EZB_OK;
 }
 
-size_t ezb_linear_workspace_bytes(int M, int N, int K, int activation) {
-    if (M < 1 || N < 1 || K < 1 || activation < EZB_ACT_NONE || activation > EZB_ACT_SWIGLU) return 0;
-    return linear_workspace_bytes(M, N, K, activation);
-}
-
 int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bias_or_null, const void* residual_or_null,
-                    long long ldres, void* out, long long ldout, void* workspace_or_null, size_t workspace_bytes, int M, int N, int K,
-                    int activation, int out_f32, ezb_stream_t stream) {
+                    long long ldres, void* out, long long ldout, int M, int N, int K, int activation, int out_f32, ezb_stream_t stream) {
     EZB_REQUIRE(X && W && out, "null pointer");
     EZB_REQUIRE(M >= 1 && N >= 1 && K >= 1, "M, N and K must be positive");
     EZB_REQUIRE(activation >= EZB_ACT_NONE && activation <= EZB_ACT_SWIGLU, "unknown activation");
@@ -170,12 +164,7 @@ int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bia
     const bool in_place = residual_or_null == out && ldres == ldout && !out_f32;  // every element is read by the thread that writes it
     EZB_REQUIRE(!residual_or_null || in_place || !overlap(o, {residual_or_null, M, ldres * 2, (long long)N * 2}),
                 "out overlaps residual (it may be the same bf16 tensor, not another view of it)");
-    if (workspace_or_null && (!aligned16(workspace_or_null) || workspace_bytes < linear_workspace_bytes(M, N, K, activation))) {
-        set_last_message("workspace misaligned or smaller than ezb_linear_workspace_bytes()");
-        return EZB_ERR_WORKSPACE;
-    }
     LinearArgs a;
-    a.workspace = workspace_or_null;
     a.x = static_cast<const bf16*>(X), a.W = static_cast<const bf16*>(W), a.bias = static_cast<const bf16*>(bias_or_null);
     a.residual = static_cast<const bf16*>(residual_or_null), a.out = out;
     a.ldx = ldx, a.ldres = ldres, a.ldout = ldout;

@@ -169,8 +169,6 @@ class PagedQkNormRopeSm100Kernel(BaseKernel):
 
 @register_kernel("linear", "cuda", family="prompt")
 class LinearSm100Kernel(BaseKernel):
-    """Owns workspaces (``_Workspaces``) for the numbers of rows that have a use for one."""
-
     def __init__(self, out_features, in_features, bias=False, activation=None, residual=False, out_dtype=_BF16):
         from ..ops.linear import ACTIVATIONS
 
@@ -180,20 +178,7 @@ class LinearSm100Kernel(BaseKernel):
         rows = out_features * (2 if activation == "swiglu" else 1)
         self._w, self._bias = (rows, in_features), (rows,)
         self._f32 = int(out_dtype == torch.float32)
-        self._lib = _lib.load()
         self._entry, self._pack = _packed("ezb_linear_bf16")
-        self._need: dict[int, int] = {}  # rows -> workspace bytes
-        self._spaces, self._ws = _Workspaces(self._lib), None
-
-    def workspace(self, rows: int, device):
-        """The workspace for so many rows, or None; it never has to grow."""
-        need = self._need.get(rows)
-        if need is None:
-            need = self._need[rows] = self._lib.ezb_linear_workspace_bytes(rows, self.N, self.K, self.act)
-        if not need:
-            return None
-        self._ws = self._spaces.get(need, device.index, _raw_stream(device.index))
-        return self._ws
 
     def __call__(self, X, W, bias=None, residual=None, out=None):
         dev, M, N, K = _device(X, "X"), X.shape[0], self.N, self.K
@@ -203,10 +188,9 @@ class LinearSm100Kernel(BaseKernel):
                 and (residual is None or _rows(residual, (M, N), _BF16, dev)) and _rows(out, (M, N), self.out_dtype, dev)):
             _refuse([("X", X, (M, K), _BF16, True), ("W", W, self._w, _BF16, False), ("bias", bias, self._bias, _BF16, False),
                      ("residual", residual, (M, N), _BF16, True), ("out", out, (M, N), self.out_dtype, True)], dev)
-        ws = self.workspace(M, X.device) if self._need.get(M) != 0 else None
         rc = self._entry(self._pack(
             X.data_ptr(), _distance(X), W.data_ptr(), _ptr(bias), _ptr(residual), N if residual is None else _distance(residual),
-            out.data_ptr(), _distance(out), _ptr(ws), 0 if ws is None else ws.numel(), M, N, K, self.act, self._f32, _raw_stream(dev)))
+            out.data_ptr(), _distance(out), M, N, K, self.act, self._f32, _raw_stream(dev)))
         if rc:
             _lib.check(rc)
         return out

@@ -375,19 +375,17 @@ int ezb_paged_qk_norm_rope(const void* qkv, long long ldqkv, const void* qw_or_n
  * the gate rows, then the up rows, and act is silu(gate) * up.  Rows of X, residual
  * (bf16) and out may be further apart than they are long (ldx, ldres, ldout in
  * elements; ldx a multiple of 8).  residual may be out itself.  K % 8 == 0.  The path,
- * and with it the order of the sums, follows from M, N, K, whether rows of out (32 bytes)
- * and residual (16) start at their boundaries, and whether there is a workspace: with one, sizes whose tiles would leave part of the GPU idle have some
- * tiles cut along K (ezb_linear_workspace_bytes() > 0; without one they are slower).
+ * and with it the order of the sums, follows from M, N, K, the types and whether rows of
+ * out (32 bytes) and residual (16) start at their boundaries.  fp32 results are added up
+ * every 512 elements of K, rounded to nearest (the tensor cores cut towards zero).
  * Equal calls give equal bits.  activation is one of EZB_ACT_*. */
 #define EZB_ACT_NONE 0
 #define EZB_ACT_SILU 1
 #define EZB_ACT_GELU 2 /* x/2 * (1 + erf(x / sqrt 2)) */
 #define EZB_ACT_RELU 3
 #define EZB_ACT_SWIGLU 4
-size_t ezb_linear_workspace_bytes(int M, int N, int K, int activation); /* 0 when the sizes have no use for one */
 int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bias_or_null, const void* residual_or_null,
-                    long long ldres, void* out, long long ldout, void* workspace_or_null, size_t workspace_bytes, int M, int N, int K,
-                    int activation, int out_f32, ezb_stream_t stream);
+                    long long ldres, void* out, long long ldout, int M, int N, int K, int activation, int out_f32, ezb_stream_t stream);
 
 /* Causal grouped-query attention of the step's tokens over the pools.  Row b holds
  * tokens cu_tokens[b] .. cu_tokens[b+1] of Q [T, ldq] (H heads of D) and has

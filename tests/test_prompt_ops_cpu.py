@@ -158,9 +158,9 @@ def test_c_entries_refuse_without_a_gpu():
     assert rope(ld=500) == bad and rope(ld=516) == bad and rope(qkv=odd) == bad and rope(out=a) == bad
     assert rope(pages=1 << 25) == shape
 
-    def linear(M=4, N=8, K=16, X=a, ldx=None, W=b, bias=None, res=None, ldres=None, out=c, ldout=None, act=0, f32=0, ws=None, size=0):
+    def linear(M=4, N=8, K=16, X=a, ldx=None, W=b, bias=None, res=None, ldres=None, out=c, ldout=None, act=0, f32=0):
         return lib.ezb_linear_bf16(X, K if ldx is None else ldx, W, bias, res, N if ldres is None else ldres, out,
-                                   N if ldout is None else ldout, ws, size, M, N, K, act, f32, None)
+                                   N if ldout is None else ldout, M, N, K, act, f32, None)
 
     assert linear(M=0) == bad and linear(K=12) == shape and linear(act=5) == bad and linear(act=-1) == bad
     assert linear(X=odd) == bad and linear(W=odd) == bad and linear(ldx=8) == bad and linear(ldx=20) == bad and linear(ldout=7) == bad
@@ -169,11 +169,6 @@ def test_c_entries_refuse_without_a_gpu():
     assert linear(res=P(0x4000010)) == bad and linear(res=c, ldres=9) == bad and linear(res=c, f32=1) == bad
     assert b"overlaps residual" in lib.ezb_last_error_message()
     assert linear(M=1 << 30, N=1 << 30) == shape
-    need = lib.ezb_linear_workspace_bytes(100, 8, 8192, 0)
-    assert need > 0 and lib.ezb_linear_workspace_bytes(64, 8, 8192, 0) == 0 and lib.ezb_linear_workspace_bytes(0, 8, 8192, 0) == 0
-    far = P(0x40000000)
-    assert linear(M=100, K=8192, out=far, ws=P(0x80000000), size=need - 1) == _lib.EZB_ERR_WORKSPACE
-    assert linear(M=100, K=8192, out=far, ws=P(0x80000004), size=need) == _lib.EZB_ERR_WORKSPACE
 
     def attn(B=2, T=8, H=4, NKV=2, D=64, max_pages=4, page=64, pages=9, Q=a, ldq=256, out=c, ldo=256, w=b, size=1 << 30):
         return lib.ezb_attn_prompt(Q, ldq, b, b, b, b, b, out, ldo, w, size, B, T, H, NKV, D, max_pages, page, pages, None)
@@ -202,7 +197,7 @@ def test_packed_entries_are_the_same_calls():
     p = 0x7F0012345600
     assert b"null" in same("ezb_paged_plan", *[None] * 10, 2, 8, 4, 64, 8, 8, None)
     assert b"8192" in same("ezb_paged_plan", *[p] * 10, 9000, 8, 4, 64, 8, 8, None)
-    assert b"positive" in same("ezb_linear_bf16", p, 64, p, None, None, 8, p, 8, None, 0, -3, 8, 64, 0, 0, None)
+    assert b"positive" in same("ezb_linear_bf16", p, 64, p, None, None, 8, p, 8, -3, 8, 64, 0, 0, None)
     assert b"128 query" in same("ezb_attn_prompt", p, 1 << 40, p, p, p, p, p, p, 1 << 41, p, 1 << 33, 1, 1, 129, 1, 64, 1, 64, 1, None)
     assert b"apart" in same("ezb_paged_qk_norm_rope", p, 8, None, None, *[p] * 7, 1, 8, 8, 64, 16, 1, p, 0, 64, 1, 1e-6, None)
     assert lib.ezb_attn_prompt_packed(None) == lib.ezb_paged_plan(*[None] * 10, 2, 8, 4, 64, 8, 8, None)
