@@ -8,8 +8,8 @@
 // K blocks by TMA (both CTAs' bytes are counted on the first CTA's barrier), one thread of the first CTA issues the MMAs,
 // eight warps of each CTA drain one of two accumulators while the next tile is multiplied: bias, activation, residual and
 // rounding happen there, in registers.  Grid: one CTA per SM, tiles in groups of kLtGroup tiles along A so that the x and W
-// tiles in flight stay in L2.  BN = 256 reads least per product; narrower tiles (128, 64) are taken when the wide ones would
-// leave clusters without work (linear_plan).
+// tiles in flight stay in L2.  BN = 256 reads least per product; narrower tiles, in steps of 16 or 32, are taken where the rounds of
+// tiles come out even with them (linear_widths: 777 x 4096, K = 12288 in four rows of tiles of 208 instead of 256, 74 -> 64 us).
 //   A = x: a lane of the epilogue has a row of the result and stores whole sectors of it.
 //   A = W: a lane has a column, and a warp's stores run along a row: for rows that start anywhere (a vocabulary or a number of
 // experts that is no multiple of 16, columns of a wider tensor), where a lane with a row would write parts of sectors, and for
@@ -18,14 +18,14 @@
 // columns: 154 and 163); 4530 x 3350, K = 720, fp32 62 and 32; 104 x 22304, K = 7360 86 and 67; 128 rows of 4096 through SwiGLU to
 // 12288 61 to 67 and 50; 300 x 4096, K = 4096 15.2 to 16.6 and 16.0 to 16.9; 8192 x 4096, K = 4096 193 and 188 to 193.
 // What bounds it: the tensor cores where tiles fill the clusters evenly (4096 rows of 4096 through SwiGLU to 12288: 516 us,
-// 1600 TFLOP/s; 587 at the 1.3 GHz of the power cap); else the operands' way from L2 (777 x 4096, K = 12288: 64 tiles on 74 clusters bring
-// 0.7 GB into the SMs in 72 us); from a few hundred rows down the weights' bytes (104 x 22304, K = 7360: 5.1 TB/s).
+// 1600 TFLOP/s, tensor pipe active 98 % of the time; 587 at the 1.3 GHz of the power cap), with 64 to 74 of them busy to the end; the
+// operands' way from L2 for narrow tiles; from a few hundred rows down the weights' bytes (104 x 22304, K = 7360: 5.1 TB/s).
 // fp32 results of more than kLtSegment k blocks: the tensor cores cut their sums towards zero (gemm_tc.cu), so the sums leave them
 // every kLtSegment blocks and are added up, rounded to nearest, in the registers of the lane whose column it is (A = W); the relative
 // error is 4.8e-7 for any K (1.4e-5 at K = 12800 otherwise), and 8192 x 4096, K = 4096 takes 193 us instead of 191.  Rounded to
 // bf16 that error does not show.
-// Few rows or few results (linear_in_groups): the kernel of the batched decode projections (gemm_tc.cu) with this epilogue (17 x 6144, K = 4096: 10.3 us, 4.9 TB/s;
-// 64 x 151936, K = 1024 to fp32: 57 us, 6.1 TB/s).
+// Few rows or few results (linear_in_groups): the kernel of the batched decode projections (gemm_tc.cu) with this epilogue
+// (17 x 6144, K = 4096: 10.5 us, 4.8 TB/s; 64 x 151936, K = 1024 to fp32: 58 us, 6.0 TB/s).
 #include <atomic>
 
 #include "prompt.h"
@@ -44,7 +44,7 @@ struct LtParams {
     void* out;
     long long ldres, ldout;
     int M, N, kblocks;
-    int tiles_a, tiles_b, act, out_f32;  // tiles along A's and B's rows
+    int bn, tiles_a, tiles_b, act, out_f32;  // rows of B in a tile (SwiGLU with A = x: the template's); tiles along A's and B's rows
     int rows_aligned;  // rows of out start at 32-byte, of residual at 16-byte boundaries
     int vec_bias;      // so does bias
     unsigned int* status;
@@ -113,14 +113,14 @@ __device__ __forceinline__ void load_packed(const bf16* src, int left, int vec, 
     }
 }
 
-// SEG: the products of kLtSegment k blocks at a time, added up in registers (fp32 results, swapped form).
+// BN: the most rows of B in a tile (p.bn).  SEG: the products of kLtSegment k blocks at a time, added up in registers (fp32 results, swapped form).
 template <int BN, bool PAIR, bool SWAP, bool SEG>
 __global__ void __launch_bounds__(kLtThreads, 1)
 linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant__ CUtensorMap mapW0,
                  const __grid_constant__ CUtensorMap mapW1, const __grid_constant__ LtParams p) {
     using L = LtSmem<BN, PAIR, SWAP>;
-    constexpr uint32_t IDESC = umma_idesc_bf16(256, BN);
-    constexpr int UNITS = PAIR && !SWAP ? BN / 2 : BN;  // output columns of a tile; swapped: rows
+    const int bn = PAIR && !SWAP ? BN : p.bn, units = PAIR && !SWAP ? BN / 2 : bn;  // output columns of a tile; swapped: rows
+    const uint32_t idesc = umma_idesc_bf16(256, bn);
     constexpr int ACC = PAIR && SWAP ? 2 * BN : BN;     // columns of tensor memory of a tile
     static_assert(2 * ACC <= 512);
     extern __shared__ unsigned char lt_raw[];
@@ -168,12 +168,12 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                 const int y_a = tm * 256 + rank * 128;
                 // SwiGLU: the second CTA brings the up rows
                 const CUtensorMap *mapA = SWAP ? &mapW0 : &mapX, *mapB = SWAP ? &mapX : PAIR && rank ? &mapW1 : &mapW0;
-                const int y_b = PAIR && !SWAP ? tn * UNITS : tn * BN + rank * (BN / 2);
+                const int y_b = PAIR && !SWAP ? tn * units : tn * bn + rank * (bn / 2);
                 for (int kb = 0; kb < p.kblocks; ++kb, ++it) {
                     const int s = it % L::kStages;
                     if (!mbar_wait_bounded(smem_u32(&empty[s]), (uint32_t)(((it / L::kStages) & 1) ^ 1), abort_flag, p.status, FAULT_GEMV_EMPTY_WAIT)) break;
                     const uint32_t bar = smem_u32(&full[s]), a = smem_u32(smem) + s * L::kStage;
-                    if (rank == 0) mbar_arrive_expect_tx(bar, 2 * L::kStage);
+                    if (rank == 0) mbar_arrive_expect_tx(bar, 2 * (L::kA + bn * kLtBlockK));  // both CTAs' halves of B
                     tma_load_2d_pair(a, mapA, kb * kLtBlockK, y_a, bar);
                     if constexpr (PAIR && SWAP) tma_load_2d_pair(a + L::kARows, &mapW1, kb * kLtBlockK, y_a, bar);
                     tma_load_2d_pair(a + L::kA, mapB, kb * kLtBlockK, y_b, bar);
@@ -195,12 +195,12 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
                     const uint32_t a = smem_u32(smem) + s * L::kStage;
                     const uint64_t ad = umma_desc_sw128(a), bd = umma_desc_sw128(a + L::kA);
 #pragma unroll
-                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * ACC, ad + 2 * k, bd + 2 * k, IDESC, kb > k0 || k > 0);
+                    for (int k = 0; k < kLtBlockK / 16; ++k) tc_mma_bf16_pair(tmem + acc * ACC, ad + 2 * k, bd + 2 * k, idesc, kb > k0 || k > 0);
                     if constexpr (PAIR && SWAP) {
                         const uint64_t ud = umma_desc_sw128(a + L::kARows);
 #pragma unroll
                         for (int k = 0; k < kLtBlockK / 16; ++k)
-                            tc_mma_bf16_pair(tmem + acc * ACC + BN, ud + 2 * k, bd + 2 * k, IDESC, kb > k0 || k > 0);
+                            tc_mma_bf16_pair(tmem + acc * ACC + BN, ud + 2 * k, bd + 2 * k, idesc, kb > k0 || k > 0);
                     }
                     tc_commit_pair(smem_u32(&empty[s]));
                 }
@@ -217,8 +217,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
         for (int tile = cluster, n = 0; tile < n_tiles; tile += n_clusters, ++n) {
             int ta, tb;
             tile_at(tile, ta, tb);
-            const int n0 = ta * 256 + rank * 128 + q * 32, col = n0 + lane, m0 = tb * BN;
-            const int rows = n0 < p.N ? min(BN, p.M - m0) : 0;
+            const int n0 = ta * 256 + rank * 128 + q * 32, col = n0 + lane, m0 = tb * units;
+            const int rows = n0 < p.N ? min(units, p.M - m0) : 0;
             const bool live = col < p.N;
             const bf16* res_col = p.residual && live ? p.residual + (long long)m0 * p.ldres + col : nullptr;
             const float bias = p.bias && live ? __bfloat162float(p.bias[col]) : 0.f;
@@ -340,8 +340,8 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             const int acc = n & 1;
             const int m = tm * 256 + rank * 128 + row;
             const bool live_row = m < p.M;
-            const int n0 = tn * UNITS;
-            const int cols = min(UNITS, p.N - n0);
+            const int n0 = tn * units;
+            const int cols = min(units, p.N - n0);
             const bf16* res_row = p.residual && p.rows_aligned ? p.residual + (long long)m * p.ldres + n0 : nullptr;
             uint32_t ahead[W / 2];  // residual values of the next step, packed
             if (res_row && live_row && cols - c0 >= W) load_packed<W>(res_row + c0, W, 1, ahead);
@@ -357,7 +357,7 @@ linear_tc_kernel(const __grid_constant__ CUtensorMap mapX, const __grid_constant
             for (int c = c0; c < cols; c += 2 * W) {
                 float v[W], up[PAIR ? W : 1];
                 tmem_ld32(t + c, v);
-                if constexpr (PAIR) tmem_ld32(t + UNITS + c, up);
+                if constexpr (PAIR) tmem_ld32(t + units + c, up);
                 const int left = cols - c, col = n0 + c;
                 uint32_t res[W / 2];
                 if (res_row) {
@@ -467,28 +467,38 @@ static bool encode_rows(CUtensorMap* map, const bf16* base, long long rows, long
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// The width of the tiles.  A k block of a tile costs a cluster what its two SMs need to bring the operands in (measured 520, 490
-// and 410 cycles for 256, 128 and 64 columns), so the widest tile that leaves no more rounds is taken.
+// The form and the width of the tiles.  With all SMs busy a k block of a tile takes its cluster the longer of its products (368 ns
+// for 256 x 256, at the clock that the power cap leaves) and of its operands' way from L2 (98 bytes per ns and SM; measured 368, 251
+// and 209 ns for 256, 128 and 64 rows of B), and the last round of tiles takes as long as a full one: the width with the least sum is
+// taken, the narrower of equal rounds, so that a last tile is not left nearly empty.
 struct LtPlan {
     int bn, clusters;
     bool swap, seg;
+    double cost;
 };
 static constexpr int kLtSwapRows = 128;  // rows of x up to which W's rows are A
-static LtPlan linear_plan(int M, int N, int K, int act, bool aligned, bool f32) {
-    const long long kb = (K + kLtBlockK - 1) / kLtBlockK, most = sm_count() / 2;
-    LtPlan best = {256, 1, false, f32 && kb > kLtSegment};
-    best.swap = !aligned || M <= kLtSwapRows || best.seg;
-    const bool pair = act == ACT_SWIGLU;
-    const long long a_rows = best.swap ? N : M, b_rows = best.swap ? M : pair ? 2ll * N : N;
-    const int widths[3] = {256, 128, 64};
-    const double block[3] = {520., 490., 410.};
-    double least = -1.;
-    for (int i = best.swap && pair ? 1 : 0; i < 3; ++i) {
-        const long long tiles = (a_rows + 255) / 256 * ((b_rows + widths[i] - 1) / widths[i]);
-        const double cost = (double)((tiles + most - 1) / most) * (double)kb * block[i];
-        if (least < 0. || cost < least) least = cost, best.bn = widths[i], best.clusters = (int)(tiles < most ? tiles : most);
+static LtPlan linear_widths(int M, int N, bool pair, bool swap) {
+    const long long most = sm_count() / 2, a_tiles = ((swap ? N : M) + 255ll) / 256;
+    // what the epilogue takes at a time without a remainder; SwiGLU, swapped: two A operands, and two accumulators
+    const int step = swap ? 16 : 32, widest = swap && pair ? 128 : 256, halves = swap && pair ? 2 : 1;
+    LtPlan best = {0, 0, swap, false, 0.};
+    for (int bn = widest; bn >= 64; bn = pair && !swap ? bn / 2 : bn - step) {
+        const long long per = pair && !swap ? bn / 2 : bn, tiles = a_tiles * (((swap ? M : N) + per - 1) / per);
+        const double products = 368. / 256. * bn * halves, operands = 1.306 * (128 * halves + bn / 2.);
+        const double cost = (double)((tiles + most - 1) / most) * (products > operands ? products : operands);
+        if (best.bn == 0 || cost < best.cost) best.bn = bn, best.cost = cost, best.clusters = (int)(tiles < most ? tiles : most);
     }
     return best;
+}
+static LtPlan linear_plan(int M, int N, int K, int act, bool aligned, bool f32) {
+    const bool pair = act == ACT_SWIGLU, seg = f32 && (K + kLtBlockK - 1) / kLtBlockK > kLtSegment;
+    LtPlan plan = linear_widths(M, N, pair, !aligned || M <= kLtSwapRows || seg);
+    if (!plan.swap && !pair) {  // scattered rows cost a little: swapped only for a better fit
+        const LtPlan other = linear_widths(M, N, pair, true);
+        if (other.cost < 0.95 * plan.cost) plan = other;  // 776 x 5984, K = 3712 39 -> 28 us, 500 x 24576, K = 4096 101 -> 87
+    }
+    plan.seg = seg;
+    return plan;
 }
 
 // Few rows, or few results behind a long K, for which pairs of CTAs would leave most SMs idle: groups of 64 rows, each with the
@@ -504,15 +514,15 @@ static bool linear_in_groups(int M, int N, int K) {
 
 template <int BN, bool PAIR, bool SWAP, bool SEG = false>
 static cudaError_t launch_linear_tile(const LinearArgs& a, const LtPlan& plan, LtParams& p, cudaStream_t stream) {
-    constexpr int UNITS = PAIR && !SWAP ? BN / 2 : BN, kBytes = LtSmem<BN, PAIR, SWAP>::kBytes;
+    constexpr int kBytes = LtSmem<BN, PAIR, SWAP>::kBytes;
     alignas(64) CUtensorMap mx, w0, w1;
-    const int box_x = SWAP ? BN / 2 : 128, box_w = SWAP ? 128 : BN / 2;
+    const int box_x = SWAP ? plan.bn / 2 : 128, box_w = SWAP ? 128 : plan.bn / 2, units = PAIR && !SWAP ? plan.bn / 2 : plan.bn;
     if (!encode_rows(&mx, a.x, a.M, a.K, a.ldx, box_x) || !encode_rows(&w0, a.W, a.N, a.K, a.K, box_w)) return cudaErrorInvalidValue;
     if (!PAIR) w1 = w0;
     else if (!encode_rows(&w1, a.W + (long long)a.N * a.K, a.N, a.K, a.K, box_w)) return cudaErrorInvalidValue;
     static std::atomic<bool> configured[64];
     if (cudaError_t e = allow_smem_once(linear_tc_kernel<BN, PAIR, SWAP, SEG>, kBytes, configured)) return e;
-    p.tiles_a = ((SWAP ? a.N : a.M) + 255) / 256, p.tiles_b = ((SWAP ? a.M : a.N) + UNITS - 1) / UNITS;
+    p.tiles_a = ((SWAP ? a.N : a.M) + 255) / 256, p.tiles_b = ((SWAP ? a.M : a.N) + units - 1) / units, p.bn = plan.bn;
     chain_begin();
     return launch_pdl_cluster(linear_tc_kernel<BN, PAIR, SWAP, SEG>, dim3(2u * plan.clusters), dim3(kLtThreads), 2, kBytes, stream, mx, w0, w1, p);
 }
@@ -520,16 +530,16 @@ template <bool PAIR>
 static cudaError_t launch_linear_form(const LinearArgs& a, const LtPlan& plan, LtParams& p, cudaStream_t stream) {
     if (plan.seg) {
         if constexpr (!PAIR)
-            if (plan.bn == 256) return launch_linear_tile<256, PAIR, true, true>(a, plan, p, stream);
-        return plan.bn == 128 ? launch_linear_tile<128, PAIR, true, true>(a, plan, p, stream) : launch_linear_tile<64, PAIR, true, true>(a, plan, p, stream);
+            if (plan.bn > 128) return launch_linear_tile<256, PAIR, true, true>(a, plan, p, stream);
+        return plan.bn > 64 ? launch_linear_tile<128, PAIR, true, true>(a, plan, p, stream) : launch_linear_tile<64, PAIR, true, true>(a, plan, p, stream);
     }
     if (plan.swap) {
         if constexpr (!PAIR)
-            if (plan.bn == 256) return launch_linear_tile<256, PAIR, true>(a, plan, p, stream);
-        return plan.bn == 128 ? launch_linear_tile<128, PAIR, true>(a, plan, p, stream) : launch_linear_tile<64, PAIR, true>(a, plan, p, stream);
+            if (plan.bn > 128) return launch_linear_tile<256, PAIR, true>(a, plan, p, stream);
+        return plan.bn > 64 ? launch_linear_tile<128, PAIR, true>(a, plan, p, stream) : launch_linear_tile<64, PAIR, true>(a, plan, p, stream);
     }
-    if (plan.bn == 256) return launch_linear_tile<256, PAIR, false>(a, plan, p, stream);
-    return plan.bn == 128 ? launch_linear_tile<128, PAIR, false>(a, plan, p, stream) : launch_linear_tile<64, PAIR, false>(a, plan, p, stream);
+    if (plan.bn > 128) return launch_linear_tile<256, PAIR, false>(a, plan, p, stream);
+    return plan.bn > 64 ? launch_linear_tile<128, PAIR, false>(a, plan, p, stream) : launch_linear_tile<64, PAIR, false>(a, plan, p, stream);
 }
 
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t stream) {
