@@ -146,12 +146,13 @@ cudaError_t launch_paged_plan(const PlanArgs& a, cudaStream_t stream) {
 //   n = x / sqrt(mean(x^2) + eps) * w
 //   y_i = n_i cos[p, i] - n_{i+D/2} sin[p, i],   y_{i+D/2} = n_{i+D/2} cos[p, i+D/2] + n_i sin[p, i+D/2]
 // in fp32 with one rounding, as the stand-alone operator of a decode step and the decode attention do.
-// What bounds it: HBM for prompts (every head is read and written once: 8189 tokens of 32 heads with three axes 28 us, 137 MB,
-// 4.9 TB/s), latency for a handful of tokens (32 tokens of 48 heads 2.2 us).  A head is D/8 lanes, each with four elements of
+// What bounds it: HBM for prompts (every head is read and written once: 8189 tokens of 32 heads with three axes 27 us, 137 MB,
+// 5.1 TB/s), latency for a handful of tokens (32 tokens of 48 heads 2.2 us).  A head is D/8 lanes, each with four elements of
 // its first half and their partners in the second, so that a rotation stays inside a lane, and two elements share an
 // instruction.  A warp keeps the cos and sin values of ONE token in registers for all the heads it walks; how many that are
 // (`steps`) follows from the number of tokens: one group of heads per warp while there are fewer warps than the chip holds,
-// more when the table rows would otherwise be fetched again for every group (36.8 -> 27.9 us).
+// more when the table rows would otherwise be fetched again for every group (36.8 -> 27.9 us, and 27.0 with the next heads
+// requested before these are worked off).
 struct PagedRopeParams {
     const bf16* qkv;
     long long ld;
@@ -165,7 +166,7 @@ struct PagedRopeParams {
     alignas(4) unsigned char axis[64];  // axis of frequency i
 };
 
-static constexpr int kRopeBatch = 4;  // heads in flight per lane
+static constexpr int kRopeBatch = 2;  // heads that a lane works off while as many are on their way (more take too many registers)
 __device__ __forceinline__ uint2 ld_stream8(const bf16* p) {  // read once
     uint2 v;
     asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
@@ -186,14 +187,14 @@ __global__ void __launch_bounds__(128, 7) paged_qk_norm_rope_kernel(const __grid
     // Everything that does not depend on the position is requested together with it: the heads, the weights, the slot.
     const int h0 = chunk * p.steps * HPW + lane / LPH;
     const bf16* src = p.qkv + (long long)t * p.ld + (long long)h0 * D + f0;
-    uint2 lo[kRopeBatch], hi[kRopeBatch];
-    auto load = [&](int i) {
+    uint2 lo[2][kRopeBatch], hi[2][kRopeBatch];
+    auto load = [&](int i, int z) {
 #pragma unroll
         for (int u = 0; u < kRopeBatch; ++u)
             if (i + u < p.steps && h0 + (i + u) * HPW < heads)
-                lo[u] = ld_stream8(src + (long long)(i + u) * HPW * D), hi[u] = ld_stream8(src + (long long)(i + u) * HPW * D + D / 2);
+                lo[z][u] = ld_stream8(src + (long long)(i + u) * HPW * D), hi[z][u] = ld_stream8(src + (long long)(i + u) * HPW * D + D / 2);
     };
-    load(0);
+    load(0, 0);
     int pos[3];
     bool real = true, inside = true;
 #pragma unroll
@@ -244,47 +245,52 @@ __global__ void __launch_bounds__(128, 7) paged_qk_norm_rope_kernel(const __grid
     bf16* q_row = p.q_out + (long long)t * p.H * D + f0;
     const long long kv_row = ((page * p.NKV) << p.page_shift) + off;  // + kv head * page size
 #pragma unroll 1
-    for (int i = 0; i < p.steps; i += kRopeBatch) {
-    if (i > 0) load(i);
+    for (int i2 = 0; i2 < p.steps; i2 += 2 * kRopeBatch) {
 #pragma unroll
-    for (int u = 0; u < kRopeBatch; ++u) {
-        if (i + u >= p.steps) break;
-        const int h = h0 + (i + u) * HPW;
-        const bool live = h < heads, is_v = h >= p.H + p.NKV, is_q = h < p.H;
-        uint2 out1 = lo[u], out2 = hi[u];
-        if ((chunk * p.steps + i + u) * HPW < p.H + p.NKV) {  // the same for the whole warp
-            float2 a[2], b[2], w1[2], w2[2];
-            unpack(lo[u], a), unpack(hi[u], b);
-            unpack(is_q ? qw1 : kw1, w1), unpack(is_q ? qw2 : kw2, w2);
-            float2 sq = mul2(a[0], a[0]);
-            sq = fma2(a[1], a[1], sq), sq = fma2(b[0], b[0], sq), sq = fma2(b[1], b[1], sq);
-            float ssq = sq.x + sq.y;
+        for (int z = 0; z < 2; ++z) {
+            const int i = i2 + z * kRopeBatch;
+            if (i >= p.steps) break;
+            load(i + kRopeBatch, 1 - z);
 #pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
-            const float r = rsqrtf(ssq * (1.0f / D) + p.eps);
-            const float2 r2 = make_float2(r, r);
-            float2 y1[2], y2[2];
+            for (int u = 0; u < kRopeBatch; ++u) {
+                if (i + u >= p.steps) break;
+                const int h = h0 + (i + u) * HPW;
+                const bool live = h < heads, is_v = h >= p.H + p.NKV, is_q = h < p.H;
+                uint2 out1 = lo[z][u], out2 = hi[z][u];
+                if ((chunk * p.steps + i + u) * HPW < p.H + p.NKV) {  // the same for the whole warp
+                    float2 a[2], b[2], w1[2], w2[2];
+                    unpack(lo[z][u], a), unpack(hi[z][u], b);
+                    unpack(is_q ? qw1 : kw1, w1), unpack(is_q ? qw2 : kw2, w2);
+                    float2 sq = mul2(a[0], a[0]);
+                    sq = fma2(a[1], a[1], sq), sq = fma2(b[0], b[0], sq), sq = fma2(b[1], b[1], sq);
+                    float ssq = sq.x + sq.y;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float2 n1 = mul2(mul2(a[e], r2), w1[e]), n2 = mul2(mul2(b[e], r2), w2[e]);
-                y1[e] = add2(mul2(n1, c1[e]), mul2(n2, s1[e]));
-                y2[e] = add2(mul2(n2, c2[e]), mul2(n1, s2[e]));
+                    for (int o = LPH / 2; o > 0; o >>= 1) ssq += __shfl_xor_sync(0xffffffffu, ssq, o);
+                    const float r = rsqrtf(ssq * (1.0f / D) + p.eps);
+                    const float2 r2 = make_float2(r, r);
+                    float2 y1[2], y2[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float2 n1 = mul2(mul2(a[e], r2), w1[e]), n2 = mul2(mul2(b[e], r2), w2[e]);
+                        y1[e] = add2(mul2(n1, c1[e]), mul2(n2, s1[e]));
+                        y2[e] = add2(mul2(n2, c2[e]), mul2(n1, s2[e]));
+                    }
+                    if (!is_v) {
+                        out1 = make_uint2(pack_bf16(y1[0].x, y1[0].y), pack_bf16(y1[1].x, y1[1].y));
+                        out2 = make_uint2(pack_bf16(y2[0].x, y2[0].y), pack_bf16(y2[1].x, y2[1].y));
+                    }
+                }
+                bf16* dst = q_row + (long long)h * D;
+                if (!is_q) {
+                    const long long row = kv_row + ((long long)(h - p.H - (is_v ? p.NKV : 0)) << p.page_shift);
+                    dst = (is_v ? p.V : p.K) + row * D + f0;
+                }
+                if (live && (is_q || cached)) {
+                    *reinterpret_cast<uint2*>(dst) = out1;
+                    *reinterpret_cast<uint2*>(dst + D / 2) = out2;
+                }
             }
-            if (!is_v) {
-                out1 = make_uint2(pack_bf16(y1[0].x, y1[0].y), pack_bf16(y1[1].x, y1[1].y));
-                out2 = make_uint2(pack_bf16(y2[0].x, y2[0].y), pack_bf16(y2[1].x, y2[1].y));
-            }
         }
-        bf16* dst = q_row + (long long)h * D;
-        if (!is_q) {
-            const long long row = kv_row + ((long long)(h - p.H - (is_v ? p.NKV : 0)) << p.page_shift);
-            dst = (is_v ? p.V : p.K) + row * D + f0;
-        }
-        if (live && (is_q || cached)) {
-            *reinterpret_cast<uint2*>(dst) = out1;
-            *reinterpret_cast<uint2*>(dst + D / 2) = out2;
-        }
-    }
     }
 }
 
