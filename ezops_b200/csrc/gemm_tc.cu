@@ -347,10 +347,11 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                     const int n_own = tile * p.units + row;
                     const bool own = row < p.units && n_own < p.N && !*abort_flag;
                     const float bias = p.bias && own ? __bfloat162float(p.bias[n_own]) : 0.f;
-#pragma unroll 1
+#pragma unroll 2
                     for (int c = 0; c < HC; c += 8) {
                         if (b_half + c >= B) break;
                         float v[8], r8[8];
+                        const long long o0 = (long long)(row0 + b_half + c) * p.ldout + n_own;
                         tmem_ld8(t_addr + (uint32_t)c, v);
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
@@ -365,9 +366,8 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap mapW0, const __grid_constant_
                         for (int e = 0; e < 8; ++e) {
                             if (own && b_half + c + e < B) {
                                 const float x = v[e] + r8[e];
-                                const long long o = (long long)(row0 + b_half + c + e) * p.ldout + n_own;
-                                if (p.out_f32) static_cast<float*>(p.out)[o] = x;
-                                else static_cast<bf16*>(p.out)[o] = __float2bfloat16_rn(x);
+                                if (p.out_f32) static_cast<float*>(p.out)[o0 + e * p.ldout] = x;
+                                else static_cast<bf16*>(p.out)[o0 + e * p.ldout] = __float2bfloat16_rn(x);
                             }
                         }
                         __syncwarp();

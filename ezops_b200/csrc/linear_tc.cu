@@ -25,7 +25,7 @@
 // error is 4.8e-7 for any K (1.4e-5 at K = 12800 otherwise), and 8192 x 4096, K = 4096 takes 193 us instead of 191.  Rounded to
 // bf16 that error does not show.
 // Few rows or few results (linear_in_groups): the kernel of the batched decode projections (gemm_tc.cu) with this epilogue
-// (17 x 6144, K = 4096: 10.5 us, 4.8 TB/s; 64 x 151936, K = 1024 to fp32: 58 us, 6.0 TB/s).
+// (17 x 6144, K = 4096: 10.4 us, 4.9 TB/s; 64 x 151936, K = 1024 to fp32: 57 us, 6.1 TB/s).
 #include <atomic>
 
 #include "prompt.h"
