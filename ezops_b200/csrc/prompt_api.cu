@@ -44,8 +44,14 @@ T from_word(long long w) {
         return f;
     } else return static_cast<T>(w);
 }
+template <class T>
+bool holds(long long w) {  // whether an argument of this type keeps the whole word (a float is its low 32 bits)
+    if constexpr (std::is_same_v<T, int>) return w == static_cast<int>(w);
+    else return true;
+}
 template <class... A, size_t... I>
 int call_words(int (*f)(A...), const long long* w, std::index_sequence<I...>) {
+    EZB_REQUIRE_SHAPE((holds<A>(w[I]) && ...), "a size does not fit in 32 bits");
     return f(from_word<A>(w[I])...);
 }
 template <class... A>

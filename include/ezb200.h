@@ -409,7 +409,8 @@ int ezb_attn_prompt(const void* Q, long long ldq, const void* K_pool, const void
                     int D, int max_pages, int page_size, int num_pages, ezb_stream_t stream);
 
 /* The four calls above with their arguments, in their order, as 64-bit words (pointers, sizes, a float as
- * its bits): for bindings to which every argument costs (Python's ctypes 2 us a call). */
+ * its bits): for bindings to which every argument costs (Python's ctypes 2 us a call).  A size
+ * that does not fit in 32 bits is refused (EZB_ERR_UNSUPPORTED_SHAPE). */
 int ezb_paged_plan_packed(const long long* words);
 int ezb_paged_qk_norm_rope_packed(const long long* words);
 int ezb_linear_bf16_packed(const long long* words);

@@ -201,3 +201,19 @@ def test_packed_entries_are_the_same_calls():
     assert b"128 query" in same("ezb_attn_prompt", p, 1 << 40, p, p, p, p, p, p, 1 << 41, p, 1 << 33, 1, 1, 129, 1, 64, 1, 64, 1, None)
     assert b"apart" in same("ezb_paged_qk_norm_rope", p, 8, None, None, *[p] * 7, 1, 8, 8, 64, 16, 1, p, 0, 64, 1, 1e-6, None)
     assert lib.ezb_attn_prompt_packed(None) == lib.ezb_paged_plan(*[None] * 10, 2, 8, 4, 64, 8, 8, None)
+
+
+@pytest.mark.parametrize("name", ["ezb_paged_plan", "ezb_paged_qk_norm_rope", "ezb_linear_bf16", "ezb_attn_prompt"])
+def test_packed_sizes_beyond_32_bits_are_refused(name):
+    """A size that a 32-bit argument cannot hold is refused; cut off, 2**32 + 8 would be a call for 8."""
+    import struct
+
+    lib, kinds = _lib.load(), _lib.SIGNATURES[name][1]
+    sizes = [i for i, kind in enumerate(kinds) if kind is ctypes.c_int]
+    assert len(sizes) >= 5
+    for at in sizes:
+        for size in (1 << 31, (1 << 32) + 8, (1 << 62) + 64, -(1 << 31) - 1):
+            words = [8 if kind is ctypes.c_int else 0 for kind in kinds]
+            words[at] = size
+            assert getattr(lib, name + "_packed")(struct.pack(f"{len(words)}q", *words)) == _lib.EZB_ERR_UNSUPPORTED_SHAPE
+            assert b"32 bits" in lib.ezb_last_error_message()
