@@ -160,10 +160,16 @@ def get_tuning(key: str) -> int:
     return load().ezb_get_tuning(TUNE[key])
 
 
+faults_read = 0  # faults that device_status() has read: the prompt operators then start from cleared workspaces
+
+
 def device_status(clear: bool = True) -> int:
     """Synchronise the current device and return its status word (0 = healthy)."""
+    global faults_read
     word = c_uint(0)
     rc = load().ezb_device_status(ctypes.byref(word), 1 if clear else 0)
     if rc not in (EZB_OK, EZB_ERR_DEVICE_FAULT):
         check(rc)
+    if word.value:
+        faults_read += 1
     return int(word.value)

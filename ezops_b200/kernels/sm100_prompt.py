@@ -76,12 +76,15 @@ class _Workspaces:
     """The workspaces of one operator: one per device and stream, and one per stream of a graph capture, so that neither calls on
     several streams nor graphs that are replayed side by side meet in one.  A captured call never uses an eager one's, nor the
     other way round: the counters in front (all that has to be zero) are cleared where the memory is first used, in a graph
-    once per replay.  A capture's are dropped when the next one begins: they lie in its graph's own pool."""
+    once per replay.  A capture's are dropped when the next one begins: they lie in its graph's own pool.
+
+    A call that gives up a wait leaves its counters half counted.  Once ``_lib.device_status`` has read a fault (any: the word
+    keeps the first one only), the eager workspaces are dropped, and calls go on with cleared ones."""
 
     _COUNTERS = 4096
 
     def __init__(self, lib):
-        self._lib, self._eager, self._captured, self._capture = lib, {}, {}, 0
+        self._lib, self._eager, self._captured, self._capture, self._faults = lib, {}, {}, 0, _lib.faults_read
 
     def get(self, nbytes: int, device: int, stream: int):
         held = self._eager
@@ -90,6 +93,9 @@ class _Workspaces:
             if capture != self._capture:
                 self._capture, self._captured = capture, {}
             held = self._captured
+        elif self._faults != _lib.faults_read:
+            self._faults = _lib.faults_read
+            held.clear()
         ws = held.get((device, stream))
         if ws is None:
             ws = held[device, stream] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))

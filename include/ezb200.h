@@ -398,8 +398,8 @@ int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bia
  * cu_tokens is cut to [0, T], seq_lens to [0, max_pages * page_size].  Equal calls
  * give equal bits; where a row's sums are cut may depend on the other rows.
  * The workspace depends on D only; as everywhere it is zero-filled once and serves one
- * stream at a time; after a recorded wait that ran out (0x1xx) it has to be zero-filled
- * again.  D in {64, 128}; H / NKV <= 128; page_size a power of two >= 64. */
+ * stream at a time; after a recorded wait that ran out (0x1xx) its first 4096 bytes have to
+ * be zero-filled again (the word keeps the first fault only: best after any).  D in {64, 128}; H / NKV <= 128; page_size a power of two >= 64. */
 size_t ezb_attn_prompt_workspace_bytes(int D);
 /* Identity of the graph capture that `stream` takes part in, 0 when there is none: a
  * binding that keeps workspaces gives a captured call one of its capture's. */

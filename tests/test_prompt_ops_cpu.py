@@ -217,3 +217,50 @@ def test_packed_sizes_beyond_32_bits_are_refused(name):
             words[at] = size
             assert getattr(lib, name + "_packed")(struct.pack(f"{len(words)}q", *words)) == _lib.EZB_ERR_UNSUPPORTED_SHAPE
             assert b"32 bits" in lib.ezb_last_error_message()
+
+
+class _FaultyLib:
+    """A library whose status word reads ``word`` once (cleared by the read)."""
+
+    def __init__(self, word):
+        self.word = word
+
+    def ezb_device_status(self, out, clear):
+        out._obj.value, word = self.word, self.word
+        self.word = 0 if clear else self.word
+        return _lib.EZB_ERR_DEVICE_FAULT if word else _lib.EZB_OK
+
+    def ezb_stream_capture_id(self, stream):
+        return 0
+
+
+@pytest.fixture
+def host_workspaces(monkeypatch):
+    """``_Workspaces`` on the host: its tensors come from there, and nothing is being captured."""
+    from ezops_b200.kernels import sm100_prompt
+
+    empty = torch.empty
+    monkeypatch.setattr(sm100_prompt, "_capturing", lambda: False)
+    monkeypatch.setattr(sm100_prompt.torch, "empty", lambda n, dtype, device: empty(n, dtype=dtype).fill_(9))
+    return sm100_prompt._Workspaces
+
+
+@pytest.mark.parametrize("word", [0x105, 0x302])
+def test_workspaces_are_renewed_after_a_recorded_fault(monkeypatch, host_workspaces, word):
+    """A call that gave up leaves its counters half counted; reading the fault has every operator start from cleared ones.  Any
+    fault does: the word keeps the first one only."""
+    lib = _FaultyLib(0)
+    monkeypatch.setattr(_lib, "_lib", lib)
+    spaces = [host_workspaces(lib) for _ in range(2)]
+    before = [s.get(8192, 0, stream) for s in spaces for stream in (1, 2)]
+    for ws in before:
+        assert (ws[:4096] == 0).all()
+        ws[:4096] = 3  # what a call that gave up leaves
+    assert _lib.device_status() == 0
+    assert all(s.get(8192, 0, stream) is before[2 * i + stream - 1] for i, s in enumerate(spaces) for stream in (1, 2))
+    lib.word = word
+    assert _lib.device_status() == word
+    for s in spaces:
+        for stream in (1, 2):
+            ws = s.get(8192, 0, stream)
+            assert (ws[:4096] == 0).all() and ws is s.get(8192, 0, stream)
