@@ -82,6 +82,7 @@ class _Workspaces:
     keeps the first one only), the eager workspaces are dropped, and calls go on with cleared ones."""
 
     _COUNTERS = 4096
+    _STREAMS = 8  # eager ones that are kept: of more streams the oldest one's goes (its memory is reused behind its stream's work)
 
     def __init__(self, lib):
         self._lib, self._eager, self._captured, self._capture, self._faults = lib, {}, {}, 0, _lib.faults_read
@@ -98,6 +99,8 @@ class _Workspaces:
             held.clear()
         ws = held.get((device, stream))
         if ws is None:
+            if held is self._eager and len(held) >= self._STREAMS:
+                held.pop(list(held)[0], None)
             ws = held[device, stream] = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
             ws[: self._COUNTERS].zero_()
         return ws

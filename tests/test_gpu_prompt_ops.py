@@ -709,3 +709,17 @@ def test_attn_goes_on_after_a_recorded_fault():
     other(*args[:3], bad, *args[4:])
     assert _lib.device_status() == 0x302
     assert torch.equal(op(*args), want) and torch.equal(op(*args), want)
+
+
+def test_attn_on_more_streams_than_workspaces():
+    op, args = attn_rows(2, 128, 4)
+    want = op(*args)
+    streams = [torch.cuda.Stream() for _ in range(12)]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(op(*args))
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, want) for r in results) and len(op._kernel._spaces._eager) <= 8

@@ -264,3 +264,15 @@ def test_workspaces_are_renewed_after_a_recorded_fault(monkeypatch, host_workspa
         for stream in (1, 2):
             ws = s.get(8192, 0, stream)
             assert (ws[:4096] == 0).all() and ws is s.get(8192, 0, stream)
+
+
+def test_workspaces_of_many_streams_do_not_pile_up(host_workspaces):
+    spaces = host_workspaces(_FaultyLib(0))
+    kept = spaces.get(8192, 0, 0)
+    for stream in range(1, 8):
+        spaces.get(8192, 0, stream)
+    assert spaces.get(8192, 0, 0) is kept
+    for stream in range(8, 500):
+        ws = spaces.get(8192, stream % 2, stream)
+        assert ws is spaces.get(8192, stream % 2, stream) and (ws[:4096] == 0).all()
+        assert len(spaces._eager) <= 8
