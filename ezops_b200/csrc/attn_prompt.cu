@@ -340,6 +340,13 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
     if (tid == 32) {
         prefetch_map(&mapQ), prefetch_map(&mapK), prefetch_map(&mapV);
     }
+    // The tensor memory is taken before the next kernel may start: one that came to this SM first would hold some of it while it
+    // waits for this kernel.
+    if (warp == 9) {
+        tmem_alloc(smem_u32(&t.tmem), 512);
+        tmem_relinquish();
+    }
+    __syncthreads();
     pdl_open(1);
 
     // ---- where this CTA's share starts: running sums of the rows' costs, rows spread over the threads
@@ -409,10 +416,6 @@ attn_prompt_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_consta
             }
             base += sum;
         }
-    }
-    if (warp == 9) {
-        tmem_alloc(smem_u32(&t.tmem), 512);
-        tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
