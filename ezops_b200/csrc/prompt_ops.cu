@@ -25,15 +25,16 @@ struct PlanParams {
     int B, T, max_pages, page_shift, num_pages, free_size;
 };
 
-// Exclusive running sum over the block's threads; the total in `total`.  Sums are cut at `cap` (no overflow: every
-// value is at most cap <= 2^30).
+// a + b, cut at cap.  All three lie between 0 and 2^30, so that the sum may reach 2^31: one more than an int holds.
+__device__ __forceinline__ int cut_add(int a, int b, int cap) { return (int)min((unsigned)a + (unsigned)b, (unsigned)cap); }
+// Exclusive running sum over the block's threads; the total in `total`.  Sums are cut at `cap`, and every value is at most that.
 __device__ __forceinline__ int block_prefix(int v, int cap, int* warp_sums, int& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s = min(s + up, cap);
+        if (lane >= o) s = cut_add(s, up, cap);
     }
     __syncthreads();  // warp_sums may still be read from the sum before
     if (lane == 31) warp_sums[warp] = s;
@@ -42,12 +43,12 @@ __device__ __forceinline__ int block_prefix(int v, int cap, int* warp_sums, int&
 #pragma unroll
     for (int w = 0; w < kPlanThreads / 32; ++w) {
         if (w == warp) before = all;
-        all = min(all + warp_sums[w], cap);
+        all = cut_add(all, warp_sums[w], cap);
     }
     total = all;
     int up = __shfl_up_sync(0xffffffffu, s, 1);
     if (lane == 0) up = 0;
-    return min(before + up, cap);
+    return cut_add(before, up, cap);
 }
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanParams p) {
@@ -63,17 +64,18 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     const int count = min(__ldg(p.free_count), p.free_size);
     auto cached = [&](int b) { return min(max(__ldg(p.ctx + b), 0), cap); };
     auto held = [&](int c) { return (int)(((long long)c + page - 1) >> p.page_shift); };
+    auto fresh = [&](int b) { return min(max(__ldg(p.fresh + b), 0), p.T); };
 
     int sum = 0, total = 0;
-    for (int b = b0; b < b1; ++b) sum = min(sum + min(max(__ldg(p.fresh + b), 0), p.T), p.T);
+    for (int b = b0; b < b1; ++b) sum = cut_add(sum, fresh(b), p.T);
     int at = block_prefix(sum, p.T, warp_sums, total);
     if (tid == 0) cu[p.B] = total;
     sum = 0;
     for (int b = b0; b < b1; ++b) {
         cu[b] = at;
-        const int next = min(at + min(max(__ldg(p.fresh + b), 0), p.T), p.T), c = cached(b);
+        const int next = cut_add(at, fresh(b), p.T), c = cached(b);
         base[b] = sum;  // completed below
-        sum += held(min(c + next - at, cap)) - held(c);
+        sum += held(cut_add(c, next - at, cap)) - held(c);
         at = next;
     }
     int pages = 0;
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     if (blockIdx.x == 0) {
         for (int b = tid; b <= p.B; b += kPlanThreads) {
             p.cu[b] = cu[b];
-            if (b < p.B) p.lens[b] = min(cached(b) + cu[b + 1] - cu[b], cap);
+            if (b < p.B) p.lens[b] = cut_add(cached(b), cu[b + 1] - cu[b], cap);
         }
         if (tid == 0) *p.free_left = count - pages;
     }
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PlanPara
     for (int b = blockIdx.x * (kPlanThreads / 32) + (tid >> 5); b < p.B; b += gridDim.x * (kPlanThreads / 32)) {
         const int n = cu[b + 1] - cu[b];
         if (n == 0) continue;
-        const int c = cached(b), h = held(c), need = held(min(c + n, cap));
+        const int c = cached(b), h = held(c), need = held(cut_add(c, n, cap));
         for (int j = h + (tid & 31); j < need; j += 32) p.table[(long long)b * p.max_pages + j] = new_page(base[b] + j - h);
     }
     for (int t = blockIdx.x * kPlanTokens + tid; t < min((blockIdx.x + 1) * kPlanTokens, p.T); t += kPlanThreads) {

@@ -723,3 +723,34 @@ def test_attn_on_more_streams_than_workspaces():
                 results.append(op(*args))
     torch.cuda.synchronize()
     assert all(torch.equal(r, want) for r in results) and len(op._kernel._spaces._eager) <= 8
+
+
+@pytest.mark.parametrize("ctx,new,cu,lens", [([0, 0], [2**30, 2**30], [0, 2**30, 2**30], [2**30, 0]),
+                                             ([2**30, 5], [2**30, 7], [0, 2**30, 2**30], [2**30, 5]),
+                                             ([2**29, 0], [2**29, 2**30], [0, 2**29, 2**30], [2**30, 2**29])])
+def test_plan_of_the_largest_sizes(ctx, new, cu, lens):
+    """2^30 token slots, rows of 2^30 positions: sums of two such numbers do not fit in 32 bits."""
+    page, pages, T = 1 << 20, 1024, 1 << 30
+    op = ez.PagedPlanOp(2, T, pages, page, pages, backend="cuda")
+    table = (torch.arange(2 * pages, dtype=I32, device=DEV) % pages).view(2, pages)  # (the rows share pages)
+    free = (torch.arange(2 * pages, dtype=I32, device=DEV) % pages).flip(0).contiguous()  # taken in the order of their numbers
+    held = [-(-c // page) for c in ctx]
+    first = free.numel()
+    plan = op(ints(*ctx), ints(*new), table, free, ints(first))
+    assert plan.cu_tokens.tolist() == cu and plan.seq_lens.tolist() == lens
+    need = [-(-n // page) for n in lens]
+    assert int(plan.free_count) == first - sum(need) + sum(held)
+    taken = 0
+    for b in range(2):
+        for j in (held[b], need[b] - 1):
+            if held[b] <= j < need[b]:
+                assert int(table[b, j]) == (taken + j - held[b]) % pages
+        taken += need[b] - held[b]
+        lo, hi = cu[b], cu[b + 1]
+        for at in range(lo, hi, 1 << 28):
+            pos = torch.arange(ctx[b] + at - lo, ctx[b] + min(at + (1 << 28), hi) - lo, device=DEV)
+            part = slice(at, at + pos.numel())
+            assert torch.equal(plan.positions[part].long(), pos)
+            slot = table[b].long()[(pos // page).clamp(max=pages - 1)] * page + pos % page
+            assert torch.equal(plan.slots[part].long(), torch.where(pos < pages * page, slot, -1))
+    assert (plan.positions[cu[2] :] == -1).all() and (plan.slots[cu[2] :] == -1).all()
