@@ -30,6 +30,18 @@ bool overlap(const Rect& a, const Rect& b) {
     const long long off = ((pb - pa) % a.ld + a.ld) % a.ld;
     return off < a.width || off + b.width > a.ld;
 }
+Rect span(const void* base, long long bytes) { return {base, 1, bytes, bytes}; }
+// Whether any of the arrays that a call writes meets another of them, or one that it only reads (null: not there).
+template <size_t W, size_t R>
+bool any_overlap(const Rect (&writes)[W], const Rect (&reads)[R]) {
+    for (size_t i = 0; i < W; ++i) {
+        for (size_t j = 0; j < i; ++j)
+            if (overlap(writes[i], writes[j])) return true;
+        for (const Rect& r : reads)
+            if (r.base && overlap(writes[i], r)) return true;
+    }
+    return false;
+}
 
 constexpr int kMost = 1 << 30;  // sizes, positions and slots are 32-bit on the device
 
@@ -74,18 +86,10 @@ int ezb_paged_plan(const int* ctx_lens, const int* new_lens, int* page_table, co
     EZB_REQUIRE_SHAPE(B <= kPlanMaxRows, "at most 8192 rows");
     EZB_REQUIRE_SHAPE(max_tokens <= kMost && (long long)max_pages * page_size <= kMost && (long long)num_pages * page_size <= kMost,
                       "max_tokens, max_pages * page_size and num_pages * page_size are limited to 2^30");
-    const Rect in[5] = {{ctx_lens, 1, 0, 4ll * B}, {new_lens, 1, 0, 4ll * B}, {free_pages, 1, 0, 4ll * free_size}, {free_count, 1, 0, 4},
-                        {page_table, 1, 0, 4ll * B * max_pages}};
-    const Rect out[5] = {{seq_lens, 1, 0, 4ll * B}, {cu_tokens, 1, 0, 4ll * (B + 1)}, {positions, 1, 0, 4ll * max_tokens},
-                         {slots, 1, 0, 4ll * max_tokens}, {free_left, 1, 0, 4}};
-    for (const Rect& o : out) {
-        // single rows: byte ranges
-        const uintptr_t a = reinterpret_cast<uintptr_t>(o.base);
-        for (const Rect& i : in) {
-            const uintptr_t b = reinterpret_cast<uintptr_t>(i.base);
-            EZB_REQUIRE(a + o.width <= b || b + i.width <= a, "an output overlaps an input (results go to tensors of their own)");
-        }
-    }
+    const Rect writes[] = {span(page_table, 4ll * B * max_pages), span(seq_lens, 4ll * B), span(cu_tokens, 4ll * (B + 1)),
+                           span(positions, 4ll * max_tokens), span(slots, 4ll * max_tokens), span(free_left, 4)};
+    const Rect reads[] = {span(ctx_lens, 4ll * B), span(new_lens, 4ll * B), span(free_pages, 4ll * free_size), span(free_count, 4)};
+    EZB_REQUIRE(!any_overlap(writes, reads), "an output overlaps an input or another output (results go to tensors of their own)");
     PlanArgs p;
     p.ctx_lens = ctx_lens, p.new_lens = new_lens, p.free_pages = free_pages, p.free_count = free_count, p.page_table = page_table;
     p.seq_lens = seq_lens, p.cu_tokens = cu_tokens, p.positions = positions, p.slots = slots, p.free_left = free_left;
@@ -122,7 +126,11 @@ int ezb_paged_qk_norm_rope(const void* qkv, long long ldqkv, const void* qw_or_n
                               "interleaved sections do not fit: axis a takes the frequencies a, a + axes, ...");
     }
     EZB_REQUIRE_SHAPE(sum == half, "the sections must add up to head_dim / 2");
-    EZB_REQUIRE(!overlap({qkv, T, ldqkv * 2, width * 2}, {q_out, T, (long long)H * D * 2, (long long)H * D * 2}), "q_out overlaps qkv");
+    const long long pool = (long long)num_pages * NKV * page_size * D * 2, table = (long long)table_rows * D * 2;
+    const Rect writes[] = {{q_out, T, (long long)H * D * 2, (long long)H * D * 2}, span(K_pool, pool), span(V_pool, pool)};
+    const Rect reads[] = {{qkv, T, ldqkv * 2, width * 2}, span(qw_or_null, D * 2), span(kw_or_null, D * 2), span(cos, table), span(sin, table),
+                          span(positions, 4ll * axes * T), span(slots, 4ll * T)};
+    EZB_REQUIRE(!any_overlap(writes, reads), "q_out, K_pool and V_pool must not overlap each other or an input");
     unsigned char axis[64];
     for (int i = 0, a = 0, left = sections_host[0]; i < half; ++i) {
         if (interleaved) {
@@ -195,11 +203,15 @@ int ezb_attn_prompt(const void* Q, long long ldq, const void* K_pool, const void
     const long long width = (long long)H * D;
     EZB_REQUIRE(ldq >= width && ldq % 8 == 0 && ldo >= width && ldo % 8 == 0, "rows of Q and Out must be at least H * D elements apart, a multiple of 8");
     EZB_REQUIRE(aligned16(Q) && aligned16(K_pool) && aligned16(V_pool) && aligned16(Out), "Q, Out and the page pools must be 16-byte aligned");
-    EZB_REQUIRE(!overlap({Q, T, ldq * 2, width * 2}, {Out, T, ldo * 2, width * 2}), "Out overlaps Q");
     if (!workspace || !aligned16(workspace) || workspace_bytes < attn_prompt_workspace_bytes(D)) {
         set_last_message("workspace missing, misaligned or smaller than ezb_attn_prompt_workspace_bytes()");
         return EZB_ERR_WORKSPACE;
     }
+    const long long pool = (long long)num_pages * NKV * page_size * D * 2;
+    const Rect writes[] = {{Out, T, ldo * 2, width * 2}, span(workspace, (long long)attn_prompt_workspace_bytes(D))};
+    const Rect reads[] = {{Q, T, ldq * 2, width * 2}, span(K_pool, pool), span(V_pool, pool), span(page_table, 4ll * B * max_pages),
+                          span(seq_lens, 4ll * B), span(cu_tokens, 4ll * (B + 1))};
+    EZB_REQUIRE(!any_overlap(writes, reads), "Out or the workspace overlaps an input, or each other");
     AttnPromptArgs a;
     a.Q = static_cast<const bf16*>(Q), a.K = static_cast<const bf16*>(K_pool), a.V = static_cast<const bf16*>(V_pool);
     a.Out = static_cast<bf16*>(Out), a.ldq = ldq, a.ldo = ldo;

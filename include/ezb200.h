@@ -343,8 +343,8 @@ int ezb_qwen3_decode_stack_paged(const void* hidden, void* out, const ezb_layer_
  *                             and slots are then -1
  * Tokens beyond max_tokens are dropped (cu_tokens stops there); a token beyond the
  * max_pages * page_size positions of its row gets slot -1, and seq_lens stops
- * there; an id outside [0, num_pages) is written and used as -1.  Outputs must not
- * overlap inputs.  B <= 8192. */
+ * there; an id outside [0, num_pages) is written and used as -1.  Outputs (page_table among
+ * them) must not overlap inputs or each other.  B <= 8192. */
 int ezb_paged_plan(const int* ctx_lens, const int* new_lens, int* page_table, const int* free_pages, const int* free_count,
                    int* seq_lens, int* cu_tokens, int* positions, int* slots, int* free_left, int B, int max_tokens, int max_pages,
                    int page_size, int num_pages, int free_size, ezb_stream_t stream);
@@ -362,8 +362,8 @@ int ezb_paged_plan(const int* ctx_lens, const int* new_lens, int* page_table, co
  * A token with a negative position is padding: nothing is written for it.  A
  * negative slot writes q only.  A position behind the tables (fault 0x301, nothing
  * written) or a slot behind the pools (fault 0x303, q only) is recorded in the
- * status word.  Two tokens with one slot leave either's k and v there.
- * D in {64, 128}. */
+ * status word.  Two tokens with one slot leave either's k and v there, head by
+ * head.  q_out, K_pool and V_pool must not overlap each other or an input.  D in {64, 128}. */
 int ezb_paged_qk_norm_rope(const void* qkv, long long ldqkv, const void* qw_or_null, const void* kw_or_null, const void* cos,
                            const void* sin, const int* positions, const int* slots, void* K_pool, void* V_pool, void* q_out, int T,
                            int H, int NKV, int D, int table_rows, int axes, const int* sections_host, int interleaved, int page_size,
@@ -397,6 +397,7 @@ int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bia
  * outside [0, num_pages) inside a row's length read as zeros and record fault 0x302.
  * cu_tokens is cut to [0, T], seq_lens to [0, max_pages * page_size].  Equal calls
  * give equal bits; where a row's sums are cut may depend on the other rows.
+ * Out and the workspace must not overlap each other or an input.
  * The workspace depends on D only; as everywhere it is zero-filled once and serves one
  * stream at a time; after a recorded wait that ran out (0x1xx) its first 4096 bytes have to
  * be zero-filled again (the word keeps the first fault only: best after any).  D in {64, 128}; H / NKV <= 128; page_size a power of two >= 64. */

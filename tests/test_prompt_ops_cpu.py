@@ -276,3 +276,55 @@ def test_workspaces_of_many_streams_do_not_pile_up(host_workspaces):
         ws = spaces.get(8192, stream % 2, stream)
         assert ws is spaces.get(8192, stream % 2, stream) and (ws[:4096] == 0).all()
         assert len(spaces._eager) <= 8
+
+
+def _spans(**at):
+    """Addresses of a call's arrays, far apart, but for those given."""
+    names = ("ctx", "new", "table", "free", "count", "lens", "cu", "positions", "slots", "left", "qkv", "qw", "kw", "cos", "sin", "K", "V",
+             "Q", "out", "ws")
+    return {name: at.get(name, 0x1000000 * (i + 1)) for i, name in enumerate(names)}
+
+
+def test_results_that_overlap_are_refused():
+    """Whatever a call writes has to lie apart from all else that it reads or writes."""
+    lib, bad = _lib.load(), _lib.EZB_ERR_INVALID_ARGUMENT
+
+    def refused(code, what):
+        assert code == bad, what
+        assert b"overlap" in lib.ezb_last_error_message(), (what, lib.ezb_last_error_message())
+
+    def plan(**at):
+        a = _spans(**at)
+        return lib.ezb_paged_plan(*[a[n] for n in ("ctx", "new", "table", "free", "count", "lens", "cu", "positions", "slots", "left")],
+                                  4, 100, 8, 64, 32, 40, None)
+
+    base = _spans()
+    writes, reads = ("table", "lens", "cu", "positions", "slots", "left"), ("ctx", "new", "free", "count")
+    for w in writes:
+        for other in (*writes, *reads):
+            if w != other:
+                refused(plan(**{w: base[other]}), (w, other))
+    refused(plan(lens=base["cu"] + 16), "last entry of cu")
+    refused(plan(free=base["table"] + 4 * 31), "last entry of the table")
+
+    def rope(**at):
+        a, sections = _spans(**at), (ctypes.c_int * 1)(32)
+        return lib.ezb_paged_qk_norm_rope(a["qkv"], 520, a["qw"], a["kw"], a["cos"], a["sin"], a["positions"], a["slots"], a["K"], a["V"],
+                                          a["out"], 4, 4, 2, 64, 10, 1, sections, 0, 64, 3, 1e-6, None)
+
+    for w in ("K", "V", "out"):
+        for other in ("qkv", "qw", "kw", "cos", "sin", "positions", "slots", "K", "V", "out"):
+            if w != other:
+                refused(rope(**{w: base[other]}), (w, other))
+    refused(rope(V=base["K"] + 2 * (3 * 2 * 64 * 64 - 8)), "end of K")
+
+    def attn(**at):
+        a = _spans(**at)
+        return lib.ezb_attn_prompt(a["Q"], 256, a["K"], a["V"], a["table"], a["lens"], a["cu"], a["out"], 256, a["ws"], 1 << 25, 2, 8, 4, 2,
+                                   64, 4, 64, 9, None)
+
+    for other in ("Q", "K", "V", "table", "lens", "cu", "ws"):
+        refused(attn(out=base[other]), ("out", other))
+        if other != "ws":
+            refused(attn(ws=base[other]), ("ws", other))
+    refused(attn(out=base["ws"] + 512), "inside the workspace")
