@@ -37,8 +37,9 @@ def _device(t: torch.Tensor, name: str) -> int:
     return _current_device()
 
 
-def _refuse(checks, device: int):
-    """Raises for the first of ``checks`` - (name, tensor, shape, dtype, rows may lie apart) - that does not hold."""
+def _refuse(checks, device: int, no_rows: bool = False):
+    """Raises for the first of ``checks`` - (name, tensor, shape, dtype, rows may lie apart) - that does not hold.  It returns when
+    all hold but for tensors that are empty because the call has ``no_rows``: then there is nothing to do."""
     for name, t, shape, dtype, apart in checks:
         if t is None:
             continue
@@ -50,7 +51,7 @@ def _refuse(checks, device: int):
             raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
         if tuple(t.shape) != tuple(shape):
             raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-        if t.numel() == 0:
+        if t.numel() == 0 and not no_rows:
             raise ValueError(f"{name} is empty")
         if not t.is_contiguous() and not (apart and t[0].is_contiguous()):
             raise ValueError(f"{name} must be contiguous" + (" within a row" if apart else ""))
@@ -167,7 +168,9 @@ class PagedQkNormRopeSm100Kernel(BaseKernel):
             _refuse([("qkv", qkv, row, _BF16, True), ("q_norm_w", q_norm_w, w, _BF16, False), ("k_norm_w", k_norm_w, w, _BF16, False),
                      ("cos", cos, table, _BF16, False), ("sin", sin, table, _BF16, False), ("positions", positions, where, _I32, False),
                      ("slots", slots, (T,), _I32, False), ("K_pool", K_pool, pool, _BF16, False), ("V_pool", V_pool, pool, _BF16, False),
-                     ("out", out, heads, _BF16, False)], dev)
+                     ("out", out, heads, _BF16, False)], dev, T == 0)
+            if T == 0:
+                return out
         rc = self._entry(self._pack(
             qkv.data_ptr(), _distance(qkv), _ptr(q_norm_w), _ptr(k_norm_w), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
             slots.data_ptr(), K_pool.data_ptr(), V_pool.data_ptr(), out.data_ptr(), T, *self._sizes, _raw_stream(dev)))
@@ -196,7 +199,9 @@ class LinearSm100Kernel(BaseKernel):
         if not (_rows(X, (M, K), _BF16, dev) and _whole(W, self._w, _BF16, dev) and (bias is None or _whole(bias, self._bias, _BF16, dev))
                 and (residual is None or _rows(residual, (M, N), _BF16, dev)) and _rows(out, (M, N), self.out_dtype, dev)):
             _refuse([("X", X, (M, K), _BF16, True), ("W", W, self._w, _BF16, False), ("bias", bias, self._bias, _BF16, False),
-                     ("residual", residual, (M, N), _BF16, True), ("out", out, (M, N), self.out_dtype, True)], dev)
+                     ("residual", residual, (M, N), _BF16, True), ("out", out, (M, N), self.out_dtype, True)], dev, M == 0)
+            if M == 0:
+                return out
         rc = self._entry(self._pack(
             X.data_ptr(), _distance(X), W.data_ptr(), _ptr(bias), _ptr(residual), N if residual is None else _distance(residual),
             out.data_ptr(), _distance(out), M, N, K, self.act, self._f32, _raw_stream(dev)))
@@ -228,7 +233,9 @@ class AttnPromptSm100Kernel(BaseKernel):
                 and _whole(cu_tokens, self._cu, _I32, dev) and _rows(out, heads, _BF16, dev)):
             _refuse([("Q", Q, heads, _BF16, True), ("K_pool", K_pool, pool, _BF16, False), ("V_pool", V_pool, pool, _BF16, False),
                      ("page_table", page_table, self._table, _I32, False), ("seq_lens", seq_lens, self._lens, _I32, False),
-                     ("cu_tokens", cu_tokens, self._cu, _I32, False), ("out", out, heads, _BF16, True)], dev)
+                     ("cu_tokens", cu_tokens, self._cu, _I32, False), ("out", out, heads, _BF16, True)], dev, T == 0)
+            if T == 0:
+                return out
         stream = _raw_stream(dev)
         ws = self._spaces.get(self._need, dev, stream)
         rc = self._entry(self._pack(

@@ -9,7 +9,7 @@ values are already in the pools as the last n_b of its ``seq_lens[b]`` keys.  Qu
 
 Q, out [T, H, D] bf16 (rows of one step behind each other, token rows may lie further apart); K_pool, V_pool [pages,
 NKV, page_size, D]; page_table [batch, max_pages], seq_lens [batch], cu_tokens [batch + 1] int32 - the tensors of a
-``PagedPlan``.  Rows of ``out`` behind ``cu_tokens[batch]`` are left as they were.  What the pools hold behind a row's last key
+``PagedPlan``.  Rows of ``out`` behind ``cu_tokens[batch]`` are left as they were; T may be 0.  What the pools hold behind a row's last key
 is never used.  Equal calls give equal bits; the order of a row's sums may depend on the other rows.
 """
 

@@ -19,7 +19,7 @@ equal positions on all axes give its result.
 A token with a negative position is padding (nothing is written for it), a token with a negative slot is not cached.
 Tensors (bf16 unless noted): qkv [T, (H+2*NKV)*D], rows may lie further apart; q_norm_w, k_norm_w [D] or None (unit);
 cos, sin [max_positions, D]; positions int32 [T] or [axes, T]; slots int32 [T]; K_pool, V_pool [num_pages, NKV,
-page_size, D].  Returns q_out [T, H, D].
+page_size, D].  Returns q_out [T, H, D]; T may be 0.
 """
 
 from __future__ import annotations

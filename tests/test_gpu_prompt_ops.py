@@ -754,3 +754,38 @@ def test_plan_of_the_largest_sizes(ctx, new, cu, lens):
             slot = table[b].long()[(pos // page).clamp(max=pages - 1)] * page + pos % page
             assert torch.equal(plan.slots[part].long(), torch.where(pos < pages * page, slot, -1))
     assert (plan.positions[cu[2] :] == -1).all() and (plan.slots[cu[2] :] == -1).all()
+
+
+def test_steps_without_tokens():
+    """No rows in, no rows out; nothing is written, and what would be refused otherwise still is."""
+    op = ez.LinearOp(4, 24, 64, backend="cuda", bias=True, residual=True, activation="swiglu")
+    X, W, b, r = op.gen_data()
+    out = op(X[:0], W, bias=b, residual=r[:0])
+    assert out.shape == (0, 24) and out.dtype == BF16 and out.is_cuda
+    given = torch.empty(0, 24, device=DEV, dtype=BF16)
+    assert op(X[:0], W, bias=b, residual=r[:0], out=given) is given
+    with pytest.raises(ValueError, match="W must have shape"):
+        op(X[:0], W[:5], bias=b, residual=r[:0])
+    with pytest.raises(ValueError, match="residual must have shape"):
+        op(X[:0], W, bias=b, residual=r)
+
+    for sections in (None, (12, 10, 10)):
+        op = ez.PagedQkNormRopeOp(4, 8, 64, 50, 64, 3, backend="cuda", num_kv_heads=2, sections=sections)
+        qkv, qw, kw, cos, sin, positions, slots, K, V = op.gen_data()
+        K0, V0 = K.clone(), V.clone()
+        out = op(qkv[:0], qw, kw, cos, sin, positions[:, :0].contiguous(), slots[:0], K, V)
+        assert out.shape == (0, 8, 64) and torch.equal(K, K0) and torch.equal(V, V0)
+        with pytest.raises(ValueError, match="slots must have shape"):
+            op(qkv[:0], qw, kw, cos, sin, positions[:, :0].contiguous(), slots, K, V)
+
+    Q, K, V, table, _, _ = attn_data([4], [0], 8, 2, 128, 64)
+    op = ez.AttnPromptOp(1, 4, 8, 128, table.shape[1], 64, backend="cuda", num_kv_heads=2)
+    out = op(Q[:0], K, V, table, ints(4), ints(0, 0))
+    assert out.shape == (0, 8, 128) and out.dtype == BF16
+    with pytest.raises(ValueError, match="page_table must have shape"):
+        op(Q[:0], K, V, table[:, :1].contiguous(), ints(4), ints(0, 0))
+    with pytest.raises(ValueError):
+        op(Q, K[:0], V[:0], table, ints(4), ints(0, 4))
+    with pytest.raises(ValueError, match="free_pages is empty"):
+        plan = ez.PagedPlanOp(1, 4, 2, 64, 4, backend="cuda")
+        plan(ints(0), ints(1), torch.zeros(1, 2, dtype=I32, device=DEV), ints(), ints(0))
