@@ -10,6 +10,9 @@ entered into the page table, and every token gets its position and its cache slo
     token t of row b:  position = ctx_lens[b] + t - cu_tokens[b]
                        slot = page_table[b, position // page_size] * page_size + position % page_size
 
+``positions`` has one axis and counts the tokens of a row; a program with positions of its own (images: several axes, and text
+behind them that does not go on at its place in the cache) takes the slots and offsets from here and brings its positions.
+
 All tensors are int32.  ``page_table`` [batch, max_pages] is changed in place; the other results come in a ``PagedPlan``
 whose tensors have fixed sizes, so that a step can be captured in a CUDA graph: ``positions`` and ``slots`` hold -1 behind
 the last token, and tokens beyond ``max_tokens`` are dropped.  ``free_count`` [1] counts what is left; it is negative when the

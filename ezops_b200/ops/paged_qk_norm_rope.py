@@ -14,7 +14,8 @@ Images and video have positions of several axes (time, height, width): ``positio
 i < D/2 is turned by the position of its axis.  ``sections`` holds the number of frequencies per axis (they add up to
 D/2).  Chunked (default): the first ``sections[0]`` frequencies belong to axis 0, the next to axis 1, ...  ``interleaved``:
 axis a > 0 has the frequencies a + axes*j for j < sections[a], axis 0 all others.  One axis is the ordinary rotation;
-equal positions on all axes give its result.
+equal positions on all axes give its result.  Behind an image the position of a token is no longer its place in the cache:
+single tokens of such a request come through this operator as well, since ``Qwen3DecodeStackOp`` rotates a token by its slot.
 
 A token with a negative position is padding (nothing is written for it), a token with a negative slot is not cached.
 Tensors (bf16 unless noted): qkv [T, (H+2*NKV)*D], rows may lie further apart; q_norm_w, k_norm_w [D] or None (unit);

@@ -15,7 +15,9 @@ with, optionally,
 * per-row lengths (``seq_lens``, each in 1..seq_len): row b's new token goes to cache slot
   ``seq_lens[b] - 1``, attends to its first ``seq_lens[b]`` keys and is rotated with the table
   row of that slot - the per-row position of sequences of different lengths in one batch
-  (the reference's attention and RoPE operators each take one length / position for all rows);
+  (the reference's attention and RoPE operators each take one length / position for all rows).
+  Tokens whose position is not their slot - those behind an image, or with several position axes -
+  go through ``PagedQkNormRopeOp`` and ``AttnPromptOp`` instead, which take single tokens too;
 
 and feeds layer ``l + 1``.  ``gen_data`` returns ``(hidden, layers, cos, sin)``
 where ``layers`` is a list of dicts of bf16 tensors: ``K_cache``, ``V_cache``

@@ -237,6 +237,8 @@ int ezb_residual_add_f32(const void* x2, const float* summed_d, void* out, int B
  * first seq_lens[b] keys and is rotated with the table row of that slot
  * (rope_position is ignored; the tables must have S rows).  That is the
  * per-row position a serving loop with sequences of different lengths needs.
+ * A token whose position is not its slot (behind an image, or with several
+ * position axes) goes through ezb_paged_qk_norm_rope and ezb_attn_prompt instead.
  * `layers` is a host array, read during the call. */
 typedef struct ezb_layer_t {
     void* K_cache;
@@ -326,7 +328,9 @@ int ezb_qwen3_decode_stack_paged(const void* hidden, void* out, const ezb_layer_
  *   ezb_paged_qk_norm_rope   head norm, rotary embedding, write into the pools
  *   ezb_attn_prompt          causal attention over the pools
  * Pools and tables are those of ezb_attn_decode_paged; a decode step can follow
- * a prompt step on them without a copy.  All index arrays are device int32. */
+ * a prompt step on them without a copy, as long as every token's rotary position is
+ * its place in the cache (the decode stack rotates by that; behind an image, single
+ * tokens go through the entries here).  All index arrays are device int32. */
 
 /* The plan of a step, on the device.  Row b has ctx_lens[b] cached and
  * new_lens[b] new tokens (values below 0 count as 0).  Its first

@@ -162,3 +162,50 @@ def test_prompts_in_pieces_then_single_tokens(cuda_device):
         assert rel(y, expected[b]) < 1e-2 * math.sqrt(LAYERS)
         worst = ((y.double() - expected[b]).norm(dim=-1) / expected[b].norm(dim=-1)).max().item()
         assert worst < 2e-2 * math.sqrt(LAYERS)
+
+
+def test_images_in_pieces_then_single_tokens(cuda_device):
+    """Requests with an image in them: positions of three axes, which the program brings and which run behind the place in the cache
+    from the image on, first in pieces, then token by token through the same operators."""
+    _lib.device_status()
+    sections = (12, 10, 10)
+    model = Model()
+    model.rope = ez.PagedQkNormRopeOp(T_MAX, SH.num_heads, SH.head_dim, MAX_PAGES * PAGE, PAGE, PAGES, num_kv_heads=SH.num_kv_heads,
+                                      sections=sections, interleaved=True, backend="cuda")
+    torch.manual_seed(1)
+    lengths, positions = [180, 70, 131], []
+    for n, (at, rows, columns) in zip(lengths, ((20, 6, 8), (0, 4, 4), (50, 2, 30))):  # text, an image of so many patches, text
+        text = torch.arange(at).expand(3, -1)
+        image = at + torch.stack([torch.zeros(rows * columns, dtype=torch.int64), torch.arange(rows).repeat_interleave(columns),
+                                  torch.arange(columns).repeat(rows)])
+        rest = at + max(rows, columns) + torch.arange(n - at - rows * columns)
+        positions.append(torch.cat([text, image, rest.expand(3, -1)], 1))
+        assert positions[-1].shape == (3, n) and int(positions[-1][:, -1].max()) < n - 1
+    sequences = [torch.randn(n, SH.hidden, device="cuda").to(torch.bfloat16) for n in lengths]
+    got, done = [[] for _ in range(B)], [0] * B
+    for new in ([100, 0, 60], [79, 66, 68], [1, 1, 1], [0, 2, 1], [0, 1, 1]):
+        x = torch.zeros(T_MAX, SH.hidden, device="cuda", dtype=torch.bfloat16)
+        where = torch.full((3, T_MAX), -1, dtype=I32)
+        at = 0
+        for b, n in enumerate(new):
+            x[at : at + n], where[:, at : at + n] = sequences[b][done[b] : done[b] + n], positions[b][:, done[b] : done[b] + n]
+            at += n
+        where = where.cuda()
+        model.new.copy_(torch.tensor(new, dtype=I32))
+        rope = model.rope
+        model.rope = lambda qkv, qw, kw, cos, sin, _, *rest, where=where, **kw2: rope(qkv, qw, kw, cos, sin, where, *rest, **kw2)
+        y, at = model.step(x), 0
+        model.rope = rope
+        for b, n in enumerate(new):
+            got[b].append(y[at : at + n])
+            at += n
+            done[b] += n
+    assert done == lengths and _lib.device_status() == 0
+    axis = torch.tensor([i % 3 if i // 3 < sections[i % 3] else 0 for i in range(SH.head_dim // 2)] * 2)
+    for b in range(B):
+        at = positions[b][axis].T.cuda()  # [tokens, D]
+        column = torch.arange(SH.head_dim, device="cuda")
+        tables = Model.__new__(Model)
+        tables.layers, tables.cos, tables.sin = model.layers, model.cos[at, column], model.sin[at, column]
+        (expected,) = whole_sequences64(tables, sequences[b : b + 1])
+        assert rel(torch.cat(got[b]), expected) < 1e-2 * math.sqrt(LAYERS)
