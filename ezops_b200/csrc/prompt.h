@@ -50,8 +50,10 @@ cudaError_t launch_paged_qk_norm_rope(const PagedRopeArgs& a, cudaStream_t strea
 
 // out[M, N] = act(x[M, K] W^T + bias) + residual; SwiGLU: W [2N, K], bias [2N], gate rows first
 enum LinearAct { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_RELU = 3, ACT_SWIGLU = 4 };
-// x / (1 + e^-x) and x (1 - erfc(x / sqrt 2) / 2) from one or two MUFU results each, to a few units of 2^-23: a result is
-// rounded to bf16, or is as uncertain from its own sum.  (With the division and erfcf a product of 5772 x 14592 results took
+// x / (1 + e^-x) and x (1 - erfc(x / sqrt 2) / 2) from two MUFU results each.  Relative error, in units of 2^-23: at most |x| + 4
+// and 3/4 x^2 + 17, the first terms from the rounding of the exponent (an exponent e has an error of up to |e| 2^-23, and the result
+// that times ln 2).  So they are exact to a few units near zero and above it, and lose bits where a negative x makes them vanish (below -87 and
+// -13 they are 0).  A result is rounded to bf16, or is as uncertain from its own sum, whose absolute error does not vanish there.  (With the division and erfcf a product of 5772 x 14592 results took
 // 512 and 429 us instead of 201 without an activation.)
 __device__ __forceinline__ float ex2_ftz(float x) {
     float y;
@@ -65,7 +67,7 @@ __device__ __forceinline__ float rcp_ftz(float x) {
 }
 __device__ __forceinline__ float silu_fast(float x) { return x * rcp_ftz(1.0f + ex2_ftz(x * -1.4426950408889634f)); }
 __device__ __forceinline__ float gelu_fast(float x) {
-    // erfc(y) = e^(-y^2) t P(t), t = 1 / (1 + 0.45 y), y >= 0: P of degree 7 with least maximum relative error (3.8e-7), found by
+    // erfc(y) = e^(-y^2) t P(t), t = 1 / (1 + 0.45 y), y >= 0: P of degree 7 with least maximum relative error (3.9e-7), found by
     // reweighted least squares
     const float t = rcp_ftz(fmaf(fabsf(x), 0.45f * 0.70710678118654752f, 1.0f));
     float s = 0.06947775930166245f;

@@ -789,3 +789,31 @@ def test_steps_without_tokens():
     with pytest.raises(ValueError, match="free_pages is empty"):
         plan = ez.PagedPlanOp(1, 4, 2, 64, 4, backend="cuda")
         plan(ints(0), ints(1), torch.zeros(1, 2, dtype=I32, device=DEV), ints(), ints(0))
+
+
+@pytest.mark.parametrize("M,N", [(5, 4000), (40, 1999), (100, 1999), (700, 2048), (700, 2001)])
+@pytest.mark.parametrize("act", ["silu", "gelu", "swiglu"])
+def test_linear_activations_in_their_tails(M, N, act):
+    """Relative bounds down to where the results vanish; the arguments are exact (a bf16 value times a power of two).  In units of
+    2^-23: silu's exponent x log2(e) is off by two roundings, |x| log2(e), which makes |x| of e^-x; ex2 2, rcp 1, sum and product 1
+    (times one more product in swiglu, half a unit).  gelu's exponent has three roundings of x^2 log2(e) / 2, which make 3/4 x^2;
+    the fit 3.3, t = rcp(..) 2 times the condition of t P(t) (below 2.5), its seven fma 4, ex2 2, products 2.  Behind that: flushed."""
+    low = -87.0 if act != "gelu" else -12.5
+    op = ez.LinearOp(M, N, 8, backend="cuda", activation=act, out_dtype=torch.float32)
+    X, W = torch.zeros(M, 8, device=DEV, dtype=BF16), torch.zeros(op.weight_rows, 8, device=DEV, dtype=BF16)
+    X[:, 0] = 2.0 ** -(torch.arange(M, device=DEV) % 5)
+    W[:N, 0] = torch.linspace(-100.0 if act != "gelu" else -16.0, 30.0, N, device=DEV)
+    if act == "swiglu":
+        W[N:, 0] = torch.linspace(1.0, 2.0, N, device=DEV)
+    out = op(X, W)
+    z = X[:, :1].double() @ W[:, 0].double()[None]
+    x = z[:, :N]
+    if act == "gelu":
+        y, units = 0.5 * x * torch.special.erfc(-x * 0.5**0.5), 0.75 * x * x + 17
+    else:
+        y, units = x / (1 + torch.exp(-x)), x.abs() + 5
+        if act == "swiglu":
+            y = y * z[:, N:]
+    # below `low` the results are smaller than 2^-118 (87 e^-87 times a factor of up to 2) and 2^-114 (12.5 erfc(12.5 / sqrt 2) / 2)
+    tol = torch.where(x < low, 2.0**-117 if act != "gelu" else 2.0**-113, units * 2**-23 * y.abs() + 2.0**-149)
+    close(out, y, tol)
