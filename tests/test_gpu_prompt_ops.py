@@ -817,3 +817,11 @@ def test_linear_activations_in_their_tails(M, N, act):
     # below `low` the results are smaller than 2^-118 (87 e^-87 times a factor of up to 2) and 2^-114 (12.5 erfc(12.5 / sqrt 2) / 2)
     tol = torch.where(x < low, 2.0**-117 if act != "gelu" else 2.0**-113, units * 2**-23 * y.abs() + 2.0**-149)
     close(out, y, tol)
+
+
+@pytest.mark.parametrize("new,ctx,H,NKV,D", [([4096], [0], 32, 8, 128), ([8191], [0], 8, 2, 128), ([4097], [0], 32, 8, 64),
+                                             ([8192], [0], 4, 4, 64), ([700, 2500, 1], [5000, 3001, 9000], 16, 4, 128),
+                                             ([1100, 1, 2300], [6000, 4000, 77], 14, 2, 64), ([939, 313, 626], [0, 0, 0], 8, 8, 64)])
+def test_attn_long_prompts(new, ctx, H, NKV, D):
+    """Thousands of tokens per row: many units per CTA, cut at both ends of a share, of both head sizes."""
+    attn_case(new, ctx, H, NKV, D, 256)
