@@ -19,8 +19,10 @@
 // last part joins them in the order of the keys (equal calls give equal bits).  Units of up to kApWhole tiles stay whole: a part
 // costs a trip through the workspace (short prompts of 14 heads of 64: 37.7 -> 17.6 us).
 //
-// What bounds it: for prompts the exponentials and the products together - 128 x 128 scores take 512 cycles each for QK^T
-// and PV (D = 128) and 1024 cycles of the MUFU, twice per step.  8192 tokens, 32/8 heads of 128: 439 us, 1250
+// What bounds it: for prompts the exponentials and the products, one behind the other - 128 x 128 scores take 512 cycles each for
+// QK^T and PV (D = 128) and 1024 cycles of the MUFU, twice per step, so either alone needs 2048 cycles of a step that takes about 3700.
+// The two were meant to overlap, and hardly do (4096 tokens: tensor pipe busy for 51.5 % of the time, MUFU 51.7 %); where a step waits has not
+// been measured.  8192 tokens, 32/8 heads of 128: 439 us, 1250
 // TFLOP/s of the products that the mask leaves (505 us at the 1.6 GHz of the power cap; the MMAs alone in this order 355 to 370
 // us); 8 prompts of 65 to 600 tokens behind 300 to 7400: 232 us (277 capped); 8192 tokens of D = 64: 380 us, of which 240 are
 // exponentials.  For single tokens the bytes

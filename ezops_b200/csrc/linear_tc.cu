@@ -9,7 +9,7 @@
 // eight warps of each CTA drain one of two accumulators while the next tile is multiplied: bias, activation, residual and
 // rounding happen there, in registers.  Grid: one CTA per SM, tiles in groups of kLtGroup tiles along A so that the x and W
 // tiles in flight stay in L2.  BN = 256 reads least per product; narrower tiles, in steps of 16 or 32, are taken where the rounds of
-// tiles come out even with them (linear_widths: 777 x 4096, K = 12288 in four rows of tiles of 208 instead of 256, 74 -> 64 us).
+// tiles come out even with them (linear_widths: 777 x 4096, K = 12288 in four rows of tiles of 208 instead of 256, 74 -> 63 us).
 //   A = x: a lane of the epilogue has a row of the result and stores whole sectors of it.
 //   A = W: a lane has a column, and a warp's stores run along a row: for rows that start anywhere (a vocabulary or a number of
 // experts that is no multiple of 16, columns of a wider tensor), where a lane with a row would write parts of sectors, and for
@@ -18,12 +18,12 @@
 // columns: 154 and 163); 4530 x 3350, K = 720, fp32 62 and 32; 104 x 22304, K = 7360 86 and 67; 128 rows of 4096 through SwiGLU to
 // 12288 61 to 67 and 50; 300 x 4096, K = 4096 15.2 to 16.6 and 16.0 to 16.9; 8192 x 4096, K = 4096 193 and 188 to 193.
 // What bounds it: the tensor cores where tiles fill the clusters evenly (4096 rows of 4096 through SwiGLU to 12288: 516 us,
-// 1600 TFLOP/s, tensor pipe active 98 % of the time; 587 at the 1.3 GHz of the power cap), with 64 to 74 of them busy to the end; the
+// 1600 TFLOP/s, tensor pipe active 98 % of the time; 587 to 640 at the 1.3 GHz of the power cap, by the card), with 64 to 74 of them busy to the end; the
 // operands' way from L2 for narrow tiles; from a few hundred rows down the weights' bytes (104 x 22304, K = 7360: 5.1 TB/s).
 // fp32 results of more than kLtSegment k blocks: the tensor cores cut their sums towards zero (gemm_tc.cu), so the sums leave them
 // every kLtSegment blocks and are added up, rounded to nearest, in the registers of the lane whose column it is (A = W); the relative
-// error is 4.8e-7 for any K (1.4e-5 at K = 12800 otherwise), and 8192 x 4096, K = 4096 takes 193 us instead of 191.  Rounded to
-// bf16 that error does not show.
+// error is 4.7e-7 for K = 512 to 12800 (1.4e-5 at K = 12800 otherwise) and grows with the root of the number of segments, one rounding
+// each, beside that (5.0e-7 at K = 204800); 8192 x 4096, K = 4096 takes 193 us instead of 191.  Rounded to bf16 that error does not show.
 // Few rows or few results (linear_in_groups): the kernel of the batched decode projections (gemm_tc.cu) with this epilogue
 // (17 x 6144, K = 4096: 10.4 us, 4.9 TB/s; 64 x 151936, K = 1024 to fp32: 57 us, 6.1 TB/s).
 #include <atomic>
@@ -505,7 +505,8 @@ static LtPlan linear_plan(int M, int N, int K, int act, bool aligned, bool f32) 
 // weight cut along K over clusters that add their parts up in shared memory (us, pairs against groups: 128 x 64, K = 4096 10.3 and
 // 5.8; 128 x 515, K = 4600 20.8 and 7.3; 300 x 512, K = 2048 8.7 and 7.3, but 555 rows 8.6 and 10.0; 2048 x 128, K = 4096 13.3 and 9.0;
 // 400 x 128, K = 512 5.2 and 4.8, but 800 rows 5.2 and 5.7; 128 x 4096, K = 12288 32.6 and 28.4, K = 4096 14.3 and 15.0, K = 1024 6.8
-// and 9.3).
+// and 9.3).  The border is a fit to these: 128 x 4096, K = 4096 lies on it and takes the groups, the slower side by 5 %.  Above 64 rows
+// each group brings the weight through L2 again, and the pairs do not cut K: neither is near the weight's bytes (5.4 us there).
 static bool linear_in_groups(int M, int N, int K) {
     const long long tiles = ((long long)M + kLinearGroupRows - 1) / kLinearGroupRows * ((N + 127ll) / 128);
     if (((long long)M + kLinearGroupRows - 1) / kLinearGroupRows > sm_count()) return false;  // a cluster each at least

@@ -16,8 +16,10 @@ behind them that does not go on at its place in the cache) takes the slots and o
 All tensors are int32.  ``page_table`` [batch, max_pages] is changed in place; the other results come in a ``PagedPlan``
 whose tensors have fixed sizes, so that a step can be captured in a CUDA graph: ``positions`` and ``slots`` hold -1 behind
 the last token, and tokens beyond ``max_tokens`` are dropped.  ``free_count`` [1] counts what is left; it is negative when the
-list was too short, and the table entries and slots of the missing pages are -1.  The reference has contiguous caches only
-(ezops/ops/attn_decode.py:52-56).
+list was too short, and the table entries and slots of the missing pages are -1.  A row holds ``max_pages * page_size`` positions:
+tokens beyond them keep their place in the step with slot -1, and ``seq_lens`` stops there.  Such a row has to be ended before its
+step: ``seq_lens`` no longer counts all of its tokens, from which attention tells what each of them sees.  The reference has
+contiguous caches only (ezops/ops/attn_decode.py:52-56).
 """
 
 from __future__ import annotations

@@ -347,7 +347,8 @@ int ezb_qwen3_decode_stack_paged(const void* hidden, void* out, const ezb_layer_
  *                             and slots are then -1
  * Tokens beyond max_tokens are dropped (cu_tokens stops there); a token beyond the
  * max_pages * page_size positions of its row gets slot -1, and seq_lens stops
- * there; an id outside [0, num_pages) is written and used as -1.  Outputs (page_table among
+ * there (ezb_attn_prompt's results for such a row mean nothing in that step: its
+ * tokens are no longer the last of seq_lens keys); an id outside [0, num_pages) is written and used as -1.  Outputs (page_table among
  * them) must not overlap inputs or each other.  B <= 8192. */
 int ezb_paged_plan(const int* ctx_lens, const int* new_lens, int* page_table, const int* free_pages, const int* free_count,
                    int* seq_lens, int* cu_tokens, int* positions, int* slots, int* free_left, int B, int max_tokens, int max_pages,
@@ -399,7 +400,7 @@ int ezb_linear_bf16(const void* X, long long ldx, const void* W, const void* bia
  * seq_lens[b] are never used, whatever they hold; the values of a row's own keys must
  * be finite (a masked key counts with weight 0, and 0 * inf is not 0).  Table entries
  * outside [0, num_pages) inside a row's length read as zeros and record fault 0x302.
- * cu_tokens is cut to [0, T], seq_lens to [0, max_pages * page_size].  Equal calls
+ * cu_tokens must not decrease; it is cut to [0, T], seq_lens to [0, max_pages * page_size].  Equal calls
  * give equal bits; where a row's sums are cut may depend on the other rows.
  * Out and the workspace must not overlap each other or an input.
  * The workspace depends on D only; as everywhere it is zero-filled once and serves one
