@@ -8,7 +8,7 @@ all (``out_dtype=torch.float32``, e.g. for scores over a vocabulary).  ``activat
 ezops/ops/qwen3_dense_decode.py:35), and act is ``silu(gate) * up``.
 
 Rows of X, residual and ``out`` may lie further apart than they are long; ``residual`` may be ``out`` itself (the residual
-stream updated in place).  X may have no rows.
+stream updated in place).  X may have no rows; sizes above 2^30 are refused.
 """
 
 from __future__ import annotations

@@ -379,7 +379,7 @@ int ezb_paged_qk_norm_rope(const void* qkv, long long ldqkv, const void* qw_or_n
  * (or none: out_f32 = 1 stores fp32).  EZB_ACT_SWIGLU: W [2N, K] and bias [2N] hold
  * the gate rows, then the up rows, and act is silu(gate) * up.  Rows of X, residual
  * (bf16) and out may be further apart than they are long (ldx, ldres, ldout in
- * elements; ldx a multiple of 8).  residual may be out itself.  K % 8 == 0.  The path,
+ * elements; ldx a multiple of 8).  residual may be out itself.  K % 8 == 0; M, N and K up to 2^30.  The path,
  * and with it the order of the sums, follows from M, N, K, the types and whether rows of
  * out (32 bytes) and residual (16) start at their boundaries.  fp32 results are added up
  * every 512 elements of K, rounded to nearest (the tensor cores cut towards zero).
